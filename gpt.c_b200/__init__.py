@@ -37,6 +37,8 @@ SIGNATURES = {
     "attn_sm100_forward_static": (_c.c_int, [_c.c_void_p] * 3 + [_c.c_int] * 4 + [_c.c_void_p]),
     "attn_sm100_static_status": (_c.c_int, [_c.POINTER(_c.c_int), _c.c_int]),
     "attn_sm100_selftest_wait_limit": (_c.c_int, [_c.c_uint, _c.c_void_p]),
+    "attn_sm100_paged_append": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_longlong] * 2 + [_c.c_int] * 12 + [_c.c_void_p]),
+    "attn_sm100_paged_forward": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_longlong] * 2 + [_c.c_int] * 10 + [_c.c_float, _c.c_void_p]),
     "attn_sm100_device_status": (_c.c_int, [_c.POINTER(_c.c_int), _c.c_int]),
     "attn_sm100_strerror": (_c.c_char_p, [_c.c_int]),
     "linear_sm100_forward": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 3 + [_c.c_void_p]),
@@ -53,6 +55,7 @@ SIGNATURES = {
     "tensor_sm100_gelu_backward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "xent_sm100_forward": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 2 + [_c.c_void_p]),
     "xent_sm100_selftest_wait_limit": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 3 + [_c.c_uint, _c.c_void_p]),
+    "xent_sm100_sample": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_longlong] + [_c.c_int] * 2 + [_c.c_void_p]),
     "xent_sm100_backward": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 2 + [_c.c_void_p]),
     "adamw_sm100_step": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] + [_c.c_float] * 5 + [_c.c_int, _c.c_void_p]),
 }
@@ -229,3 +232,45 @@ def layernorm_forward(x, w, b=None, eps: float = 1e-5, stream=None):
 def layernorm_backward(dy, x, mean, rstd, w, dw, db, dx, stream=None) -> None:
     """Accumulates into dw, db (may be None) and dx, like the reference."""
     _calls().layernorm_backward(dy, x, mean, rstd, w, dw, db, dx, _raw(stream))
+
+
+# ---------------------------------------------------------------------------------------------
+# Generation: a paged key/value cache with the attention that reads it (include/attn_sm100.h), and the draw of the next
+# token (include/xent_sm100.h).  The reference's infer_gpt.c:341-408 has no cache and draws on the host.
+#
+# A layer's cache is k_pages and v_pages [pages, kv_heads, page_size, head_size], fp32 or bf16.  A step brings rows of several
+# sequences, one behind the other: page_table [sequences, pages], cu_seqlens [sequences + 1] (first row of each, and the
+# end) and past [sequences] (positions before the step) are int32 tensors beside them.
+# ---------------------------------------------------------------------------------------------
+def paged_append(qkv, k_pages, v_pages, page_table, cu_seqlens, past, rotary=None, rotary_pairs: bool = False, stream=None):
+    """Stores the keys and values of qkv [tokens, (n_heads + 2 kv_heads) * head_size] in their sequences' pages and returns the
+    queries [tokens, n_heads * head_size]: a view of qkv, or with `rotary` (see rotary_table) a tensor of queries rotated by
+    their positions, as the stored keys are.  Columns i and i + R/2 of a head make a pair, or 2i and 2i + 1 with rotary_pairs."""
+    return _calls().paged_append(qkv, k_pages, v_pages, page_table, cu_seqlens, past, rotary, rotary_pairs, _raw(stream))
+
+
+def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, past, max_new: int = 0, scale=None, out=None, stream=None):
+    """Causal attention of q [tokens, n_heads * head_size] over the pages, the new tokens' own keys among them.  `max_new`: the
+    largest number of new tokens of a sequence, 0 where the program does not know it; `scale`: head_size ** -0.5 if None.
+    Rows behind the last sequence are not written."""
+    return _calls().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, past, max_new, scale, out, _raw(stream))
+
+
+def rotary_table(positions: int, dim: int, base: float = 10000.0, device="cuda"):
+    """The table [positions, dim] that paged_append takes as `rotary`: cosines, then sines, of position * base ** (-2 i / dim),
+    the angles in 64 bits."""
+    import torch
+
+    if positions < 1 or dim < 2 or dim % 2:
+        raise ValueError("positions must be positive and dim even")
+    freq = base ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """One class (int32) for each row of logits [rows, classes], drawn with u [rows] from [0, 1).  temperature, top_p and min_p
+    (fp32) and top_k (int32) have one value a row, or are None: exp((x - max) / temperature) are the weights, the largest top_k
+    classes are kept, of these the shortest run with top_p of their weight, of these the ones with min_p of the largest
+    weight.  temperature 0 takes the largest logit.  A row with a NaN, or of -inf alone, gives -1."""
+    return _calls().sample(logits, u, temperature, top_k, top_p, min_p, _raw(stream))

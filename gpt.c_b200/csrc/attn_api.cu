@@ -341,6 +341,7 @@ const char *attn_sm100_strerror(int code) {
         case ATTN_ERR_KERNEL: return "a kernel gave up a bounded wait (see attn_sm100_device_status)";
         case ATTN_ERR_STATIC_CAPACITY:
             return "attn_sm100_forward_static: B*T*3*H*D exceeds the 4,194,304 elements the built-in scratch array holds";
+        case ATTN_ERR_ARGUMENT: return "an argument (a size, stride, type or count) is outside what the entry point's description allows";
         default: break;
     }
     if (code > 0) return cudaGetErrorString(static_cast<cudaError_t>(code));

@@ -1,4 +1,4 @@
-// The tensor-level calls of the Python package (forward, backward, linear_*, layernorm_*) as a CPython extension
+// The tensor-level calls of the Python package (forward, backward, linear_*, layernorm_*, paged_*, sample) as a CPython extension
 // over the C ABI of libattn_sm100.so.
 //
 // What bounds small calls is the host: with these functions written in Python, a forward and backward of
@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -21,6 +22,7 @@
 #include "../../include/tensor_sm100.h"
 #include "../../include/xent_sm100.h"
 
+#include <cmath>
 #include <tuple>
 #include <utility>
 
@@ -312,6 +314,166 @@ PyObject *layernorm_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------
+// Generation: the paged cache and the draw of a token.  These take tensors on any one device, current or not, and views
+// whose rows lie apart; without a stream they run on the current stream of that device.
+// ------------------------------------------------------------------------------------------
+// The device of a call's tensors made current, and the stream of the call: outputs are allocated for it.
+struct On {
+    c10::cuda::CUDAGuard device;
+    c10::cuda::OptionalCUDAStreamGuard own;
+    void *stream;
+    On(const at::Tensor &t, PyObject *s) : device(t.device()) {
+        if (s == Py_None) {
+            stream = c10::cuda::getCurrentCUDAStream().stream();
+        } else {
+            stream = PyLong_AsVoidPtr(s);
+            if (!PyErr_Occurred()) own.reset_stream(c10::cuda::getStreamFromExternal(static_cast<cudaStream_t>(stream), t.device().index()));
+        }
+    }
+};
+
+bool is(const at::Tensor &t, at::ScalarType type, const at::Tensor &beside) {
+    return t.scalar_type() == type && t.device() == beside.device();
+}
+
+struct Pages {
+    const at::Tensor *k, *v, *table, *cu, *past;
+    int type = 0, tokens = 0, seqs = 0, kv_heads = 0, D = 0, page_size = 0, pages = 0, width = 0;
+    long long stride = 0;
+
+    // `x` [tokens, ...] beside the cache in arguments i .. i + 4; false with a Python error set
+    bool read(Args &a, const at::Tensor &x, int i) {
+        k = a.tensor(i), v = a.tensor(i + 1), table = a.tensor(i + 2), cu = a.tensor(i + 3), past = a.tensor(i + 4);
+        if (!a.ok) return false;
+        if (!(x.is_cuda() && x.scalar_type() == at::kFloat && x.dim() == 2 && (x.size(1) < 2 || x.stride(1) == 1)))
+            return value_error("the first argument must be an fp32 CUDA tensor of shape [tokens, columns] with its columns side by side") != nullptr;
+        if (!((k->scalar_type() == at::kFloat || k->scalar_type() == at::kBFloat16) && k->dim() == 4 && k->device() == x.device()))
+            return value_error("k_pages must be an fp32 or bf16 tensor of shape [pages, kv_heads, page_size, head_size] on the same device") != nullptr;
+        if (!(v->scalar_type() == k->scalar_type() && v->sizes() == k->sizes() && v->device() == x.device()))
+            return value_error("v_pages must be like k_pages") != nullptr;
+        for (const at::Tensor *t : {k, v})
+            if (!t->numel() || !t->select(0, 0).is_contiguous() || (t->size(0) > 1 && (t->stride(0) != k->stride(0) || t->stride(0) < t->select(0, 0).numel())))
+                return value_error("pages must each be contiguous, and as far apart in v_pages as in k_pages") != nullptr;
+        if (!(is(*table, at::kInt, x) && table->dim() == 2 && table->is_contiguous()))
+            return value_error("page_table must be a contiguous int32 tensor of shape [sequences, pages] on the same device") != nullptr;
+        if (!(is(*cu, at::kInt, x) && cu->dim() == 1 && cu->is_contiguous() && cu->size(0) == table->size(0) + 1))
+            return value_error("cu_seqlens must be an int32 tensor of sequences + 1 values on the same device") != nullptr;
+        if (!(is(*past, at::kInt, x) && past->dim() == 1 && past->is_contiguous() && past->size(0) == table->size(0)))
+            return value_error("past must be an int32 tensor of one value a sequence on the same device") != nullptr;
+        for (int64_t n : {x.size(0), k->size(0), k->size(1), k->size(2), table->size(0), table->size(1)})
+            if (n > 0x7fffffff) return value_error("a size does not fit 31 bits") != nullptr;
+        if (x.size(0) > 1 && x.stride(0) < x.size(1)) return value_error("rows must not overlap") != nullptr;
+        type = k->scalar_type() == at::kBFloat16 ? ATTN_CACHE_BF16 : ATTN_CACHE_F32;
+        tokens = (int)x.size(0), seqs = (int)table->size(0), width = (int)table->size(1);
+        pages = (int)k->size(0), kv_heads = (int)k->size(1), page_size = (int)k->size(2), D = (int)k->size(3);
+        stride = pages > 1 ? k->stride(0) : (long long)kv_heads * page_size * D;
+        return true;
+    }
+};
+
+long long row_stride(const at::Tensor &x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+// paged_append(qkv, k_pages, v_pages, page_table, cu_seqlens, past, rotary or None, rotary_pairs, stream) -> q
+PyObject *paged_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 9);
+    const at::Tensor *qkv = a.tensor(0);
+    Pages p;
+    if (!a.ok || !p.read(a, *qkv, 1)) return nullptr;
+    const at::Tensor *rotary = args[6] == Py_None ? nullptr : a.tensor(6);
+    const int pairs = a.ok ? PyObject_IsTrue(args[7]) : 0;
+    if (!a.ok || pairs < 0) return nullptr;
+    const int64_t C = qkv->size(1) - 2 * (int64_t)p.kv_heads * p.D;
+    if (C <= 0 || C % ((int64_t)p.kv_heads * p.D)) return value_error("qkv must have (n_heads + 2 kv_heads) * head_size columns, n_heads a multiple of kv_heads");
+    if (rotary && !(is(*rotary, at::kFloat, *qkv) && rotary->dim() == 2 && rotary->is_contiguous() && rotary->size(0) > 0 && rotary->size(0) <= 0x7fffffff &&
+                    rotary->size(1) > 0 && rotary->size(1) <= p.D && rotary->size(1) % 2 == 0))
+        return value_error("rotary must be a contiguous fp32 tensor of shape [positions, an even number of columns up to head_size] on the same device");
+    const On on(*qkv, args[8]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor q = rotary ? alloc({qkv->size(0), C}, at::kFloat, *qkv) : qkv->narrow(1, 0, C);
+    const int heads = (int)(C / p.D), positions = rotary ? (int)rotary->size(0) : 0, dim = rotary ? (int)rotary->size(1) : 0;
+    const float *x = static_cast<const float *>(qkv->data_ptr()), *angles = rotary ? static_cast<const float *>(rotary->data_ptr()) : nullptr;
+    float *out = rotary ? static_cast<float *>(q.data_ptr()) : nullptr;
+    int rc = ATTN_OK;
+    Py_BEGIN_ALLOW_THREADS
+    if (p.tokens)
+        rc = attn_sm100_paged_append(x, out, p.k->data_ptr(), p.v->data_ptr(), static_cast<const int *>(p.table->data_ptr()),
+                                     static_cast<const int *>(p.cu->data_ptr()), static_cast<const int *>(p.past->data_ptr()), angles, row_stride(*qkv), p.stride,
+                                     p.type, p.tokens, p.seqs, heads, p.kv_heads, p.D, p.page_size, p.pages, p.width, positions, dim, pairs, on.stream);
+    Py_END_ALLOW_THREADS
+    if (failed(rc, "attn_sm100_paged_append")) return nullptr;
+    return THPVariable_Wrap(q);
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, past, max_new, scale or None, out or None, stream) -> out
+PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 10);
+    const at::Tensor *q = a.tensor(0);
+    Pages p;
+    if (!a.ok || !p.read(a, *q, 1)) return nullptr;
+    const long max_new = a.integer(6);
+    const double scale = args[7] == Py_None ? 1.0 / std::sqrt((double)p.D) : a.real(7);
+    const at::Tensor *given = args[8] == Py_None ? nullptr : a.tensor(8);
+    if (!a.ok) return nullptr;
+    if (q->size(1) == 0 || q->size(1) % ((int64_t)p.kv_heads * p.D)) return value_error("q must have n_heads * head_size columns, n_heads a multiple of kv_heads");
+    if (max_new < 0 || max_new > 0x7fffffff) return value_error("max_new must be a count, or 0 where it is not known");
+    if (given && !(is(*given, at::kFloat, *q) && given->is_contiguous() && given->sizes() == q->sizes()))
+        return value_error("out must be a contiguous fp32 tensor of the shape of q on the same device");
+    const On on(*q, args[9]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor out = given ? *given : alloc(q->sizes(), at::kFloat, *q);
+    const int heads = (int)(q->size(1) / p.D);
+    const float *x = static_cast<const float *>(q->data_ptr());
+    float *y = static_cast<float *>(out.data_ptr());
+    int rc = ATTN_OK;
+    Py_BEGIN_ALLOW_THREADS
+    if (p.tokens)
+        rc = attn_sm100_paged_forward(x, p.k->data_ptr(), p.v->data_ptr(), static_cast<const int *>(p.table->data_ptr()),
+                                      static_cast<const int *>(p.cu->data_ptr()), static_cast<const int *>(p.past->data_ptr()), y, row_stride(*q), p.stride, p.type,
+                                      p.tokens, p.seqs, heads, p.kv_heads, p.D, p.page_size, p.pages, p.width, (int)max_new, (float)scale, on.stream);
+    Py_END_ALLOW_THREADS
+    if (failed(rc, "attn_sm100_paged_forward")) return nullptr;
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, u, temperature or None, top_k or None, top_p or None, min_p or None, stream) -> tokens
+PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 7);
+    const at::Tensor *x = a.tensor(0);
+    if (!a.ok) return nullptr;
+    if (!(x->is_cuda() && x->scalar_type() == at::kFloat && x->dim() == 2 && x->size(1) > 0 && (x->size(1) == 1 || x->stride(1) == 1) &&
+          (x->size(0) < 2 || x->stride(0) >= x->size(1)) && x->size(0) <= 0x7fffffff && x->size(1) <= 0x7fffffff))
+        return value_error("logits must be an fp32 CUDA tensor of shape [rows, classes] with a row's values side by side");
+    const void *each[5] = {};  // u, temperature, top_k, top_p, min_p
+    for (int i = 0; i < 5; i++) {
+        if (i > 0 && args[1 + i] == Py_None) continue;
+        const at::Tensor *t = a.tensor(1 + i);
+        if (!a.ok) return nullptr;
+        if (!(is(*t, i == 2 ? at::kInt : at::kFloat, *x) && t->is_contiguous() && t->dim() == 1 && t->size(0) == x->size(0)))
+            return value_error("u, temperature, top_p and min_p must be fp32, top_k int32, with one value a row of logits, on the same device");
+        each[i] = t->data_ptr();
+    }
+    const On on(*x, args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    at::Tensor out = alloc({x->size(0)}, at::kInt, *x);
+    const float *logits = static_cast<const float *>(x->data_ptr());
+    int *y = static_cast<int *>(out.data_ptr()), rc = ATTN_OK;
+    const int rows = (int)x->size(0), C = (int)x->size(1);
+    Py_BEGIN_ALLOW_THREADS
+    if (rows)
+        rc = xent_sm100_sample(logits, static_cast<const float *>(each[0]), static_cast<const float *>(each[1]), static_cast<const int *>(each[2]),
+                               static_cast<const float *>(each[3]), static_cast<const float *>(each[4]), y, rows > 1 ? x->stride(0) : C, rows, C, on.stream);
+    Py_END_ALLOW_THREADS
+    if (failed(rc, "xent_sm100_sample")) return nullptr;
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------
 // What calling a ctypes function of the library does instead, as the tp_call of its function object's class: a call with
 // exactly as many plain numbers (or None for a pointer) as the function has arguments goes to the C ABI from here, every
 // other one to ctypes.
@@ -382,7 +544,7 @@ PyObject *set_error(PyObject *, PyObject *cls) {
 
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(forward), FAST(backward), FAST(forward_into), FAST(backward_into), FAST(linear_forward),
-                          FAST(linear_backward), FAST(layernorm_forward), FAST(layernorm_backward),
+                          FAST(linear_backward), FAST(layernorm_forward), FAST(layernorm_backward), FAST(paged_append), FAST(paged_attention), FAST(sample),
                           {"set_error", set_error, METH_O, nullptr}, {"shorten_calls", shorten_calls, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "gptc_b200_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -69,6 +69,7 @@ extern "C" {
 #define ATTN_ERR_DEVICE (-5)      /* current device is not an sm_100 GPU, or a driver entry point is missing */
 #define ATTN_ERR_KERNEL (-6)      /* reported by attn_sm100_device_status: a kernel gave up a bounded wait */
 #define ATTN_ERR_STATIC_CAPACITY (-7) /* attn_sm100_forward_static: the problem needs more than ATTN_STATIC_SCRATCH_BYTES */
+#define ATTN_ERR_ARGUMENT (-8)        /* attn_sm100_paged_*, xent_sm100_sample: an argument outside what its description allows */
 
 /* flags */
 #define ATTN_FLAG_FORCE_GENERIC 1 /* use the general kernels even when those for D = 64 apply */
@@ -192,6 +193,58 @@ int attn_sm100_selftest_wait_limit(unsigned limit_us, void *stream);
  * word is reset.  Returns ATTN_OK, ATTN_ERR_KERNEL when *status != 0, or a cudaError_t.
  */
 int attn_sm100_device_status(int *status, int clear);
+
+/*
+ * Paged key/value cache, for generation.  (No counterpart in the reference: infer_gpt.c:341-408 runs the whole context again
+ * for every token.)
+ *
+ * A layer's cache is two arrays of pages, k_pages and v_pages, of fp32 (ATTN_CACHE_F32) or bf16 (ATTN_CACHE_BF16) elements:
+ * page n holds page_size positions of every key/value head, [kv_heads, page_size, D], and begins n * page_stride elements
+ * behind page 0 (page_stride >= kv_heads * page_size * D; a larger one lets keys and values, or layers, share an allocation).
+ * A step brings `tokens` rows of `seqs` sequences, one sequence behind the other:
+ *   page_table [seqs, table_width]   the pages of each sequence in the order of its positions; entries behind its last
+ *                                    position are not read
+ *   cu_seqlens [seqs + 1]            first row of each sequence's new tokens, and the end; rows from cu_seqlens[seqs] on
+ *                                    belong to no sequence: nothing is read from or written for them.  A sequence may bring none
+ *   past       [seqs]                positions that each sequence holds before the step: its i-th new token has position past + i
+ * all 32-bit, on the device: a captured step may be replayed with other lengths and pages in them.
+ *   n_heads    query heads, a multiple of kv_heads: query head h reads key/value head h / (n_heads / kv_heads)
+ *   D          a multiple of 8, up to 256; page_size any, up to 2^20, with table_width * page_size below 2^31 - 2^20
+ * A position outside the page table, a page number outside 0 .. pages - 1, a negative `past`, or more new tokens in a sequence than
+ * max_new touch no memory: the token is not stored, the key has no weight, the sequence's rows are not written; and
+ * attn_sm100_device_status reports 2001 (append) or 2002 (attention).
+ * Pages must not be shared between sequences that write to them in the same step.
+ */
+#define ATTN_CACHE_F32 0
+#define ATTN_CACHE_BF16 1
+
+/*
+ * Stores a step's keys and values in the pages of their sequences, with the rotation by position on the way.
+ *   qkv    [tokens, (n_heads + 2 kv_heads) * D] fp32, rows `ld` elements apart (a multiple of 4): queries | keys | values
+ *   rotary NULL, or [positions, rotary_dim] fp32: for each position rotary_dim / 2 cosines and as many sines.  The first
+ *          rotary_dim columns (even, up to D) of every query and key head are rotated in pairs, (a, b) to
+ *          (a cos - b sin, b cos + a sin): columns i and i + rotary_dim / 2, or 2i and 2i + 1 with rotary_pairs not 0
+ *   q_out  [tokens, n_heads * D] fp32: the rotated queries; may be NULL, and is not written, without `rotary`
+ * Values are rounded to the cache's type once, to nearest.
+ */
+int attn_sm100_paged_append(const float *qkv, float *q_out, void *k_pages, void *v_pages, const int *page_table, const int *cu_seqlens,
+                            const int *past, const float *rotary, long long ld, long long page_stride, int cache_type, int tokens, int seqs,
+                            int n_heads, int kv_heads, int D, int page_size, int pages, int table_width, int positions, int rotary_dim,
+                            int rotary_pairs, void *stream);
+
+/*
+ * Attention of a step's new tokens over the pages, in which their own keys and values are already (attn_sm100_paged_append):
+ *     out[t, h] = sum_{j <= past + i} softmax_j( scale * q[t, h] . k[j] ) v[j]       t the i-th new token of its sequence
+ *   q       [tokens, n_heads * D] fp32, rows `ld` elements apart (a multiple of 4)
+ *   out     [tokens, n_heads * D] fp32; rows of no sequence are left as they were
+ *   max_new the largest number of new tokens that a sequence may bring (0: not known); the kernel and the size of its launch go by it
+ * Scores and sums are fp32, from q in fp32 and the cache's elements as they are.  A score of -inf has no weight, a row without any
+ * weight is 0; NaN and infinities among keys and values that a row does not see do not reach it.
+ */
+int attn_sm100_paged_forward(const float *q, const void *k_pages, const void *v_pages, const int *page_table, const int *cu_seqlens,
+                             const int *past, float *out, long long ld, long long page_stride, int cache_type, int tokens, int seqs,
+                             int n_heads, int kv_heads, int D, int page_size, int pages, int table_width, int max_new, float scale,
+                             void *stream);
 
 /* Human-readable text for a return value of this library (static storage). */
 const char *attn_sm100_strerror(int code);

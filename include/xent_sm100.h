@@ -41,6 +41,25 @@ int xent_sm100_selftest_wait_limit(const float *logits, const float *targets, fl
  */
 int xent_sm100_backward(const float *g, const float *targets, const float *logsm, float *dout, int rows, int C, void *stream);
 
+/*
+ * Draws a class from each row of logits with given random numbers.  (The reference's infer_gpt.c:341-408 divides by the temperature,
+ * takes the softmax on the GPU and draws on the host; it has no top-k, top-p or min-p.)  Row r, with classes in the order of falling
+ * logits, equal ones by index:
+ *     w_i = exp((x_i - max x) / temperature[r])
+ *     kept: the first top_k[r] classes; of these the shortest run from the front with at least top_p[r] of their weight, one at
+ *           least; of these the ones with w_i >= min_p[r]
+ *     tokens[r] = the first class, in the order of the index, at which the running sum of the kept weights exceeds u[r] times their sum
+ * Each of temperature, top_k, top_p and min_p has one value a row, or is NULL (1, all, all, all).  temperature <= 0 or NaN: the
+ * largest logit, the first of equal ones.  top_k outside 1 .. C - 1, top_p >= 1 and min_p <= 0, or NaN, restrict nothing; top_p <= 0 and
+ * min_p >= 1 keep the classes of the largest logit only, the first of them and all of them.  u is in [0, 1) (outside: the nearest
+ * number inside; NaN: 0).  A logit of +inf has all the weight, one of -inf none; a row with a NaN, or of -inf alone, has no
+ * class to draw: its token is -1.
+ * Weights are 64-bit whole numbers, 2^-44 of the largest one each, so that every sum is exact and the token does not depend on the order in
+ * which they are added; C is at most 425984.  Rows are `ld` elements apart (any number from C on).
+ */
+int xent_sm100_sample(const float *logits, const float *u, const float *temperature, const int *top_k, const float *top_p,
+                      const float *min_p, int *tokens, long long ld, int rows, int C, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
