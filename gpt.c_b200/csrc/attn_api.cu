@@ -2,6 +2,7 @@
 // and kernel dispatch.  Declarations and the reference interfaces they replace are in
 // include/attn_sm100.h.
 #include "attn_internal.h"
+#include "paged_attn.cuh"
 #include "tc05.cuh"
 
 #include <math.h>
@@ -177,6 +178,7 @@ int attn_sm100_init(void) {
     if ((e = attn::fast_bwd_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = attn::attn24_fwd_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = attn::attn24_bwd_set_attributes()) != cudaSuccess) return (int)e;
+    if ((e = paged::tiles_set_attributes()) != cudaSuccess) return (int)e;
 
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return (int)e;

@@ -12,6 +12,7 @@
 
 #include "attn_internal.h"
 #include "paged.cuh"
+#include "paged_attn.cuh"
 #include "tc05.cuh"
 
 #include "../../include/attn_sm100.h"
@@ -67,7 +68,8 @@ __device__ __forceinline__ uint4 load16(const void *p) {
 // kLanes: lanes of a key; kChunks: 16-byte words of a lane
 template <class T, int kLanes, int kChunks, int kRows>
 __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float *q, float *out, long long ld, int heads,
-                                                            int groups, int max_new, float scale_log2, int *status) {
+                                                            int groups, int few, int max_new, float scale_log2,
+                                                            int *status) {
     constexpr int kN = Words<T>::kN, kWidth = kLanes * kChunks * kN, kKeys = 32 / kLanes, kBatch = 4 / kChunks;
     __shared__ Partial<kRows, kWidth> part[kWarps];
     cg::cluster_group cluster = cg::this_cluster();
@@ -80,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
     const Span w = span_of(c, s);
     const int rows = w.count * G;
     if (unit % groups == 0 && kvh == 0 && rank == 0 && threadIdx.x == 0 && (w.count > max_new || (w.count > 0 && w.past < 0))) report(status, ST_ATTEND);
-    if (row0 >= rows || w.past < 0 || w.count > max_new) return;  // the whole cluster
+    if (row0 >= rows || rows > few || w.past < 0 || w.count > max_new) return;  // the whole cluster
     const int last = min(row0 + kRows, rows) - 1;
     const long long room = (long long)c.width * c.page_size;
     const int keys = (int)min((long long)w.past + last / G + 1, room);
@@ -250,20 +252,9 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
 // ------------------------------------------------------------------------------------------
 // launch
 // ------------------------------------------------------------------------------------------
-struct Call {
-    Cache c;
-    const float *q;
-    float *out;
-    long long ld;
-    int heads, max_new, type;
-    float scale_log2;
-    int *status;
-    cudaStream_t s;
-};
-
 template <class T, int kLanes, int kChunks, int kRows>
-cudaError_t launch_few(const Call &a) {
-    const int G = a.heads / a.c.kv_heads, groups = (int)(((long long)a.max_new * G + kRows - 1) / kRows);
+cudaError_t launch_few(const Call &a, int few) {
+    const int G = a.heads / a.c.kv_heads, groups = (int)((min((long long)a.max_new * G, (long long)few) + kRows - 1) / kRows);
     const long long units = (long long)a.c.seqs * groups, all = units * a.c.kv_heads;
     const int sms = attn::sm_count();
     unsigned ranks = 1;
@@ -272,25 +263,40 @@ cudaError_t launch_few(const Call &a) {
     while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
     if (units * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     return attn::launch_clusters_after_previous(few_rows_kernel<T, kLanes, kChunks, kRows>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(kThreads),
-                                                0, ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, groups, a.max_new, a.scale_log2, a.status);
+                                                0, ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, groups, few, a.max_new, a.scale_log2, a.status);
 }
 
 template <class T, int kLanes, int kChunks>
-cudaError_t launch_rows(const Call &a) {
-    const long long rows = (long long)a.max_new * (a.heads / a.c.kv_heads);
-    if (rows == 1) return launch_few<T, kLanes, kChunks, 1>(a);
-    if (rows == 2) return launch_few<T, kLanes, kChunks, 2>(a);
-    return launch_few<T, kLanes, kChunks, 4>(a);
+cudaError_t launch_rows(const Call &a, int few) {
+    const long long rows = min((long long)a.max_new * (a.heads / a.c.kv_heads), (long long)few);
+    if (rows == 1) return launch_few<T, kLanes, kChunks, 1>(a, few);
+    if (rows == 2) return launch_few<T, kLanes, kChunks, 2>(a, few);
+    return launch_few<T, kLanes, kChunks, 4>(a, few);
 }
 
 template <class T>
-cudaError_t launch(const Call &a) {
+cudaError_t launch(const Call &a, int few) {
     const int words = a.c.D / Words<T>::kN;  // of 16 bytes
-    if (words <= 4) return launch_rows<T, 4, 1>(a);
-    if (words <= 8) return launch_rows<T, 8, 1>(a);
-    if (words <= 16) return launch_rows<T, 16, 1>(a);
-    if (words <= 32) return launch_rows<T, 32, 1>(a);
-    return launch_rows<T, 32, 2>(a);
+    if (words <= 4) return launch_rows<T, 4, 1>(a, few);
+    if (words <= 8) return launch_rows<T, 8, 1>(a, few);
+    if (words <= 16) return launch_rows<T, 16, 1>(a, few);
+    if (words <= 32) return launch_rows<T, 32, 1>(a, few);
+    return launch_rows<T, 32, 2>(a, few);
+}
+
+// Sequences of up to kFewRows rows go to the kernel above, which reads their keys at the HBM rate, the others to the tensor
+// cores; both kernels find their own sequences on the device, so a step that mixes them takes two launches.
+constexpr int kFewRows = 4;
+constexpr int kMeanRows = 128;  // from this many rows a sequence on, on average, the tensor cores take all of them in one launch
+
+cudaError_t forward(const Call &a) {
+    const long long G = a.heads / a.c.kv_heads, most = a.max_new * G;
+    if (most <= kFewRows || a.c.D > 128) return a.type == ATTN_CACHE_BF16 ? launch<__nv_bfloat16>(a, 0x7fffffff) : launch<float>(a, 0x7fffffff);
+    const bool both = G <= kFewRows && a.c.tokens * G < (long long)kMeanRows * a.c.seqs;
+    const int few = both ? kFewRows : 0;
+    const cudaError_t e = launch_tiles(a, few);
+    if (e != cudaSuccess || !both) return e;
+    return a.type == ATTN_CACHE_BF16 ? launch<__nv_bfloat16>(a, few) : launch<float>(a, few);
 }
 
 }  // namespace
@@ -310,9 +316,9 @@ extern "C" int attn_sm100_paged_forward(const float *q, const void *k_pages, con
     if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
     if (tokens == 0) return ATTN_OK;
     const int most = max_new == 0 || max_new > tokens ? tokens : max_new;
-    if ((long long)most * (n_heads / kv_heads) > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;
+    if ((long long)tokens * (n_heads / kv_heads) > 0x3fffffffll) return ATTN_ERR_UNSUPPORTED;
     const paged::Call a{{const_cast<void *>(k_pages), const_cast<void *>(v_pages), page_table, cu_seqlens, past, page_stride, seqs, kv_heads, D, page_size, pages,
                          table_width, tokens},
                         q, out, ld, n_heads, most, cache_type, scale * 1.4426950408889634f, status, static_cast<cudaStream_t>(stream)};
-    return (int)(cache_type == ATTN_CACHE_BF16 ? paged::launch<__nv_bfloat16>(a) : paged::launch<float>(a));
+    return (int)paged::forward(a);
 }
