@@ -126,3 +126,7 @@ int encode_tiled(CUtensorMap *map, CUtensorMapDataType dtype, unsigned rank, con
 int device_status_word(int **status);
 
 }  // namespace attn
+
+namespace sample {
+cudaError_t set_attributes();  // of the kernel that draws a class from each row of logits (sample_sm100.cu)
+}
