@@ -4,12 +4,15 @@
 // that order, so the classes kept are those above one logit and, of those equal to it, the ones up to an index.  A weight is a
 // whole number, round(2^44 exp((x - max) / T)): sums of up to 2^19 of them fit 64 bits and are exact in any order.
 //
-// A cluster of 1 to 8 CTAs holds a row in shared memory, each CTA a piece, and reads it once.  Where a run ends (the k-th class, or the
-// one at which the weight reaches p of all) is found by a histogram over 2048 steps of max - x: counts or weights are added up in shared
-// memory, the step in which the run ends is taken from their sums over the cluster, and the classes of that step, some dozens,
-// are put in order by comparing each with each.  Where they are more than that (equal logits, outliers that stretch the steps)
-// the histogram is taken again over their order-preserving 32-bit keys, 2048 times finer each time.  Then one pass adds up what is kept, in
-// the order of the index, and one warp walks the stretch in which the draw falls.
+// A cluster of 1 to 8 CTAs holds a row in shared memory, each CTA a piece, and reads it once, 16 bytes at a time.
+//
+// Few classes matter where top-k or min-p is given: min-p leaves those within T ln(1 / min_p) of the largest logit; and no
+// fewer than k logits lie at or above the k-th largest of the maxima of four neighbours each, which a histogram over a quarter as
+// many values finds.  They go to a list in one CTA (up to 2048, most often little more than k), which ends the runs and draws.
+// Otherwise, and where the list is too short, the cluster looks through the row: where a run ends is found by a histogram of counts or
+// weights over 2048 steps of max - x, and the classes of the step in which it ends are put in order by comparing
+// each with each; where they are too many for that, the histogram is taken again over their keys, 2048 times finer each time.
+//
 #include <cooperative_groups.h>
 
 #include "attn_internal.h"
@@ -22,10 +25,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kRanks = 8;      // CTAs of a row at most
 constexpr int kBins = 2048;    // of a histogram
 constexpr int kList = 512;     // classes that are compared each with each
+constexpr int kMost = 2048;    // classes of the list
 constexpr int kMaxC = 425984;  // a piece of kMaxC / kRanks logits fits shared memory beside the rest
 typedef unsigned long long u64;
 
@@ -39,17 +42,26 @@ struct Smem {
             int index[kList];
             u64 weight[kList];
         };
+        struct {  // the same, of the list
+            u64 order[kList], value[kList];
+        };
+        struct {
+            uint32_t list_key[kMost];
+            int list_index[kMost];
+        };
     };
+    double powers[64];              // 2^(i / 64)
     u64 sums[kRanks];               // of the CTAs, in the order of their pieces
-    u64 at[kWarps];
+    u64 at[32];                     // of this CTA's warps
     u64 before;                     // what lies in front of `bin`
-    float2 range[kRanks];           // each CTA's largest logit and smallest finite one
-    int nan[kRanks];
+    u64 end, omin, omax;            // in the list
+    float2 range[kRanks];           // each CTA's largest logit, NaN if one is, and its smallest maximum of four
     int bin;
     uint32_t count, kmin, kmax;     // rank 0: classes of the step, and the range of their keys
     uint32_t edge;                  // the last class kept
     int upto;
-    int found;
+    int taken, counts[kRanks];      // classes that this CTA, each CTA has put in the list
+    int first;                      // rank 0: the first class with the largest logit
 };
 
 // The order of fp32 numbers as that of 32-bit ones (-0 counts as +0).
@@ -75,13 +87,15 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
 }
 
 // One row as its cluster sees it.
+template <int kThreads>
 struct Row {
+    static constexpr int kWarps = kThreads / 32, kEach = kMost / kThreads;
     Smem &sm;
-    const float *x;  // this CTA's piece, in shared memory
-    int n, base;     // its length, and its first class
-    int ranks, rank;
+    const float *x;    // this CTA's piece, in shared memory, from a 16-byte boundary of the row's memory on
+    int begin, end;    // the logits in it; class of the first place: base
+    int base, ranks, rank;
     float max;
-    double inv_t;
+    double by;         // 64 log2(e) / T
 
     __device__ __forceinline__ void sync() const {
         if (ranks > 1) cg::this_cluster().sync();
@@ -93,20 +107,31 @@ struct Row {
         return ranks > 1 ? cg::this_cluster().map_shared_rank(p, r) : p;
     }
 
+    // 2^44 exp((v - max) / T) by 2^(n / 64) from a table and the series of exp for what is left, |r| <= ln(2) / 128: the first term
+    // left out is 2^-44 of the result.  Adding 2^52 rounds it to a whole number.
     __device__ __forceinline__ u64 weight(float v) const {
-        if (v == max) return 1ull << 44;
-        if (v == -INFINITY || max == INFINITY) return 0;
-        return __double2ull_rn(exp(((double)v - (double)max) * inv_t) * 17592186044416.0);
+        constexpr double kWhole = 6755399441055744.0, kLn = 0.010830424696249145;  // 1.5 * 2^52, ln(2) / 64
+        const double d = (double)v - (double)max, k = fma(d, by, kWhole);
+        const int n = __double2loint(k);
+        const double r = fma(d, by, kWhole - k);
+        const double s = r * fma(r, fma(r, fma(r, kLn * kLn * kLn * kLn / 24, kLn * kLn * kLn / 6), kLn * kLn / 2), kLn);
+        const double p = sm.powers[n & 63], w = fma(p, s, p);
+        const double whole = __hiloint2double(__double2hiint(w) + (((n >> 6) + 44) << 20), __double2loint(w)) + 4503599627370496.0;
+        // no branches: several of these are under way at a time
+        const bool some = v > -INFINITY && max < INFINITY && d * by >= -46.0 * 64, all = v == max;
+        const uint32_t low = some && !all ? (uint32_t)__double2loint(whole) : 0, high = all ? 1u << 12 : some ? (uint32_t)__double2hiint(whole) & 0xfffffu : 0;
+        return (u64)high << 32 | low;
     }
 
     // f(i) of the classes of all pieces in the order of the index: the class at which their running sum exceeds above(total of
     // all).  The thread that finds it calls then(class).
     template <class F, class A, class Then>
     __device__ void first_above(F f, A above, Then then) const {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-        const int begin = min(warp * each, n), end = min(begin + each, n);
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
+        const int from = min(begin + warp * each, end), to = min(from + each, end);
         u64 sum = 0;
-        for (int i = begin + lane; i < end; i += 32) sum += f(i);
+#pragma unroll 4
+        for (int i = from + lane; i < to; i += 32) sum += f(i);
         sum = warp_sum(sum);
         if (lane == 0) sm.at[warp] = sum;
         __syncthreads();
@@ -123,8 +148,8 @@ struct Row {
         for (int w = 0; w < warp; w++) before += sm.at[w];
         const u64 target = above(total);
         if (before <= target && before + sum > target) {  // one warp of the cluster
-            for (int i = begin + lane; i - lane < end; i += 32) {
-                const u64 run = before + warp_scan(i < end ? f(i) : 0, lane);
+            for (int i = from + lane; i - lane < to; i += 32) {
+                const u64 run = before + warp_scan(i < to ? f(i) : 0, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, run > target);
                 if (hit) {
                     if (lane == __ffs(hit) - 1) then(base + i);
@@ -132,6 +157,157 @@ struct Row {
                 }
                 before = __shfl_sync(0xffffffffu, run, 31);
             }
+        }
+    }
+
+    // The cluster's histograms are there: the first step at which their running sum, from `before` on, reaches need_of(total); bin
+    // and before (what lies in front of it) are set in every CTA.  Returns what was needed.
+    template <bool kMass, class Need>
+    __device__ u64 find_bin(u64 before, Need need_of) const {
+        sync();
+        // every CTA adds up its share of the steps over the cluster
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = kBins / ranks, per = share / kWarps >= 32 ? share / kWarps : 32;
+        const int from = rank * share + warp * per, to = min(from + per, (rank + 1) * share);
+        u64 part[kBins / kThreads] = {}, mine = 0;  // of steps from + 32 j + lane
+#pragma unroll
+        for (int j = 0; j < kBins / kThreads; j++) {
+            const int b = from + 32 * j + lane;
+            if (b < to)
+                for (int r = 0; r < ranks; r++) {
+                    part[j] += *there(&sm.lo[b], r);
+                    if (kMass) part[j] += (u64)*there(&sm.hi[b], r) << 32;
+                }
+            mine += part[j];
+        }
+        mine = warp_sum(mine);
+        if (lane == 0) sm.at[warp] = mine;
+        __syncthreads();
+        if (warp == 0) {
+            const u64 all = warp_sum(lane < kWarps ? sm.at[lane] : 0);
+            if (lane < ranks) *there(&sm.sums[rank], lane) = all;
+        }
+        sync();
+        u64 run = before, total = 0;
+        for (int r = 0; r < ranks; r++) {
+            if (r < rank) run += sm.sums[r];
+            total += sm.sums[r];
+        }
+        const u64 need = need_of(total);
+        for (int w = 0; w < warp; w++) run += sm.at[w];
+        if (run < need && run + mine >= need) {  // one warp of the cluster
+#pragma unroll
+            for (int j = 0; j < kBins / kThreads; j++) {
+                const u64 sum = run + warp_scan(part[j], lane);
+                const uint32_t hit = __ballot_sync(0xffffffffu, sum >= need);
+                if (hit) {
+                    if (lane == __ffs(hit) - 1)
+                        for (int r = 0; r < ranks; r++) *there(&sm.bin, r) = from + 32 * j + lane, *there(&sm.before, r) = sum - part[j];
+                    break;
+                }
+                run = __shfl_sync(0xffffffffu, sum, 31);
+            }
+        }
+        sync();
+        return need;
+    }
+    __device__ __forceinline__ void clear() const {
+        for (int b = threadIdx.x; b < kBins / 2; b += kThreads) reinterpret_cast<uint4 *>(sm.lo)[b] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    __device__ __forceinline__ void add(int b, u64 w) const {
+        const uint32_t low = (uint32_t)w, old = atomicAdd(&sm.lo[b], low), up = (uint32_t)(w >> 32) + (old + low < low);
+        if (up) atomicAdd(&sm.hi[b], up);
+    }
+    __device__ __forceinline__ int step_of(float v, float s) const { return (int)fminf((max - v) * s, (float)(kBins - 1)); }
+
+    // The classes for which take(logit) is true, which grows with the logit, to the list at rank 0.  Returns their number; those
+    // above kMost are not there.
+    template <class Take>
+    __device__ int gather(Take take) const {
+        if (threadIdx.x == 0) sm.count = 0, sm.taken = 0;
+        sync();
+        uint32_t *count = there(&sm.count, 0), *keys = there(&sm.list_key[0], 0);
+        int *indexes = there(&sm.list_index[0], 0);
+        for (int i = 4 * threadIdx.x; i < end; i += 4 * kThreads) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + i);
+            if (!take(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)))) continue;
+            const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (!take(f[e]) || i + e < begin || i + e >= end) continue;
+                const uint32_t slot = atomicAdd(count, 1u);
+                atomicAdd(&sm.taken, 1);
+                if (slot < kMost) keys[slot] = key_of(f[e]), indexes[slot] = base + i + e;
+            }
+        }
+        __syncthreads();
+        if (threadIdx.x < ranks) *there(&sm.counts[rank], threadIdx.x) = sm.taken;
+        sync();  // from here on rank 0 may go on alone
+        int all = 0;
+        for (int r = 0; r < ranks; r++) all += sm.counts[r];
+        return all;
+    }
+
+    // In the list: the class at which the values, in rising order, add up to `need` (at most their sum).  Values of 0 take no part, orders
+    // differ from each other; bins: steps of the first histogram, rising with the order.
+    __device__ u64 cut(const u64 (&order)[kEach], const u64 (&value)[kEach], const int (&bins)[kEach], u64 need) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        u64 before = 0, omin = 0, omax = ~0ull;
+        int shift = -1;
+#pragma unroll 1
+        while (true) {
+            auto step = [&](int j) { return value[j] == 0 || order[j] < omin || order[j] > omax ? -1 : shift < 0 ? bins[j] : (int)((order[j] - omin) >> shift); };
+            __syncthreads();
+            clear();
+#pragma unroll
+            for (int j = 0; j < kEach; j++)
+                if (step(j) >= 0) add(step(j), value[j]);
+            if (threadIdx.x == 0) sm.count = 0, sm.omin = ~0ull, sm.omax = 0;
+            __syncthreads();
+            u64 part[kBins / kThreads], mine = 0;
+#pragma unroll
+            for (int j = 0; j < kBins / kThreads; j++) {
+                const int b = threadIdx.x * (kBins / kThreads) + j;
+                part[j] = (u64)sm.hi[b] << 32 | sm.lo[b];
+                mine += part[j];
+            }
+            const u64 scan = warp_scan(mine, lane);
+            if (lane == 31) sm.at[warp] = scan;
+            __syncthreads();
+            u64 run = before + scan - mine;
+            for (int w = 0; w < warp; w++) run += sm.at[w];
+#pragma unroll
+            for (int j = 0; j < kBins / kThreads; j++) {
+                if (run < need && run + part[j] >= need) sm.bin = threadIdx.x * (kBins / kThreads) + j, sm.before = run;
+                run += part[j];
+            }
+            __syncthreads();
+            const int bin = sm.bin;
+            before = sm.before;
+#pragma unroll
+            for (int j = 0; j < kEach; j++)
+                if (step(j) == bin) {
+                    const uint32_t slot = atomicAdd(&sm.count, 1u);
+                    if (slot < kList) sm.order[slot] = order[j], sm.value[slot] = value[j];
+                }
+            __syncthreads();
+            const int n = (int)sm.count;
+            if (n <= kList) {
+                for (int i = threadIdx.x; i < n; i += kThreads) {
+                    const u64 own = sm.order[i];
+                    u64 sum = before;
+                    for (int j = 0; j < n; j++) sum += sm.order[j] < own ? sm.value[j] : 0;
+                    if (sum < need && sum + sm.value[i] >= need) sm.end = own;
+                }
+                __syncthreads();
+                return sm.end;
+            }
+#pragma unroll
+            for (int j = 0; j < kEach; j++)
+                if (step(j) == bin) atomicMin(&sm.omin, order[j]), atomicMax(&sm.omax, order[j]);
+            __syncthreads();
+            omin = sm.omin, omax = sm.omax;
+            shift = ::max(0, 64 - __clzll((long long)(omax - omin)) - 11);
         }
     }
 
@@ -145,77 +321,32 @@ struct Row {
         int shift = -1;  // of keys; the first histogram goes by values
 #pragma unroll 1
         while (true) {
-            auto bin_of = [&](float v, uint32_t key) { return shift < 0 ? (int)fminf((max - v) * s, (float)(kBins - 1)) : (int)((khi - key) >> shift); };
-            for (int b = threadIdx.x; b < kBins; b += kThreads) sm.lo[b] = sm.hi[b] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < n; i += kThreads) {
+            auto bin_of = [&](float v, uint32_t key) { return shift < 0 ? step_of(v, s) : (int)((khi - key) >> shift); };
+            clear();
+            for (int i = begin + threadIdx.x; i < end; i += kThreads) {
                 const float v = x[i];
                 const uint32_t key = key_of(v);
                 if (key < klo || key > khi || !in(key, i)) continue;
                 const int b = bin_of(v, key);
                 if (kMass) {
                     const u64 w = weight(v);
-                    if (w == 0) continue;
-                    const uint32_t low = (uint32_t)w, old = atomicAdd(&sm.lo[b], low), up = (uint32_t)(w >> 32) + (old + low < low);
-                    if (up) atomicAdd(&sm.hi[b], up);
+                    if (w) add(b, w);
                 } else {
                     atomicAdd(&sm.lo[b], 1u);
                 }
             }
             sync();
-            // every CTA adds up its share of the steps over the cluster
-            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = kBins / ranks, per = share / kWarps >= 32 ? share / kWarps : 32;
-            const int from = rank * share + warp * per, to = min(from + per, (rank + 1) * share);
-            u64 part[kBins / kThreads] = {}, mine = 0;  // of steps from + 32 j + lane
-#pragma unroll
-            for (int j = 0; j < kBins / kThreads; j++) {
-                const int b = from + 32 * j + lane;
-                if (b < to)
-                    for (int r = 0; r < ranks; r++) {
-                        part[j] += *there(&sm.lo[b], r);
-                        if (kMass) part[j] += (u64)*there(&sm.hi[b], r) << 32;
-                    }
-                mine += part[j];
-            }
-            mine = warp_sum(mine);
-            if (lane == 0) sm.at[warp] = mine;
-            __syncthreads();
-            if (warp == 0) {
-                const u64 all = warp_sum(lane < kWarps ? sm.at[lane] : 0);
-                if (lane < ranks) *there(&sm.sums[rank], lane) = all;
-            }
             if (rank == 0 && threadIdx.x == 0) sm.count = 0, sm.kmin = 0xffffffffu, sm.kmax = 0;
-            sync();
-            u64 run = before, total = 0;
-            for (int r = 0; r < ranks; r++) {
-                if (r < rank) run += sm.sums[r];
-                total += sm.sums[r];
-            }
-            if (shift < 0) need = need_of(total);
-            for (int w = 0; w < warp; w++) run += sm.at[w];
-            if (run < need && run + mine >= need) {  // one warp of the cluster
-#pragma unroll
-                for (int j = 0; j < kBins / kThreads; j++) {
-                    const u64 sum = run + warp_scan(part[j], lane);
-                    const uint32_t hit = __ballot_sync(0xffffffffu, sum >= need);
-                    if (hit) {
-                        if (lane == __ffs(hit) - 1)
-                            for (int r = 0; r < ranks; r++) *there(&sm.bin, r) = from + 32 * j + lane, *there(&sm.before, r) = sum - part[j];
-                        break;
-                    }
-                    run = __shfl_sync(0xffffffffu, sum, 31);
-                }
-            }
-            sync();
-            const int bin = sm.bin;
+            need = find_bin<kMass>(before, [&](u64 total) { return shift < 0 ? need_of(total) : need; });
+            const int bin = sm.bin, lane = threadIdx.x & 31;
             before = sm.before;
             // the classes of that step, at rank 0
             uint32_t *count = there(&sm.count, 0), *keys = there(&sm.key[0], 0), kmin = 0xffffffffu, kmax = 0;
             int *indexes = there(&sm.index[0], 0);
-            for (int i = threadIdx.x; i - lane < n; i += kThreads) {
-                const float v = i < n ? x[i] : 0.f;
+            for (int i = begin + threadIdx.x; i - lane < end; i += kThreads) {
+                const float v = i < end ? x[i] : 0.f;
                 const uint32_t key = key_of(v);
-                const bool hit = i < n && key >= klo && key <= khi && in(key, i) && bin_of(v, key) == bin;
+                const bool hit = i < end && key >= klo && key <= khi && in(key, i) && bin_of(v, key) == bin;
                 const uint32_t hits = __ballot_sync(0xffffffffu, hit);
                 if (hits == 0) continue;
                 uint32_t slot = 0;
@@ -269,104 +400,224 @@ struct Row {
     }
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// The smallest whole number that is at least p * mass, 1 at least.
+__device__ __forceinline__ u64 part_of(float p, u64 mass) {
+    const u64 share = p > 0.f ? (u64)((double)p * 18446744073709551616.0) : 0;
+    const u64 need = __umul64hi(share, mass) + (share * mass != 0);
+    return need ? need : 1;
+}
+
+template <int kThreads>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, const float *u, const float *temperature, const int *top_k,
-                                                          const float *top_p, const float *min_p, int *tokens, long long ld, int C, int piece) {
+                                                          const float *top_p, const float *min_p, int *tokens, long long ld, int rows, int C, int words, int ahead) {
     extern __shared__ __align__(16) uint8_t raw[];
     Smem &sm = *reinterpret_cast<Smem *>(raw);
     float *x = reinterpret_cast<float *>(raw + sizeof(Smem));
     const int ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank(), row = blockIdx.x / ranks;
+    constexpr int kWarps = kThreads / 32, kEach = kMost / kThreads;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x < 64) sm.powers[threadIdx.x] = exp2((double)threadIdx.x / 64);
     tc05::pdl_launch_dependents();
     tc05::pdl_wait();
-    Row r{sm, x, max(0, min(piece, C - rank * piece)), rank * piece, ranks, rank, -INFINITY, 1.0};
-    const float *src = logits + row * ld + r.base;
+    // the row in words of 16 bytes as they lie in memory, `words` of them a CTA; what is not in the row is -inf
+    const float *src = logits + row * ld;
+    const int skip = (int)((reinterpret_cast<uintptr_t>(src) >> 2) & 3), base = 4 * rank * words - skip;
+    Row<kThreads> r{sm, x, max(0, -base), max(0, min(4 * words, C - base)), base, ranks, rank, -INFINITY, 1.0};
     float top = -INFINITY, low = INFINITY;
-    bool bad = false;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < r.n; i += kThreads) {
-        const float v = src[i];
-        x[i] = v;
-        top = fmaxf(top, v);
-        if (v > -INFINITY) low = fminf(low, v);
-        bad |= v != v;
+    if (ahead > 0 && threadIdx.x == 0 && row + ahead < rows) {  // the row that this SM takes next, to L2
+        const char *from = reinterpret_cast<const char *>((reinterpret_cast<uintptr_t>(src + ahead * ld) + 15) & ~(uintptr_t)15);
+        const int bytes = (4 * (C - 3)) & ~15;
+        for (int i = 0; i < bytes; i += 16384)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from + i), "r"(min(16384, bytes - i)) : "memory");
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+#pragma unroll 4
+    for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
+        float4 v;
+        if (i >= r.begin && i + 4 <= r.end) {
+            v = *reinterpret_cast<const float4 *>(src + base + i);
+        } else {
+            float f[4];
+            for (int e = 0; e < 4; e++) f[e] = i + e >= r.begin && i + e < r.end ? src[base + i + e] : -INFINITY;
+            v = make_float4(f[0], f[1], f[2], f[3]);
+        }
+        *reinterpret_cast<float4 *>(x + i) = v;
+        const float most = max_nan(max_nan(v.x, v.y), max_nan(v.z, v.w));
+        top = max_nan(top, most);
+        if (most > -INFINITY) low = fminf(low, most);
     }
-    float2 *most = reinterpret_cast<float2 *>(sm.at);
-    if (lane == 0) most[warp] = make_float2(top, low);
-    bad = __syncthreads_or(bad);
-    if (warp == 0) {
-        const float2 v = most[lane % kWarps];
-        top = v.x, low = v.y;
+    auto both = [&](float2 v) {  // over the warp
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+            v.x = max_nan(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
+            v.y = fminf(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
         }
-        if (lane < ranks) *r.there(&sm.range[rank], lane) = make_float2(top, low), *r.there(&sm.nan[rank], lane) = bad;
+        return v;
+    };
+    float2 *most = reinterpret_cast<float2 *>(sm.at);
+    const float2 own = both(make_float2(top, low));
+    if (lane == 0) most[warp] = own;
+    if (threadIdx.x == 0) sm.first = 0x7fffffff;
+    __syncthreads();
+    if (warp == 0) {
+        const float2 all = both(most[lane % kWarps]);
+        if (lane < ranks) *r.there(&sm.range[rank], lane) = all;
     }
-    const float T = temperature ? temperature[row] : 1.f, p = top_p ? top_p[row] : 1.f, least = min_p ? min_p[row] : 0.f, v = u[row];
+    const float T = temperature ? temperature[row] : 1.f, p = top_p ? top_p[row] : 1.f, least = min_p ? min_p[row] : 0.f, draw = u[row];
     const int k = top_k ? top_k[row] : 0;
     r.sync();
-    low = INFINITY, bad = false;
-    for (int i = 0; i < ranks; i++) r.max = fmaxf(r.max, sm.range[i].x), low = fminf(low, sm.range[i].y), bad |= sm.nan[i] != 0;
-    if (bad || r.max == -INFINITY) {  // the whole cluster; nobody looks at another CTA's memory any more
+    low = INFINITY;
+    for (int i = 0; i < ranks; i++) r.max = max_nan(r.max, sm.range[i].x), low = fminf(low, sm.range[i].y);
+    if (!(r.max > -INFINITY)) {  // the whole cluster; nobody looks at another CTA's memory any more
         if (rank == 0 && threadIdx.x == 0) tokens[row] = -1;
         return;
     }
-    auto write = [&](int i) { tokens[row] = i; };
-    if (!(T > 0.f)) {
-        r.first_above([&](int i) { return (u64)(x[i] == r.max); }, [](u64) { return 0ull; }, write);
+    if (!(T > 0.f) || k == 1 || p <= 0.f) {  // the first of the largest
+        int first = 0x7fffffff;
+        for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + i);
+            if (first < 0x7fffffff || !(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) == r.max)) continue;
+            first = base + i + (v.x == r.max ? 0 : v.y == r.max ? 1 : v.z == r.max ? 2 : 3);
+        }
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0 && first < 0x7fffffff) atomicMin(r.there(&sm.first, 0), first);
+        r.sync();
+        if (rank == 0 && threadIdx.x == 0) tokens[row] = sm.first;
         return;
     }
-    r.inv_t = 1.0 / (double)T;
+    r.by = 64 * 1.4426950408889634 / (double)T;
+    const u64 lowest = least > 0.f ? (least < 1.f ? (u64)ceil((double)least * 17592186044416.0) : 1ull << 44) : 0;
+    const u64 part = draw >= 1.f ? ~0ull : draw > 0.f ? (u64)((double)draw * 18446744073709551616.0) : 0;
+    const bool by_k = k > 1 && k < C, by_p = p < 1.f;
+
+    // the list of classes that matter, if it is a short one
+    const float s = (float)(kBins - 1) / (r.max - low);
+    u64 mass = 0;
+    int listed = kMost + 1;
+    if (by_k && k <= kMost) {
+        r.clear();
+        u64 words_in_all = 0;
+        for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + i);
+            atomicAdd(&sm.lo[r.step_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), s)], 1u);
+        }
+        r.find_bin<false>(0, [&](u64 total) { return words_in_all = total, min((u64)k, total); });
+        const int bin = sm.bin;
+        if (words_in_all >= (u64)k) listed = r.gather([&](float v) { return r.step_of(v, s) <= bin; });
+    } else if (!by_k && lowest) {
+        if (by_p) {
+            u64 sum = 0;
+#pragma unroll 4
+            for (int i = r.begin + threadIdx.x; i < r.end; i += kThreads) sum += r.weight(x[i]);
+            sum = warp_sum(sum);
+            if (lane == 0) sm.at[warp] = sum;
+            __syncthreads();
+            if (warp == 0) {
+                sum = warp_sum(lane < kWarps ? sm.at[lane] : 0);
+                if (lane < ranks) *r.there(&sm.sums[rank], lane) = sum;
+            }
+        }
+        // a little more than T ln(1 / min_p), and than what rounding to 2^-44 makes of it: the list is looked through by weight
+        const float reach = T * (1e-5f - 1.00001f * logf(fmaxf(fminf(least, 1.f) - 1.2e-13f, 1.4e-14f)));
+        listed = r.gather([&](float v) { return r.max - v <= reach || v == r.max; });
+        for (int i = 0; i < ranks; i++) mass += sm.sums[i];
+    }
+    if (listed <= kMost) {
+        if (rank > 0) return;
+        u64 order[kEach], weight[kEach], value[kEach];
+        int bins[kEach], index[kEach];
+        const float per = 64.f / T;
+#pragma unroll
+        for (int j = 0; j < kEach; j++) {
+            const int i = threadIdx.x + j * kThreads;
+            const bool in = i < listed;
+            const uint32_t key = in ? sm.list_key[i] : 0;
+            index[j] = in ? sm.list_index[i] : 0;
+            order[j] = (u64)~key << 32 | (uint32_t)index[j];
+            weight[j] = in ? r.weight(value_of(key)) : 0;
+            value[j] = in;
+            bins[j] = by_k ? r.step_of(value_of(key), s) : r.step_of(value_of(key), per);
+        }
+        u64 end = ~0ull;
+        if (by_k) end = r.cut(order, value, bins, (u64)k);
+        u64 sum = 0;
+        auto total = [&] {  // of the weights up to the end
+            u64 v = 0;
+#pragma unroll
+            for (int j = 0; j < kEach; j++) v += value[j] = order[j] <= end ? weight[j] : 0;
+            v = warp_sum(v);
+            __syncthreads();
+            if (lane == 0) sm.at[warp] = v;
+            __syncthreads();
+            return warp_sum(lane < kWarps ? sm.at[lane] : 0);
+        };
+        sum = total();
+        if (by_p) {
+            const u64 need = part_of(p, by_k ? sum : mass);
+            if (need <= sum) {  // else all of the list is within it
+#pragma unroll
+                for (int j = 0; j < kEach; j++) bins[j] = r.step_of(value_of(~(uint32_t)(order[j] >> 32)), per);
+                end = r.cut(order, value, bins, need);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; j++)
+            if (weight[j] < lowest) weight[j] = 0;
+        sum = total();
+        int step = 0;
+        while ((C - 1) >> step >= kBins) step++;
+#pragma unroll
+        for (int j = 0; j < kEach; j++) order[j] = (uint32_t)index[j], bins[j] = index[j] >> step;
+        const u64 token = r.cut(order, value, bins, __umul64hi(part, sum) + 1);
+        if (threadIdx.x == 0) tokens[row] = (int)token;
+        return;
+    }
 
     // the classes kept: keys above `edge`, and those equal to it up to class `upto`
     uint32_t edge = 0;
     int upto = C;
     auto in = [&](uint32_t key, int i) { return key > edge || (key == edge && r.base + i <= upto); };
-    if (k >= 1 && k < C) {
-        r.find_end<false>([](uint32_t, int) { return true; }, [&](u64) { return (u64)k; }, (float)(kBins - 1) / (r.max - low));
+    if (by_k) {
+        r.find_end<false>([](uint32_t, int) { return true; }, [&](u64) { return (u64)k; }, s);
         edge = sm.edge, upto = sm.upto;
     }
-    if (p < 1.f) {
-        const u64 share = p > 0.f ? (u64)((double)p * 18446744073709551616.0) : 0;
-        r.find_end<true>(in,
-                         [&](u64 mass) {  // the smallest whole number that is at least p * mass
-                             const u64 need = __umul64hi(share, mass) + (share * mass != 0);
-                             return need ? need : 1;
-                         },
-                         64.f / T);
+    if (by_p) {
+        r.find_end<true>(in, [&](u64 total) { return part_of(p, total); }, 64.f / T);
         edge = sm.edge, upto = sm.upto;
     }
-    const u64 lowest = least > 0.f ? (least < 1.f ? (u64)ceil((double)least * 17592186044416.0) : 1ull << 44) : 0;
-    const u64 part = v >= 1.f ? ~0ull : v > 0.f ? (u64)((double)v * 18446744073709551616.0) : 0;
     r.first_above(
         [&](int i) -> u64 {
             if (!in(key_of(x[i]), i)) return 0;
             const u64 w = r.weight(x[i]);
             return w >= lowest ? w : 0;
         },
-        [&](u64 total) { return __umul64hi(part, total); }, write);
+        [&](u64 total) { return __umul64hi(part, total); }, [&](int i) { tokens[row] = i; });
 }
 
-// CTAs of a row: as many as keep the SMs busy, with at least 2048 logits each, and enough for several to share an SM's memory.
+// CTAs of a row: one, of 1024 threads, where there are enough rows to fill the SMs or a row is short, else as many, of 512,
+// as give each SM one, with at least 2048 logits each; and enough for a row to fit.
+constexpr int kAlone = 53000;  // logits that one CTA can hold
 int ranks_of(int rows, int C) {
     const int sms = attn::sm_count();
     int ranks = 1;
-    while (ranks < kRanks && ((long long)rows * ranks < 2 * sms || C / ranks > 12800) && C / (2 * ranks) >= 2048) ranks *= 2;
+    while (ranks < kRanks && (C / ranks > kAlone || ((long long)rows * ranks * 2 <= sms && C / (2 * ranks) >= 2048))) ranks *= 2;
     return ranks;
 }
 
-size_t smem_bytes(int piece) { return sizeof(Smem) + sizeof(float) * (size_t)piece; }
+size_t smem_bytes(int words) { return sizeof(Smem) + 16 * (size_t)words; }
+int words_of(int C, int ranks) { return (C + 3 + 4 * ranks - 1) / (4 * ranks); }  // of 16 bytes, wherever the row begins
 
 }  // namespace
 
 cudaError_t set_attributes() {
-    return cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(kMaxC / kRanks));
+    const cudaFuncAttribute at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<512>, at, (int)smem_bytes(words_of(kMaxC, kRanks)));
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(sample_kernel<1024>, at, (int)smem_bytes(words_of(kAlone, 1)));
 }
 
 }  // namespace sample
@@ -380,8 +631,10 @@ extern "C" int xent_sm100_sample(const float *logits, const float *u, const floa
     const int rc = attn::device_status_word(&status);
     if (rc != ATTN_OK) return rc;
     if (rows == 0) return ATTN_OK;
-    const int ranks = sample::ranks_of(rows, C), piece = (C + ranks - 1) / ranks;
-    return (int)attn::launch_clusters_after_previous(sample::sample_kernel, dim3((unsigned)rows * ranks), dim3(sample::kThreads), sample::smem_bytes(piece),
-                                                     (unsigned)ranks, static_cast<cudaStream_t>(stream), logits, u, temperature, top_k, top_p, min_p, tokens, ld,
-                                                     C, piece);
+    const int ranks = sample::ranks_of(rows, C), words = sample::words_of(C, ranks);
+    const bool alone = ranks == 1;
+    return (int)attn::launch_clusters_after_previous(alone ? sample::sample_kernel<1024> : sample::sample_kernel<512>, dim3((unsigned)rows * ranks),
+                                                     dim3(alone ? 1024 : 512), sample::smem_bytes(words), (unsigned)ranks, static_cast<cudaStream_t>(stream),
+                                                     logits, u, temperature, top_k, top_p, min_p, tokens, ld, rows, C, words,
+                                                     alone && C > 3 ? attn::sm_count() * (int)(200000 / sample::smem_bytes(words) + 1) : 0);
 }
