@@ -15,6 +15,8 @@
 //
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "attn_internal.h"
 #include "tc05.cuh"
 
@@ -29,6 +31,8 @@ constexpr int kRanks = 8;      // CTAs of a row at most
 constexpr int kBins = 2048;    // of a histogram
 constexpr int kList = 512;     // classes that are compared each with each
 constexpr int kMost = 2048;    // classes of the list
+constexpr int kFew = 128;      // classes of a list that one thread each compares with all others
+constexpr int kListThreads = 512, kEach = kMost / kListThreads;  // who works on it, and the classes of each
 constexpr int kMaxC = 425984;  // a piece of kMaxC / kRanks logits fits shared memory beside the rest
 typedef unsigned long long u64;
 
@@ -55,6 +59,8 @@ struct Smem {
     u64 at[32];                     // of this CTA's warps
     u64 before;                     // what lies in front of `bin`
     u64 end, omin, omax;            // in the list
+    u64 front;                      // what lies in front of a stretch of the piece
+    int stretch[2];
     float2 range[kRanks];           // each CTA's largest logit, NaN if one is, and its smallest maximum of four
     int bin;
     uint32_t count, kmin, kmax;     // rank 0: classes of the step, and the range of their keys
@@ -77,19 +83,25 @@ __device__ __forceinline__ T warp_sum(T v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
+template <class T>
+__device__ __forceinline__ T warp_scan(T v, int lane) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const u64 left = __shfl_up_sync(0xffffffffu, v, o);
+        const T left = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += left;
     }
     return v;
 }
 
+// For the threads that work on the list.
+__device__ __forceinline__ void list_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kListThreads) : "memory"); }
+
+__device__ __forceinline__ void few_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kFew) : "memory"); }
+
 // One row as its cluster sees it.
 template <int kThreads>
 struct Row {
-    static constexpr int kWarps = kThreads / 32, kEach = kMost / kThreads;
+    static constexpr int kWarps = kThreads / 32;
     Smem &sm;
     const float *x;    // this CTA's piece, in shared memory, from a 16-byte boundary of the row's memory on
     int begin, end;    // the logits in it; class of the first place: base
@@ -108,7 +120,7 @@ struct Row {
     }
 
     // 2^44 exp((v - max) / T) by 2^(n / 64) from a table and the series of exp for what is left, |r| <= ln(2) / 128: the first term
-    // left out is 2^-44 of the result.  Adding 2^52 rounds it to a whole number.
+    // left out is 2^-44 of the result.  Adding 2^52 rounds it to a whole number.  max is finite.
     __device__ __forceinline__ u64 weight(float v) const {
         constexpr double kWhole = 6755399441055744.0, kLn = 0.010830424696249145;  // 1.5 * 2^52, ln(2) / 64
         const double d = (double)v - (double)max, k = fma(d, by, kWhole);
@@ -117,24 +129,29 @@ struct Row {
         const double s = r * fma(r, fma(r, fma(r, kLn * kLn * kLn * kLn / 24, kLn * kLn * kLn / 6), kLn * kLn / 2), kLn);
         const double p = sm.powers[n & 63], w = fma(p, s, p);
         const double whole = __hiloint2double(__double2hiint(w) + (((n >> 6) + 44) << 20), __double2loint(w)) + 4503599627370496.0;
-        // no branches: several of these are under way at a time
-        const bool some = v > -INFINITY && max < INFINITY && d * by >= -46.0 * 64, all = v == max;
-        const uint32_t low = some && !all ? (uint32_t)__double2loint(whole) : 0, high = all ? 1u << 12 : some ? (uint32_t)__double2hiint(whole) & 0xfffffu : 0;
-        return (u64)high << 32 | low;
+        const bool some = k >= kWhole - 46.0 * 64;  // not where v is -inf
+        return some ? (u64)(__double2hiint(whole) & 0xfffff) << 32 | (uint32_t)__double2loint(whole) : 0;
     }
 
     // f(i) of the classes of all pieces in the order of the index: the class at which their running sum exceeds above(total of
     // all).  The thread that finds it calls then(class).
     template <class F, class A, class Then>
     __device__ void first_above(F f, A above, Then then) const {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, each = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
-        const int from = min(begin + warp * each, end), to = min(from + each, end);
-        u64 sum = 0;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        // a stretch of the piece for each warp, added up; what lies in front of this warp's, and its own
+        auto stretch = [&](int lo, int hi, int &from, int &to) {
+            const int each = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+            from = min(lo + warp * each, hi), to = min(from + each, hi);
+            u64 sum = 0;
 #pragma unroll 4
-        for (int i = from + lane; i < to; i += 32) sum += f(i);
-        sum = warp_sum(sum);
-        if (lane == 0) sm.at[warp] = sum;
-        __syncthreads();
+            for (int i = from + lane; i < to; i += 32) sum += f(i);
+            sum = warp_sum(sum);
+            if (lane == 0) sm.at[warp] = sum;
+            __syncthreads();
+            return sum;
+        };
+        int from, to;
+        u64 sum = stretch(begin, end, from, to);
         if (warp == 0) {
             const u64 all = warp_sum(lane < kWarps ? sm.at[lane] : 0);
             if (lane < ranks) *there(&sm.sums[rank], lane) = all;
@@ -145,9 +162,16 @@ struct Row {
             if (r < rank) before += sm.sums[r];
             total += sm.sums[r];
         }
-        for (int w = 0; w < warp; w++) before += sm.at[w];
         const u64 target = above(total);
-        if (before <= target && before + sum > target) {  // one warp of the cluster
+        if (before > target || before + sm.sums[rank] <= target) return;  // not in this CTA's piece
+        // the stretch in which it is, once more, by all warps
+        for (int w = 0; w < warp; w++) before += sm.at[w];
+        if (before <= target && before + sum > target && lane == 0) sm.stretch[0] = from, sm.stretch[1] = to, sm.front = before;
+        __syncthreads();
+        before = sm.front;
+        sum = stretch(sm.stretch[0], sm.stretch[1], from, to);
+        for (int w = 0; w < warp; w++) before += sm.at[w];
+        if (before <= target && before + sum > target) {  // one warp
             for (int i = from + lane; i - lane < to; i += 32) {
                 const u64 run = before + warp_scan(i < to ? f(i) : 0, lane);
                 const uint32_t hit = __ballot_sync(0xffffffffu, run > target);
@@ -168,14 +192,15 @@ struct Row {
         // every CTA adds up its share of the steps over the cluster
         const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = kBins / ranks, per = share / kWarps >= 32 ? share / kWarps : 32;
         const int from = rank * share + warp * per, to = min(from + per, (rank + 1) * share);
-        u64 part[kBins / kThreads] = {}, mine = 0;  // of steps from + 32 j + lane
+        using Sum = std::conditional_t<kMass, u64, uint32_t>;
+        Sum part[kBins / kThreads] = {}, mine = 0;  // of steps from + 32 j + lane
 #pragma unroll
         for (int j = 0; j < kBins / kThreads; j++) {
             const int b = from + 32 * j + lane;
             if (b < to)
                 for (int r = 0; r < ranks; r++) {
                     part[j] += *there(&sm.lo[b], r);
-                    if (kMass) part[j] += (u64)*there(&sm.hi[b], r) << 32;
+                    if constexpr (kMass) part[j] += (u64)*there(&sm.hi[b], r) << 32;
                 }
             mine += part[j];
         }
@@ -220,25 +245,44 @@ struct Row {
     }
     __device__ __forceinline__ int step_of(float v, float s) const { return (int)fminf((max - v) * s, (float)(kBins - 1)); }
 
-    // The classes for which take(logit) is true, which grows with the logit, to the list at rank 0.  Returns their number; those
-    // above kMost are not there.
-    template <class Take>
-    __device__ int gather(Take take) const {
+    // The classes with logits of `least` (finite) and more to the list at rank 0.  Returns their number; those above kMost are not there.
+    __device__ int gather(float least) const {
         if (threadIdx.x == 0) sm.count = 0, sm.taken = 0;
         sync();
-        uint32_t *count = there(&sm.count, 0), *keys = there(&sm.list_key[0], 0);
+        uint32_t *count = there(&sm.count, 0), *keys = there(&sm.list_key[0], 0), words = 0;
         int *indexes = there(&sm.list_index[0], 0);
-        for (int i = 4 * threadIdx.x; i < end; i += 4 * kThreads) {
+        const int lane = threadIdx.x & 31;
+        // a bit for each of this thread's words of four that has one; few have
+        int j = 0;
+#pragma unroll 4
+        for (int i = 4 * threadIdx.x; i < end; i += 4 * kThreads, j++) {
             const float4 v = *reinterpret_cast<const float4 *>(x + i);
-            if (!take(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)))) continue;
+            words |= (uint32_t)(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least) << j;
+        }
+        int mine = 0;
+        for (uint32_t left = words; left; left &= left - 1) {
+            const float4 v = *reinterpret_cast<const float4 *>(x + 4 * (threadIdx.x + (__ffs(left) - 1) * kThreads));
+            mine += (v.x >= least) + (v.y >= least) + (v.z >= least) + (v.w >= least);
+        }
+        int run = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int left = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += left;
+        }
+        uint32_t slot = 0;
+        if (lane == 31 && run) slot = atomicAdd(count, (uint32_t)run), atomicAdd(&sm.taken, run);
+        slot = __shfl_sync(0xffffffffu, slot, 31) + run - mine;
+        for (uint32_t left = words; left; left &= left - 1) {
+            const int i = 4 * (threadIdx.x + (__ffs(left) - 1) * kThreads);
+            const float4 v = *reinterpret_cast<const float4 *>(x + i);
             const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (!take(f[e]) || i + e < begin || i + e >= end) continue;
-                const uint32_t slot = atomicAdd(count, 1u);
-                atomicAdd(&sm.taken, 1);
-                if (slot < kMost) keys[slot] = key_of(f[e]), indexes[slot] = base + i + e;
-            }
+            for (int e = 0; e < 4; e++)
+                if (f[e] >= least) {
+                    if (slot < kMost) keys[slot] = key_of(f[e]), indexes[slot] = base + i + e;
+                    slot++;
+                }
         }
         __syncthreads();
         if (threadIdx.x < ranks) *there(&sm.counts[rank], threadIdx.x) = sm.taken;
@@ -257,31 +301,32 @@ struct Row {
 #pragma unroll 1
         while (true) {
             auto step = [&](int j) { return value[j] == 0 || order[j] < omin || order[j] > omax ? -1 : shift < 0 ? bins[j] : (int)((order[j] - omin) >> shift); };
-            __syncthreads();
-            clear();
+            list_sync();
+            for (int b = threadIdx.x; b < kBins / 2; b += kListThreads) reinterpret_cast<uint4 *>(sm.lo)[b] = make_uint4(0, 0, 0, 0);
+            list_sync();
 #pragma unroll
             for (int j = 0; j < kEach; j++)
                 if (step(j) >= 0) add(step(j), value[j]);
             if (threadIdx.x == 0) sm.count = 0, sm.omin = ~0ull, sm.omax = 0;
-            __syncthreads();
-            u64 part[kBins / kThreads], mine = 0;
+            list_sync();
+            u64 part[kBins / kListThreads], mine = 0;
 #pragma unroll
-            for (int j = 0; j < kBins / kThreads; j++) {
-                const int b = threadIdx.x * (kBins / kThreads) + j;
+            for (int j = 0; j < kBins / kListThreads; j++) {
+                const int b = threadIdx.x * (kBins / kListThreads) + j;
                 part[j] = (u64)sm.hi[b] << 32 | sm.lo[b];
                 mine += part[j];
             }
             const u64 scan = warp_scan(mine, lane);
             if (lane == 31) sm.at[warp] = scan;
-            __syncthreads();
+            list_sync();
             u64 run = before + scan - mine;
             for (int w = 0; w < warp; w++) run += sm.at[w];
 #pragma unroll
-            for (int j = 0; j < kBins / kThreads; j++) {
-                if (run < need && run + part[j] >= need) sm.bin = threadIdx.x * (kBins / kThreads) + j, sm.before = run;
+            for (int j = 0; j < kBins / kListThreads; j++) {
+                if (run < need && run + part[j] >= need) sm.bin = threadIdx.x * (kBins / kListThreads) + j, sm.before = run;
                 run += part[j];
             }
-            __syncthreads();
+            list_sync();
             const int bin = sm.bin;
             before = sm.before;
 #pragma unroll
@@ -290,22 +335,22 @@ struct Row {
                     const uint32_t slot = atomicAdd(&sm.count, 1u);
                     if (slot < kList) sm.order[slot] = order[j], sm.value[slot] = value[j];
                 }
-            __syncthreads();
+            list_sync();
             const int n = (int)sm.count;
             if (n <= kList) {
-                for (int i = threadIdx.x; i < n; i += kThreads) {
+                for (int i = threadIdx.x; i < n; i += kListThreads) {
                     const u64 own = sm.order[i];
                     u64 sum = before;
                     for (int j = 0; j < n; j++) sum += sm.order[j] < own ? sm.value[j] : 0;
                     if (sum < need && sum + sm.value[i] >= need) sm.end = own;
                 }
-                __syncthreads();
+                list_sync();
                 return sm.end;
             }
 #pragma unroll
             for (int j = 0; j < kEach; j++)
                 if (step(j) == bin) atomicMin(&sm.omin, order[j]), atomicMax(&sm.omax, order[j]);
-            __syncthreads();
+            list_sync();
             omin = sm.omin, omax = sm.omax;
             shift = ::max(0, 64 - __clzll((long long)(omax - omin)) - 11);
         }
@@ -321,13 +366,14 @@ struct Row {
         int shift = -1;  // of keys; the first histogram goes by values
 #pragma unroll 1
         while (true) {
-            auto bin_of = [&](float v, uint32_t key) { return shift < 0 ? step_of(v, s) : (int)((khi - key) >> shift); };
+            auto bin_of = [&](float v) { return shift < 0 ? step_of(v, s) : (int)((khi - key_of(v)) >> shift); };
+            auto there_is = [&](float v, int i) { return in(v, i) && (shift < 0 || (key_of(v) >= klo && key_of(v) <= khi)); };
             clear();
+#pragma unroll 4
             for (int i = begin + threadIdx.x; i < end; i += kThreads) {
                 const float v = x[i];
-                const uint32_t key = key_of(v);
-                if (key < klo || key > khi || !in(key, i)) continue;
-                const int b = bin_of(v, key);
+                if (!there_is(v, i)) continue;
+                const int b = bin_of(v);
                 if (kMass) {
                     const u64 w = weight(v);
                     if (w) add(b, w);
@@ -345,10 +391,10 @@ struct Row {
             int *indexes = there(&sm.index[0], 0);
             for (int i = begin + threadIdx.x; i - lane < end; i += kThreads) {
                 const float v = i < end ? x[i] : 0.f;
-                const uint32_t key = key_of(v);
-                const bool hit = i < end && key >= klo && key <= khi && in(key, i) && bin_of(v, key) == bin;
+                const bool hit = i < end && there_is(v, i) && bin_of(v) == bin;
                 const uint32_t hits = __ballot_sync(0xffffffffu, hit);
                 if (hits == 0) continue;
+                const uint32_t key = key_of(v);
                 uint32_t slot = 0;
                 if (lane == 0) slot = atomicAdd(count, (uint32_t)__popc(hits));
                 slot = __shfl_sync(0xffffffffu, slot, 0) + __popc(hits & ((1u << lane) - 1u));
@@ -387,7 +433,7 @@ struct Row {
             if (klo == khi) {  // equal logits: so many of them, by the index
                 const u64 own = kMass ? weight(value_of(klo)) : 1, some = (need - before + own - 1) / own;
                 if (threadIdx.x == 0) sm.edge = klo;
-                first_above([&](int i) { return (u64)(key_of(x[i]) == klo && in(klo, i)); }, [&](u64) { return some - 1; },
+                first_above([&](int i) { return (u64)(key_of(x[i]) == klo && in(x[i], i)); }, [&](u64) { return some - 1; },
                             [&](int index) {
                                 for (int r = 0; r < ranks; r++) *there(&sm.upto, r) = index;
                             });
@@ -420,7 +466,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
     Smem &sm = *reinterpret_cast<Smem *>(raw);
     float *x = reinterpret_cast<float *>(raw + sizeof(Smem));
     const int ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank(), row = blockIdx.x / ranks;
-    constexpr int kWarps = kThreads / 32, kEach = kMost / kThreads;
+    constexpr int kWarps = kThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x < 64) sm.powers[threadIdx.x] = exp2((double)threadIdx.x / 64);
     tc05::pdl_launch_dependents();
@@ -477,6 +523,12 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
         if (rank == 0 && threadIdx.x == 0) tokens[row] = -1;
         return;
     }
+    if (r.max == INFINITY) {  // it has all the weight
+        for (int i = threadIdx.x; i < r.end; i += kThreads) x[i] = x[i] == INFINITY ? 0.f : -INFINITY;
+        r.max = low = 0.f;
+        top = top == INFINITY ? 0.f : -INFINITY;
+        __syncthreads();
+    }
     if (!(T > 0.f) || k == 1 || p <= 0.f) {  // the first of the largest
         int first = 0x7fffffff;
         for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
@@ -502,13 +554,18 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
     if (by_k && k <= kMost) {
         r.clear();
         u64 words_in_all = 0;
-        for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
-            const float4 v = *reinterpret_cast<const float4 *>(x + i);
-            atomicAdd(&sm.lo[r.step_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), s)], 1u);
+        if (3 * k <= kThreads * ranks) {  // few: the largest of each thread are enough of them
+            atomicAdd(&sm.lo[r.step_of(top, s)], 1u);
+        } else {
+            for (int i = 4 * threadIdx.x; i < r.end; i += 4 * kThreads) {
+                const float4 v = *reinterpret_cast<const float4 *>(x + i);
+                atomicAdd(&sm.lo[r.step_of(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)), s)], 1u);
+            }
         }
         r.find_bin<false>(0, [&](u64 total) { return words_in_all = total, min((u64)k, total); });
-        const int bin = sm.bin;
-        if (words_in_all >= (u64)k) listed = r.gather([&](float v) { return r.step_of(v, s) <= bin; });
+        // the logits at the end of that step, and what its rounding may hide; the last step has no end
+        const float least_of_them = sm.bin == kBins - 1 ? -INFINITY : r.max - (float)(sm.bin + 1) / s * 1.00001f - 1e-6f * fabsf(r.max);
+        if (words_in_all >= (u64)k) listed = r.gather(fmaxf(least_of_them, -3.402823466e38f));
     } else if (!by_k && lowest) {
         if (by_p) {
             u64 sum = 0;
@@ -522,19 +579,55 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
                 if (lane < ranks) *r.there(&sm.sums[rank], lane) = sum;
             }
         }
-        // a little more than T ln(1 / min_p), and than what rounding to 2^-44 makes of it: the list is looked through by weight
+        // T ln(1 / min_p) below the largest, and a little more than rounding, to 2^-44 too, may hide: the list is looked through by weight
         const float reach = T * (1e-5f - 1.00001f * logf(fmaxf(fminf(least, 1.f) - 1.2e-13f, 1.4e-14f)));
-        listed = r.gather([&](float v) { return r.max - v <= reach || v == r.max; });
+        listed = r.gather(fmaxf(r.max - reach - 1e-6f * fabsf(r.max), -3.402823466e38f));
         for (int i = 0; i < ranks; i++) mass += sm.sums[i];
     }
+    if (listed <= kFew) {
+        // every class against each other, one a thread
+        if (rank > 0 || threadIdx.x >= kFew) return;
+        const int i = threadIdx.x;
+        const bool in = i < listed;
+        const uint32_t key = in ? sm.list_key[i] : 0, index = in ? sm.list_index[i] : 0;
+        const u64 order = (u64)~key << 32 | index;
+        u64 weight = in ? r.weight(value_of(key)) : 0;
+        few_sync();
+        sm.order[i] = order, sm.value[i] = weight;
+        few_sync();
+        u64 front = 0, all = 0;  // the weight of the classes before this one
+        int place = 0;           // their number
+        for (int j = 0; j < listed; j++) {
+            const bool before = sm.order[j] < order;
+            place += before;
+            front += before ? sm.value[j] : 0;
+        }
+        if (by_k && place >= k) weight = 0;
+        auto total = [&] {  // of the weights left
+            const u64 v = warp_sum(weight);
+            if (lane == 0) sm.at[warp] = v;
+            few_sync();
+            return warp_sum(lane < kFew / 32 ? sm.at[lane] : 0);
+        };
+        all = total();
+        if (by_p && front >= part_of(p, by_k ? all : mass)) weight = 0;
+        if (weight < lowest) weight = 0;
+        sm.order[i] = index, sm.value[i] = weight;
+        few_sync();
+        const u64 target = __umul64hi(part, total());
+        front = 0;
+        for (int j = 0; j < listed; j++) front += sm.order[j] < index ? sm.value[j] : 0;
+        if (front <= target && front + weight > target) tokens[row] = (int)index;
+        return;
+    }
     if (listed <= kMost) {
-        if (rank > 0) return;
+        if (rank > 0 || threadIdx.x >= kListThreads) return;
         u64 order[kEach], weight[kEach], value[kEach];
         int bins[kEach], index[kEach];
         const float per = 64.f / T;
 #pragma unroll
         for (int j = 0; j < kEach; j++) {
-            const int i = threadIdx.x + j * kThreads;
+            const int i = threadIdx.x + j * kListThreads;
             const bool in = i < listed;
             const uint32_t key = in ? sm.list_key[i] : 0;
             index[j] = in ? sm.list_index[i] : 0;
@@ -544,17 +637,17 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
             bins[j] = by_k ? r.step_of(value_of(key), s) : r.step_of(value_of(key), per);
         }
         u64 end = ~0ull;
-        if (by_k) end = r.cut(order, value, bins, (u64)k);
+        if (by_k && listed > k) end = r.cut(order, value, bins, (u64)k);  // fewer than k: the others are at -inf
         u64 sum = 0;
         auto total = [&] {  // of the weights up to the end
             u64 v = 0;
 #pragma unroll
             for (int j = 0; j < kEach; j++) v += value[j] = order[j] <= end ? weight[j] : 0;
             v = warp_sum(v);
-            __syncthreads();
+            list_sync();
             if (lane == 0) sm.at[warp] = v;
-            __syncthreads();
-            return warp_sum(lane < kWarps ? sm.at[lane] : 0);
+            list_sync();
+            return warp_sum(lane < kListThreads / 32 ? sm.at[lane] : 0);
         };
         sum = total();
         if (by_p) {
@@ -578,25 +671,30 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
         return;
     }
 
-    // the classes kept: keys above `edge`, and those equal to it up to class `upto`
-    uint32_t edge = 0;
+    // the classes kept: logits above `edge`, and those equal to it up to class `upto`
+    float edge = -INFINITY;
     int upto = C;
-    auto in = [&](uint32_t key, int i) { return key > edge || (key == edge && r.base + i <= upto); };
+    auto in = [&](float v, int i) { return v > edge || (v == edge && r.base + i <= upto); };
     if (by_k) {
-        r.find_end<false>([](uint32_t, int) { return true; }, [&](u64) { return (u64)k; }, s);
-        edge = sm.edge, upto = sm.upto;
+        r.find_end<false>([](float, int) { return true; }, [&](u64) { return (u64)k; }, s);
+        edge = value_of(sm.edge), upto = sm.upto;
     }
     if (by_p) {
         r.find_end<true>(in, [&](u64 total) { return part_of(p, total); }, 64.f / T);
-        edge = sm.edge, upto = sm.upto;
+        edge = value_of(sm.edge), upto = sm.upto;
     }
-    r.first_above(
-        [&](int i) -> u64 {
-            if (!in(key_of(x[i]), i)) return 0;
-            const u64 w = r.weight(x[i]);
-            return w >= lowest ? w : 0;
-        },
-        [&](u64 total) { return __umul64hi(part, total); }, [&](int i) { tokens[row] = i; });
+    auto target = [&](u64 total) { return __umul64hi(part, total); };
+    auto write = [&](int i) { tokens[row] = i; };
+    if (!by_k && !by_p && !lowest)
+        r.first_above([&](int i) { return r.weight(x[i]); }, target, write);
+    else
+        r.first_above(
+            [&](int i) -> u64 {
+                if (!in(x[i], i)) return 0;
+                const u64 w = r.weight(x[i]);
+                return w >= lowest ? w : 0;
+            },
+            target, write);
 }
 
 // CTAs of a row: one, of 1024 threads, where there are enough rows to fill the SMs or a row is short, else as many, of 512,
@@ -605,7 +703,7 @@ constexpr int kAlone = 53000;  // logits that one CTA can hold
 int ranks_of(int rows, int C) {
     const int sms = attn::sm_count();
     int ranks = 1;
-    while (ranks < kRanks && (C / ranks > kAlone || ((long long)rows * ranks * 2 <= sms && C / (2 * ranks) >= 2048))) ranks *= 2;
+    while (ranks < kRanks && (C / ranks > kAlone || ((long long)rows * ranks * 2 <= sms - 20 && C / (2 * ranks) >= 2048))) ranks *= 2;
     return ranks;
 }
 

@@ -109,7 +109,8 @@ def test_borders(pkg):
 @pytest.mark.parametrize("C", [5, 1500, 50257])
 def test_infinities_and_nan(pkg, C):
     """-inf has no weight, +inf all of it; a row with a NaN or of -inf alone draws nothing, and keeps that to itself."""
-    x, u = rows_of(12, C)
+    x, u = rows_of(13, C)
+    x[12, : C // 2] = torch.finfo(torch.float32).min
     x[0, : C - 2] = -INF
     x[1] = -INF
     x[2, C // 2] = NAN
@@ -121,10 +122,11 @@ def test_infinities_and_nan(pkg, C):
     x[9] = -3e38
     x[9, 4] = 3e38
     x[10, : C - 1] = -INF
-    for settings in (dict(), dict(temperature=0.0), dict(top_k=2), dict(top_k=C - 1, top_p=0.9), dict(min_p=0.5), dict(temperature=1e-30), dict(temperature=1e30),
+    x[11] = torch.finfo(torch.float32).min
+    for settings in (dict(), dict(temperature=0.0), dict(top_k=2), dict(top_k=C - 1, top_p=0.9), dict(top_k=3), dict(top_k=C // 2 + 1), dict(min_p=0.5), dict(temperature=1e-30), dict(temperature=1e30),
                      dict(temperature=INF), dict(temperature=INF, top_p=0.5), dict(temperature=NAN), dict(top_p=NAN), dict(min_p=NAN), dict(top_p=1e-38)):
         if settings.get("temperature") == INF:  # infinite logits over an infinite temperature
-            keep = [r for r in range(12) if r not in (3, 4, 5, 7)]
+            keep = [r for r in range(13) if r not in (3, 4, 5, 7)]
             check(pkg, x[keep], u[keep], **settings)
         else:
             check(pkg, x, u, **settings)
