@@ -19,5 +19,6 @@ struct Call {
 // Sequences with more than `few` rows (new tokens x query heads of a group), D <= 128.
 cudaError_t launch_tiles(const Call &a, int few);
 cudaError_t tiles_set_attributes();
+cudaError_t few_rows_set_attributes();
 
 }  // namespace paged

@@ -3,13 +3,15 @@
 //   out[t, h] = sum_j p_j v[j] / sum_j p_j,   p_j = exp(scale q[t, h] . k[j] - m),   j = 0 .. position of t
 //
 // A unit is one sequence, one key/value head and up to kRows of its rows (row = new token x query head of the group); a
-// cluster of 1 to 8 CTAs takes it, each CTA one run of the keys, each warp every fourth batch of that run.  LPR lanes hold
-// one key (16 bytes each, twice that for the widest heads), so a warp reads 32 / LPR keys in one request; every such group
+// cluster of 1 to 8 CTAs takes it, each CTA one run of the keys.  One warp brings them: pages are contiguous for a head, so it asks
+// the copy engine for whole runs of a page at a time, four stages ahead.  Four warps compute: LPR lanes hold
+// one key (16 bytes each, twice that for the widest heads), so a warp reads 32 / LPR keys at a time; every such group
 // of lanes keeps a running maximum, sum and output of its own for its keys, in fp32 and in registers, and they are joined
 // only at the end: over the lanes by shuffles, over the warps in shared memory, over the cluster through distributed shared
 // memory.  No atomics, no scratch buffer, one launch; the order of every sum is fixed.
 #include <cooperative_groups.h>
 
+#include "attn24.cuh"
 #include "attn_internal.h"
 #include "paged.cuh"
 #include "paged_attn.cuh"
@@ -22,8 +24,11 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+using namespace tc05;
+
+constexpr int kWarps = 4;  // that compute, and one that brings keys and values
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kStages = 4;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -39,17 +44,17 @@ struct Words;  // 16 bytes of the cache as floats
 template <>
 struct Words<float> {
     static constexpr int kN = 4;
-    static __device__ __forceinline__ void open(const uint4 &w, float (&f)[4]) {
-        f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y), f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+    static __device__ __forceinline__ void open(const uint4 &w, float2 (&f)[2]) {
+        f[0] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y)), f[1] = make_float2(__uint_as_float(w.z), __uint_as_float(w.w));
     }
 };
 template <>
 struct Words<__nv_bfloat16> {
     static constexpr int kN = 8;
-    static __device__ __forceinline__ void open(const uint4 &w, float (&f)[8]) {
+    static __device__ __forceinline__ void open(const uint4 &w, float2 (&f)[4]) {
         const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) f[2 * i] = __uint_as_float(v[i] << 16), f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        for (int i = 0; i < 4; i++) f[i] = make_float2(__uint_as_float(v[i] << 16), __uint_as_float(v[i] & 0xffff0000u));
     }
 };
 
@@ -59,26 +64,50 @@ struct Partial {
     float o[kRows][kWidth];
 };
 
-__device__ __forceinline__ uint4 load16(const void *p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-    return v;
-}
+enum Site : int { SITE_FULL = 451, SITE_EMPTY };
 
 // kLanes: lanes of a key; kChunks: 16-byte words of a lane
 template <class T, int kLanes, int kChunks, int kRows>
-__global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float *q, float *out, long long ld, int heads,
-                                                            int groups, int few, int max_new, float scale_log2,
-                                                            int *status) {
-    constexpr int kN = Words<T>::kN, kWidth = kLanes * kChunks * kN, kKeys = 32 / kLanes, kBatch = 4 / kChunks;
-    __shared__ Partial<kRows, kWidth> part[kWarps];
+struct FewSmem {
+    static constexpr int kWidth = kLanes * kChunks * Words<T>::kN;
+    static constexpr int kKeys = 32 / kLanes, kBatch = 4 / kChunks;  // keys of a warp at a time, and how often in a stage
+    static constexpr int kStep = kKeys * kBatch * kWarps;            // keys of a stage
+    uint8_t k[kStages][kStep * kWidth * sizeof(T)], v[kStages][kStep * kWidth * sizeof(T)];  // rows of D elements, one behind the other
+    Partial<kRows, kWidth> part[kWarps];
+    uint64_t full[kStages], empty[kStages];
+    int holes[kStages];  // whether a key of the stage has no page
+    int abort_flag;
+};
+
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+
+template <class T, int kLanes, int kChunks, int kRows>
+__global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float *q, float *out, long long ld, int heads, int groups, int few, int max_new,
+                                                            float scale_log2, int *status) {
+    using Smem = FewSmem<T, kLanes, kChunks, kRows>;
+    constexpr int kN = Words<T>::kN, kPairs = kN / 2, kKeys = Smem::kKeys, kBatch = Smem::kBatch, kStep = Smem::kStep;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane % kLanes, mine = lane / kLanes;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, sub = lane % kLanes, mine = lane / kLanes;
     const int unit = blockIdx.x / ranks, s = unit / groups, row0 = (unit % groups) * kRows, kvh = blockIdx.y;
     const int G = heads / c.kv_heads;
-    tc05::pdl_launch_dependents();
-    tc05::pdl_wait();
+    WaitCtx ctx{&sm.abort_flag, status};
+    if (threadIdx.x == 0) {
+        sm.abort_flag = 0;
+        for (int i = 0; i < kStages; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], kWarps);
+        }
+        fence_barrier_init();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
     const Span w = span_of(c, s);
     const int rows = w.count * G;
     if (unit % groups == 0 && kvh == 0 && rank == 0 && threadIdx.x == 0 && (w.count > max_new || (w.count > 0 && w.past < 0))) report(status, ST_ATTEND);
@@ -88,144 +117,180 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
     const int keys = (int)min((long long)w.past + last / G + 1, room);
     if (w.past + (long long)w.count > room && row0 == 0 && threadIdx.x == 0) report(status, ST_ATTEND);
     const int *table = c.table + (long long)s * c.width;
+    // this CTA's run of keys, in whole stages
+    const int all = (keys + kStep - 1) / kStep, each = (all + ranks - 1) / ranks;
+    const int begin = rank * each * kStep, end = min(keys, begin + each * kStep), steps = max(0, (end - begin + kStep - 1) / kStep);
+    const int row_bytes = c.D * (int)sizeof(T);
+    __syncthreads();
 
-    float qv[kRows][kChunks][kN], m[kRows], l[kRows], o[kRows][kChunks][kN];
-    int seen[kRows];  // keys that the row sees
-#pragma unroll
-    for (int r = 0; r < kRows; r++) {
-        const int at = min(row0 + r, last), t = at / G;
-        seen[r] = row0 + r <= last ? w.past + t + 1 : 0;
-        m[r] = -INFINITY, l[r] = 0.f;
-        const float *src = q + (w.first + t) * ld + (long long)(kvh * G + at % G) * c.D;
-#pragma unroll
-        for (int ch = 0; ch < kChunks; ch++) {
-            const int d = (ch * kLanes + sub) * kN;
-#pragma unroll
-            for (int e = 0; e < kN; e += 4) {
-                const float4 v = d < c.D ? *reinterpret_cast<const float4 *>(src + d + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-                qv[r][ch][e] = v.x * scale_log2, qv[r][ch][e + 1] = v.y * scale_log2;
-                qv[r][ch][e + 2] = v.z * scale_log2, qv[r][ch][e + 3] = v.w * scale_log2;
+    if (warp == kWarps) {
+        // ------------------------------ keys and values ------------------------------
+        const T *kp = static_cast<const T *>(c.k) + (long long)kvh * c.page_size * c.D, *vp = static_cast<const T *>(c.v) + (long long)kvh * c.page_size * c.D;
+        for (int n = 0; n < steps; n++) {
+            const int st = n % kStages, from = begin + n * kStep, to = min(end, from + kStep);
+            const int first = from / c.page_size, runs = (to - 1) / c.page_size - first + 1;  // runs of keys within a page, one a lane
+            if (n >= kStages) attn24::await(&sm.empty[st], (n / kStages - 1) & 1, ctx, SITE_EMPTY);
+            if (lane == 0) sm.holes[st] = 0;
+            __syncwarp();
+            int missing = 0;
+            for (int i = lane; i < runs; i += 32) {
+                const int slot = first + i, page = table[slot], j0 = max(from, slot * c.page_size), j1 = min(to, (slot + 1) * c.page_size);
+                const bool there = page >= 0 && page < c.pages;
+                if (!there) missing += j1 - j0;
             }
-#pragma unroll
-            for (int e = 0; e < kN; e++) o[r][ch][e] = 0.f;
+            const int lost = __reduce_add_sync(0xffffffffu, missing);
+            if (lane == 0) {
+                if (lost) sm.holes[st] = 1, report(status, ST_ATTEND);
+                mbar_expect_tx(&sm.full[st], 2u * (uint32_t)((to - from - lost) * row_bytes));
+            }
+            __syncwarp();
+            for (int i = lane; i < runs; i += 32) {
+                const int slot = first + i, page = table[slot], j0 = max(from, slot * c.page_size), j1 = min(to, (slot + 1) * c.page_size);
+                if (page < 0 || page >= c.pages) continue;
+                const long long at = page * c.page_stride + (long long)(j0 - slot * c.page_size) * c.D;
+                const uint32_t bytes = (uint32_t)((j1 - j0) * row_bytes);
+                bulk_load(sm.k[st] + (j0 - from) * row_bytes, kp + at, bytes, &sm.full[st]);
+                bulk_load(sm.v[st] + (j0 - from) * row_bytes, vp + at, bytes, &sm.full[st]);
+            }
+            __syncwarp();
         }
-    }
-
-    // this CTA's run of keys, in whole batches of all its warps
-    constexpr int kRound = kKeys * kBatch * kWarps;
-    const int rounds = (keys + kRound - 1) / kRound, each = (rounds + ranks - 1) / ranks;
-    const int begin = rank * each * kRound, end = min(keys, begin + each * kRound);
-    const T *kp = static_cast<const T *>(c.k) + (long long)kvh * c.page_size * c.D, *vp = static_cast<const T *>(c.v) + (long long)kvh * c.page_size * c.D;
-    bool missing = false;
-    // the first element of a key's row, -1 where there is no such key
-    auto place = [&](int j) -> long long {
-        if (j >= end) return -1;
-        const int slot = j / c.page_size, page = table[slot];
-        if (page < 0 || page >= c.pages) {
-            missing = true;
-            return -1;
-        }
-        return page * c.page_stride + (long long)(j - slot * c.page_size) * c.D;
-    };
-    long long where[kBatch];
+    } else {
+        // ------------------------------ softmax and sums ------------------------------
+        float2 qv[kRows][kChunks][kPairs], o[kRows][kChunks][kPairs];
+        float m[kRows], l[kRows];
+        int seen[kRows];  // keys that the row sees
 #pragma unroll
-    for (int u = 0; u < kBatch; u++) where[u] = place(begin + warp * kKeys * kBatch + u * kKeys + mine);
-    for (int j0 = begin + warp * kKeys * kBatch; j0 < end; j0 += kRound) {
-        uint4 kw[kBatch][kChunks], vw[kBatch][kChunks];
-        bool there[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; u++) {
-            there[u] = where[u] >= 0;
+        for (int r = 0; r < kRows; r++) {
+            const int at = min(row0 + r, last), t = at / G;
+            seen[r] = row0 + r <= last ? w.past + t + 1 : 0;
+            m[r] = -INFINITY, l[r] = 0.f;
+            const float *src = q + (w.first + t) * ld + (long long)(kvh * G + at % G) * c.D;
 #pragma unroll
             for (int ch = 0; ch < kChunks; ch++) {
                 const int d = (ch * kLanes + sub) * kN;
-                const bool ok = there[u] && d < c.D;
-                kw[u][ch] = ok ? load16(kp + where[u] + d) : make_uint4(0, 0, 0, 0);
-                vw[u][ch] = ok ? load16(vp + where[u] + d) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < kPairs; e += 2) {
+                    const float4 v = d < c.D ? *reinterpret_cast<const float4 *>(src + d + 2 * e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    qv[r][ch][e] = make_float2(v.x * scale_log2, v.y * scale_log2);
+                    qv[r][ch][e + 1] = make_float2(v.z * scale_log2, v.w * scale_log2);
+                }
+#pragma unroll
+                for (int e = 0; e < kPairs; e++) o[r][ch][e] = make_float2(0.f, 0.f);
             }
         }
+        const int most = min(end, w.past + row0 / G + 1);  // keys that every row sees
+        for (int n = 0; n < steps; n++) {
+            const int st = n % kStages, j0 = begin + n * kStep + warp * (kKeys * kBatch) + mine;
+            attn24::await(&sm.full[st], (n / kStages) & 1, ctx, SITE_FULL);
+            const bool whole = begin + (n + 1) * kStep <= most && !sm.holes[st];
+            bool there[kBatch];
 #pragma unroll
-        for (int u = 0; u < kBatch; u++) where[u] = place(j0 + kRound + u * kKeys + mine);
-        float sc[kBatch][kRows];
+            for (int u = 0; u < kBatch; u++) there[u] = whole || j0 + u * kKeys < end;
+            if (!whole && sm.holes[st]) {
 #pragma unroll
-        for (int u = 0; u < kBatch; u++) {
-#pragma unroll
-            for (int r = 0; r < kRows; r++) sc[u][r] = 0.f;
-#pragma unroll
-            for (int ch = 0; ch < kChunks; ch++) {
-                float f[kN];
-                Words<T>::open(kw[u][ch], f);
-#pragma unroll
-                for (int r = 0; r < kRows; r++)
-#pragma unroll
-                    for (int e = 0; e < kN; e++) sc[u][r] = fmaf(qv[r][ch][e], f[e], sc[u][r]);
+                for (int u = 0; u < kBatch; u++)
+                    if (there[u]) {
+                        const int page = table[(j0 + u * kKeys) / c.page_size];
+                        there[u] = page >= 0 && page < c.pages;
+                    }
             }
-#pragma unroll
-            for (int r = 0; r < kRows; r++)
-#pragma unroll
-                for (int x = kLanes / 2; x > 0; x >>= 1) sc[u][r] += __shfl_xor_sync(0xffffffffu, sc[u][r], x);
-        }
-#pragma unroll
-        for (int r = 0; r < kRows; r++) {
-            bool ok[kBatch];
-            float top = m[r];
+            const int at = (warp * (kKeys * kBatch) + mine) * row_bytes;
+            float sc[kBatch][kRows];
 #pragma unroll
             for (int u = 0; u < kBatch; u++) {
-                ok[u] = there[u] && j0 + u * kKeys + mine < seen[r];
-                if (ok[u]) top = fmaxf(top, sc[u][r]);
-            }
-            const float keep = weight(m[r], top);
-            m[r] = top;
-            l[r] *= keep;
+                float2 sum[kRows];
 #pragma unroll
-            for (int ch = 0; ch < kChunks; ch++)
+                for (int r = 0; r < kRows; r++) sum[r] = make_float2(0.f, 0.f);
 #pragma unroll
-                for (int e = 0; e < kN; e++) o[r][ch][e] *= keep;
+                for (int ch = 0; ch < kChunks; ch++) {
+                    const int d = (ch * kLanes + sub) * kN;
+                    uint4 word = make_uint4(0, 0, 0, 0);
+                    if (there[u] && d < c.D) word = *reinterpret_cast<const uint4 *>(sm.k[st] + at + u * kKeys * row_bytes + d * (int)sizeof(T));
+                    float2 f[kPairs];
+                    Words<T>::open(word, f);
 #pragma unroll
-            for (int u = 0; u < kBatch; u++) {
-                sc[u][r] = ok[u] ? weight(sc[u][r], top) : 0.f;
-                l[r] += sc[u][r];
-            }
-        }
+                    for (int r = 0; r < kRows; r++)
 #pragma unroll
-        for (int u = 0; u < kBatch; u++)
-#pragma unroll
-            for (int ch = 0; ch < kChunks; ch++) {
-                float f[kN];
-                Words<T>::open(vw[u][ch], f);
+                        for (int e = 0; e < kPairs; e++) sum[r] = fma2(qv[r][ch][e], f[e], sum[r]);
+                }
 #pragma unroll
                 for (int r = 0; r < kRows; r++) {
-                    // a value that the row does not see may be anything, and 0 times it not 0
-                    if (kRows > 1 && sc[u][r] == 0.f) continue;
+                    sc[u][r] = sum[r].x + sum[r].y;
 #pragma unroll
-                    for (int e = 0; e < kN; e++) o[r][ch][e] = fmaf(sc[u][r], f[e], o[r][ch][e]);
+                    for (int x = kLanes / 2; x > 0; x >>= 1) sc[u][r] += __shfl_xor_sync(0xffffffffu, sc[u][r], x);
                 }
             }
-    }
-    if (missing) report(status, ST_ATTEND);
+#pragma unroll
+            for (int r = 0; r < kRows; r++) {
+                float top = m[r];
+                if (!whole) {
+#pragma unroll
+                    for (int u = 0; u < kBatch; u++)
+                        if (!there[u] || j0 + u * kKeys >= seen[r]) sc[u][r] = -INFINITY;
+                }
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) top = fmaxf(top, sc[u][r]);
+                const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[r] - base);  // nothing has weight yet
+                m[r] = top;
+                l[r] *= keep;
+#pragma unroll
+                for (int ch = 0; ch < kChunks; ch++)
+#pragma unroll
+                    for (int e = 0; e < kPairs; e++) o[r][ch][e] = mul2(o[r][ch][e], make_float2(keep, keep));
+#pragma unroll
+                for (int u = 0; u < kBatch; u++) {
+                    sc[u][r] = ex2(sc[u][r] - base);
+                    l[r] += sc[u][r];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; u++)
+#pragma unroll
+                for (int ch = 0; ch < kChunks; ch++) {
+                    const int d = (ch * kLanes + sub) * kN;
+                    uint4 word = make_uint4(0, 0, 0, 0);
+                    if (there[u] && d < c.D) word = *reinterpret_cast<const uint4 *>(sm.v[st] + at + u * kKeys * row_bytes + d * (int)sizeof(T));
+                    float2 f[kPairs];
+                    Words<T>::open(word, f);
+#pragma unroll
+                    for (int r = 0; r < kRows; r++) {
+                        // a value that the row does not see may be anything, and 0 times it not 0
+                        if (kRows > 1 && !whole && sc[u][r] == 0.f) continue;
+#pragma unroll
+                        for (int e = 0; e < kPairs; e++) o[r][ch][e] = fma2(make_float2(sc[u][r], sc[u][r]), f[e], o[r][ch][e]);
+                    }
+                }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
+        }
 
-    // join the groups of lanes, then the warps, then the CTAs
+        // join the groups of lanes, then the warps, then the CTAs
 #pragma unroll
-    for (int r = 0; r < kRows; r++) {
+        for (int r = 0; r < kRows; r++) {
 #pragma unroll
-        for (int x = kLanes; x < 32; x <<= 1) {
-            const float mo = __shfl_xor_sync(0xffffffffu, m[r], x), top = fmaxf(m[r], mo);
-            const float a = weight(m[r], top), b = weight(mo, top);
-            l[r] = l[r] * a + __shfl_xor_sync(0xffffffffu, l[r], x) * b;
+            for (int x = kLanes; x < 32; x <<= 1) {
+                const float mo = __shfl_xor_sync(0xffffffffu, m[r], x), top = fmaxf(m[r], mo);
+                const float a = weight(m[r], top), b = weight(mo, top);
+                l[r] = l[r] * a + __shfl_xor_sync(0xffffffffu, l[r], x) * b;
 #pragma unroll
-            for (int ch = 0; ch < kChunks; ch++)
+                for (int ch = 0; ch < kChunks; ch++)
 #pragma unroll
-                for (int e = 0; e < kN; e++) o[r][ch][e] = o[r][ch][e] * a + __shfl_xor_sync(0xffffffffu, o[r][ch][e], x) * b;
-            m[r] = top;
-        }
-        if (mine == 0) {
-            if (sub == 0) part[warp].m[r] = m[r], part[warp].l[r] = l[r];
+                    for (int e = 0; e < kPairs; e++) {
+                        o[r][ch][e].x = o[r][ch][e].x * a + __shfl_xor_sync(0xffffffffu, o[r][ch][e].x, x) * b;
+                        o[r][ch][e].y = o[r][ch][e].y * a + __shfl_xor_sync(0xffffffffu, o[r][ch][e].y, x) * b;
+                    }
+                m[r] = top;
+            }
+            if (mine == 0) {
+                if (sub == 0) sm.part[warp].m[r] = m[r], sm.part[warp].l[r] = l[r];
 #pragma unroll
-            for (int ch = 0; ch < kChunks; ch++)
+                for (int ch = 0; ch < kChunks; ch++)
 #pragma unroll
-                for (int e = 0; e < kN; e++) part[warp].o[r][(ch * kLanes + sub) * kN + e] = o[r][ch][e];
+                    for (int e = 0; e < kPairs; e++) *reinterpret_cast<float2 *>(&sm.part[warp].o[r][(ch * kLanes + sub) * kN + 2 * e]) = o[r][ch][e];
+            }
         }
     }
+    if (sm.abort_flag) __nanosleep(50000);  // let copies that are still in flight land
     if (ranks > 1) cluster.sync();
     else __syncthreads();
     if (rank == 0) {
@@ -234,7 +299,7 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
             if (row0 + r > last) break;
             float top = -INFINITY, sum = 0.f, acc = 0.f;
             for (int k = 0; k < ranks; k++) {
-                const Partial<kRows, kWidth> *p = ranks > 1 ? cluster.map_shared_rank(&part[0], k) : part;
+                const Partial<kRows, Smem::kWidth> *p = ranks > 1 ? cluster.map_shared_rank(&sm.part[0], k) : sm.part;
                 for (int x = 0; x < kWarps; x++) {
                     const float mo = p[x].m[r], t2 = fmaxf(top, mo), a = weight(top, t2), b = weight(mo, t2);
                     sum = sum * a + p[x].l[r] * b;
@@ -263,7 +328,7 @@ cudaError_t launch_few(const Call &a, int few) {
     while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
     if (units * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     return attn::launch_clusters_after_previous(few_rows_kernel<T, kLanes, kChunks, kRows>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(kThreads),
-                                                0, ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, groups, few, a.max_new, a.scale_log2, a.status);
+                                                sizeof(FewSmem<T, kLanes, kChunks, kRows>), ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, groups, few, a.max_new, a.scale_log2, a.status);
 }
 
 template <class T, int kLanes, int kChunks>
@@ -284,6 +349,24 @@ cudaError_t launch(const Call &a, int few) {
     return launch_rows<T, 32, 2>(a, few);
 }
 
+template <class T, int kLanes, int kChunks>
+cudaError_t set_rows() {
+    const cudaFuncAttribute at = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    cudaError_t e = cudaFuncSetAttribute(few_rows_kernel<T, kLanes, kChunks, 1>, at, (int)sizeof(FewSmem<T, kLanes, kChunks, 1>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_rows_kernel<T, kLanes, kChunks, 2>, at, (int)sizeof(FewSmem<T, kLanes, kChunks, 2>));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_rows_kernel<T, kLanes, kChunks, 4>, at, (int)sizeof(FewSmem<T, kLanes, kChunks, 4>));
+    return e;
+}
+template <class T>
+cudaError_t set_all() {
+    cudaError_t e = set_rows<T, 4, 1>();
+    if (e == cudaSuccess) e = set_rows<T, 8, 1>();
+    if (e == cudaSuccess) e = set_rows<T, 16, 1>();
+    if (e == cudaSuccess) e = set_rows<T, 32, 1>();
+    if (e == cudaSuccess) e = set_rows<T, 32, 2>();
+    return e;
+}
+
 // Sequences of up to kFewRows rows go to the kernel above, which reads their keys at the HBM rate, the others to the tensor
 // cores; both kernels find their own sequences on the device, so a step that mixes them takes two launches.
 constexpr int kFewRows = 4;
@@ -300,6 +383,12 @@ cudaError_t forward(const Call &a) {
 }
 
 }  // namespace
+
+cudaError_t few_rows_set_attributes() {
+    const cudaError_t e = set_all<__nv_bfloat16>();
+    return e != cudaSuccess ? e : set_all<float>();
+}
+
 }  // namespace paged
 
 extern "C" int attn_sm100_paged_forward(const float *q, const void *k_pages, const void *v_pages, const int *page_table, const int *cu_seqlens,
