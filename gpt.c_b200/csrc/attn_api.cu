@@ -180,6 +180,7 @@ int attn_sm100_init(void) {
     if ((e = attn::attn24_bwd_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = paged::tiles_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = paged::few_rows_set_attributes()) != cudaSuccess) return (int)e;
+    if ((e = paged::decode_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = sample::set_attributes()) != cudaSuccess) return (int)e;
 
     int sms = 0;

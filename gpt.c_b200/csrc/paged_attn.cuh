@@ -1,9 +1,90 @@
-// The call that the two attention kernels over a paged cache share (paged_attn_sm100.cu, paged_tile_sm100.cu).
+// What the attention kernels over a paged cache share (paged_attn_sm100.cu, paged_decode_sm100.cu, paged_tile_sm100.cu).
 #pragma once
 
+#include "attn24.cuh"
+#include "attn_internal.h"
 #include "paged.cuh"
 
 namespace paged {
+
+using namespace attn24;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
+
+// A warp's arrival after what its lanes did to tensor memory.
+__device__ __forceinline__ void arrive_tmem(uint64_t *bar, int lane) {
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
+// p = hi + mid + lo, each the next eight bits cut off: exact.
+__device__ __forceinline__ void cut3(float2 p, uint32_t &hi, uint32_t &mid, uint32_t &lo) { split3(p, hi, mid, lo, 0u); }
+
+// Element offset of key j's row from that of its head, -1 where it has no page.
+__device__ __forceinline__ long long place(const Cache &c, const int *table, int j, int end, bool &missing) {
+    if (j >= end) return -1;
+    const int slot = j / c.page_size, page = table[slot];
+    if (page < 0 || page >= c.pages) {
+        missing = true;
+        return -1;
+    }
+    return page * c.page_stride + (long long)(j - slot * c.page_size) * c.D;
+}
+
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// One row over again in fp32 arithmetic, by a warp: keys from .. to - 1.
+template <class T, int kDP>
+__device__ __noinline__ void exact_row(const Cache &c, const float *q, const int *table, int kvh, int from, int to, float scale_log2, float *o, float *m_out,
+                                       float *l_out) {
+    constexpr int kE = kDP / 32, kAhead = 4;
+    const int lane = threadIdx.x & 31;
+    const T *kp = static_cast<const T *>(c.k) + (long long)kvh * c.page_size * c.D, *vp = static_cast<const T *>(c.v) + (long long)kvh * c.page_size * c.D;
+    float x[kE], acc[kE], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kE; e++) x[e] = lane + 32 * e < c.D ? q[lane + 32 * e] * scale_log2 : 0.f, acc[e] = 0.f;
+    bool missing = false, is_nan = false;
+#pragma unroll 1
+    for (int j = from; j < to && !is_nan; j += kAhead) {
+        float s[kAhead], v[kAhead][kE];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const long long at = place(c, table, j + u, to, missing);
+            s[u] = 0.f;
+#pragma unroll
+            for (int e = 0; e < kE; e++) {
+                const bool in = at >= 0 && lane + 32 * e < c.D;
+                s[u] = fmaf(x[e], in ? as_float(kp[at + lane + 32 * e]) : 0.f, s[u]);
+                v[u][e] = in ? as_float(vp[at + lane + 32 * e]) : 0.f;
+            }
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
+            if (at < 0) s[u] = -INFINITY;
+            is_nan = is_nan || !(s[u] < INFINITY);  // an infinite maximum is subtracted from itself
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            const float top = fmaxf(m, s[u]);
+            if (top == -INFINITY || s[u] == -INFINITY) continue;  // no weight
+            const float keep = ex2f(m - top), p = ex2f(s[u] - top);
+            l = l * keep + p;
+#pragma unroll
+            for (int e = 0; e < kE; e++) acc[e] = acc[e] * keep + p * v[u][e];
+            m = top;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kE; e++) o[lane + 32 * e] = is_nan ? NAN : acc[e];
+    if (lane == 0) *m_out = is_nan ? 0.f : m, *l_out = is_nan ? NAN : l;
+}
+
 
 struct Call {
     Cache c;
@@ -18,6 +99,18 @@ struct Call {
 
 // Sequences with more than `few` rows (new tokens x query heads of a group), D <= 128.
 cudaError_t launch_tiles(const Call &a, int few);
+// Sequences with up to `few` rows, 8 at most; bf16 pages, D <= 128.
+cudaError_t launch_decode(const Call &a, int few);
+cudaError_t decode_set_attributes();
+// CTAs of one of `units`, which share its keys: enough for two on each SM, and for no more than 4096 keys each.
+inline unsigned ranks_of(const Call &a, long long units) {
+    const int sms = attn::sm_count();
+    unsigned ranks = 1;
+    while (ranks < 8 && units * ranks < 2 * sms) ranks *= 2;
+    const long long keys = (long long)a.c.width * a.c.page_size;
+    while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
+    return ranks;
+}
 cudaError_t tiles_set_attributes();
 cudaError_t few_rows_set_attributes();
 

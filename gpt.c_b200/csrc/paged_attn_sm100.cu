@@ -24,8 +24,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-using namespace tc05;
-
 constexpr int kWarps = 4;  // that compute, and one that brings keys and values
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kStages = 4;
@@ -321,11 +319,7 @@ template <class T, int kLanes, int kChunks, int kRows>
 cudaError_t launch_few(const Call &a, int few) {
     const int G = a.heads / a.c.kv_heads, groups = (int)((min((long long)a.max_new * G, (long long)few) + kRows - 1) / kRows);
     const long long units = (long long)a.c.seqs * groups, all = units * a.c.kv_heads;
-    const int sms = attn::sm_count();
-    unsigned ranks = 1;
-    while (ranks < 8 && all * ranks < 2 * sms) ranks *= 2;
-    const long long keys = (long long)a.c.width * a.c.page_size;
-    while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
+    const unsigned ranks = ranks_of(a, all);
     if (units * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     return attn::launch_clusters_after_previous(few_rows_kernel<T, kLanes, kChunks, kRows>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(kThreads),
                                                 sizeof(FewSmem<T, kLanes, kChunks, kRows>), ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, groups, few, a.max_new, a.scale_log2, a.status);
@@ -339,14 +333,14 @@ cudaError_t launch_rows(const Call &a, int few) {
     return launch_few<T, kLanes, kChunks, 4>(a, few);
 }
 
-template <class T>
 cudaError_t launch(const Call &a, int few) {
-    const int words = a.c.D / Words<T>::kN;  // of 16 bytes
-    if (words <= 4) return launch_rows<T, 4, 1>(a, few);
-    if (words <= 8) return launch_rows<T, 8, 1>(a, few);
-    if (words <= 16) return launch_rows<T, 16, 1>(a, few);
-    if (words <= 32) return launch_rows<T, 32, 1>(a, few);
-    return launch_rows<T, 32, 2>(a, few);
+    if (a.type == ATTN_CACHE_BF16) return launch_rows<__nv_bfloat16, 32, 1>(a, few);  // D > 128
+    const int words = a.c.D / Words<float>::kN;  // of 16 bytes
+    if (words <= 4) return launch_rows<float, 4, 1>(a, few);
+    if (words <= 8) return launch_rows<float, 8, 1>(a, few);
+    if (words <= 16) return launch_rows<float, 16, 1>(a, few);
+    if (words <= 32) return launch_rows<float, 32, 1>(a, few);
+    return launch_rows<float, 32, 2>(a, few);
 }
 
 template <class T, int kLanes, int kChunks>
@@ -357,36 +351,33 @@ cudaError_t set_rows() {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(few_rows_kernel<T, kLanes, kChunks, 4>, at, (int)sizeof(FewSmem<T, kLanes, kChunks, 4>));
     return e;
 }
-template <class T>
-cudaError_t set_all() {
-    cudaError_t e = set_rows<T, 4, 1>();
-    if (e == cudaSuccess) e = set_rows<T, 8, 1>();
-    if (e == cudaSuccess) e = set_rows<T, 16, 1>();
-    if (e == cudaSuccess) e = set_rows<T, 32, 1>();
-    if (e == cudaSuccess) e = set_rows<T, 32, 2>();
-    return e;
-}
-
-// Sequences of up to kFewRows rows go to the kernel above, which reads their keys at the HBM rate, the others to the tensor
-// cores; both kernels find their own sequences on the device, so a step that mixes them takes two launches.
-constexpr int kFewRows = 4;
-constexpr int kMeanRows = 128;  // from this many rows a sequence on, on average, the tensor cores take all of them in one launch
+// Sequences of few rows go to the kernels that read their keys at the HBM rate, the others to the tile kernel; all find
+// their own sequences on the device, so a step that mixes them takes two launches.
+constexpr int kFewRows16 = 8, kFewRows32 = 4;
+constexpr int kMeanRows = 128;  // from this many rows a sequence on, on average, the tile kernel takes all of them in one launch
 
 cudaError_t forward(const Call &a) {
+    const bool narrow = a.type == ATTN_CACHE_BF16 && a.c.D <= 128;
     const long long G = a.heads / a.c.kv_heads, most = a.max_new * G;
-    if (most <= kFewRows || a.c.D > 128) return a.type == ATTN_CACHE_BF16 ? launch<__nv_bfloat16>(a, 0x7fffffff) : launch<float>(a, 0x7fffffff);
-    const bool both = G <= kFewRows && a.c.tokens * G < (long long)kMeanRows * a.c.seqs;
-    const int few = both ? kFewRows : 0;
-    const cudaError_t e = launch_tiles(a, few);
-    if (e != cudaSuccess || !both) return e;
-    return a.type == ATTN_CACHE_BF16 ? launch<__nv_bfloat16>(a, few) : launch<float>(a, few);
+    const int limit = narrow ? kFewRows16 : kFewRows32;
+    auto launch_few_rows = [&](int few) { return narrow ? launch_decode(a, few) : launch(a, few); };
+    if (a.c.D > 128) return launch_few_rows(0x7fffffff);
+    const bool far = narrow && a.c.pages * a.c.page_stride > 1ll << 34;  // beyond that kernel's 32-bit places: the tile kernel takes all
+    if (most <= limit && !far) return launch_few_rows(limit);
+    const bool both = !far && G <= limit && a.c.tokens * G < (long long)kMeanRows * a.c.seqs;
+    const cudaError_t e = launch_tiles(a, both ? limit : 0);
+    return e != cudaSuccess || !both ? e : launch_few_rows(limit);
 }
 
 }  // namespace
 
 cudaError_t few_rows_set_attributes() {
-    const cudaError_t e = set_all<__nv_bfloat16>();
-    return e != cudaSuccess ? e : set_all<float>();
+    cudaError_t e = set_rows<float, 4, 1>();
+    if (e == cudaSuccess) e = set_rows<float, 8, 1>();
+    if (e == cudaSuccess) e = set_rows<float, 16, 1>();
+    if (e == cudaSuccess) e = set_rows<float, 32, 1>();
+    if (e == cudaSuccess) e = set_rows<float, 32, 2>();
+    return e != cudaSuccess ? e : set_rows<__nv_bfloat16, 32, 1>();
 }
 
 }  // namespace paged

@@ -69,23 +69,6 @@ struct __align__(1024) TileSmem {
 
 enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_O_FREE, SITE_Q_READY, SITE_ALIGN };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kN>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
-
-// A warp's arrival after what its lanes did to tensor memory.
-__device__ __forceinline__ void arrive_tmem(uint64_t *bar, int lane) {
-    tc_fence_before_sync();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar);
-}
-
-// p = hi + mid + lo, each the next eight bits cut off: exact.
-__device__ __forceinline__ void cut3(float2 p, uint32_t &hi, uint32_t &mid, uint32_t &lo) { split3(p, hi, mid, lo, 0u); }
-
 // The sequence and tile of unit `u`, tiles counted over the sequences with more than `few` rows and no more new tokens than max_new;
 // tile -1 past the last.  A whole warp.  check: reports lengths that the call does not allow.
 __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int max_new, int u, bool check, int *status, int &seq, int &tile) {
@@ -117,65 +100,6 @@ __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int ma
         u -= __shfl_sync(0xffffffffu, run, 31);
         if (tile >= 0) u = 0x7fffffff;  // only the check goes on
     }
-}
-
-// Element offset of key j's row from that of its head, -1 where it has no page.
-__device__ __forceinline__ long long place(const Cache &c, const int *table, int j, int end, bool &missing) {
-    if (j >= end) return -1;
-    const int slot = j / c.page_size, page = table[slot];
-    if (page < 0 || page >= c.pages) {
-        missing = true;
-        return -1;
-    }
-    return page * c.page_stride + (long long)(j - slot * c.page_size) * c.D;
-}
-
-__device__ __forceinline__ float as_float(float x) { return x; }
-__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-// One row over again in fp32 arithmetic, by a warp: keys from .. to - 1.
-template <class T, int kDP>
-__device__ __noinline__ void exact_row(const Cache &c, const float *q, const int *table, int kvh, int from, int to, float scale_log2, float *o, float *m_out,
-                                       float *l_out) {
-    constexpr int kE = kDP / 32, kAhead = 4;
-    const int lane = threadIdx.x & 31;
-    const T *kp = static_cast<const T *>(c.k) + (long long)kvh * c.page_size * c.D, *vp = static_cast<const T *>(c.v) + (long long)kvh * c.page_size * c.D;
-    float x[kE], acc[kE], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < kE; e++) x[e] = lane + 32 * e < c.D ? q[lane + 32 * e] * scale_log2 : 0.f, acc[e] = 0.f;
-    bool missing = false, is_nan = false;
-#pragma unroll 1
-    for (int j = from; j < to && !is_nan; j += kAhead) {
-        float s[kAhead], v[kAhead][kE];
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const long long at = place(c, table, j + u, to, missing);
-            s[u] = 0.f;
-#pragma unroll
-            for (int e = 0; e < kE; e++) {
-                const bool in = at >= 0 && lane + 32 * e < c.D;
-                s[u] = fmaf(x[e], in ? as_float(kp[at + lane + 32 * e]) : 0.f, s[u]);
-                v[u][e] = in ? as_float(vp[at + lane + 32 * e]) : 0.f;
-            }
-#pragma unroll
-            for (int w = 16; w > 0; w >>= 1) s[u] += __shfl_xor_sync(0xffffffffu, s[u], w);
-            if (at < 0) s[u] = -INFINITY;
-            is_nan = is_nan || !(s[u] < INFINITY);  // an infinite maximum is subtracted from itself
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            const float top = fmaxf(m, s[u]);
-            if (top == -INFINITY || s[u] == -INFINITY) continue;  // no weight
-            const float keep = ex2f(m - top), p = ex2f(s[u] - top);
-            l = l * keep + p;
-#pragma unroll
-            for (int e = 0; e < kE; e++) acc[e] = acc[e] * keep + p * v[u][e];
-            m = top;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < kE; e++) o[lane + 32 * e] = is_nan ? NAN : acc[e];
-    if (lane == 0) *m_out = is_nan ? 0.f : m, *l_out = is_nan ? NAN : l;
 }
 
 template <class T, int kDP>
