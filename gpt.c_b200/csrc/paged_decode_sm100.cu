@@ -9,7 +9,7 @@
 // K and V come by asynchronous 16-byte copies from wherever their pages are, V transposed by the load from shared memory.
 //
 // Up to 2 rows (packed_kernel): the terms of q, and of p, are columns of one product.  Each warp works by itself: it brings its stages,
-// two ahead, and keeps a maximum, a sum and an output of its own.  Where there are many units a warp takes one; else four
+// one ahead, and keeps a maximum, a sum and an output of its own.  Where there are many units a warp takes one; else four
 // warps of a CTA, and the CTAs of a cluster, share it and are joined at the end.
 // Up to 8 rows (rows_kernel): a product for each term; one warp of a CTA brings the stages, four take every fourth.
 //
@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, kDP == 64 ? 3 : 2) rows_kernel(Cache
 // ------------------------------------------------------------------------------------------
 // one or two rows
 // ------------------------------------------------------------------------------------------
-constexpr int kAhead = 3;  // stages of a warp
+constexpr int kAhead = 2;  // stages of a warp: with 3, fewer warps fit an SM (96 sequences, 12 heads of 64: 40 us with 2, 51 with 3)
 
 template <int kDP, int kW>
 struct __align__(128) PackedSmem {
@@ -567,11 +567,12 @@ cudaError_t launch_packed(const Call &a, int few, unsigned ranks) {
                                                 sizeof(PackedSmem<kDP, kW>), ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, a.status);
 }
 
-// One warp a unit where that leaves each SM enough of them (16 or 32 KB on their way each) and no sequence can be long; else four
-// warps and as many CTAs as fit the GPU at a time, and enough for 2048 keys a warp.
+// One warp a unit where that leaves each SM enough of them and no sequence can be long; else four warps and as many CTAs as fit the
+// GPU at a time, and enough for 2048 keys a warp.  Lengths up to 1022 positions, one warp / four, us: 12 heads of 64, 30 sequences 34 / 17,
+// 96 43 / 40, 400 119 / 130; heads of 128, 96 sequences 80 / 115.
 template <int kDP, int kR>
 cudaError_t launch_packed_width(const Call &a, int few) {
-    constexpr int kFull = kDP == 64 ? 3 : 2, kResident = kDP == 64 ? 2 : 1;
+    constexpr int kFull = kDP == 64 ? 8 : 2, kResident = kDP == 64 ? 3 : 1;
     const long long units = (long long)a.c.seqs * a.c.kv_heads, keys = (long long)a.c.width * a.c.page_size;
     const int sms = attn::sm_count();
     if (units >= (long long)kFull * sms && keys <= 2048) return launch_packed<kDP, 1, kR>(a, few, 1);
