@@ -29,9 +29,6 @@ constexpr int kRows = 8, kKeys = 32;                     // its rows; keys of a 
 
 enum Site : int { SITE_FULL = 461, SITE_EMPTY };
 
-__device__ __forceinline__ void arrive_when_copied(uint64_t *bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void ldsm(uint32_t (&a)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(at) : "memory");
 }

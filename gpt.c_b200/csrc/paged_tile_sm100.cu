@@ -7,11 +7,13 @@
 // (attn24.cuh), so q and p take part exactly; bf16 pages are one term, fp32 pages three: 3 or 6 passes a product.  The tensor
 // cores truncate their sums, so the P V of each step starts at zero and is added to the output in registers.
 //
-// Warps: one issues the tensor-core instructions, a few bring keys and values (bf16 by asynchronous 16-byte copies, fp32
-// through registers, split on the way) from wherever their pages are into a ring, eight per group do the softmax, two
-// threads a row.  Two score buffers alternate, S of step n+2 is issued behind P V of step n.  Where a step takes the tensor
-// cores less time than a softmax step (bf16, head size up to 64: 768 cycles), two groups take every other step each, with a
-// maximum, sum and output of their own that are joined at the end.
+// Warps: one issues the tensor-core instructions, two or three bring keys and values from wherever their pages are into a ring (bf16 by
+// the copy engine, boxes of 8 to 64 rows that lie in one page; by asynchronous 16-byte copies where pages are not a multiple of 8 rows;
+// fp32 through registers, split on the way), sixteen do the softmax.  Where a step takes the tensor cores as long as a softmax step or
+// longer (1536 cycles and more: fp32, or head sizes above 64) four threads share a row and two score buffers alternate; else (768
+// cycles) two threads do, and two groups of eight warps take every other step each, with a maximum, sum and output of their own that
+// are joined at the end, and three score buffers, so that a group finds its next scores when it has done with one step (with two
+// buffers S of step n+2 had to wait for P V of step n, and a step took 1430 cycles).
 //
 // A row whose result is not finite is computed again in fp32 arithmetic: 0 times an infinite value that the row does
 // not see is NaN on the tensor cores, and so are the terms of an infinity.
@@ -30,26 +32,27 @@ using namespace attn24;
 
 constexpr int kRowsTile = 128;
 
-template <class T, int kDP>
+template <class T, int kDP, bool kTma>
 struct Shape {
     static constexpr bool kWide = sizeof(T) == 4;          // fp32 pages
     static constexpr int kTerms = kWide ? 3 : 1;           // of K and V
     static constexpr int kGroups = !kWide && kDP == 64 ? 2 : 1;
-    static constexpr int kProducers = kWide ? 7 : 3;       // warps 1 .. ; warp 0 issues
+    static constexpr int kSplit = 4 / kGroups;             // threads of a row
+    static constexpr int kGroupWarps = 4 * kSplit;
+    static constexpr int kProducers = 3;                   // warps 1 to 3; warp 0 issues
     static constexpr int kFirst = kProducers + 1;          // first softmax warp, a multiple of four
-    static constexpr int kThreads = 32 * (kFirst + 8 * kGroups);
+    static constexpr int kThreads = 32 * (kFirst + 16);
     static constexpr int kPlane = kStep * kDP * 2;         // one term of 64 keys
     static constexpr int kStage = 2 * kTerms * kPlane;     // K terms, V terms
     static constexpr int kStages = kWide ? (kDP == 64 ? 4 : 2) : (kDP == 64 ? 8 : 6);
-    static constexpr int kLag = kWide ? 0 : (kDP == 64 ? 4 : 2);  // steps between the request of a stage and its hand-over
-    static constexpr uint32_t kColO = 192, kColQ = 192 + kDP;     // scores: twice 96 columns before them
+    static constexpr int kBuffers = kGroups + 1;           // of scores, 96 columns each
+    static constexpr uint32_t kColO = 96 * kBuffers, kColQ = kColO + kGroups * kDP;  // an output for each group
     static_assert(kColQ + 3 * kDP / 2 <= 512, "tensor memory");
-    static_assert(kLag <= kStages - 2 || kLag == 0, "a step is consumed only when the next one is there");
 };
 
-template <class T, int kDP>
+template <class T, int kDP, bool kTma>
 struct __align__(1024) TileSmem {
-    using S = Shape<T, kDP>;
+    using S = Shape<T, kDP, kTma>;
     union {
         uint8_t ring[S::kStages][S::kStage];
         struct {  // at the end
@@ -57,17 +60,18 @@ struct __align__(1024) TileSmem {
             float o1[kRowsTile][kDP + 4];
         } fin;
     };
-    uint64_t kv_full[S::kStages], kv_empty[S::kStages], s_full[2], p_full[2], o_full[2], o_free, q_ready;
+    uint64_t kv_full[S::kStages], kv_empty[S::kStages], s_full[3], p_full[2], o_full[2], q_ready, tail[2];
     uint32_t valid[S::kStages][2];          // keys of the stage that are there
-    float xmax[S::kGroups][2][2][kRowsTile];  // [group][step parity][half][row]
-    float m[kRowsTile], l[kRowsTile], m1[kRowsTile], l1[kRowsTile], half_l[S::kGroups][kRowsTile];
+    float xmax[S::kGroups][2][S::kSplit][kRowsTile];  // [group][step parity][part][row]: maxima, at the end sums
+    float m[kRowsTile], l[kRowsTile], m1[kRowsTile], l1[kRowsTile];
     uint32_t odd[kRowsTile / 32];           // rows to be computed again
     int seq, tile;
+    Span span;
     uint32_t tmem_base;
     int abort_flag;
 };
 
-enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_O_FREE, SITE_Q_READY, SITE_ALIGN };
+enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_Q_READY, SITE_ALIGN, SITE_TAIL };
 
 // The sequence and tile of unit `u`, tiles counted over the sequences with more than `few` rows and no more new tokens than max_new;
 // tile -1 past the last.  A whole warp.  check: reports lengths that the call does not allow.
@@ -102,12 +106,13 @@ __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int ma
     }
 }
 
-template <class T, int kDP>
-__global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache c, const float *q, float *out, long long ld, int heads, int few, int max_new,
+template <class T, int kDP, bool kTma>
+__global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                               int box, Cache c, const float *q, float *out, long long ld, int heads, int few, int max_new,
                                                                          float scale_log2, int *status) {
-    using Sh = Shape<T, kDP>;
-    using Smem = TileSmem<T, kDP>;
-    constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups, kTerms = Sh::kTerms, kHalf = kDP / 2;
+    using Sh = Shape<T, kDP, kTma>;
+    using Smem = TileSmem<T, kDP, kTma>;
+    constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups, kBuffers = Sh::kBuffers, kTerms = Sh::kTerms, kSplit = Sh::kSplit, kPart = kDP / kSplit;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
@@ -118,17 +123,21 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
         if ((smem_u32(smem_raw) & 1023u) != 0) report(status, ST_TIMEOUT_BASE + SITE_ALIGN);
         sm.abort_flag = 0;
         for (int i = 0; i < kStages; i++) {
-            mbar_init(&sm.kv_full[i], Sh::kProducers);
+            mbar_init(&sm.kv_full[i], kTma ? 4 : Sh::kWide ? Sh::kProducers : 32 * Sh::kProducers + 1);
             mbar_init(&sm.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_full[i], 8);
+            mbar_init(&sm.p_full[i], Sh::kGroupWarps);
             mbar_init(&sm.o_full[i], 1);
+            mbar_init(&sm.tail[i], 1);
         }
-        mbar_init(&sm.o_free, 8);
-        mbar_init(&sm.q_ready, 8);
+        for (int i = 0; i < 3; i++) mbar_init(&sm.s_full[i], 1);
+        mbar_init(&sm.q_ready, Sh::kGroupWarps);
         fence_barrier_init();
+    }
+    if (kTma && threadIdx.x == 64) {
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
     }
     if (warp == 1) tmem_alloc_then_launch_dependents(&sm.tmem_base, 512);
     pdl_wait();
@@ -136,14 +145,15 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
         int seq, tile;
         const int units = gridDim.x / ranks, u = units - 1 - (int)(blockIdx.x / ranks);  // the last tiles of a sequence are its longest
         find_tile(c, G, few, max_new, u, u == 0 && kvh == 0 && rank == 0, status, seq, tile);
-        if (lane == 0) sm.seq = seq, sm.tile = tile;
+        const Span span = span_of(c, seq);
+        if (lane == 0) sm.seq = seq, sm.tile = tile, sm.span = span;
     }
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem_base, 0);
     const int seq = __shfl_sync(0xffffffffu, sm.seq, 0), tile = __shfl_sync(0xffffffffu, sm.tile, 0);
-    const Span w = span_of(c, seq);
+    const Span w = sm.span;
     const int rows = w.count * G, row0 = tile * kRowsTile;
     const int *table = c.table + (long long)seq * c.width;
     // this CTA's run of keys: steps first .. first + nsteps - 1
@@ -166,168 +176,248 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
         auto issue_s = [&](int n) {
             const int st = n % kStages;
             await(&sm.kv_full[st], (n / kStages) & 1, ctx, SITE_KV_FULL);
+            fence_proxy_async_smem();  // here, not where they are written: there it would wait for everything that is on its way
             const uint64_t at = desc_advance(kd, st * Sh::kStage);
 #pragma unroll
             for (int i = 0; i < kPasses; i++)
 #pragma unroll
                 for (int kk = 0; kk < kK; kk++)
-                    mma_ts_lead(leader, tmem + (n & 1) * 96, tmem + Sh::kColQ + kHalf * term_a(i) + 8 * kk,
+                    mma_ts_lead(leader, tmem + n % kBuffers * 96, tmem + Sh::kColQ + kDP / 2 * term_a(i) + 8 * kk,
                                 desc_advance(at, term_b(i) * kPlane + (kk >> 2) * (kStep * 128) + (kk & 3) * 32), idesc_s, i > 0 || kk > 0 ? 1u : 0u);
-            tc_commit_lead(leader, &sm.s_full[n & 1]);
+            tc_commit_lead(leader, &sm.s_full[n % kBuffers]);
         };
         await(&sm.q_ready, 0, ctx, SITE_Q_READY);
-        issue_s(0);
-        if (nsteps > 1) issue_s(1);
+        for (int n = 0; n < min(kBuffers, nsteps); n++) issue_s(n);
         for (int n = 0; n < nsteps; n++) {
             const int st = n % kStages;
             await(&sm.p_full[n & 1], (n >> 1) & 1, ctx, SITE_P_FULL);
-            if (kGroups == 2 && n > 0) await(&sm.o_free, (n - 1) & 1, ctx, SITE_O_FREE);
             const uint64_t at = desc_advance(vd, st * Sh::kStage);
 #pragma unroll
             for (int i = 0; i < kPasses; i++)
 #pragma unroll
                 for (int kk = 0; kk < kStep / 16; kk++)
-                    mma_ts_lead(leader, tmem + Sh::kColO, tmem + (n & 1) * 96 + term_column(term_a(i), kk), desc_advance(at, term_b(i) * kPlane + kk * 2048),
+                    mma_ts_lead(leader, tmem + Sh::kColO + n % kGroups * kDP, tmem + n % kBuffers * 96 + term_column(term_a(i), kk), desc_advance(at, term_b(i) * kPlane + kk * 2048),
                                 idesc_o, i > 0 || kk > 0 ? 1u : 0u);
             tc_commit_lead(leader, &sm.o_full[n & 1]);
             tc_commit_lead(leader, &sm.kv_empty[st]);
-            if (n + 2 < nsteps) issue_s(n + 2);  // where P_n was, which P V of step n, earlier in the pipe, has read by then
+            if (n + kBuffers < nsteps) issue_s(n + kBuffers);  // where P_n was, which P V of step n, earlier in the pipe, has read by then
         }
-    } else if (nsteps > 0 && warp < Sh::kFirst) {
+    } else if (kTma && nsteps > 0 && (warp == 2 || warp == 3)) {
+        // ------------------------------ producers of K and of V: boxes, one a lane ------------------------------
+        // Few instructions a step: beside sixteen busy warps each of them takes this one about six cycles.
+        const int boxes = kStep / box, slots = kStep / c.page_size, row_step = kStep % c.page_size;
+        const uint32_t all_boxes = boxes == 32 ? 0xffffffffu : (1u << boxes) - 1u;
+        bool missing = false;
+        int j = first * kStep + lane * box, slot = j / c.page_size, row = j % c.page_size, row_here = row;
+        auto page_of = [&] {  // of key j; past the last one where there is none: that reads as zeros
+            int page = lane < boxes && j < keys ? table[slot] : c.pages;
+            if ((unsigned)page > (unsigned)c.pages || (page == c.pages && lane < boxes && j < keys)) missing = true, page = c.pages;
+            row_here = row;
+            j += kStep, slot += slots, row += row_step;
+            if (row >= c.page_size) row -= c.page_size, slot++;
+            return page;
+        };
+        int page = page_of(), at_row = row_here;  // looked up a step ahead
+        const int kv = warp - 2;
+        const CUtensorMap *map = kv ? &map_v : &map_k;
+        uint8_t *const tile_at = sm.ring[0] + kv * kPlane, *const to = tile_at + (lane < boxes ? lane : 0) * box * 128;
+        for (int n = 0; n < nsteps; n++) {
+            const int st = n % kStages, here = page, here_row = at_row;
+            page = page_of(), at_row = row_here;
+            if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
+            const int key0 = (first + n) * kStep;
+            const bool last_part = key0 + kStep > keys;
+            uint64_t *bar = last_part ? &sm.tail[kv] : &sm.kv_full[st];
+            const uint32_t found = __ballot_sync(0xffffffffu, here < c.pages);
+            if (lane == 0) mbar_expect_tx(bar, kPlane);
+            __syncwarp();
+            if (lane < boxes) {
+#pragma unroll
+                for (int b = 0; b < kDP / 64; b++) tma_load_4d(to + st * Sh::kStage + b * (kStep * 128), map, bar, 64 * b, here_row, kvh, here);
+            }
+            uint32_t there[2] = {0xffffffffu, 0xffffffffu};  // the keys of the stage that have a page
+            if (found != all_boxes) {
+                const uint32_t row_bits = box >= 32 ? 0xffffffffu : (1u << box) - 1u;
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    there[i] = 0;
+                    for (int b = 32 * i / box; b * box < 32 * (i + 1); b++)
+                        if (found >> b & 1u) there[i] |= row_bits << (b * box & 31);
+                }
+            }
+            if (lane == 0 && kv == 0) sm.valid[st][0] = there[0], sm.valid[st][1] = there[1];
+            if (last_part) {  // rows of the last page that nothing has been stored in: 0 times what they hold need not be 0
+                await(&sm.tail[kv], 0, ctx, SITE_TAIL);
+                for (int r = keys - key0; r < kStep; r++)
+                    for (int i = lane; i < (kDP / 64) * 8; i += 32)
+                        *reinterpret_cast<uint4 *>(tile_at + st * Sh::kStage + (i >> 3) * (kStep * 128) + r * 128 + ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.kv_full[st]);  // in the place of the copies' arrival
+            }
+            if (lane == 0) mbar_arrive(&sm.kv_full[st]);
+        }
+        if (missing) report(status, ST_ATTEND);
+    } else if (!kTma && nsteps > 0 && warp < Sh::kFirst) {
         // ------------------------------ producers ------------------------------
         constexpr int kChunks = kDP / 8, kPer = 32 / kChunks;  // pieces of 8 columns of a row; rows that a warp takes at once
+        constexpr int kIts = 64 / kPer;                        // of a tile
         const int mine = lane / kChunks, ch = lane % kChunks, from = warp - 1;
-        const T *kp = static_cast<const T *>(c.k) + head, *vp = static_cast<const T *>(c.v) + head;
         const bool col = 8 * ch < c.D;
+        const T *kp = static_cast<const T *>(c.k) + head + (col ? 8 * ch : 0), *vp = static_cast<const T *>(c.v) + head + (col ? 8 * ch : 0);
+        const uint32_t column = (ch >> 3) * (kStep * 128);
+        auto spot = [&](int r) { return column + r * 128 + (((ch & 7) ^ (r & 7)) << 4); };
         bool missing = false;
-        for (int n = 0; n < nsteps; n++) {
-            const int st = n % kStages, key0 = (first + n) * kStep;
-            const long long lo = place(c, table, key0 + lane, keys, missing), hi = place(c, table, key0 + 32 + lane, keys, missing);
-            const uint32_t there0 = __ballot_sync(0xffffffffu, lo >= 0), there1 = __ballot_sync(0xffffffffu, hi >= 0);
-            if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
-            if (from == 0 && lane == 0) sm.valid[st][0] = there0, sm.valid[st][1] = there1;
-            uint8_t *kt = sm.ring[st], *vt = kt + kTerms * kPlane;
-            if constexpr (!Sh::kWide) {
+        // of keys `lane` and 32 + `lane` of a step, looked up a step ahead
+        long long lo = place(c, table, first * kStep + lane, keys, missing), hi = place(c, table, first * kStep + 32 + lane, keys, missing);
+        if constexpr (!Sh::kWide) {
+            for (int n = 0; n < nsteps; n++) {
+                const int st = n % kStages, next0 = (first + n + 1) * kStep;
+                const long long lo1 = place(c, table, next0 + lane, keys, missing), hi1 = place(c, table, next0 + 32 + lane, keys, missing);
+                const uint32_t there0 = __ballot_sync(0xffffffffu, lo >= 0), there1 = __ballot_sync(0xffffffffu, hi >= 0);
+                if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
+                if (from == 0 && lane == 0) {
+                    sm.valid[st][0] = there0, sm.valid[st][1] = there1;
+                    mbar_arrive(&sm.kv_full[st]);
+                }
+                const uint32_t kt = smem_u32(sm.ring[st]), vt = kt + kPlane;
 #pragma unroll
-                for (int i = 0; i < (64 / kPer + Sh::kProducers - 1) / Sh::kProducers; i++) {
-                    const int it = i * Sh::kProducers + from;
-                    if (it >= 64 / kPer) break;
+                for (int i = 0; i < (kIts + 2) / 3; i++) {
+                    const int it = 3 * i + from;
+                    if (it >= kIts) break;
                     const int r = it * kPer + mine;
                     const long long off = __shfl_sync(0xffffffffu, it * kPer < 32 ? lo : hi, r & 31);
                     const bool in = off >= 0 && col;
-                    const long long at = in ? off + 8 * ch : 0;
-                    const uint32_t to = (ch >> 3) * (kStep * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-                    cp16(smem_u32(kt) + to, kp + at, in);
-                    cp16(smem_u32(vt) + to, vp + at, in);
+                    const uint32_t to = spot(r);
+                    cp16(kt + to, kp + max(off, 0ll), in);
+                    cp16(vt + to, vp + max(off, 0ll), in);
                 }
-                cp_commit();
-                if (n >= Sh::kLag) {
-                    cp_wait<Sh::kLag>();
-                    warp_arrive(&sm.kv_full[(n - Sh::kLag) % kStages], lane);
-                }
-            } else {
-                constexpr int kEach = (64 / kPer + Sh::kProducers - 1) / Sh::kProducers;
-#pragma unroll 1
-                for (int kv = 0; kv < 2; kv++) {
-                    const float *src = reinterpret_cast<const float *>(kv ? vp : kp);
-                    float4 f[kEach][2];
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        const int it = i * Sh::kProducers + from, r = it * kPer + mine;
-                        const long long off = __shfl_sync(0xffffffffu, it * kPer < 32 ? lo : hi, r & 31);
-                        f[i][0] = f[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (it < 64 / kPer && off >= 0 && col) {
-                            f[i][0] = *reinterpret_cast<const float4 *>(src + off + 8 * ch);
-                            f[i][1] = *reinterpret_cast<const float4 *>(src + off + 8 * ch + 4);
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < kEach; i++) {
-                        const int it = i * Sh::kProducers + from, r = it * kPer + mine;
-                        if (it >= 64 / kPer) break;
-                        const float g[8] = {f[i][0].x, f[i][0].y, f[i][0].z, f[i][0].w, f[i][1].x, f[i][1].y, f[i][1].z, f[i][1].w};
-                        store_split3<true>(kv ? vt : kt, kPlane, (ch >> 3) * (kStep * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), g);
-                    }
-                }
-                warp_arrive(&sm.kv_full[st], lane);
+                arrive_when_copied(&sm.kv_full[st]);
+                lo = lo1, hi = hi1;
             }
-        }
-        if constexpr (!Sh::kWide) {
             cp_wait<0>();
-            for (int n = max(0, nsteps - Sh::kLag); n < nsteps; n++) warp_arrive(&sm.kv_full[n % kStages], lane);
+        } else {
+            // three pieces at a time in registers, the next three on their way
+            constexpr int kMine = (2 * kIts + 2) / 3, kParts = (kMine + 5) / 6 * 2;
+            float4 f[2][3][2];
+            auto load = [&](int buf, int part, long long a, long long b) {
+#pragma unroll
+                for (int i = 0; i < 3; i++) {
+                    const int item = 3 * (3 * part + i) + from, it = item % kIts, r = it * kPer + mine;
+                    const long long off = __shfl_sync(0xffffffffu, it * kPer < 32 ? a : b, r & 31);
+                    f[buf][i][0] = f[buf][i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (item < 2 * kIts && off >= 0 && col) {
+                        const float *src = reinterpret_cast<const float *>(item < kIts ? kp : vp) + off;
+                        f[buf][i][0] = *reinterpret_cast<const float4 *>(src), f[buf][i][1] = *reinterpret_cast<const float4 *>(src + 4);
+                    }
+                }
+            };
+            load(0, 0, lo, hi);
+            for (int n = 0; n < nsteps; n++) {
+                const int st = n % kStages, next0 = (first + n + 1) * kStep;
+                const long long lo1 = place(c, table, next0 + lane, keys, missing), hi1 = place(c, table, next0 + 32 + lane, keys, missing);
+                const uint32_t there0 = __ballot_sync(0xffffffffu, lo >= 0), there1 = __ballot_sync(0xffffffffu, hi >= 0);
+                if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
+                if (from == 0 && lane == 0) sm.valid[st][0] = there0, sm.valid[st][1] = there1;
+#pragma unroll
+                for (int part = 0; part < kParts; part++) {
+                    if (part + 1 < kParts) load((part + 1) & 1, part + 1, lo, hi);
+                    else load(0, 0, lo1, hi1);
+#pragma unroll
+                    for (int i = 0; i < 3; i++) {
+                        const int item = 3 * (3 * part + i) + from, it = item % kIts;
+                        if (item >= 2 * kIts) break;
+                        const float4 x = f[part & 1][i][0], y = f[part & 1][i][1];
+                        const float g[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+                        store_split3<true>(sm.ring[st] + (item < kIts ? 0 : kTerms * kPlane), kPlane, spot(it * kPer + mine), g);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.kv_full[st]);
+                lo = lo1, hi = hi1;
+            }
         }
         if (missing) report(status, ST_ATTEND);
     }
-    float o[kHalf], m = -INFINITY, l = 0.f;
-    const int group = (warp - Sh::kFirst) >> 3, half = ((warp - Sh::kFirst) >> 2) & 1, quarter = warp & 3, row = 32 * quarter + lane;
+    float o[kPart], m = -INFINITY, l = 0.f;
+    const int group = (warp - Sh::kFirst) / Sh::kGroupWarps, part = ((warp - Sh::kFirst) >> 2) % kSplit, quarter = warp & 3, row = 32 * quarter + lane;
     const uint32_t lane_addr = (uint32_t)(quarter << 5) << 16;
     const bool softmax = warp >= Sh::kFirst;
     if (softmax) {
         // ------------------------------ softmax ------------------------------
+        constexpr int kCols = kStep / kSplit;  // scores of this thread
         const int at = row0 + row;
         const int seen = tile >= 0 && at < rows ? w.past + at / G + 1 : 0;  // keys that this row sees
 #pragma unroll
-        for (int e = 0; e < kHalf; e++) o[e] = 0.f;
+        for (int e = 0; e < kPart; e++) o[e] = 0.f;
         if (nsteps > 0 && group == 0) {
-            const float *src = q + (w.first + at / G) * ld + (long long)(kvh * G + at % G) * c.D + half * kHalf;
+            const float *src = q + (w.first + at / G) * ld + (long long)(kvh * G + at % G) * c.D + part * kPart;
+            uint32_t x[3][kPart / 2];
 #pragma unroll
-            for (int b = 0; b < kHalf; b += 32) {
-                uint32_t t[3][16];
+            for (int e = 0; e < kPart; e += 4) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (at < rows && part * kPart + e < c.D) v = *reinterpret_cast<const float4 *>(src + e);
+                cut3(make_float2(v.x * scale_log2, v.y * scale_log2), x[0][e / 2], x[1][e / 2], x[2][e / 2]);
+                cut3(make_float2(v.z * scale_log2, v.w * scale_log2), x[0][e / 2 + 1], x[1][e / 2 + 1], x[2][e / 2 + 1]);
+            }
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (at < rows && half * kHalf + b + e < c.D) v = *reinterpret_cast<const float4 *>(src + b + e);
-                    cut3(make_float2(v.x * scale_log2, v.y * scale_log2), t[0][e / 2], t[1][e / 2], t[2][e / 2]);
-                    cut3(make_float2(v.z * scale_log2, v.w * scale_log2), t[0][e / 2 + 1], t[1][e / 2 + 1], t[2][e / 2 + 1]);
-                }
-#pragma unroll
-                for (int i = 0; i < 3; i++) tmem_st16(tmem + lane_addr + Sh::kColQ + kHalf * i + (half * kHalf + b) / 2, t[i]);
+            for (int i = 0; i < 3; i++) {
+                const uint32_t to = tmem + lane_addr + Sh::kColQ + kDP / 2 * i + part * (kPart / 2);
+                if constexpr (kPart == 16) tmem_st8(to, x[i]);
+                else tmem_st16(to, x[i]);
             }
             tmem_wait_st();
             arrive_tmem(&sm.q_ready, lane);
         }
-        const uint32_t t_o = tmem + lane_addr + Sh::kColO + half * kHalf;
+        const uint32_t t_o = tmem + lane_addr + Sh::kColO + group * kDP + part * kPart;
         auto add_output = [&](int n, float by) {
             await(&sm.o_full[n & 1], (n >> 1) & 1, ctx, SITE_O_FULL);
+            const float2 by2 = make_float2(by, by);
 #pragma unroll
-            for (int b = 0; b < kHalf; b += 16) {
+            for (int b = 0; b < kPart; b += 16) {
                 uint32_t r[16];
                 tmem_ld16(t_o + b, r);
                 tmem_wait_ld();
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[b + e] = fmaf(o[b + e], by, __uint_as_float(r[e]));
+                for (int e = 0; e < 16; e += 2) {
+                    const float2 sum = fma2(make_float2(o[b + e], o[b + e + 1]), by2, make_float2(__uint_as_float(r[e]), __uint_as_float(r[e + 1])));
+                    o[b + e] = sum.x, o[b + e + 1] = sum.y;
+                }
             }
         };
         float alpha_before = 1.f;
         for (int n = group; n < nsteps; n += kGroups) {
-            const int st = n % kStages, key0 = (first + n) * kStep + 32 * half;
-            const uint32_t t_s = tmem + lane_addr + (n & 1) * 96;
-            await(&sm.kv_full[st], (n / kStages) & 1, ctx, SITE_KV_FULL);  // for what it says of the keys
+            const int st = n % kStages, key0 = (first + n) * kStep + kCols * part;
+            const uint32_t t_s = tmem + lane_addr + n % kBuffers * 96;
+            await(&sm.s_full[n % kBuffers], (n / kBuffers) & 1, ctx, SITE_S_FULL);
+            uint32_t s[kCols];
+            if constexpr (kCols == 32) tmem_ld32(t_s + kCols * part, s);
+            else tmem_ld16(t_s + kCols * part, s);
+            // what the warps that brought the keys say of them: it was there before the scores were asked for
+            const uint32_t there = sm.valid[st][part * kCols / 32] >> (part * kCols % 32);
             const int lim = seen - key0;
-            const uint32_t bits = sm.valid[st][half] & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u);
-            await(&sm.s_full[n & 1], (n >> 1) & 1, ctx, SITE_S_FULL);
-            uint32_t s[32];
-            tmem_ld32(t_s + 32 * half, s);
+            const uint32_t bits = there & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u), full = kCols == 32 ? 0xffffffffu : (1u << (kCols & 31)) - 1u;
             tmem_wait_ld();
-            if (__any_sync(0xffffffffu, bits != 0xffffffffu)) {
+            if (__any_sync(0xffffffffu, (bits & full) != full)) {
 #pragma unroll
-                for (int e = 0; e < 32; e++)
+                for (int e = 0; e < kCols; e++)
                     if (!(bits >> e & 1u)) s[e] = 0xff800000u;  // -inf
             }
             float mx = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+            for (int e = 0; e < kCols; e += 2) mx = max3(mx, __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
             const int par = (n / kGroups) & 1;
-            sm.xmax[group][par][half][row] = mx;
-            named_sync(1 + 4 * group + quarter, 64);
-            mx = max3(m, mx, sm.xmax[group][par][half ^ 1][row]);
+            sm.xmax[group][par][part][row] = mx;
+            named_sync(1 + 4 * group + quarter, 32 * kSplit);
+            if constexpr (kSplit == 2) mx = max3(m, mx, sm.xmax[group][par][part ^ 1][row]);
+            else mx = fmaxf(m, fmaxf(max3(sm.xmax[group][par][0][row], sm.xmax[group][par][1][row], sm.xmax[group][par][2][row]), sm.xmax[group][par][kSplit - 1][row]));
             const float base = mx == -INFINITY ? 0.f : mx;  // nothing but -inf so far
             const float alpha = ex2f(m - base);
             m = mx;
             const float2 minus = make_float2(-base, -base);
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int b = 0; b < 2; b++) {  // 16 columns make 8 of each term
+            for (int b = 0; b < kCols / 16; b++) {  // 16 columns make 8 of each term
                 uint32_t hi[8], mid[8], lo[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -336,22 +426,20 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
                     sum = add2(sum, p);
                     cut3(p, hi[e], mid[e], lo[e]);
                 }
-                tmem_st8(t_s + term_column(0, 2 * half + b), hi);
-                tmem_st8(t_s + term_column(1, 2 * half + b), mid);
-                tmem_st8(t_s + term_column(2, 2 * half + b), lo);
+                tmem_st8(t_s + term_column(0, part * (kCols / 16) + b), hi);
+                tmem_st8(t_s + term_column(1, part * (kCols / 16) + b), mid);
+                tmem_st8(t_s + term_column(2, part * (kCols / 16) + b), lo);
             }
             l = l * alpha + (sum.x + sum.y);
             tmem_wait_st();
-            if (kGroups == 1 && n > 0) add_output(n - 1, alpha_before);
+            if (n >= kGroups) add_output(n - kGroups, alpha_before);  // this group's output is free for the next P V
             alpha_before = alpha;
             arrive_tmem(&sm.p_full[n & 1], lane);
-            if (kGroups == 2) {
-                add_output(n, alpha);
-                arrive_tmem(&sm.o_free, lane);
-            }
         }
-        if (kGroups == 1 && nsteps > 0) add_output(nsteps - 1, alpha_before);
-        if (half == 1) sm.half_l[group][row] = l;
+        if (nsteps > group) add_output(nsteps - 1 - (nsteps - 1 - group) % kGroups, alpha_before);
+        // each part's share of the sum; the step that last used this parity is behind a barrier that all have passed
+        named_sync(1 + 4 * group + quarter, 32 * kSplit);
+        sm.xmax[group][0][part][row] = l;
     }
     if (sm.abort_flag) __nanosleep(50000);  // let products that are still in flight end
     if (threadIdx.x < kRowsTile / 32) sm.odd[threadIdx.x] = 0;
@@ -361,12 +449,14 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
     if (warp == 1) tmem_dealloc(tmem, 512);  // before anything that waits for the other CTAs of the cluster
     if (tile >= 0) {
         if (softmax) {
-            if (half == 0) l += sm.half_l[group][row];
+            l = 0.f;
+#pragma unroll
+            for (int i = 0; i < kSplit; i++) l += sm.xmax[group][0][i][row];
             if (kGroups == 2 && group == 1) {
 #pragma unroll
-                for (int e = 0; e < kHalf; e += 4)
-                    *reinterpret_cast<float4 *>(&sm.fin.o1[row][half * kHalf + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                if (half == 0) sm.m1[row] = m, sm.l1[row] = l;
+                for (int e = 0; e < kPart; e += 4)
+                    *reinterpret_cast<float4 *>(&sm.fin.o1[row][part * kPart + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (part == 0) sm.m1[row] = m, sm.l1[row] = l;
             }
         }
         if (kGroups == 2) __syncthreads();
@@ -374,17 +464,17 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
             if (kGroups == 2) {
                 const float mo = sm.m1[row], top = fmaxf(m, mo), base = top == -INFINITY ? 0.f : top, a = ex2f(m - base), b = ex2f(mo - base);
 #pragma unroll
-                for (int e = 0; e < kHalf; e++) o[e] = o[e] * a + sm.fin.o1[row][half * kHalf + e] * b;
-                l = l * a + sm.l1[row] * b;  // of the first half
+                for (int e = 0; e < kPart; e++) o[e] = o[e] * a + sm.fin.o1[row][part * kPart + e] * b;
+                l = l * a + sm.l1[row] * b;
                 m = top;
             }
-            float zero = half == 0 ? l * 0.f : 0.f;  // what is finite times zero is zero
+            float zero = l * 0.f;  // what is finite times zero is zero
 #pragma unroll
-            for (int e = 0; e < kHalf; e++) zero = fmaf(o[e], 0.f, zero);
+            for (int e = 0; e < kPart; e++) zero = fmaf(o[e], 0.f, zero);
 #pragma unroll
-            for (int e = 0; e < kHalf; e += 4)
-                *reinterpret_cast<float4 *>(&sm.fin.o[row][half * kHalf + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-            if (half == 0) sm.m[row] = m, sm.l[row] = l;
+            for (int e = 0; e < kPart; e += 4)
+                *reinterpret_cast<float4 *>(&sm.fin.o[row][part * kPart + e]) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            if (part == 0) sm.m[row] = m, sm.l[row] = l;
             const uint32_t odd = __ballot_sync(0xffffffffu, !(zero == 0.f) && row0 + row < rows);
             if (lane == 0 && odd) atomicOr(&sm.odd[quarter], odd);
         }
@@ -423,31 +513,56 @@ __global__ void __launch_bounds__(Shape<T, kDP>::kThreads, 1) tile_kernel(Cache 
     }
 }
 
-template <class T, int kDP>
-cudaError_t launch_tile(const Call &a, int few) {
-    using Sh = Shape<T, kDP>;
+template <class T, int kDP, bool kTma>
+cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUtensorMap &v, int box) {
+    using Sh = Shape<T, kDP, kTma>;
     const int G = a.heads / a.c.kv_heads, sms = attn::sm_count();
     const long long units = (long long)a.c.tokens * G / kRowsTile + a.c.seqs;
     unsigned ranks = 1;
     while (ranks < 8 && units * a.c.kv_heads * ranks * 2 <= sms) ranks *= 2;
     if (units * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    return attn::launch_clusters_after_previous(tile_kernel<T, kDP>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(Sh::kThreads),
-                                                sizeof(TileSmem<T, kDP>), ranks, a.s, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, a.status);
+    return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(Sh::kThreads),
+                                                sizeof(TileSmem<T, kDP, kTma>), ranks, a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2,
+                                                a.status);
+}
+
+// Pages as a map {D, rows of a page, heads, pages}, boxes of 64 columns by `box` rows; columns past the D-th read as zeros.
+int pages_map(CUtensorMap *map, const Cache &c, const void *base, int box) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c.D, (cuuint64_t)c.page_size, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)c.D * 2, (cuuint64_t)c.D * 2 * c.page_size, (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+    return attn::encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides, boxes);
+}
+
+template <int kDP>
+cudaError_t launch_narrow(const Call &a, int few) {
+    const int box = kStep < (a.c.page_size & -a.c.page_size) ? kStep : a.c.page_size & -a.c.page_size;  // the largest power of two in the page size
+    CUtensorMap k{}, v{};
+    if (box < 8 || a.c.page_stride >= 1ll << 39 || pages_map(&k, a.c, a.c.k, box) != 0 || pages_map(&v, a.c, a.c.v, box) != 0)
+        return launch_tile<__nv_bfloat16, kDP, false>(a, few, k, v, 0);
+    return launch_tile<__nv_bfloat16, kDP, true>(a, few, k, v, box);
+}
+
+template <class T, int kDP, bool kTma>
+cudaError_t set_one() {
+    return cudaFuncSetAttribute(tile_kernel<T, kDP, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(TileSmem<T, kDP, kTma>));
 }
 
 }  // namespace
 
 cudaError_t launch_tiles(const Call &a, int few) {
-    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_tile<__nv_bfloat16, 64>(a, few) : launch_tile<__nv_bfloat16, 128>(a, few);
-    return a.c.D <= 64 ? launch_tile<float, 64>(a, few) : launch_tile<float, 128>(a, few);
+    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_narrow<64>(a, few) : launch_narrow<128>(a, few);
+    const CUtensorMap none{};
+    return a.c.D <= 64 ? launch_tile<float, 64, false>(a, few, none, none, 0) : launch_tile<float, 128, false>(a, few, none, none, 0);
 }
 
 cudaError_t tiles_set_attributes() {
-    const cudaFuncAttribute at = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    cudaError_t e = cudaFuncSetAttribute(tile_kernel<__nv_bfloat16, 64>, at, (int)sizeof(TileSmem<__nv_bfloat16, 64>));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(tile_kernel<__nv_bfloat16, 128>, at, (int)sizeof(TileSmem<__nv_bfloat16, 128>));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(tile_kernel<float, 64>, at, (int)sizeof(TileSmem<float, 64>));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(tile_kernel<float, 128>, at, (int)sizeof(TileSmem<float, 128>));
+    cudaError_t e = set_one<__nv_bfloat16, 64, true>();
+    if (e == cudaSuccess) e = set_one<__nv_bfloat16, 64, false>();
+    if (e == cudaSuccess) e = set_one<__nv_bfloat16, 128, true>();
+    if (e == cudaSuccess) e = set_one<__nv_bfloat16, 128, false>();
+    if (e == cudaSuccess) e = set_one<float, 64, false>();
+    if (e == cudaSuccess) e = set_one<float, 128, false>();
     return e;
 }
 
