@@ -27,8 +27,22 @@ __device__ __forceinline__ void arrive_tmem(uint64_t *bar, int lane) {
     if (lane == 0) mbar_arrive(bar);
 }
 
+// x - hi for both halves of a pair of bf16 values, exact where hi is the upper half of x.
+__device__ __forceinline__ float2 less(float2 x, uint32_t hi) {
+    float2 r;
+    asm("{\n\t.reg .b16 a, b, m;\n\tmov.b32 {a, b}, %2;\n\tmov.b16 m, 0xbf80;\n\tfma.rn.f32.bf16 %0, a, m, %3;\n\tfma.rn.f32.bf16 %1, b, m, %4;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(hi), "f"(x.x), "f"(x.y));
+    return r;
+}
 // p = hi + mid + lo, each the next eight bits cut off: exact.
-__device__ __forceinline__ void cut3(float2 p, uint32_t &hi, uint32_t &mid, uint32_t &lo) { split3(p, hi, mid, lo, 0u); }
+__device__ __forceinline__ void cut3(float2 p, uint32_t &hi, uint32_t &mid, uint32_t &lo) {
+    hi = __byte_perm(__float_as_uint(p.x), __float_as_uint(p.y), 0x7632);
+    const float2 r = less(p, hi);
+    mid = __byte_perm(__float_as_uint(r.x), __float_as_uint(r.y), 0x7632);
+    const float2 s = less(r, mid);
+    lo = __byte_perm(__float_as_uint(s.x), __float_as_uint(s.y), 0x7632);
+}
 
 // Element offset of key j's row from that of its head, -1 where it has no page.
 __device__ __forceinline__ long long place(const Cache &c, const int *table, int j, int end, bool &missing) {

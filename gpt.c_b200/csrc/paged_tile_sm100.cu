@@ -71,45 +71,48 @@ struct __align__(1024) TileSmem {
     int abort_flag;
 };
 
+enum Chain : int { kGoesOn = 1, kSecond = 2 };  // a launch that another one goes on with, and that other one
 enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_Q_READY, SITE_ALIGN, SITE_TAIL };
 
 // The sequence and tile of unit `u`, tiles counted over the sequences with more than `few` rows and no more new tokens than max_new;
-// tile -1 past the last.  A whole warp.  check: reports lengths that the call does not allow.
+// tile -1 past the last.  Up to 32 sequences are taken in the order of falling length, and the tiles of each from its last, so that the
+// longest units begin first and the shortest fill the end.  A whole warp.  check: reports lengths that the call does not allow.
 __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int max_new, int u, bool check, int *status, int &seq, int &tile) {
     const int lane = threadIdx.x & 31;
     seq = 0, tile = -1;
     for (int base = 0; base < c.seqs; base += 32) {
         const int s = base + lane;
-        int tiles = 0;
+        int tiles = 0, length = 0;
         if (s < c.seqs) {
             const Span w = span_of(c, s);
             const bool good = w.count <= max_new && w.past >= 0;
             if (check && w.count > 0 && (!good || w.past + (long long)w.count > (long long)c.width * c.page_size)) report(status, ST_ATTEND);
             const long long rows = (long long)w.count * G;
             tiles = good && rows > few ? (int)((rows + kRowsTile - 1) / kRowsTile) : 0;
+            length = w.past + w.count;
         }
-        int run = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int left = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += left;
+        int before = 0, all = 0;  // tiles in front of this lane's
+        for (int j = 0; j < min(32, c.seqs - base); j++) {
+            const int other = __shfl_sync(0xffffffffu, tiles, j), longer = __shfl_sync(0xffffffffu, length, j);
+            before += longer > length || (longer == length && j < lane) ? other : 0;
+            all += other;
         }
-        const uint32_t past = __ballot_sync(0xffffffffu, run > u);
-        if (past != 0 && tile < 0) {
-            const int at = __ffs(past) - 1;
+        const uint32_t mine = __ballot_sync(0xffffffffu, u >= before && u < before + tiles);
+        if (mine != 0) {
+            const int at = __ffs(mine) - 1;
             seq = base + at;
-            tile = u - __shfl_sync(0xffffffffu, run - tiles, at);
+            tile = __shfl_sync(0xffffffffu, before + tiles, at) - 1 - u;
             if (!check) return;
+            u = 0x7fffffff;  // only the check goes on
         }
-        u -= __shfl_sync(0xffffffffu, run, 31);
-        if (tile >= 0) u = 0x7fffffff;  // only the check goes on
+        u -= all;
     }
 }
 
 template <class T, int kDP, bool kTma>
 __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                int box, Cache c, const float *q, float *out, long long ld, int heads, int few, int max_new,
-                                                                         float scale_log2, int *status) {
+                                                                         float scale_log2, int from_unit, int chain, int *status) {
     using Sh = Shape<T, kDP, kTma>;
     using Smem = TileSmem<T, kDP, kTma>;
     constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups, kBuffers = Sh::kBuffers, kTerms = Sh::kTerms, kSplit = Sh::kSplit, kPart = kDP / kSplit;
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, kvh = blockIdx.y, G = heads / c.kv_heads;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, unit = from_unit + (int)blockIdx.x / ranks, kvh = unit % c.kv_heads, G = heads / c.kv_heads;
     WaitCtx ctx{&sm.abort_flag, status};
     if (threadIdx.x == 0) {
         if ((smem_u32(smem_raw) & 1023u) != 0) report(status, ST_TIMEOUT_BASE + SITE_ALIGN);
@@ -132,18 +135,21 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             mbar_init(&sm.tail[i], 1);
         }
         for (int i = 0; i < 3; i++) mbar_init(&sm.s_full[i], 1);
-        mbar_init(&sm.q_ready, Sh::kGroupWarps);
+        mbar_init(&sm.q_ready, 16);
         fence_barrier_init();
     }
     if (kTma && threadIdx.x == 64) {
         tma_prefetch_desc(&map_k);
         tma_prefetch_desc(&map_v);
     }
+    // The second of two launches runs beside the end of the first: the first lets it start only when what was before both has
+    // completed, and it waits for the first before it ends itself.
+    if (chain & kGoesOn) pdl_wait();
     if (warp == 1) tmem_alloc_then_launch_dependents(&sm.tmem_base, 512);
-    pdl_wait();
+    if (!(chain & (kGoesOn | kSecond))) pdl_wait();
     if (warp == 0) {
         int seq, tile;
-        const int units = gridDim.x / ranks, u = units - 1 - (int)(blockIdx.x / ranks);  // the last tiles of a sequence are its longest
+        const int u = unit / c.kv_heads;
         find_tile(c, G, few, max_new, u, u == 0 && kvh == 0 && rank == 0, status, seq, tile);
         const Span span = span_of(c, seq);
         if (lane == 0) sm.seq = seq, sm.tile = tile, sm.span = span;
@@ -159,8 +165,10 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
     // this CTA's run of keys: steps first .. first + nsteps - 1
     const int last = (min(row0 + kRowsTile, rows) - 1) / G;
     const int keys = tile < 0 ? 0 : (int)min((long long)w.past + last + 1, (long long)c.width * c.page_size);
-    const int all = (keys + kStep - 1) / kStep, each = (all + ranks - 1) / ranks;
-    const int first = min(rank * each, all), nsteps = min(each, all - first);
+    const int all = (keys + kStep - 1) / kStep, each = (all + ranks - 1) / ranks, first = min(rank * each, all), nsteps = min(each, all - first);
+    // new token and head of a row
+    auto token_of = [&](int at) { return G == 1 ? at : at / G; };
+    auto head_of = [&](int at) { return kvh * G + (G == 1 ? 0 : at % G); };
     const long long head = (long long)kvh * c.page_size * c.D;
 
     if (nsteps > 0 && warp == 0) {
@@ -209,9 +217,8 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         const uint32_t all_boxes = boxes == 32 ? 0xffffffffu : (1u << boxes) - 1u;
         bool missing = false;
         int j = first * kStep + lane * box, slot = j / c.page_size, row = j % c.page_size, row_here = row;
-        auto page_of = [&] {  // of key j; past the last one where there is none: that reads as zeros
-            int page = lane < boxes && j < keys ? table[slot] : c.pages;
-            if ((unsigned)page > (unsigned)c.pages || (page == c.pages && lane < boxes && j < keys)) missing = true, page = c.pages;
+        auto page_of = [&] {  // of key j; -1 where there is no key
+            const int page = lane < boxes && j < keys ? table[slot] : -1;
             row_here = row;
             j += kStep, slot += slots, row += row_step;
             if (row >= c.page_size) row -= c.page_size, slot++;
@@ -222,13 +229,17 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         const CUtensorMap *map = kv ? &map_v : &map_k;
         uint8_t *const tile_at = sm.ring[0] + kv * kPlane, *const to = tile_at + (lane < boxes ? lane : 0) * box * 128;
         for (int n = 0; n < nsteps; n++) {
-            const int st = n % kStages, here = page, here_row = at_row;
+            const int st = n % kStages, here_row = at_row;
+            // past the last page where there is none: that reads as zeros
+            const bool wanted = lane < boxes && (first + n) * kStep + lane * box < keys, there_is = wanted && (unsigned)page < (unsigned)c.pages;
+            const int here = there_is ? page : c.pages;
+            missing |= wanted && !there_is;
             page = page_of(), at_row = row_here;
             if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
             const int key0 = (first + n) * kStep;
             const bool last_part = key0 + kStep > keys;
             uint64_t *bar = last_part ? &sm.tail[kv] : &sm.kv_full[st];
-            const uint32_t found = __ballot_sync(0xffffffffu, here < c.pages);
+            const uint32_t found = __ballot_sync(0xffffffffu, there_is);
             if (lane == 0) mbar_expect_tx(bar, kPlane);
             __syncwarp();
             if (lane < boxes) {
@@ -347,23 +358,26 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         // ------------------------------ softmax ------------------------------
         constexpr int kCols = kStep / kSplit;  // scores of this thread
         const int at = row0 + row;
-        const int seen = tile >= 0 && at < rows ? w.past + at / G + 1 : 0;  // keys that this row sees
+        const int seen = tile >= 0 && at < rows ? w.past + token_of(at) + 1 : 0;  // keys that this row sees
+        const int all_see = __reduce_min_sync(0xffffffffu, seen);           // and every row of this warp
 #pragma unroll
         for (int e = 0; e < kPart; e++) o[e] = 0.f;
-        if (nsteps > 0 && group == 0) {
-            const float *src = q + (w.first + at / G) * ld + (long long)(kvh * G + at % G) * c.D + part * kPart;
-            uint32_t x[3][kPart / 2];
+        if (nsteps > 0) {
+            constexpr int kShare = kDP / 4;  // columns of Q for each thread of a row, of both groups
+            const int from = (group * kSplit + part) * kShare;
+            const float *src = q + (w.first + token_of(at)) * ld + (long long)head_of(at) * c.D + from;
+            uint32_t x[3][kShare / 2];
 #pragma unroll
-            for (int e = 0; e < kPart; e += 4) {
+            for (int e = 0; e < kShare; e += 4) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (at < rows && part * kPart + e < c.D) v = *reinterpret_cast<const float4 *>(src + e);
+                if (at < rows && from + e < c.D) v = *reinterpret_cast<const float4 *>(src + e);
                 cut3(make_float2(v.x * scale_log2, v.y * scale_log2), x[0][e / 2], x[1][e / 2], x[2][e / 2]);
                 cut3(make_float2(v.z * scale_log2, v.w * scale_log2), x[0][e / 2 + 1], x[1][e / 2 + 1], x[2][e / 2 + 1]);
             }
 #pragma unroll
             for (int i = 0; i < 3; i++) {
-                const uint32_t to = tmem + lane_addr + Sh::kColQ + kDP / 2 * i + part * (kPart / 2);
-                if constexpr (kPart == 16) tmem_st8(to, x[i]);
+                const uint32_t to = tmem + lane_addr + Sh::kColQ + kDP / 2 * i + from / 2;
+                if constexpr (kShare == 16) tmem_st8(to, x[i]);
                 else tmem_st16(to, x[i]);
             }
             tmem_wait_st();
@@ -394,11 +408,11 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             if constexpr (kCols == 32) tmem_ld32(t_s + kCols * part, s);
             else tmem_ld16(t_s + kCols * part, s);
             // what the warps that brought the keys say of them: it was there before the scores were asked for
-            const uint32_t there = sm.valid[st][part * kCols / 32] >> (part * kCols % 32);
-            const int lim = seen - key0;
-            const uint32_t bits = there & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u), full = kCols == 32 ? 0xffffffffu : (1u << (kCols & 31)) - 1u;
+            const uint32_t there = sm.valid[st][part * kCols / 32] >> (part * kCols % 32), full = kCols == 32 ? 0xffffffffu : (1u << (kCols & 31)) - 1u;
             tmem_wait_ld();
-            if (__any_sync(0xffffffffu, (bits & full) != full)) {
+            if ((first + n + 1) * kStep > all_see || (there & full) != full) {
+                const int lim = seen - key0;
+                const uint32_t bits = there & (lim >= 32 ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u);
 #pragma unroll
                 for (int e = 0; e < kCols; e++)
                     if (!(bits >> e & 1u)) s[e] = 0xff800000u;  // -inf
@@ -418,17 +432,16 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
             for (int b = 0; b < kCols / 16; b++) {  // 16 columns make 8 of each term
-                uint32_t hi[8], mid[8], lo[8];
+                uint32_t hi[8], rest[16];  // mid and lo lie side by side
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float2 x = add2(make_float2(__uint_as_float(s[16 * b + 2 * e]), __uint_as_float(s[16 * b + 2 * e + 1])), minus);
                     const float2 p = make_float2(ex2f(x.x), ex2f(x.y));
                     sum = add2(sum, p);
-                    cut3(p, hi[e], mid[e], lo[e]);
+                    cut3(p, hi[e], rest[e], rest[8 + e]);
                 }
                 tmem_st8(t_s + term_column(0, part * (kCols / 16) + b), hi);
-                tmem_st8(t_s + term_column(1, part * (kCols / 16) + b), mid);
-                tmem_st8(t_s + term_column(2, part * (kCols / 16) + b), lo);
+                tmem_st16(t_s + term_column(1, part * (kCols / 16) + b), rest);
             }
             l = l * alpha + (sum.x + sum.y);
             tmem_wait_st();
@@ -483,8 +496,8 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             for (int r = warp; r < kRowsTile; r += Sh::kThreads / 32) {
                 if (!(sm.odd[r >> 5] >> (r & 31) & 1u)) continue;
                 const int at = row0 + r;
-                exact_row<T, kDP>(c, q + (w.first + at / G) * ld + (long long)(kvh * G + at % G) * c.D, table, kvh, first * kStep,
-                                  min(min((first + nsteps) * kStep, keys), w.past + at / G + 1), scale_log2, sm.fin.o[r], &sm.m[r], &sm.l[r]);
+                exact_row<T, kDP>(c, q + (w.first + token_of(at)) * ld + (long long)head_of(at) * c.D, table, kvh, first * kStep,
+                                  min(min((first + nsteps) * kStep, keys), w.past + token_of(at) + 1), scale_log2, sm.fin.o[r], &sm.m[r], &sm.l[r]);
             }
         }
         if (ranks > 1) cluster.sync();
@@ -506,11 +519,12 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             const int at = row0 + r;
             const float by = sum == 0.f ? 0.f : 1.f / sum;
             if (4 * word < c.D)
-                *reinterpret_cast<float4 *>(out + ((long long)(w.first + at / G) * heads + kvh * G + at % G) * c.D + 4 * word) =
+                *reinterpret_cast<float4 *>(out + ((long long)(w.first + token_of(at)) * heads + head_of(at)) * c.D + 4 * word) =
                     make_float4(acc.x * by, acc.y * by, acc.z * by, acc.w * by);
         }
         if (ranks > 1) cluster.sync();  // shared memory of the others is read until here
     }
+    if (chain & kSecond) pdl_wait();
 }
 
 template <class T, int kDP, bool kTma>
@@ -518,12 +532,20 @@ cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUte
     using Sh = Shape<T, kDP, kTma>;
     const int G = a.heads / a.c.kv_heads, sms = attn::sm_count();
     const long long units = (long long)a.c.tokens * G / kRowsTile + a.c.seqs;
-    unsigned ranks = 1;
-    while (ranks < 8 && units * a.c.kv_heads * ranks * 2 <= sms) ranks *= 2;
-    if (units * ranks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-    return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)(units * ranks), (unsigned)a.c.kv_heads), dim3(Sh::kThreads),
-                                                sizeof(TileSmem<T, kDP, kTma>), ranks, a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2,
-                                                a.status);
+    const long long all = units * a.c.kv_heads;
+    if (all > 0x7fffffffll / 8) return cudaErrorInvalidConfiguration;
+    auto launch = [&](int from, int count, int chain) {
+        unsigned ranks = 1;
+        while (ranks < 8 && (long long)count * ranks * 2 <= sms) ranks *= 2;  // few units share their keys among the SMs that are left
+        return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)count * ranks), dim3(Sh::kThreads), sizeof(TileSmem<T, kDP, kTma>), ranks,
+                                                    a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, from, chain, a.status);
+    };
+    // What is left behind full rounds of one unit an SM, where that is less than half a round, would hold a few SMs for as long as a full
+    // one: a second launch cuts each of those units among several SMs (324 units of 102 steps 225 -> XXX us).
+    const int rest = (int)(all % sms);
+    if (all < sms || rest == 0 || 2 * rest > sms) return launch(0, (int)all, 0);
+    const cudaError_t e = launch(0, (int)all - rest, kGoesOn);
+    return e != cudaSuccess ? e : launch((int)all - rest, rest, kSecond);
 }
 
 // Pages as a map {D, rows of a page, heads, pages}, boxes of 64 columns by `box` rows; columns past the D-th read as zeros.
