@@ -7,9 +7,10 @@
 // (attn24.cuh), so q and p take part exactly; bf16 pages are one term, fp32 pages three: 3 or 6 passes a product.  The tensor
 // cores truncate their sums, so the P V of each step starts at zero and is added to the output in registers.
 //
-// Warps: one issues the tensor-core instructions, two or three bring keys and values from wherever their pages are into a ring (bf16 by
-// the copy engine, boxes of 8 to 64 rows that lie in one page; by asynchronous 16-byte copies where pages are not a multiple of 8 rows;
-// fp32 through registers, split on the way), sixteen do the softmax.  Where a step takes the tensor cores as long as a softmax step or
+// Warps: one issues the tensor-core instructions, two or three bring keys and values of bf16 from wherever their pages are into a ring
+// (the copy engine, boxes of 8 to 64 rows that lie in one page; asynchronous 16-byte copies where pages are not a multiple of 8 rows),
+// sixteen do the softmax and, of fp32 pages, bring keys and values through registers, split on the way (three warps for that alone took
+// 4000 cycles a step).  Where a step takes the tensor cores as long as a softmax step or
 // longer (1536 cycles and more: fp32, or head sizes above 64) four threads share a row and two score buffers alternate; else (768
 // cycles) two threads do, and two groups of eight warps take every other step each, with a maximum, sum and output of their own that
 // are joined at the end, and three score buffers, so that a group finds its next scores when it has done with one step (with two
@@ -45,6 +46,7 @@ struct Shape {
     static constexpr int kPlane = kStep * kDP * 2;         // one term of 64 keys
     static constexpr int kStage = 2 * kTerms * kPlane;     // K terms, V terms
     static constexpr int kStages = kWide ? (kDP == 64 ? 4 : 2) : (kDP == 64 ? 8 : 6);
+    static constexpr int kLead = kWide ? kStages / 2 : 0;  // steps that the softmax warps are ahead with fp32 keys and values
     static constexpr int kBuffers = kGroups + 1;           // of scores, 96 columns each
     static constexpr uint32_t kColO = 96 * kBuffers, kColQ = kColO + kGroups * kDP;  // an output for each group
     static_assert(kColQ + 3 * kDP / 2 <= 512, "tensor memory");
@@ -62,6 +64,7 @@ struct __align__(1024) TileSmem {
     };
     uint64_t kv_full[S::kStages], kv_empty[S::kStages], s_full[3], p_full[2], o_full[2], q_ready, tail[2];
     uint32_t valid[S::kStages][2];          // keys of the stage that are there
+    uint8_t nibble[S::kStages][16];         // fp32 pages: of the four rows of each warp
     float xmax[S::kGroups][2][S::kSplit][kRowsTile];  // [group][step parity][part][row]: maxima, at the end sums
     float m[kRowsTile], l[kRowsTile], m1[kRowsTile], l1[kRowsTile];
     uint32_t odd[kRowsTile / 32];           // rows to be computed again
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         if ((smem_u32(smem_raw) & 1023u) != 0) report(status, ST_TIMEOUT_BASE + SITE_ALIGN);
         sm.abort_flag = 0;
         for (int i = 0; i < kStages; i++) {
-            mbar_init(&sm.kv_full[i], kTma ? 4 : Sh::kWide ? Sh::kProducers : 32 * Sh::kProducers + 1);
+            mbar_init(&sm.kv_full[i], kTma ? 4 : Sh::kWide ? 16 : 32 * Sh::kProducers + 1);
             mbar_init(&sm.kv_empty[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             if (lane == 0) mbar_arrive(&sm.kv_full[st]);
         }
         if (missing) report(status, ST_ATTEND);
-    } else if (!kTma && nsteps > 0 && warp < Sh::kFirst) {
+    } else if (!kTma && !Sh::kWide && nsteps > 0 && warp < Sh::kFirst) {
         // ------------------------------ producers ------------------------------
         constexpr int kChunks = kDP / 8, kPer = 32 / kChunks;  // pieces of 8 columns of a row; rows that a warp takes at once
         constexpr int kIts = 64 / kPer;                        // of a tile
@@ -307,46 +310,6 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
                 lo = lo1, hi = hi1;
             }
             cp_wait<0>();
-        } else {
-            // three pieces at a time in registers, the next three on their way
-            constexpr int kMine = (2 * kIts + 2) / 3, kParts = (kMine + 5) / 6 * 2;
-            float4 f[2][3][2];
-            auto load = [&](int buf, int part, long long a, long long b) {
-#pragma unroll
-                for (int i = 0; i < 3; i++) {
-                    const int item = 3 * (3 * part + i) + from, it = item % kIts, r = it * kPer + mine;
-                    const long long off = __shfl_sync(0xffffffffu, it * kPer < 32 ? a : b, r & 31);
-                    f[buf][i][0] = f[buf][i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (item < 2 * kIts && off >= 0 && col) {
-                        const float *src = reinterpret_cast<const float *>(item < kIts ? kp : vp) + off;
-                        f[buf][i][0] = *reinterpret_cast<const float4 *>(src), f[buf][i][1] = *reinterpret_cast<const float4 *>(src + 4);
-                    }
-                }
-            };
-            load(0, 0, lo, hi);
-            for (int n = 0; n < nsteps; n++) {
-                const int st = n % kStages, next0 = (first + n + 1) * kStep;
-                const long long lo1 = place(c, table, next0 + lane, keys, missing), hi1 = place(c, table, next0 + 32 + lane, keys, missing);
-                const uint32_t there0 = __ballot_sync(0xffffffffu, lo >= 0), there1 = __ballot_sync(0xffffffffu, hi >= 0);
-                if (n >= kStages) await(&sm.kv_empty[st], (n / kStages - 1) & 1, ctx, SITE_KV_EMPTY);
-                if (from == 0 && lane == 0) sm.valid[st][0] = there0, sm.valid[st][1] = there1;
-#pragma unroll
-                for (int part = 0; part < kParts; part++) {
-                    if (part + 1 < kParts) load((part + 1) & 1, part + 1, lo, hi);
-                    else load(0, 0, lo1, hi1);
-#pragma unroll
-                    for (int i = 0; i < 3; i++) {
-                        const int item = 3 * (3 * part + i) + from, it = item % kIts;
-                        if (item >= 2 * kIts) break;
-                        const float4 x = f[part & 1][i][0], y = f[part & 1][i][1];
-                        const float g[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-                        store_split3<true>(sm.ring[st] + (item < kIts ? 0 : kTerms * kPlane), kPlane, spot(it * kPer + mine), g);
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.kv_full[st]);
-                lo = lo1, hi = hi1;
-            }
         }
         if (missing) report(status, ST_ATTEND);
     }
@@ -362,6 +325,61 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         const int all_see = __reduce_min_sync(0xffffffffu, seen);           // and every row of this warp
 #pragma unroll
         for (int e = 0; e < kPart; e++) o[e] = 0.f;
+        // fp32 pages: eight threads a row, each with 8 columns of every 64 of K and of V; loads of a step are under way while the one
+        // before is split
+        constexpr int kBlocks = kDP / 64, kLead = Sh::kLead;
+        const int mine = (int)threadIdx.x - 32 * Sh::kFirst, k_row = mine >> 3, k_ch = mine & 7;
+        float4 kf[Sh::kWide ? kBlocks : 1][2], vf[Sh::kWide ? kBlocks : 1][2];
+        bool have = false, missing = false;
+        int j = first * kStep + k_row, slot = 0, in_page = 0, page = -1;
+        const int end_key = min(keys, (first + nsteps) * kStep), slots = kStep / c.page_size, page_step = kStep % c.page_size;
+        auto look_up = [&] { page = j < end_key ? table[slot] : -1; };
+        auto fetch = [&] {
+            const bool wanted = j < end_key;
+            have = wanted && (unsigned)page < (unsigned)c.pages;
+            missing |= wanted && !have;
+            const long long at = have ? page * c.page_stride + (long long)in_page * c.D + head + 8 * k_ch : 0;
+#pragma unroll
+            for (int i = 0; i < kBlocks; i++) {
+                const bool in = have && 64 * i + 8 * k_ch < c.D;
+                const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 *kp = reinterpret_cast<const float4 *>(static_cast<const float *>(c.k) + at + 64 * i);
+                const float4 *vp = reinterpret_cast<const float4 *>(static_cast<const float *>(c.v) + at + 64 * i);
+                kf[i][0] = in ? kp[0] : zero, kf[i][1] = in ? kp[1] : zero;
+                vf[i][0] = in ? vp[0] : zero, vf[i][1] = in ? vp[1] : zero;
+            }
+            j += kStep, slot += slots, in_page += page_step;
+            if (in_page >= c.page_size) in_page -= c.page_size, slot++;
+            look_up();
+        };
+        auto put = [&](int n) {  // into the stage of step n
+            uint8_t *to = sm.ring[n % kStages] + k_row * 128 + ((k_ch ^ (k_row & 7)) << 4);
+#pragma unroll
+            for (int i = 0; i < kBlocks; i++)
+#pragma unroll
+                for (int kv = 0; kv < 2; kv++) {
+                    const float4 x = kv ? vf[i][0] : kf[i][0], y = kv ? vf[i][1] : kf[i][1];
+                    uint32_t h[4], m[4], l[4];
+                    cut3(make_float2(x.x, x.y), h[0], m[0], l[0]);
+                    cut3(make_float2(x.z, x.w), h[1], m[1], l[1]);
+                    cut3(make_float2(y.x, y.y), h[2], m[2], l[2]);
+                    cut3(make_float2(y.z, y.w), h[3], m[3], l[3]);
+                    uint8_t *at = to + kv * kTerms * kPlane + i * (kStep * 128);
+                    *reinterpret_cast<uint4 *>(at) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(at + kPlane) = make_uint4(m[0], m[1], m[2], m[3]);
+                    *reinterpret_cast<uint4 *>(at + 2 * kPlane) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            const uint32_t rows4 = __ballot_sync(0xffffffffu, have);
+            if (lane == 0) {
+                sm.nibble[n % kStages][mine >> 5] = (uint8_t)((rows4 & 1) | (rows4 >> 7 & 2) | (rows4 >> 14 & 4) | (rows4 >> 21 & 8));
+                mbar_arrive(&sm.kv_full[n % kStages]);
+            }
+        };
+        if (Sh::kWide && nsteps > 0) {
+            slot = j / c.page_size, in_page = j % c.page_size;
+            look_up();
+            fetch();
+        }
         if (nsteps > 0) {
             constexpr int kShare = kDP / 4;  // columns of Q for each thread of a row, of both groups
             const int from = (group * kSplit + part) * kShare;
@@ -382,6 +400,12 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             }
             tmem_wait_st();
             arrive_tmem(&sm.q_ready, lane);
+        }
+        if (Sh::kWide) {
+            for (int n = 0; n < min(kLead, nsteps); n++) {
+                put(n);
+                fetch();
+            }
         }
         const uint32_t t_o = tmem + lane_addr + Sh::kColO + group * kDP + part * kPart;
         auto add_output = [&](int n, float by) {
@@ -404,11 +428,26 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             const int st = n % kStages, key0 = (first + n) * kStep + kCols * part;
             const uint32_t t_s = tmem + lane_addr + n % kBuffers * 96;
             await(&sm.s_full[n % kBuffers], (n / kBuffers) & 1, ctx, SITE_S_FULL);
+            if (Sh::kWide && kLead == 1) {  // two stages: the other one is free when P V of the step before has been added up
+                if (n > 0) add_output(n - 1, alpha_before);
+                if (n + 1 < nsteps) {
+                    __syncwarp();
+                    put(n + 1);
+                    fetch();
+                }
+            }
             uint32_t s[kCols];
             if constexpr (kCols == 32) tmem_ld32(t_s + kCols * part, s);
             else tmem_ld16(t_s + kCols * part, s);
             // what the warps that brought the keys say of them: it was there before the scores were asked for
-            const uint32_t there = sm.valid[st][part * kCols / 32] >> (part * kCols % 32), full = kCols == 32 ? 0xffffffffu : (1u << (kCols & 31)) - 1u;
+            uint32_t there;
+            if constexpr (Sh::kWide) {
+                const uint32_t n4 = *reinterpret_cast<const uint32_t *>(&sm.nibble[st][4 * part]);
+                there = (n4 & 0xf) | (n4 >> 4 & 0xf0) | (n4 >> 8 & 0xf00) | (n4 >> 12 & 0xf000);
+            } else {
+                there = sm.valid[st][part * kCols / 32] >> (part * kCols % 32);
+            }
+            const uint32_t full = kCols == 32 ? 0xffffffffu : (1u << (kCols & 31)) - 1u;
             tmem_wait_ld();
             if ((first + n + 1) * kStep > all_see || (there & full) != full) {
                 const int lim = seen - key0;
@@ -445,10 +484,16 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
             }
             l = l * alpha + (sum.x + sum.y);
             tmem_wait_st();
-            if (n >= kGroups) add_output(n - kGroups, alpha_before);  // this group's output is free for the next P V
+            // this group's output is free for the next P V
+            if (n >= kGroups && !(Sh::kWide && kLead == 1)) add_output(n - kGroups, alpha_before);
             alpha_before = alpha;
             arrive_tmem(&sm.p_full[n & 1], lane);
+            if (Sh::kWide && kLead == 2 && n + 2 < nsteps) {  // four stages: that of step n - 2, which has been added up
+                put(n + 2);
+                fetch();
+            }
         }
+        if (missing) report(status, ST_ATTEND);
         if (nsteps > group) add_output(nsteps - 1 - (nsteps - 1 - group) % kGroups, alpha_before);
         // each part's share of the sum; the step that last used this parity is behind a barrier that all have passed
         named_sync(1 + 4 * group + quarter, 32 * kSplit);
@@ -536,7 +581,7 @@ cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUte
     if (all > 0x7fffffffll / 8) return cudaErrorInvalidConfiguration;
     auto launch = [&](int from, int count, int chain) {
         unsigned ranks = 1;
-        while (ranks < 8 && (long long)count * ranks * 2 <= sms) ranks *= 2;  // few units share their keys among the SMs that are left
+        while (ranks < 8 && (long long)count * ranks * 2 <= (chain & kSecond ? 2 : 1) * sms) ranks *= 2;  // few units share their keys among the SMs that are left
         return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)count * ranks), dim3(Sh::kThreads), sizeof(TileSmem<T, kDP, kTma>), ranks,
                                                     a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, from, chain, a.status);
     };
