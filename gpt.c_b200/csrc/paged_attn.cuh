@@ -115,16 +115,26 @@ struct Call {
     cudaStream_t s;
 };
 
+// Launches that share nothing run side by side: one that another goes on with (kGoesOn) lets it start only when what was before both has
+// completed, and that other one (kSecond) does not wait at its start, but for the first before it ends, so that whatever
+// waits for it has both behind it.
+enum Chain : int { kGoesOn = 1, kSecond = 2 };
+__device__ __forceinline__ void chain_start(int chain) {
+    if (chain & kGoesOn && !(chain & kSecond)) pdl_wait();
+    pdl_launch_dependents();
+    if (chain == 0) pdl_wait();
+}
+
 // Sequences with more than `few` rows (new tokens x query heads of a group), D <= 128.
-cudaError_t launch_tiles(const Call &a, int few);
+cudaError_t launch_tiles(const Call &a, int few, int chain);
 // Sequences with up to `few` rows, 8 at most; bf16 pages, D <= 128.
-cudaError_t launch_decode(const Call &a, int few);
+cudaError_t launch_decode(const Call &a, int few, int chain);
 cudaError_t decode_set_attributes();
-// CTAs of one of `units`, which share its keys: enough for two on each SM, and for no more than 4096 keys each.
+// CTAs of one of `units`, which share its keys: as many as fit the GPU at a time, two an SM, and enough for no more than 4096 keys each.
 inline unsigned ranks_of(const Call &a, long long units) {
     const int sms = attn::sm_count();
     unsigned ranks = 1;
-    while (ranks < 8 && units * ranks < 2 * sms) ranks *= 2;
+    while (ranks < 8 && units * ranks * 2 <= 2 * sms) ranks *= 2;
     const long long keys = (long long)a.c.width * a.c.page_size;
     while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
     return ranks;

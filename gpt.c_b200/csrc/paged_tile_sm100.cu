@@ -74,7 +74,6 @@ struct __align__(1024) TileSmem {
     int abort_flag;
 };
 
-enum Chain : int { kGoesOn = 1, kSecond = 2 };  // a launch that another one goes on with, and that other one
 enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_Q_READY, SITE_ALIGN, SITE_TAIL };
 
 // The sequence and tile of unit `u`, tiles counted over the sequences with more than `few` rows and no more new tokens than max_new;
@@ -145,11 +144,9 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         tma_prefetch_desc(&map_k);
         tma_prefetch_desc(&map_v);
     }
-    // The second of two launches runs beside the end of the first: the first lets it start only when what was before both has
-    // completed, and it waits for the first before it ends itself.
-    if (chain & kGoesOn) pdl_wait();
+    if (chain & kGoesOn && !(chain & kSecond)) pdl_wait();
     if (warp == 1) tmem_alloc_then_launch_dependents(&sm.tmem_base, 512);
-    if (!(chain & (kGoesOn | kSecond))) pdl_wait();
+    if (chain == 0) pdl_wait();
     if (warp == 0) {
         int seq, tile;
         const int u = unit / c.kv_heads;
@@ -573,7 +570,7 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
 }
 
 template <class T, int kDP, bool kTma>
-cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUtensorMap &v, int box) {
+cudaError_t launch_tile(const Call &a, int few, int before, const CUtensorMap &k, const CUtensorMap &v, int box) {
     using Sh = Shape<T, kDP, kTma>;
     const int G = a.heads / a.c.kv_heads, sms = attn::sm_count();
     const long long units = (long long)a.c.tokens * G / kRowsTile + a.c.seqs;
@@ -588,8 +585,8 @@ cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUte
     // What is left behind full rounds of one unit an SM, where that is less than half a round, would hold a few SMs for as long as a full
     // one: a second launch cuts each of those units among several SMs (324 units of 102 steps 225 -> XXX us).
     const int rest = (int)(all % sms);
-    if (all < sms || rest == 0 || 2 * rest > sms) return launch(0, (int)all, 0);
-    const cudaError_t e = launch(0, (int)all - rest, kGoesOn);
+    if (all < sms || rest == 0 || 2 * rest > sms) return launch(0, (int)all, before);
+    const cudaError_t e = launch(0, (int)all - rest, before | kGoesOn);
     return e != cudaSuccess ? e : launch((int)all - rest, rest, kSecond);
 }
 
@@ -602,12 +599,12 @@ int pages_map(CUtensorMap *map, const Cache &c, const void *base, int box) {
 }
 
 template <int kDP>
-cudaError_t launch_narrow(const Call &a, int few) {
+cudaError_t launch_narrow(const Call &a, int few, int chain) {
     const int box = kStep < (a.c.page_size & -a.c.page_size) ? kStep : a.c.page_size & -a.c.page_size;  // the largest power of two in the page size
     CUtensorMap k{}, v{};
     if (box < 8 || a.c.page_stride >= 1ll << 39 || pages_map(&k, a.c, a.c.k, box) != 0 || pages_map(&v, a.c, a.c.v, box) != 0)
-        return launch_tile<__nv_bfloat16, kDP, false>(a, few, k, v, 0);
-    return launch_tile<__nv_bfloat16, kDP, true>(a, few, k, v, box);
+        return launch_tile<__nv_bfloat16, kDP, false>(a, few, chain, k, v, 0);
+    return launch_tile<__nv_bfloat16, kDP, true>(a, few, chain, k, v, box);
 }
 
 template <class T, int kDP, bool kTma>
@@ -617,10 +614,10 @@ cudaError_t set_one() {
 
 }  // namespace
 
-cudaError_t launch_tiles(const Call &a, int few) {
-    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_narrow<64>(a, few) : launch_narrow<128>(a, few);
+cudaError_t launch_tiles(const Call &a, int few, int chain) {
+    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_narrow<64>(a, few, chain) : launch_narrow<128>(a, few, chain);
     const CUtensorMap none{};
-    return a.c.D <= 64 ? launch_tile<float, 64, false>(a, few, none, none, 0) : launch_tile<float, 128, false>(a, few, none, none, 0);
+    return a.c.D <= 64 ? launch_tile<float, 64, false>(a, few, chain, none, none, 0) : launch_tile<float, 128, false>(a, few, chain, none, none, 0);
 }
 
 cudaError_t tiles_set_attributes() {

@@ -109,6 +109,11 @@ struct Row {
     float max;
     double by;         // 64 log2(e) / T
 
+    // What the warps before this one have in `at`.
+    __device__ __forceinline__ u64 in_front(int warps) const {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        return warp_sum(lane < warp && lane < warps ? sm.at[lane] : 0);
+    }
     __device__ __forceinline__ void sync() const {
         if (ranks > 1) cg::this_cluster().sync();
         else __syncthreads();
@@ -165,12 +170,12 @@ struct Row {
         const u64 target = above(total);
         if (before > target || before + sm.sums[rank] <= target) return;  // not in this CTA's piece
         // the stretch in which it is, once more, by all warps
-        for (int w = 0; w < warp; w++) before += sm.at[w];
+        before += in_front(kWarps);
         if (before <= target && before + sum > target && lane == 0) sm.stretch[0] = from, sm.stretch[1] = to, sm.front = before;
         __syncthreads();
         before = sm.front;
         sum = stretch(sm.stretch[0], sm.stretch[1], from, to);
-        for (int w = 0; w < warp; w++) before += sm.at[w];
+        before += in_front(kWarps);
         if (before <= target && before + sum > target) {  // one warp
             for (int i = from + lane; i - lane < to; i += 32) {
                 const u64 run = before + warp_scan(i < to ? f(i) : 0, lane);
@@ -218,7 +223,7 @@ struct Row {
             total += sm.sums[r];
         }
         const u64 need = need_of(total);
-        for (int w = 0; w < warp; w++) run += sm.at[w];
+        run += in_front(kWarps);
         if (run < need && run + mine >= need) {  // one warp of the cluster
 #pragma unroll
             for (int j = 0; j < kBins / kThreads; j++) {
@@ -319,8 +324,7 @@ struct Row {
             const u64 scan = warp_scan(mine, lane);
             if (lane == 31) sm.at[warp] = scan;
             list_sync();
-            u64 run = before + scan - mine;
-            for (int w = 0; w < warp; w++) run += sm.at[w];
+            u64 run = before + scan - mine + in_front(kListThreads / 32);
 #pragma unroll
             for (int j = 0; j < kBins / kListThreads; j++) {
                 if (run < need && run + part[j] >= need) sm.bin = threadIdx.x * (kBins / kListThreads) + j, sm.before = run;
