@@ -104,6 +104,28 @@ __device__ __noinline__ void exact_row(const Cache &c, const float *q, const int
 }
 
 
+// One value of a row from the parts of a cluster's CTAs: with(k) gives part k's maximum, sum and value.  All are asked for before the
+// first is used: one after the other they took longer than the keys of a short context.
+struct Part {
+    float m, l, o;
+};
+template <class F>
+__device__ __forceinline__ float joined_value(int ranks, F with) {
+    Part p[8];
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) p[k] = k < ranks ? with(k) : Part{-INFINITY, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; k++) top = fmaxf(top, p[k].m);
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float by = ex2f(p[k].m - base);
+        sum = fmaf(p[k].l, by, sum), o = fmaf(p[k].o, by, o);
+    }
+    return sum == 0.f ? 0.f : o / sum;
+}
+
 struct Call {
     Cache c;
     const float *q;

@@ -71,7 +71,7 @@ struct FewSmem {
     static constexpr int kKeys = 32 / kLanes, kBatch = 4 / kChunks;  // keys of a warp at a time, and how often in a stage
     static constexpr int kStep = kKeys * kBatch * kWarps;            // keys of a stage
     uint8_t k[kStages][kStep * kWidth * sizeof(T)], v[kStages][kStep * kWidth * sizeof(T)];  // rows of D elements, one behind the other
-    Partial<kRows, kWidth> part[kWarps];
+    Partial<kRows, kWidth> part[kWarps], all;
     uint64_t full[kStages], empty[kStages];
     int holes[kStages];  // whether a key of the stage has no page
     int abort_flag;
@@ -104,7 +104,9 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
         }
         fence_barrier_init();
     }
-    chain_start(chain);
+    if (chain & kGoesOn) pdl_wait();
+    if (chain != 0) pdl_launch_dependents();
+    if (chain == 0) pdl_wait();
     const Span w = span_of(c, s);
     const int rows = w.count * G;
     if (unit % groups == 0 && kvh == 0 && rank == 0 && threadIdx.x == 0 && (w.count > max_new || (w.count > 0 && w.past < 0))) report(status, ST_ATTEND);
@@ -287,26 +289,34 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
             }
         }
     }
+    // Let the next kernel start only now: beside this one's loads its CTAs made one sequence of 1001 positions take 8.5 instead of 7.8 us.
+    if (chain == 0) pdl_launch_dependents();
     if (sm.abort_flag) __nanosleep(50000);  // let copies that are still in flight land
+    __syncthreads();
+    const int count = last - row0 + 1;
+    for (int i = threadIdx.x; i < count * c.D; i += kThreads) {
+        const int r = i / c.D, d = i - r * c.D;
+        float top = -INFINITY, sum = 0.f, o_all = 0.f;
+#pragma unroll
+        for (int x = 0; x < kWarps; x++) top = fmaxf(top, sm.part[x].m[r]);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int x = 0; x < kWarps; x++) {
+            const float by = ex2(sm.part[x].m[r] - base);
+            sum = fmaf(sm.part[x].l[r], by, sum), o_all = fmaf(sm.part[x].o[r][d], by, o_all);
+        }
+        sm.all.o[r][d] = o_all;
+        if (d == 0) sm.all.m[r] = top, sm.all.l[r] = sum;
+    }
     if (ranks > 1) cluster.sync();
     else __syncthreads();
-    if (rank == 0) {
-        for (int i = threadIdx.x; i < kRows * c.D; i += kThreads) {
-            const int r = i / c.D, d = i - r * c.D;
-            if (row0 + r > last) break;
-            float top = -INFINITY, sum = 0.f, acc = 0.f;
-            for (int k = 0; k < ranks; k++) {
-                const Partial<kRows, Smem::kWidth> *p = ranks > 1 ? cluster.map_shared_rank(&sm.part[0], k) : sm.part;
-                for (int x = 0; x < kWarps; x++) {
-                    const float mo = p[x].m[r], t2 = fmaxf(top, mo), a = weight(top, t2), b = weight(mo, t2);
-                    sum = sum * a + p[x].l[r] * b;
-                    acc = acc * a + p[x].o[r][d] * b;
-                    top = t2;
-                }
-            }
-            const int at = row0 + r;
-            out[((long long)(w.first + at / G) * heads + kvh * G + at % G) * c.D + d] = sum == 0.f ? 0.f : acc / sum;
-        }
+    // every CTA of the cluster writes some of the values
+    for (int i = rank * kThreads + threadIdx.x; i < count * c.D; i += ranks * kThreads) {
+        const int r = i / c.D, d = i - r * c.D, at = row0 + r;
+        out[((long long)(w.first + at / G) * heads + kvh * G + at % G) * c.D + d] = joined_value(ranks, [&](int k) {
+            const auto &p = ranks > 1 ? *cluster.map_shared_rank(&sm.all, k) : sm.all;
+            return Part{p.m[r], p.l[r], p.o[r][d]};
+        });
     }
     if (ranks > 1) cluster.sync();  // shared memory of the others is read until here
 }

@@ -278,14 +278,10 @@ __global__ void __launch_bounds__(kThreads, kDP == 64 ? 3 : 2) rows_kernel(Cache
     // every CTA of the cluster writes some of the values
     for (int i = rank * kThreads + threadIdx.x; i < rows * c.D; i += ranks * kThreads) {
         const int r = i / c.D, d = i - r * c.D;
-        float top = -INFINITY, sum = 0.f, o = 0.f;
-        for (int k = 0; k < ranks; k++) {
+        out[((long long)(w.first + r / G) * heads + kvh * G + r % G) * c.D + d] = joined_value(ranks, [&](int k) {
             const Smem &p = ranks > 1 ? *cluster.map_shared_rank(&sm, k) : sm;
-            const float mo = p.m_all[r], t2 = fmaxf(top, mo), base = t2 == -INFINITY ? 0.f : t2, a = ex2f(top - base), b = ex2f(mo - base);
-            sum = sum * a + p.l_all[r] * b, o = o * a + p.joined[r][d] * b;
-            top = t2;
-        }
-        out[((long long)(w.first + r / G) * heads + kvh * G + r % G) * c.D + d] = sum == 0.f ? 0.f : o / sum;
+            return Part{p.m_all[r], p.l_all[r], p.joined[r][d]};
+        });
     }
     if (ranks > 1) cluster.sync();  // shared memory of the others is read until here
 }
@@ -543,14 +539,10 @@ __global__ void __launch_bounds__(32 * kW) packed_kernel(Cache c, const float *q
     // every CTA of the cluster writes some of the values
     for (int i = rank * kT + threadIdx.x; i < rows * c.D; i += ranks * kT) {
         const int r = i / c.D, d = i - r * c.D;
-        float top = -INFINITY, sum = 0.f, o = 0.f;
-        for (int k = 0; k < ranks; k++) {
+        out[((long long)(w.first + r / G) * heads + kvh * G + r % G) * c.D + d] = joined_value(ranks, [&](int k) {
             const Smem &p = ranks > 1 ? *cluster.map_shared_rank(&sm, k) : sm;
-            const float mo = p.m_all[r], t2 = fmaxf(top, mo), base = t2 == -INFINITY ? 0.f : t2, a = ex2f(top - base), b = ex2f(mo - base);
-            sum = sum * a + p.l_all[r] * b, o = o * a + p.joined[r][d] * b;
-            top = t2;
-        }
-        out[((long long)(w.first + r / G) * heads + kvh * G + r % G) * c.D + d] = sum == 0.f ? 0.f : o / sum;
+            return Part{p.m_all[r], p.l_all[r], p.joined[r][d]};
+        });
     }
     if (ranks > 1) cluster.sync();  // shared memory of the others is read until here
 }

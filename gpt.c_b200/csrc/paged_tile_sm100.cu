@@ -548,15 +548,30 @@ __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(
         constexpr int kWords = kDP / 4;
         const int per = Sh::kThreads / kWords, word = threadIdx.x % kWords;
         for (int r = rank + ranks * (int)(threadIdx.x / kWords); r < kRowsTile && row0 + r < rows; r += ranks * per) {
-            float top = -INFINITY, sum = 0.f;
+            float sum = 0.f;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int k = 0; k < ranks; k++) {
-                const Smem &p = ranks > 1 ? *cluster.map_shared_rank(&sm, k) : sm;
-                const float mo = p.m[r], t2 = fmaxf(top, mo), base = t2 == -INFINITY ? 0.f : t2, a = ex2f(top - base), b = ex2f(mo - base);
-                const float4 v = *reinterpret_cast<const float4 *>(&p.fin.o[r][4 * word]);
-                sum = sum * a + p.l[r] * b;
-                acc = make_float4(acc.x * a + v.x * b, acc.y * a + v.y * b, acc.z * a + v.z * b, acc.w * a + v.w * b);
-                top = t2;
+            if (ranks == 1) {
+                sum = sm.l[r], acc = *reinterpret_cast<const float4 *>(&sm.fin.o[r][4 * word]);
+            } else {
+                float m_of[8], l_of[8], top = -INFINITY;
+                float4 v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {  // all asked for before the first is used
+                    m_of[k] = -INFINITY, l_of[k] = 0.f, v[k] = acc;
+                    if (k < ranks) {
+                        const Smem &p = *cluster.map_shared_rank(&sm, k);
+                        m_of[k] = p.m[r], l_of[k] = p.l[r], v[k] = *reinterpret_cast<const float4 *>(&p.fin.o[r][4 * word]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; k++) top = fmaxf(top, m_of[k]);
+                const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float by = ex2f(m_of[k] - base);
+                    sum = fmaf(l_of[k], by, sum);
+                    acc = make_float4(fmaf(v[k].x, by, acc.x), fmaf(v[k].y, by, acc.y), fmaf(v[k].z, by, acc.z), fmaf(v[k].w, by, acc.w));
+                }
             }
             const int at = row0 + r;
             const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -583,7 +598,7 @@ cudaError_t launch_tile(const Call &a, int few, int before, const CUtensorMap &k
                                                     a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, from, chain, a.status);
     };
     // What is left behind full rounds of one unit an SM, where that is less than half a round, would hold a few SMs for as long as a full
-    // one: a second launch cuts each of those units among several SMs (324 units of 102 steps 225 -> XXX us).
+    // one: a second launch cuts each of those units among several SMs (324 units of 102 steps 225 -> 202 us).
     const int rest = (int)(all % sms);
     if (all < sms || rest == 0 || 2 * rest > sms) return launch(0, (int)all, before);
     const cudaError_t e = launch(0, (int)all - rest, before | kGoesOn);
