@@ -453,3 +453,222 @@ def test_refusals(pkg):
     assert pkg.paged_attention(q[:0], *a).shape == (0, 128)  # no rows: nothing to do
     assert pkg.paged_append(qkv[:0], *a).shape == (0, 128)
     assert pkg.device_status() == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# what decides between the kernels and their forms, each with its neighbours
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("page", [1, 4, 8, 48, 64, 100, 128, 192])
+@pytest.mark.parametrize("D", [64, 72, 128])
+def test_page_sizes(pkg, D, page, dtype):
+    st = Step([150, 1, 20], [70, 131, 64], 2, 1, D, page, dtype, seed=page)
+    st.fill()
+    st.check(pkg, max_new=150)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("D", [64, 96])
+def test_every_small_number_of_rows(pkg, rows, D, dtype):
+    """As new tokens, and as query heads of one key/value head."""
+    for new, heads in ((rows, 1), (1, rows)):
+        st = Step([new, 1, new], [200, 40, 0], heads, 1, D, 16, dtype, seed=rows)
+        st.fill()
+        st.check(pkg, max_new=new)
+        st.check(pkg)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("seqs,heads,kv,D,new", [(110, 12, 12, 64, 1), (40, 12, 12, 128, 1), (110, 24, 12, 64, 1), (110, 12, 12, 48, 2), (45, 24, 12, 96, 1),
+                                                 (300, 4, 4, 64, 1), (1100, 1, 1, 64, 1)])
+def test_many_sequences(pkg, seqs, heads, kv, D, new, dtype):
+    """Enough of them for a warp each; none, one or `new` tokens, from no context to some pages."""
+    counts = [(0, 1, new, new)[i % 4] for i in range(seqs)]
+    st = Step(counts, [(i * 37) % 150 for i in range(seqs)], heads, kv, D, 16, dtype)
+    st.fill()
+    st.check(pkg, max_new=new)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_ragged_pieces(pkg, D, dtype):
+    """More sequences than the order of their lengths is looked at for, and pieces among single tokens."""
+    new = [(i * 53) % 140 + 1 if i % 3 else 1 for i in range(70)]
+    st = Step(new, [(i * 91) % 400 for i in range(70)], 4, 2, D, 32, dtype)
+    st.fill()
+    st.check(pkg, max_new=max(new))
+    st.check(pkg)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("new,past,heads", [([700], [500], 25), ([400, 300, 130], [64, 1000, 3], 25), ([128] * 12, [0] * 12, 13)])
+def test_more_units_than_sms(pkg, new, past, heads, dtype):
+    """Whole rounds of the SMs, and a rest of them that is cut into pieces."""
+    st = Step(new, past, heads, heads, 64, 16, dtype)
+    st.fill()
+    st.check(pkg, max_new=max(new))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("page,D", [(8, 64), (16, 128), (64, 64), (100, 64), (32, 40)])
+@pytest.mark.parametrize("n", [1, 6, 70])
+def test_holes(pkg, n, page, D, dtype):
+    """Pages that are not there at the beginning, inside and at the end of a context."""
+    st = Step([n, n], [330, 200], 2, 2, D, page, dtype)
+    st.fill()
+    q = st.normal(st.tokens, 2 * D)
+    lost = st.table.clone()
+    for where in ((0, 0), (0, 150 // page), (1, (200 + n - 1) // page)):
+        lost[where] = -7
+    out = pkg.paged_attention(q, st.k, st.v, lost, st.cu, st.before, max_new=n)
+    assert pkg.device_status() == 2002
+    for s in range(2):
+        k, v = st.context(s)
+        there = torch.tensor([0 <= int(lost[s, p // page]) < st.pages for p in range(k.shape[1])], device="cuda")
+        x = q[st.starts[s]:st.starts[s + 1]].double().view(n, 2, D).transpose(0, 1)
+        seen = (torch.arange(k.shape[1], device="cuda") <= st.past[s] + torch.arange(n, device="cuda")[:, None]) & there
+        z = (x @ k.transpose(1, 2) * D ** -0.5).masked_fill(~seen, float("-inf"))
+        size = (x.abs() @ k.abs().transpose(1, 2) * D ** -0.5).amax(-1, keepdim=True)
+        want = torch.softmax(z, -1) @ v
+        tol = 2 * (size * (D + 5) + k.shape[1] + 8) * E * (torch.softmax(z, -1) @ v.abs())
+        got = out[st.starts[s]:st.starts[s + 1]].double().view(n, 2, D).transpose(0, 1)
+        assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n", [2, 4, 6, 100])
+def test_a_bad_query_stays_by_itself(pkg, n, dtype):
+    st = Step([n, n], [150, 3], 2, 1, 64, 16, dtype)
+    st.fill()
+    q = st.normal(st.tokens, 128)
+    clean = st.check(pkg, q, max_new=n).clone()
+    q[1, 5], q[n, 70] = float("nan"), float("inf")
+    out = pkg.paged_attention(q, *st.args(), max_new=n)
+    for t in range(2 * n):
+        for h in range(2):
+            got, had = out[t, 64 * h:64 * h + 64], clean[t, 64 * h:64 * h + 64]
+            if (t, h) in ((1, 0), (n, 1)):
+                assert bool(got.isnan().all())
+            else:
+                assert torch.equal(got, had)
+
+
+@pytest.mark.parametrize("n", [1, 5, 100])
+def test_large_finite_values(pkg, n):
+    """fp32 keys and values as large as sums of them in fp32 allow: a weight is at most 1, so n of them times values below the largest
+    number over n stay below it.  Their terms are finite, too."""
+    st = Step([n], [70], 1, 1, 64, 16, "fp32")
+    st.fill()
+    q = st.normal(st.tokens, 64) * 1e-30  # times the scale above 2^-102: its terms are normal numbers
+    for p in range(70 + n):
+        page, row = st.where(0, p)
+        st.k[page, :, row] *= 1e29
+        st.v[page, :, row] = st.v[page, :, row].clamp(-1, 1) * (3.4e38 / (71 + n))
+    st.check(pkg, q, max_new=n)
+
+
+def test_rows_of_no_sequence_alone(pkg):
+    """A captured step of which nothing is left: no new token in any sequence, rows in the buffers all the same."""
+    for dtype in TYPES:
+        st = Step([0, 0, 0], [5, 0, 40], 2, 2, 64, 16, dtype, tail=7)
+        st.fill()
+        k0 = st.k.clone()
+        for max_new in (0, 1, 7):
+            st.check(pkg, max_new=max_new)
+        pkg.paged_append(st.normal(7, 384), *st.args())
+        assert torch.equal(st.k.nan_to_num(3.0), k0.nan_to_num(3.0))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_what_follows_a_call_waits_for_all_of_it(pkg, dtype):
+    """Calls of two launches side by side (single tokens and pieces; whole rounds and a rest), and kernels behind them that may start early."""
+    st = Step([1] * 20 + [200, 300], [500] * 22, 12, 12, 64, 16, dtype)
+    big = Step([700], [900], 25, 25, 64, 16, dtype)
+    w = st.normal(64, 12 * 64)
+    w2 = st.normal(64, 25 * 64)
+    for s, weights, m in ((st, w, 300), (big, w2, 700)):
+        s.fill()
+        q = s.normal(s.tokens, s.heads * 64)
+        out = s.check(pkg, q, max_new=m)
+        n = s.starts[-1]
+        torch.cuda.synchronize()
+        want = pkg.linear_forward(out[:n].contiguous(), weights)
+        torch.cuda.synchronize()
+        for i in range(30):
+            buf = torch.full_like(out, float(i))
+            got = pkg.linear_forward(pkg.paged_attention(q, *s.args(), max_new=m, out=buf)[:n], weights)
+            assert torch.equal(got, want)
+    # and the append that the next step's attention reads, over and over on one cache
+    qkv = st.normal(st.tokens, 3 * 12 * 64)
+    pkg.paged_append(qkv, *st.args())
+    torch.cuda.synchronize()
+    want = pkg.paged_attention(qkv[:, :768], *st.args(), max_new=300).clone()
+    n = st.starts[-1]
+    for i in range(20):
+        other = qkv + 1.0 + i
+        pkg.paged_attention(pkg.paged_append(other, *st.args()), *st.args(), max_new=300)
+        got = pkg.paged_attention(pkg.paged_append(qkv, *st.args()), *st.args(), max_new=300)
+        assert torch.equal(got[:n], want[:n])
+
+
+@pytest.mark.parametrize("stride", [2 ** 33, 2 ** 34])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_pages_very_far_apart(pkg, n, stride):
+    """The last page begins 2^33 or 2^34 elements behind the first: either side of what 32-bit places reach."""
+    if torch.cuda.mem_get_info()[0] < 50 << 30:
+        pytest.skip("needs 36 GB")
+    store = torch.empty(stride + 4 * 2 * 64 * 64, dtype=torch.bfloat16, device="cuda")
+    k = store.as_strided((2, 2, 64, 64), (stride, 64 * 64, 64, 1))
+    v = store.as_strided((2, 2, 64, 64), (stride, 64 * 64, 64, 1), 2 * 64 * 64)
+    st = Step([n], [80], 2, 2, 64, 64, "bf16", spare=0)
+    st.fill()
+    st.k.nan_to_num_(0.5), st.v.nan_to_num_(0.5)
+    k.copy_(st.k), v.copy_(st.v)
+    q = st.normal(st.tokens, 128)
+    want, tol = st.want(q)
+    got = pkg.paged_attention(q, k, v, st.table, st.cu, st.before, max_new=n)[:n]
+    assert bool(((got.double() - want).abs() <= tol).all())
+    qkv = st.normal(st.tokens, 384)
+    pkg.paged_append(qkv, k, v, st.table, st.cu, st.before)
+    pkg.paged_append(qkv, *st.args())
+    assert torch.equal(k, st.k) and torch.equal(v, st.v)
+    assert pkg.device_status() == 0
+
+
+SCRIPT = """
+import sys
+import torch
+import __graft_entry__ as entry
+
+pkg = entry.load_package()
+pkg.lib()
+n, bf16 = int(sys.argv[1]), sys.argv[2] == "bf16"
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+qkv = torch.randn(n, 384, device="cuda")
+k, v = (torch.randn(4, 2, 64, 64, device="cuda", dtype=torch.bfloat16 if bf16 else torch.float32) for _ in range(2))
+args = (k, v, ints([[2, 0, 1]]), ints([0, n]), ints([50]))
+logits, u, top_k = torch.randn(3, 50257, device="cuda"), torch.rand(3, device="cuda"), ints([5, 500, 5000])
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = pkg.paged_attention(pkg.paged_append(qkv, *args), *args, max_new=n)
+    drawn = pkg.sample(logits, u, None, top_k)
+graph.replay()
+torch.cuda.synchronize()
+again = pkg.paged_attention(pkg.paged_append(qkv, *args), *args, max_new=n)
+assert torch.equal(out, again) and torch.equal(drawn, pkg.sample(logits, u, None, top_k)) and bool(out.isfinite().all())
+assert pkg.device_status() == 0
+"""
+
+
+@pytest.mark.parametrize("n,dtype", [(1, "bf16"), (1, "fp32"), (5, "bf16"), (100, "bf16"), (100, "fp32")])
+def test_first_call_under_capture(n, dtype):
+    """The first call of a process may be one that a stream captures."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.abspath(os.path.join(os.path.dirname(__file__), ".."))
+    r = subprocess.run([sys.executable, "-c", SCRIPT, str(n), dtype], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
