@@ -77,8 +77,8 @@ struct __align__(1024) TileSmem {
 enum Site : int { SITE_KV_EMPTY = 401, SITE_KV_FULL, SITE_S_FULL, SITE_P_FULL, SITE_O_FULL, SITE_Q_READY, SITE_ALIGN, SITE_TAIL };
 
 // The sequence and tile of unit `u`, tiles counted over the sequences with more than `few` rows and no more new tokens than max_new;
-// tile -1 past the last.  Up to 32 sequences are taken in the order of falling length, and the tiles of each from its last, so that the
-// longest units begin first and the shortest fill the end.  A whole warp.  check: reports lengths that the call does not allow.
+// tile -1 past the last.  Up to 64 sequences are taken in the order of falling length (32 at a time), and the tiles of each from its last, so
+// that the longest units begin first and the shortest fill the end.  A whole warp.  check: reports lengths that the call does not allow.
 __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int max_new, int u, bool check, int *status, int &seq, int &tile) {
     const int lane = threadIdx.x & 31;
     seq = 0, tile = -1;
@@ -94,10 +94,20 @@ __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int ma
             length = w.past + w.count;
         }
         int before = 0, all = 0;  // tiles in front of this lane's
-        for (int j = 0; j < min(32, c.seqs - base); j++) {
-            const int other = __shfl_sync(0xffffffffu, tiles, j), longer = __shfl_sync(0xffffffffu, length, j);
-            before += longer > length || (longer == length && j < lane) ? other : 0;
-            all += other;
+        if (c.seqs <= 64) {
+            for (int j = 0; j < min(32, c.seqs - base); j++) {
+                const int other = __shfl_sync(0xffffffffu, tiles, j), longer = __shfl_sync(0xffffffffu, length, j);
+                before += longer > length || (longer == length && j < lane) ? other : 0;
+                all += other;
+            }
+        } else {
+            int run = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int left = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += left;
+            }
+            before = run - tiles, all = __shfl_sync(0xffffffffu, run, 31);
         }
         const uint32_t mine = __ballot_sync(0xffffffffu, u >= before && u < before + tiles);
         if (mine != 0) {
@@ -112,17 +122,19 @@ __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int ma
 }
 
 template <class T, int kDP, bool kTma>
-__global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                               int box, Cache c, const float *q, float *out, long long ld, int heads, int few, int max_new,
-                                                                         float scale_log2, int from_unit, int chain, int *status) {
+__global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1)
+tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box, Cache c, const float *q, float *out, long long ld, int heads,
+            int few, int max_new, float scale_log2, int from_unit, int chain, int *status) {
     using Sh = Shape<T, kDP, kTma>;
     using Smem = TileSmem<T, kDP, kTma>;
-    constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups, kBuffers = Sh::kBuffers, kTerms = Sh::kTerms, kSplit = Sh::kSplit, kPart = kDP / kSplit;
+    constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups;
+    constexpr int kBuffers = Sh::kBuffers, kTerms = Sh::kTerms, kSplit = Sh::kSplit, kPart = kDP / kSplit;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, unit = from_unit + (int)blockIdx.x / ranks, kvh = unit % c.kv_heads, G = heads / c.kv_heads;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+    const int unit = from_unit + (int)blockIdx.x / ranks, kvh = unit % c.kv_heads, G = heads / c.kv_heads;
     WaitCtx ctx{&sm.abort_flag, status};
     if (threadIdx.x == 0) {
         if ((smem_u32(smem_raw) & 1023u) != 0) report(status, ST_TIMEOUT_BASE + SITE_ALIGN);

@@ -434,6 +434,10 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (max_new < 0 || max_new > 0x7fffffff) return value_error("max_new must be a count, or 0 where it is not known");
     if (given && !(is(*given, at::kFloat, *q) && given->is_contiguous() && given->sizes() == q->sizes()))
         return value_error("out must be a contiguous fp32 tensor of the shape of q on the same device");
+    if (given && p.tokens) {
+        const char *a = static_cast<const char *>(q->data_ptr()), *b = static_cast<const char *>(given->data_ptr());
+        if (a < b + given->nbytes() && b < a + 4 * ((p.tokens - 1) * row_stride(*q) + q->size(1))) return value_error("out must not overlap q");
+    }
     const On on(*q, args[9]);
     if (PyErr_Occurred()) return nullptr;
     at::Tensor out = given ? *given : alloc(q->sizes(), at::kFloat, *q);

@@ -236,7 +236,7 @@ int attn_sm100_paged_append(const float *qkv, float *q_out, void *k_pages, void 
  * Attention of a step's new tokens over the pages, in which their own keys and values are already (attn_sm100_paged_append):
  *     out[t, h] = sum_{j <= past + i} softmax_j( scale * q[t, h] . k[j] ) v[j]       t the i-th new token of its sequence
  *   q       [tokens, n_heads * D] fp32, rows `ld` elements apart (a multiple of 4)
- *   out     [tokens, n_heads * D] fp32; rows of no sequence are left as they were
+ *   out     [tokens, n_heads * D] fp32, not overlapping q; rows of no sequence are left as they were
  *   max_new the largest number of new tokens that a sequence may bring (0: not known); the kernel and the size of its launch go by it
  * Scores and sums are fp32, from q in fp32 and the cache's elements as they are; the sum over the keys of weights of up to 1 times values
  * is one of them, so values above 3.4e38 over the number of keys may overflow.

@@ -436,6 +436,11 @@ def test_refusals(pkg):
     for bad in (q.double(), q[:, :100], q.view(5, 2, 64), q.t(), q.cpu(), q[:, ::2]):
         with pytest.raises(ValueError):
             pkg.paged_attention(bad, *a)
+    wide = st.normal(5, 384)
+    with pytest.raises(ValueError):  # out inside the rows of q
+        pkg.paged_attention(wide[:, 128:256], *a, out=wide.view(-1)[:640].view(5, 128))
+    with pytest.raises(ValueError):
+        pkg.paged_attention(q, *a, out=q)
     for more in ({"max_new": -1}, {"out": q[:4]}, {"out": q.double()}, {"out": torch.empty(128, 5, device="cuda").t()}):
         with pytest.raises(ValueError):
             pkg.paged_attention(q, *a, **more)
