@@ -152,11 +152,12 @@ cudaError_t launch_tiles(const Call &a, int few, int chain);
 // Sequences with up to `few` rows, 8 at most; bf16 pages, D <= 128.
 cudaError_t launch_decode(const Call &a, int few, int chain);
 cudaError_t decode_set_attributes();
-// CTAs of one of `units`, which share its keys: as many as fit the GPU at a time, two an SM, and enough for no more than 4096 keys each.
+// CTAs of one of `units`, which share its keys: as many as fit the GPU at a time, two an SM and a few more (160 units of up to 2000 keys, 4
+// rows: 50 us with one, 36 with two each), and enough for no more than 4096 keys each.
 inline unsigned ranks_of(const Call &a, long long units) {
     const int sms = attn::sm_count();
     unsigned ranks = 1;
-    while (ranks < 8 && units * ranks * 2 <= 2 * sms) ranks *= 2;
+    while (ranks < 8 && units * ranks * 2 <= 5 * sms / 2) ranks *= 2;
     const long long keys = (long long)a.c.width * a.c.page_size;
     while (ranks < 8 && keys / ranks > 4096) ranks *= 2;
     return ranks;
