@@ -47,7 +47,7 @@ __device__ __forceinline__ Span span_of(const Cache &c, int s) {
     Span w;
     w.first = min(max(c.cu[s], 0), c.tokens);
     w.count = min(max(c.cu[s + 1], w.first), c.tokens) - w.first;
-    w.past = c.past[s];
+    w.past = min(c.past[s], 0x7ffffffe - w.count);  // positions stay 32-bit numbers, beyond any page table if they were
     return w;
 }
 

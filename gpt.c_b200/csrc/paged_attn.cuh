@@ -137,20 +137,10 @@ struct Call {
     cudaStream_t s;
 };
 
-// Launches that share nothing run side by side: one that another goes on with (kGoesOn) lets it start only when what was before both has
-// completed, and that other one (kSecond) does not wait at its start, but for the first before it ends, so that whatever
-// waits for it has both behind it.
-enum Chain : int { kGoesOn = 1, kSecond = 2 };
-__device__ __forceinline__ void chain_start(int chain) {
-    if (chain & kGoesOn && !(chain & kSecond)) pdl_wait();
-    pdl_launch_dependents();
-    if (chain == 0) pdl_wait();
-}
-
 // Sequences with more than `few` rows (new tokens x query heads of a group), D <= 128.
-cudaError_t launch_tiles(const Call &a, int few, int chain);
+cudaError_t launch_tiles(const Call &a, int few);
 // Sequences with up to `few` rows, 8 at most; bf16 pages, D <= 128.
-cudaError_t launch_decode(const Call &a, int few, int chain);
+cudaError_t launch_decode(const Call &a, int few);
 cudaError_t decode_set_attributes();
 // CTAs of one of `units`, which share its keys: as many as fit the GPU at a time, two an SM and a few more (160 units of up to 2000 keys, 4
 // rows: 50 us with one, 36 with two each), and enough for no more than 4096 keys each.

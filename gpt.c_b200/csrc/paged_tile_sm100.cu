@@ -16,6 +16,9 @@
 // are joined at the end, and three score buffers, so that a group finds its next scores when it has done with one step (with two
 // buffers S of step n+2 had to wait for P V of step n, and a step took 1430 cycles).
 //
+// 3380 new tokens of sequences of up to 8024 positions, 12 heads of 64, bf16: 203 us, a step 1200 cycles, bound by the softmax warps'
+// instructions (63 % of issue slots; tensor pipe 64 %).  2048 new tokens, 25 heads of 64, fp32: 60 us, short units, start and end.
+//
 // A row whose result is not finite is computed again in fp32 arithmetic: 0 times an infinite value that the row does
 // not see is NaN on the tensor cores, and so are the terms of an infinity.
 #include <cooperative_groups.h>
@@ -124,7 +127,7 @@ __device__ __forceinline__ void find_tile(const Cache &c, int G, int few, int ma
 template <class T, int kDP, bool kTma>
 __global__ void __launch_bounds__(Shape<T, kDP, kTma>::kThreads, 1)
 tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, int box, Cache c, const float *q, float *out, long long ld, int heads,
-            int few, int max_new, float scale_log2, int from_unit, int chain, int *status) {
+            int few, int max_new, float scale_log2, int whole, int *status) {
     using Sh = Shape<T, kDP, kTma>;
     using Smem = TileSmem<T, kDP, kTma>;
     constexpr int kK = kDP / 16, kStages = Sh::kStages, kPlane = Sh::kPlane, kGroups = Sh::kGroups;
@@ -132,9 +135,11 @@ tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     Smem &sm = *reinterpret_cast<Smem *>(smem_raw);
     cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int size = (int)cluster.num_blocks(), which = (int)blockIdx.x / size;
+    const bool alone = which * size < whole;  // the first `whole` units have a CTA each, the others a cluster
+    const int ranks = alone ? 1 : size, rank = alone ? 0 : (int)cluster.block_rank();
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-    const int unit = from_unit + (int)blockIdx.x / ranks, kvh = unit % c.kv_heads, G = heads / c.kv_heads;
+    const int unit = alone ? (int)blockIdx.x : whole + which - whole / size, kvh = unit % c.kv_heads, G = heads / c.kv_heads;
     WaitCtx ctx{&sm.abort_flag, status};
     if (threadIdx.x == 0) {
         if ((smem_u32(smem_raw) & 1023u) != 0) report(status, ST_TIMEOUT_BASE + SITE_ALIGN);
@@ -156,9 +161,8 @@ tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         tma_prefetch_desc(&map_k);
         tma_prefetch_desc(&map_v);
     }
-    if (chain & kGoesOn && !(chain & kSecond)) pdl_wait();
     if (warp == 1) tmem_alloc_then_launch_dependents(&sm.tmem_base, 512);
-    if (chain == 0) pdl_wait();
+    pdl_wait();
     if (warp == 0) {
         int seq, tile;
         const int u = unit / c.kv_heads;
@@ -593,28 +597,31 @@ tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
         }
         if (ranks > 1) cluster.sync();  // shared memory of the others is read until here
     }
-    if (chain & kSecond) pdl_wait();
 }
 
 template <class T, int kDP, bool kTma>
-cudaError_t launch_tile(const Call &a, int few, int before, const CUtensorMap &k, const CUtensorMap &v, int box) {
+cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUtensorMap &v, int box) {
     using Sh = Shape<T, kDP, kTma>;
     const int G = a.heads / a.c.kv_heads, sms = attn::sm_count();
     const long long units = (long long)a.c.tokens * G / kRowsTile + a.c.seqs;
     const long long all = units * a.c.kv_heads;
     if (all > 0x7fffffffll / 8) return cudaErrorInvalidConfiguration;
-    auto launch = [&](int from, int count, int chain) {
-        unsigned ranks = 1;
-        while (ranks < 8 && (long long)count * ranks * 2 <= (chain & kSecond ? 2 : 1) * sms) ranks *= 2;  // few units share their keys among the SMs that are left
-        return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)count * ranks), dim3(Sh::kThreads), sizeof(TileSmem<T, kDP, kTma>), ranks,
-                                                    a.s, k, v, box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, from, chain, a.status);
-    };
     // What is left behind full rounds of one unit an SM, where that is less than half a round, would hold a few SMs for as long as a full
-    // one: a second launch cuts each of those units among several SMs (324 units of 102 steps 225 -> 202 us).
+    // one: those units, the shortest, are shared by two CTAs each, the others taken by one (324 units of up to 126 steps: 204 us without,
+    // 182 so, 207 with clusters of four, of which fewer fit the GPU).
     const int rest = (int)(all % sms);
-    if (all < sms || rest == 0 || 2 * rest > sms) return launch(0, (int)all, before);
-    const cudaError_t e = launch(0, (int)all - rest, before | kGoesOn);
-    return e != cudaSuccess ? e : launch((int)all - rest, rest, kSecond);
+    unsigned ranks = 1;
+    int whole = 0;
+    if (all < sms) {
+        while (ranks < 8 && all * ranks * 2 <= sms) ranks *= 2;  // few units share their keys among the SMs that are left
+    } else if (rest != 0 && 2 * rest <= sms) {
+        ranks = 2;
+        whole = (int)all - rest;
+        whole -= whole % ranks;
+    }
+    const long long ctas = whole + (all - whole) * ranks;
+    return attn::launch_clusters_after_previous(tile_kernel<T, kDP, kTma>, dim3((unsigned)ctas), dim3(Sh::kThreads), sizeof(TileSmem<T, kDP, kTma>), ranks, a.s, k, v,
+                                                box, a.c, a.q, a.out, a.ld, a.heads, few, a.max_new, a.scale_log2, whole, a.status);
 }
 
 // Pages as a map {D, rows of a page, heads, pages}, boxes of 64 columns by `box` rows; columns past the D-th read as zeros.
@@ -626,12 +633,12 @@ int pages_map(CUtensorMap *map, const Cache &c, const void *base, int box) {
 }
 
 template <int kDP>
-cudaError_t launch_narrow(const Call &a, int few, int chain) {
+cudaError_t launch_narrow(const Call &a, int few) {
     const int box = kStep < (a.c.page_size & -a.c.page_size) ? kStep : a.c.page_size & -a.c.page_size;  // the largest power of two in the page size
     CUtensorMap k{}, v{};
     if (box < 8 || a.c.page_stride >= 1ll << 39 || pages_map(&k, a.c, a.c.k, box) != 0 || pages_map(&v, a.c, a.c.v, box) != 0)
-        return launch_tile<__nv_bfloat16, kDP, false>(a, few, chain, k, v, 0);
-    return launch_tile<__nv_bfloat16, kDP, true>(a, few, chain, k, v, box);
+        return launch_tile<__nv_bfloat16, kDP, false>(a, few, k, v, 0);
+    return launch_tile<__nv_bfloat16, kDP, true>(a, few, k, v, box);
 }
 
 template <class T, int kDP, bool kTma>
@@ -641,10 +648,10 @@ cudaError_t set_one() {
 
 }  // namespace
 
-cudaError_t launch_tiles(const Call &a, int few, int chain) {
-    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_narrow<64>(a, few, chain) : launch_narrow<128>(a, few, chain);
+cudaError_t launch_tiles(const Call &a, int few) {
+    if (a.type == ATTN_CACHE_BF16) return a.c.D <= 64 ? launch_narrow<64>(a, few) : launch_narrow<128>(a, few);
     const CUtensorMap none{};
-    return a.c.D <= 64 ? launch_tile<float, 64, false>(a, few, chain, none, none, 0) : launch_tile<float, 128, false>(a, few, chain, none, none, 0);
+    return a.c.D <= 64 ? launch_tile<float, 64, false>(a, few, none, none, 0) : launch_tile<float, 128, false>(a, few, none, none, 0);
 }
 
 cudaError_t tiles_set_attributes() {

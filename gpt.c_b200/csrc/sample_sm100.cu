@@ -13,6 +13,8 @@
 // weights over 2048 steps of max - x, and the classes of the step in which it ends are put in order by comparing
 // each with each; where they are too many for that, the histogram is taken again over their keys, 2048 times finer each time.
 //
+// Bound by the joins of a row's phases, not by HBM: 1 row of 50257, top-k 40, 10.1 us; 96 rows, top-p and min-p, 20.9 us; 500 rows, top-k 1000 and
+// top-p, 94 us (three rounds of a row an SM), where reading takes 15.
 #include <cooperative_groups.h>
 
 #include <type_traits>

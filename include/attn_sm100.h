@@ -224,7 +224,7 @@ int attn_sm100_device_status(int *status, int clear);
  *   rotary NULL, or [positions, rotary_dim] fp32: for each position rotary_dim / 2 cosines and as many sines.  The first
  *          rotary_dim columns (even, up to D) of every query and key head are rotated in pairs, (a, b) to
  *          (a cos - b sin, b cos + a sin): columns i and i + rotary_dim / 2, or 2i and 2i + 1 with rotary_pairs not 0
- *   q_out  [tokens, n_heads * D] fp32: the rotated queries; may be NULL, and is not written, without `rotary`
+ *   q_out  [tokens, n_heads * D] fp32: the rotated queries, not overlapping qkv; may be NULL, and is not written, without `rotary`
  * Values are rounded to the cache's type once, to nearest.
  */
 int attn_sm100_paged_append(const float *qkv, float *q_out, void *k_pages, void *v_pages, const int *page_table, const int *cu_seqlens,
