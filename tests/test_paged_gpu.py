@@ -338,6 +338,41 @@ def test_pages_that_are_not_there(pkg, n):
     assert pkg.device_status() == 2002 and bool((out == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n,D", [(1, 64), (3, 64), (40, 64), (300, 64), (3, 136)])
+@pytest.mark.parametrize("past", [2 ** 31 - 1, 2 ** 31 - 20, 2 ** 30, 81])
+def test_positions_behind_the_table(pkg, past, n, D, dtype):
+    """Every new token lies behind the page table: none is stored, each sees the keys that the table has room for."""
+    st = Step([n], [80], 2, 1, D, 16, dtype, tail=0)
+    st.table = st.table[:, :5].contiguous()  # room for 80 positions
+    st.fill([80])
+    q = st.normal(n, 2 * D)
+    before = ints([past])
+    k, v = st.k.clone(), st.v.clone()
+    pkg.paged_append(st.normal(n, 4 * D), st.k, st.v, st.table, st.cu, before)
+    assert pkg.device_status() == 2001
+    assert torch.equal(st.k.nan_to_num(), k.nan_to_num()) and torch.equal(st.v.nan_to_num(), v.nan_to_num())
+    got = pkg.paged_attention(q, st.k, st.v, st.table, st.cu, before, max_new=n)
+    assert pkg.device_status() == 2002
+    st.new, st.past, st.starts = [1] * n, [79] * n, list(range(n + 1))  # the same as n sequences that share those pages
+    st.table = st.table.repeat(n, 1)
+    want, tol = st.want(q)
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
+def test_under_inference_mode(pkg):
+    """As a program that generates would call them, with tensors made there."""
+    with torch.inference_mode():
+        st = Step([1, 9], [30, 2], 2, 2, 64, 16, "bf16", tail=0)
+        st.fill([30, 2])
+        qkv = st.normal(st.tokens, 3 * 128)
+        q = pkg.paged_append(qkv, *st.args())
+        assert torch.equal(q, qkv[:, :128]) and q.data_ptr() == qkv.data_ptr()
+        st.check(pkg, q, max_new=9)
+        logits = st.normal(3, 1000)
+        assert torch.equal(pkg.sample(logits, torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda")), logits.argmax(1).int())
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_offsets_beyond_32_bits(pkg, n):
     """Pages of a cache of more than 2^32 bytes and 2^31 elements, of which only the last ones are used."""
