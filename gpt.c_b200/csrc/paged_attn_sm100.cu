@@ -360,9 +360,15 @@ cudaError_t set_rows() {
     return e;
 }
 // Sequences of few rows go to the kernels that read their keys at the HBM rate, the others to the tile kernel; all find
-// their own sequences on the device, so a step that mixes them takes two launches.
+// their own sequences on the device, so a step may mix them.  Two launches, one behind the other, for such a step only where there are more
+// sequences x key/value heads than the tile kernel takes in two rounds or so, or long contexts, which it would walk with one CTA each:
+// 32 single tokens and two pieces of up to 500, 5 heads of 128 for 20: 71 us with the tile kernel alone, 86 with both; 64 single tokens
+// 115 / 137, 128 of them 165 / 163; 32 of them with 12 heads of 64 76 / 74, 24 55 / 72, 64 125 / 110; fp32, 170 units 178 / 222, 330 319 / 298.
+// And where there are few rows on average: a step of single tokens whose program does not give max_new.
 constexpr int kFewRows16 = 8, kFewRows32 = 4;
-constexpr int kMeanRows = 128;  // from this many rows a sequence on, on average, the tile kernel takes all of them in one launch
+constexpr int kMeanRows = 128;             // from this many rows a sequence on, on average, the tile kernel takes all of them in any case
+constexpr int kUnits16 = 5, kUnits32 = 4;  // halves of a round of the SMs
+constexpr long long kShort = 8192;         // positions that the page table has room for
 
 cudaError_t forward(const Call &a) {
     const bool narrow = a.type == ATTN_CACHE_BF16 && a.c.D <= 128;
@@ -372,7 +378,9 @@ cudaError_t forward(const Call &a) {
     if (a.c.D > 128) return launch_few_rows(0x7fffffff);
     const bool far = narrow && a.c.pages * a.c.page_stride > 1ll << 34;  // beyond that kernel's 32-bit places: the tile kernel takes all
     if (most <= limit && !far) return launch_few_rows(limit);
-    const bool both = !far && G <= limit && a.c.tokens * G < (long long)kMeanRows * a.c.seqs;
+    const bool one = a.c.tokens * G > (long long)limit * a.c.seqs && (long long)a.c.width * a.c.page_size <= kShort &&
+                     2ll * a.c.seqs * a.c.kv_heads <= (narrow ? kUnits16 : kUnits32) * attn::sm_count();
+    const bool both = !far && !one && G <= limit && a.c.tokens * G < (long long)kMeanRows * a.c.seqs;
     if (both) {
         const cudaError_t e = launch_few_rows(limit);
         if (e != cudaSuccess) return e;

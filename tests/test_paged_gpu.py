@@ -232,6 +232,18 @@ def test_many_new_tokens(pkg, new, past, heads, kv, D, page, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("new,past,heads,kv,D", [([1] * 20 + [40], [17 * i for i in range(21)], 2, 2, 64), ([1, 30], [9000, 10], 4, 2, 64),
+                                                 ([1, 3, 0, 200] + [1] * 34, [5 + 11 * i for i in range(38)], 12, 12, 64),
+                                                 ([1, 100, 1], [200, 0, 64], 4, 1, 128), ([2, 60, 1], [63, 128, 700], 5, 5, 40)])
+@pytest.mark.parametrize("known", [False, True])
+def test_single_tokens_beside_pieces(pkg, known, new, past, heads, kv, D, dtype):
+    """One kernel or two, by the number of sequences, their lengths and the rows they have on average."""
+    st = Step(new, past, heads, kv, D, 16, dtype)
+    st.fill()
+    st.check(pkg, max_new=max(new) if known else 0)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 @pytest.mark.parametrize("new,past,heads,kv,D", [([1], [30011], 4, 1, 64), ([1, 1], [9000, 17], 2, 2, 128), ([40], [9001], 3, 1, 64), ([3, 150], [5000, 2500], 2, 1, 128)])
 def test_long_contexts(pkg, new, past, heads, kv, D, dtype):
     st = Step(new, past, heads, kv, D, 64, dtype)
