@@ -362,7 +362,7 @@ cudaError_t set_rows() {
 // Sequences of few rows go to the kernels that read their keys at the HBM rate, the others to the tile kernel; all find
 // their own sequences on the device, so a step may mix them.  Two launches, one behind the other, for such a step only where there are more
 // sequences x key/value heads than the tile kernel takes in two rounds or so, or long contexts, which it would walk with one CTA each:
-// 32 single tokens and two pieces of up to 500, 5 heads of 128 for 20: 71 us with the tile kernel alone, 86 with both; 64 single tokens
+// 32 single tokens and two pieces of up to 500, 5 heads of 128 for 20, short bursts: 71 us with the tile kernel alone, 86 with both; 64 single tokens
 // 115 / 137, 128 of them 165 / 163; 32 of them with 12 heads of 64 76 / 74, 24 55 / 72, 64 125 / 110; fp32, 170 units 178 / 222, 330 319 / 298.
 // And where there are few rows on average: a step of single tokens whose program does not give max_new.
 constexpr int kFewRows16 = 8, kFewRows32 = 4;

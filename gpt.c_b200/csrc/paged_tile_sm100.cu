@@ -16,7 +16,7 @@
 // are joined at the end, and three score buffers, so that a group finds its next scores when it has done with one step (with two
 // buffers S of step n+2 had to wait for P V of step n, and a step took 1430 cycles).
 //
-// 3380 new tokens of sequences of up to 8024 positions, 12 heads of 64, bf16: 181 us, a step 1200 cycles, bound by the softmax warps'
+// 3380 new tokens of sequences of up to 8024 positions, 12 heads of 64, bf16: 213 us, a step 1200 cycles, bound by the softmax warps'
 // instructions (63 % of issue slots; tensor pipe 64 %).  2048 new tokens, 25 heads of 64, fp32: 60 us, short units, start and end.
 //
 // A row whose result is not finite is computed again in fp32 arithmetic: 0 times an infinite value that the row does
@@ -607,8 +607,8 @@ cudaError_t launch_tile(const Call &a, int few, const CUtensorMap &k, const CUte
     const long long all = units * a.c.kv_heads;
     if (all > 0x7fffffffll / 8) return cudaErrorInvalidConfiguration;
     // What is left behind full rounds of one unit an SM, where that is less than half a round, would hold a few SMs for as long as a full
-    // one: those units, the shortest, are shared by two CTAs each, the others taken by one (324 units of up to 126 steps: 204 us without,
-    // 182 so, 207 with clusters of four, of which fewer fit the GPU).
+    // one: those units, the shortest, are shared by two CTAs each, the others taken by one (324 units of up to 126 steps: 228 us without,
+    // 213 so; in short bursts of calls 204, 182, and 207 with clusters of four, of which fewer fit the GPU).
     const int rest = (int)(all % sms);
     unsigned ranks = 1;
     int whole = 0;
