@@ -474,6 +474,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
     const int ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank(), row = blockIdx.x / ranks;
     constexpr int kWarps = kThreads / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (ranks > 1) tc05::cluster_arrive();  // waited for behind the loads
     if (threadIdx.x < 64) sm.powers[threadIdx.x] = exp2((double)threadIdx.x / 64);
     tc05::pdl_launch_dependents();
     tc05::pdl_wait();
@@ -516,6 +517,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const float *logits, c
     if (lane == 0) most[warp] = own;
     if (threadIdx.x == 0) sm.first = 0x7fffffff;
     __syncthreads();
+    if (ranks > 1) tc05::cluster_wait();  // the other CTAs have begun: their shared memory is there
     if (warp == 0) {
         const float2 all = both(most[lane % kWarps]);
         if (lane < ranks) *r.there(&sm.range[rank], lane) = all;
