@@ -383,6 +383,7 @@ tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ C
                     *reinterpret_cast<uint4 *>(at + 2 * kPlane) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             const uint32_t rows4 = __ballot_sync(0xffffffffu, have);
+            __syncwarp();  // lane 0 arrives for what all lanes have stored
             if (lane == 0) {
                 sm.nibble[n % kStages][mine >> 5] = (uint8_t)((rows4 & 1) | (rows4 >> 7 & 2) | (rows4 >> 14 & 4) | (rows4 >> 21 & 8));
                 mbar_arrive(&sm.kv_full[n % kStages]);
