@@ -12,6 +12,8 @@
 // 1001 positions, 12 heads of 64: 6.4 us, the chain past -> page table -> page -> sums -> join; its 6 MB alone would take 0.9.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "attn24.cuh"
 #include "attn_internal.h"
 #include "paged.cuh"
@@ -218,46 +220,58 @@ __global__ void __launch_bounds__(kThreads) few_rows_kernel(Cache c, const float
                     for (int x = kLanes / 2; x > 0; x >>= 1) sc[u][r] += __shfl_xor_sync(0xffffffffu, sc[u][r], x);
                 }
             }
+            // A key without weight (not there, not seen, or with a score of -inf) may have any value, and 0 times that need not be 0.
+            auto add_up = [&](auto careful) {
+                uint32_t without = 0;  // bit kBatch r + u
 #pragma unroll
-            for (int r = 0; r < kRows; r++) {
-                float top = m[r];
-                if (!whole) {
+                for (int r = 0; r < kRows; r++) {
+                    if (careful) {
 #pragma unroll
-                    for (int u = 0; u < kBatch; u++)
-                        if (!there[u] || j0 + u * kKeys >= seen[r]) sc[u][r] = -INFINITY;
+                        for (int u = 0; u < kBatch; u++) {
+                            if (!there[u] || j0 + u * kKeys >= seen[r]) sc[u][r] = -INFINITY;
+                            without |= (sc[u][r] == -INFINITY ? 1u : 0u) << (kBatch * r + u);
+                        }
+                    }
+                    float top = m[r];
+#pragma unroll
+                    for (int u = 0; u < kBatch; u++) top = fmaxf(top, sc[u][r]);
+                    const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[r] - base);  // nothing has weight yet
+                    m[r] = top;
+                    l[r] *= keep;
+#pragma unroll
+                    for (int ch = 0; ch < kChunks; ch++)
+#pragma unroll
+                        for (int e = 0; e < kPairs; e++) o[r][ch][e] = mul2(o[r][ch][e], make_float2(keep, keep));
+#pragma unroll
+                    for (int u = 0; u < kBatch; u++) {
+                        sc[u][r] = ex2(sc[u][r] - base);
+                        l[r] += sc[u][r];
+                    }
                 }
 #pragma unroll
-                for (int u = 0; u < kBatch; u++) top = fmaxf(top, sc[u][r]);
-                const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[r] - base);  // nothing has weight yet
-                m[r] = top;
-                l[r] *= keep;
+                for (int u = 0; u < kBatch; u++)
 #pragma unroll
-                for (int ch = 0; ch < kChunks; ch++)
+                    for (int ch = 0; ch < kChunks; ch++) {
+                        const int d = (ch * kLanes + sub) * kN;
+                        uint4 word = make_uint4(0, 0, 0, 0);
+                        if ((!careful || there[u]) && d < c.D) word = *reinterpret_cast<const uint4 *>(sm.v[st] + at + u * kKeys * row_bytes + d * (int)sizeof(T));
+                        float2 f[kPairs];
+                        Words<T>::open(word, f);
 #pragma unroll
-                    for (int e = 0; e < kPairs; e++) o[r][ch][e] = mul2(o[r][ch][e], make_float2(keep, keep));
+                        for (int r = 0; r < kRows; r++) {
+                            if (careful && (without >> (kBatch * r + u) & 1u)) continue;
 #pragma unroll
-                for (int u = 0; u < kBatch; u++) {
-                    sc[u][r] = ex2(sc[u][r] - base);
-                    l[r] += sc[u][r];
-                }
-            }
+                            for (int e = 0; e < kPairs; e++) o[r][ch][e] = fma2(make_float2(sc[u][r], sc[u][r]), f[e], o[r][ch][e]);
+                        }
+                    }
+            };
+            float low = INFINITY;
 #pragma unroll
             for (int u = 0; u < kBatch; u++)
 #pragma unroll
-                for (int ch = 0; ch < kChunks; ch++) {
-                    const int d = (ch * kLanes + sub) * kN;
-                    uint4 word = make_uint4(0, 0, 0, 0);
-                    if (there[u] && d < c.D) word = *reinterpret_cast<const uint4 *>(sm.v[st] + at + u * kKeys * row_bytes + d * (int)sizeof(T));
-                    float2 f[kPairs];
-                    Words<T>::open(word, f);
-#pragma unroll
-                    for (int r = 0; r < kRows; r++) {
-                        // a value that the row does not see may be anything, and 0 times it not 0
-                        if (kRows > 1 && !whole && sc[u][r] == 0.f) continue;
-#pragma unroll
-                        for (int e = 0; e < kPairs; e++) o[r][ch][e] = fma2(make_float2(sc[u][r], sc[u][r]), f[e], o[r][ch][e]);
-                    }
-                }
+                for (int r = 0; r < kRows; r++) low = fminf(low, sc[u][r]);
+            if (whole && low > -INFINITY) add_up(std::false_type{});
+            else add_up(std::true_type{});
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.empty[st]);
         }
