@@ -240,19 +240,21 @@ def layernorm_backward(dy, x, mean, rstd, w, dw, db, dx, stream=None) -> None:
 #
 # A layer's cache is k_pages and v_pages [pages, kv_heads, page_size, head_size], fp32 or bf16.  A step brings rows of several
 # sequences, one behind the other: page_table [sequences, pages], cu_seqlens [sequences + 1] (first row of each, and the
-# end) and past [sequences] (positions before the step) are int32 tensors beside them.
+# end) and past [sequences] (positions before the step) are int32 tensors beside them.  These calls are not differentiable:
+# their results are cut off from autograd, whatever their arguments require.
 # ---------------------------------------------------------------------------------------------
 def paged_append(qkv, k_pages, v_pages, page_table, cu_seqlens, past, rotary=None, rotary_pairs: bool = False, stream=None):
     """Stores the keys and values of qkv [tokens, (n_heads + 2 kv_heads) * head_size] in their sequences' pages and returns the
     queries [tokens, n_heads * head_size]: a view of qkv, or with `rotary` (see rotary_table) a tensor of queries rotated by
-    their positions, as the stored keys are.  Columns i and i + R/2 of a head make a pair, or 2i and 2i + 1 with rotary_pairs."""
+    their positions, as the stored keys are.  Columns i and i + R/2 of a head make a pair, or 2i and 2i + 1 with rotary_pairs.
+    Not differentiable."""
     return _calls().paged_append(qkv, k_pages, v_pages, page_table, cu_seqlens, past, rotary, rotary_pairs, _raw(stream))
 
 
 def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, past, max_new: int = 0, scale=None, out=None, stream=None):
     """Causal attention of q [tokens, n_heads * head_size] over the pages, the new tokens' own keys among them.  `max_new`: the
     largest number of new tokens of a sequence, 0 where the program does not know it; `scale`: head_size ** -0.5 if None.
-    Rows behind the last sequence are not written."""
+    Rows behind the last sequence are not written.  Not differentiable."""
     return _calls().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, past, max_new, scale, out, _raw(stream))
 
 

@@ -374,9 +374,9 @@ struct Pages {
     }
 };
 
-// x[:, :columns], without a trip through the dispatcher (a quarter of the time of a small append).
+// x[:, :columns] cut off from autograd, as every result here is: no gradient could come back for the keys and values beside
+// them.  Without a trip through the dispatcher (a quarter of the time of a small append).
 at::Tensor first_columns(const at::Tensor &x, int64_t columns) {
-    if (x.requires_grad()) return x.narrow(1, 0, columns);
     const c10::TensorImpl *impl = x.unsafeGetTensorImpl();
     auto view = impl->shallow_copy_and_detach(impl->version_counter(), true);
     const int64_t sizes[2] = {x.size(0), columns}, strides[2] = {x.stride(0), x.stride(1)};

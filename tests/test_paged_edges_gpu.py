@@ -50,3 +50,19 @@ def test_infinite_values_of_small_weight_count(pkg, new, past, heads, kv, D, dty
     out = pkg.paged_attention(q, *st.args(), max_new=max(new))[:st.starts[-1]].view(-1, heads, D)
     assert not bool(out[:, :, 3].isfinite().any())
     assert bool(out[:, :, 4:].isfinite().all()) and bool(out[:, :, :3].isfinite().all())
+
+
+@pytest.mark.parametrize("rotary", [0, 64])
+def test_queries_are_cut_off_from_autograd(pkg, rotary):
+    """No call of generation is differentiable, with and without rotation: no gradient reaches the queries alone."""
+    from test_paged_gpu import Step
+
+    st = Step([2, 5], [30, 0], 2, 2, 64, 16, "bf16", tail=0)
+    qkv = st.normal(st.tokens, 3 * 128).requires_grad_()
+    q = pkg.paged_append(qkv, *st.args(), rotary=pkg.rotary_table(40, rotary) if rotary else None)
+    assert not q.requires_grad and q.grad_fn is None
+    if not rotary:
+        assert q.data_ptr() == qkv.data_ptr() and torch.equal(q, qkv.detach()[:, :128])
+    st.fill()
+    out = pkg.paged_attention(st.normal(st.tokens, 128).requires_grad_(), *st.args(), max_new=5)
+    assert not out.requires_grad
