@@ -742,5 +742,5 @@ extern "C" int xent_sm100_sample(const float *logits, const float *u, const floa
     return (int)attn::launch_clusters_after_previous(alone ? sample::sample_kernel<1024> : sample::sample_kernel<512>, dim3((unsigned)rows * ranks),
                                                      dim3(alone ? 1024 : 512), sample::smem_bytes(words), (unsigned)ranks, static_cast<cudaStream_t>(stream),
                                                      logits, u, temperature, top_k, top_p, min_p, tokens, ld, rows, C, words,
-                                                     alone && C > 3 ? attn::sm_count() * (int)(200000 / sample::smem_bytes(words) + 1) : 0);
+                                                     alone && C > 3 ? attn::sm_count() : 0);  // 1024 threads of 64 registers: one CTA an SM
 }
