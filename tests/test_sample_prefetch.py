@@ -11,7 +11,7 @@ HERE = os.path.join(os.path.dirname(__file__), "..", "gpt.c_b200")
 def test_the_row_that_comes_next():
     text = open(os.path.join(HERE, "csrc", "sample_sm100.cu")).read()
     assert "row + ahead < rows" in text
-    distance = re.search(r"alone && C > 3 \? ([^:]*) : 0\);", text).group(1)
+    distance = re.search(r"alone && C > 3 \? (.*) : 0\);", text).group(1)
     assert distance == "attn::sm_count()"
 
 
