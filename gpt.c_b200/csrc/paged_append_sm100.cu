@@ -6,8 +6,8 @@
 //
 // Bound by HBM for a prefill step and by the chain of loads cu -> past -> table -> store for a decoding step.  A warp
 // takes 32 * kUnits units of 8 columns of one token: it asks for its part of the row before it looks for the sequence, so
-// that chain and data travel together.  10920 tokens of 20 + 2 x 5 heads of 128, rotated, bf16 pages: 54 us, 5.8 TB/s of reads and writes;
-// 24 tokens of 3 x 12 heads of 64: 3.3 us, little more than a launch.
+// that chain and data travel together.  10920 tokens of 20 + 2 x 5 heads of 128, rotated, bf16 pages: 54 to 57 us, 5.5 to 5.8 TB/s of reads
+// and writes, from GPU to GPU; 24 tokens of 3 x 12 heads of 64: 3.3 to 3.7 us, little more than a launch.
 #include "attn_internal.h"
 #include "paged.cuh"
 #include "tc05.cuh"

@@ -9,7 +9,10 @@
 // of lanes keeps a running maximum, sum and output of its own for its keys, in fp32 and in registers, and they are joined
 // only at the end: over the lanes by shuffles, over the warps in shared memory, over the cluster through distributed shared
 // memory.  No atomics, no scratch buffer; the order of every sum is fixed.  One sequence of
-// 1001 positions, 12 heads of 64: 6.4 us, the chain past -> page table -> page -> sums -> join; its 6 MB alone would take 0.9.
+// 1001 positions, 12 heads of 64: 6.5 us, the chain past -> page table -> page -> sums -> join; its 6 MB alone would take 0.9.
+//
+// Stages in which a key has no weight for one of the rows (not seen, no page, a score of -inf) leave such keys out one by one, in code of
+// their own; with the checks among the other stages' instructions six contexts of 20000 and more, 4 rows, heads of 128, took 185 us, so 177.
 #include <cooperative_groups.h>
 
 #include <type_traits>

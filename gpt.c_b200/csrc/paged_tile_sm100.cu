@@ -17,7 +17,7 @@
 // buffers S of step n+2 had to wait for P V of step n, and a step took 1430 cycles).
 //
 // 3380 new tokens of sequences of up to 8024 positions, 12 heads of 64, bf16: 213 us, a step 1200 cycles, bound by the softmax warps'
-// instructions (63 % of issue slots; tensor pipe 64 %).  2048 new tokens, 25 heads of 64, fp32: 60 us, short units, start and end.
+// instructions (61 % of issue slots; tensor pipe 62 %).  2048 new tokens, 25 heads of 64, fp32: 60 us, short units, start and end.
 //
 // A row whose result is not finite is computed again in fp32 arithmetic: 0 times an infinite value that the row does
 // not see is NaN on the tensor cores, and so are the terms of an infinity.

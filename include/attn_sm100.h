@@ -240,8 +240,8 @@ int attn_sm100_paged_append(const float *qkv, float *q_out, void *k_pages, void 
  *   max_new the largest number of new tokens that a sequence may bring (0: not known); the kernel and the size of its launch go by it
  * Scores and sums are fp32, from q in fp32 and the cache's elements as they are; the sum over the keys of weights of up to 1 times values
  * is one of them, so values above 3.4e38 over the number of keys may overflow.
- * The tensor cores take them in terms of 8 bits: of queries (times scale), and of keys and values of fp32 pages, what is below 2^-126 is lost.  A score of -inf has no weight, a row without any
- * weight is 0; NaN and infinities among keys and values that a row does not see do not reach it.
+ * The tensor cores take them in terms of 8 bits: of queries (times scale), and of keys and values of fp32 pages, what is below 2^-126 is lost.  A score of -inf has no weight, whatever the key's value is; a
+ * row without any weight is 0; NaN and infinities among keys and values that a row does not see do not reach it.
  */
 int attn_sm100_paged_forward(const float *q, const void *k_pages, const void *v_pages, const int *page_table, const int *cu_seqlens,
                              const int *past, float *out, long long ld, long long page_stride, int cache_type, int tokens, int seqs,
