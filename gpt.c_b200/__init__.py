@@ -53,9 +53,16 @@ SIGNATURES = {
     "tensor_sm100_axpy": (_c.c_int, [_c.c_size_t, _c.c_float, _c.c_void_p, _c.c_void_p, _c.c_void_p]),
     "tensor_sm100_gelu_forward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "tensor_sm100_gelu_backward": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p]),
+    "tensor_sm100_embedding_forward": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_longlong] * 3 + [_c.c_float] + [_c.c_int] * 6 + [_c.c_void_p]),
+    "tensor_sm100_embedding_backward_scratch_bytes": (_c.c_size_t, [_c.c_longlong] + [_c.c_int] * 3),
+    "tensor_sm100_embedding_backward": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_longlong] * 4 + [_c.c_float] + [_c.c_int] * 7 + [_c.c_void_p]),
     "xent_sm100_forward": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 2 + [_c.c_void_p]),
     "xent_sm100_selftest_wait_limit": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 3 + [_c.c_uint, _c.c_void_p]),
     "xent_sm100_sample": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_longlong] + [_c.c_int] * 2 + [_c.c_void_p]),
+    "xent_sm100_linear_forward_scratch_bytes": (_c.c_size_t, [_c.c_void_p] * 2 + [_c.c_longlong] * 2 + [_c.c_int] * 4),
+    "xent_sm100_linear_forward": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_longlong] * 2 + [_c.c_int] * 5 + [_c.c_void_p]),
+    "xent_sm100_linear_backward_scratch_bytes": (_c.c_size_t, [_c.c_void_p] * 2 + [_c.c_longlong] * 2 + [_c.c_int] * 4),
+    "xent_sm100_linear_backward": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_longlong] * 3 + [_c.c_int] * 6 + [_c.c_void_p]),
     "xent_sm100_backward": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 2 + [_c.c_void_p]),
     "adamw_sm100_step": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] + [_c.c_float] * 5 + [_c.c_int, _c.c_void_p]),
 }
@@ -232,6 +239,41 @@ def layernorm_forward(x, w, b=None, eps: float = 1e-5, stream=None):
 def layernorm_backward(dy, x, mean, rstd, w, dw, db, dx, stream=None) -> None:
     """Accumulates into dw, db (may be None) and dx, like the reference."""
     _calls().layernorm_backward(dy, x, mean, rstd, w, dw, db, dx, _raw(stream))
+
+
+# ---------------------------------------------------------------------------------------------
+# Token and position embedding (include/tensor_sm100.h); the reference's is embedding_{forward,backward}_cuda_kernel
+# (kernels/src/cuda/Embedding.cu:46-74).  Tables are fp32 or bf16 [rows, features], their rows may lie apart; tokens and positions are
+# int32, int64, or fp32 as gpt.c has them.  One outside its table brings zeros, and no gradient.
+# ---------------------------------------------------------------------------------------------
+def embedding_forward(tokens, table, positions=None, pos_table=None, scale: float = 1.0, stream=None):
+    """y[..., :] = scale * table[tokens] + pos_table[positions], of the type of the tables.  Without positions, a token's position is
+    its index along the last dimension of tokens [..., T]; without pos_table nothing is added."""
+    return _calls().embedding_forward(tokens, table, positions, pos_table, scale, _raw(stream))
+
+
+def embedding_backward(dy, tokens, dtable, positions=None, dpos_table=None, scale: float = 1.0, stream=None) -> None:
+    """Adds the gradients to dtable and dpos_table (either may be None), fp32 or bf16 whatever dy is: sums in fp32 and a fixed
+    order, one rounding."""
+    _calls().embedding_backward(dy, tokens, dtable, positions, dpos_table, scale, _raw(stream))
+
+
+# ---------------------------------------------------------------------------------------------
+# The vocabulary projection and its loss in one (include/xent_sm100.h): the logits, which the reference keeps three times over
+# (src/transformer.c:107-108, kernels/src/cuda/CrossEntropyLoss.cu:8-129), are not in memory.  x and w are both fp32 or both bf16; x is
+# contiguous or [rows, features] with rows apart, w and dw may have rows apart.  The calls do not record themselves for autograd.
+# ---------------------------------------------------------------------------------------------
+def linear_xent_forward(x, w, targets, stream=None):
+    """Returns (losses, lse), fp32 of the shape of targets: the cross-entropy of each row of x [..., K] @ w[V, K].T, and the
+    log of its sum of exponentials, which the backward takes.  targets (int32, int64, or fp32 as gpt.c has them): a row whose
+    target is outside 0 .. V - 1 has a loss of 0."""
+    return _calls().linear_xent_forward(x, w, targets, _raw(stream))
+
+
+def linear_xent_backward(g, x, w, targets, lse, dw=None, want_dx=True, stream=None):
+    """Gradients of sum(g * losses): returns dx, of the type of x (None when want_dx is false), and adds to dw (skipped when
+    None), which is like w.  g is fp32, one value or one for each row.  Rows without a target have no part in either."""
+    return _calls().linear_xent_backward(g, x, w, targets, lse, dw, want_dx, _raw(stream))
 
 
 # ---------------------------------------------------------------------------------------------

@@ -182,6 +182,8 @@ int attn_sm100_init(void) {
     if ((e = paged::few_rows_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = paged::decode_set_attributes()) != cudaSuccess) return (int)e;
     if ((e = sample::set_attributes()) != cudaSuccess) return (int)e;
+    if ((e = head::set_attributes()) != cudaSuccess) return (int)e;
+    if ((e = embed::set_attributes()) != cudaSuccess) return (int)e;
 
     int sms = 0;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return (int)e;

@@ -130,3 +130,9 @@ int device_status_word(int **status);
 namespace sample {
 cudaError_t set_attributes();  // of the kernel that draws a class from each row of logits (sample_sm100.cu)
 }
+namespace head {
+cudaError_t set_attributes();  // of the kernels of the projection with its loss (xent_linear_sm100.cu)
+}
+namespace embed {
+cudaError_t set_attributes();  // of the kernel that sorts tokens (embedding_sm100.cu)
+}

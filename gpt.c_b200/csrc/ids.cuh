@@ -1,0 +1,22 @@
+// Tokens, positions and targets: int32, int64, or fp32 as gpt.c's data loader makes them.
+#pragma once
+
+#include "../../include/tensor_sm100.h"
+
+struct Ids {
+    const void *p;
+    int type;
+    // The i-th one; -1 where it is none of 0 .. V - 1 (fp32: of its whole part, as the reference casts it).
+    __device__ __forceinline__ int at(long long i, int V) const {
+        if (type == TENSOR_INT64) {
+            const long long t = static_cast<const long long *>(p)[i];
+            return t >= 0 && t < V ? (int)t : -1;
+        }
+        if (type == TENSOR_INT32) {
+            const int t = static_cast<const int *>(p)[i];
+            return t >= 0 && t < V ? t : -1;
+        }
+        const float t = static_cast<const float *>(p)[i];
+        return t > -1.f && t < (float)V && (int)t < V ? (int)t : -1;
+    }
+};

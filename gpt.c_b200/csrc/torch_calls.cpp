@@ -1,4 +1,4 @@
-// The tensor-level calls of the Python package (forward, backward, linear_*, layernorm_*, paged_*, sample) as a CPython extension
+// The tensor-level calls of the Python package (forward, backward, linear_*, layernorm_*, embedding_*, paged_*, sample) as a CPython extension
 // over the C ABI of libattn_sm100.so.
 //
 // What bounds small calls is the host: with these functions written in Python, a forward and backward of
@@ -22,6 +22,7 @@
 #include "../../include/tensor_sm100.h"
 #include "../../include/xent_sm100.h"
 
+#include <algorithm>
 #include <cmath>
 #include <tuple>
 #include <utility>
@@ -491,6 +492,201 @@ PyObject *sample(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 // ------------------------------------------------------------------------------------------
+// Both ends of a training step: these take fp32 or bf16 tensors, on any one device like the calls above.
+// ------------------------------------------------------------------------------------------
+// x [..., columns] as rows `ld` elements apart: one row stride with the columns side by side.
+struct Rows {
+    const void *p = nullptr;
+    int64_t rows = 0, columns = 0;
+    long long ld = 0;
+
+    bool read(const at::Tensor &t) {
+        if (t.dim() < 1 || t.size(-1) < 1 || (t.size(-1) > 1 && t.stride(-1) != 1)) return false;
+        columns = t.size(-1), rows = t.numel() / columns, ld = columns, p = t.data_ptr();
+        if (t.dim() == 2 && rows > 1) ld = t.stride(0);
+        else if (t.dim() != 2 && !t.is_contiguous()) return false;
+        return ld >= columns && rows <= 0x7fffffff && columns <= 0x7fffffff;
+    }
+};
+// 0 fp32, 1 bf16, -1 neither
+int float_type(const at::Tensor &t) { return t.scalar_type() == at::kFloat ? TENSOR_F32 : t.scalar_type() == at::kBFloat16 ? TENSOR_BF16 : -1; }
+int id_type(const at::Tensor &t) {
+    return t.scalar_type() == at::kInt ? TENSOR_INT32 : t.scalar_type() == at::kLong ? TENSOR_INT64 : t.scalar_type() == at::kFloat ? TENSOR_IDS_F32 : -1;
+}
+
+struct Head {
+    const at::Tensor *x, *w, *targets;
+    Rows xr, wr;
+    int type, ids;
+    // x, w, targets in arguments i .. i + 2; false with a Python error set
+    bool read(Args &a, int i) {
+        x = a.tensor(i), w = a.tensor(i + 1), targets = a.tensor(i + 2);
+        if (!a.ok) return false;
+        type = float_type(*x);
+        if (!(x->is_cuda() && type >= 0 && xr.read(*x)))
+            return value_error("x must be an fp32 or bf16 CUDA tensor of shape [..., features], contiguous, or of two dimensions with its columns side by side") != nullptr;
+        if (!(is(*w, x->scalar_type(), *x) && w->dim() == 2 && wr.read(*w) && wr.rows > 0 && wr.columns == xr.columns))
+            return value_error("w must be a tensor of the type of x and of shape [classes, features] on the same device, with its columns side by side") != nullptr;
+        ids = id_type(*targets);
+        if (!(ids >= 0 && targets->device() == x->device() && targets->is_contiguous() && targets->sizes() == x->sizes().slice(0, x->dim() - 1)))
+            return value_error("targets must be a contiguous int32, int64 or fp32 tensor with one value a row of x, on the same device") != nullptr;
+        return true;
+    }
+};
+
+// linear_xent_forward(x, w, targets, stream) -> (losses, lse)
+PyObject *linear_xent_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 4);
+    Head h;
+    if (!a.ok || !h.read(a, 0)) return nullptr;
+    const On on(*h.x, args[3]);
+    if (PyErr_Occurred()) return nullptr;
+    const auto shape = h.targets->sizes();
+    const int rows = (int)h.xr.rows, V = (int)h.wr.rows, K = (int)h.xr.columns;
+    at::Tensor losses = alloc(shape, at::kFloat, *h.x), lse = alloc(shape, at::kFloat, *h.x), scratch;
+    int rc = ATTN_OK;
+    if (rows) {
+        const size_t bytes = xent_sm100_linear_forward_scratch_bytes(h.xr.p, h.wr.p, h.xr.ld, h.wr.ld, h.type, rows, V, K);
+        scratch = alloc({(int64_t)bytes}, at::kByte, *h.x);
+        float *lp = static_cast<float *>(losses.data_ptr()), *ep = static_cast<float *>(lse.data_ptr());
+        const void *tp = h.targets->data_ptr();
+        void *sp = bytes ? scratch.data_ptr() : reinterpret_cast<void *>(uintptr_t(256));  // (sizes that the call refuses)
+        Py_BEGIN_ALLOW_THREADS
+        rc = xent_sm100_linear_forward(h.xr.p, h.wr.p, tp, lp, ep, sp, h.xr.ld, h.wr.ld, h.type, h.ids, rows, V, K, on.stream);
+        Py_END_ALLOW_THREADS
+    }
+    if (failed(rc, "xent_sm100_linear_forward")) return nullptr;
+    return Py_BuildValue("(NN)", THPVariable_Wrap(losses), THPVariable_Wrap(lse));
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_xent_backward(g, x, w, targets, lse, dw or None, want_dx, stream) -> dx or None
+PyObject *linear_xent_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 8);
+    const at::Tensor *g = a.tensor(0);
+    Head h;
+    if (!a.ok || !h.read(a, 1)) return nullptr;
+    const at::Tensor *lse = a.tensor(4), *dw = args[5] == Py_None ? nullptr : a.tensor(5);
+    const int want_dx = a.ok ? PyObject_IsTrue(args[6]) : 0;
+    if (!a.ok || want_dx < 0) return nullptr;
+    if (!(is(*g, at::kFloat, *h.x) && g->is_contiguous() && (g->numel() == 1 || g->sizes() == h.targets->sizes())))
+        return value_error("g must be a contiguous fp32 tensor of one value, or of one for each row of x, on the same device");
+    if (!(is(*lse, at::kFloat, *h.x) && lse->is_contiguous() && lse->sizes() == h.targets->sizes()))
+        return value_error("lse must be a contiguous fp32 tensor with one value a row of x, on the same device");
+    Rows dr;
+    if (dw && !(is(*dw, h.w->scalar_type(), *h.w) && dw->sizes() == h.w->sizes() && dr.read(*dw)))
+        return value_error("dw must be a tensor like w, with its columns side by side");
+    if (!dw && !want_dx) return value_error("neither dx nor dw is wanted");
+    const On on(*h.x, args[7]);
+    if (PyErr_Occurred()) return nullptr;
+    const int rows = (int)h.xr.rows, V = (int)h.wr.rows, K = (int)h.xr.columns;
+    at::Tensor dx, scratch;
+    if (want_dx) dx = alloc(h.x->sizes(), h.x->scalar_type(), *h.x);
+    int rc = ATTN_OK;
+    if (rows) {
+        const size_t bytes = xent_sm100_linear_backward_scratch_bytes(h.xr.p, h.wr.p, h.xr.ld, h.wr.ld, h.type, rows, V, K);
+        scratch = alloc({(int64_t)bytes}, at::kByte, *h.x);
+        const float *gp = static_cast<const float *>(g->data_ptr()), *ep = static_cast<const float *>(lse->data_ptr());
+        const void *tp = h.targets->data_ptr();
+        void *dxp = want_dx ? dx.data_ptr() : nullptr, *dwp = dw ? dw->data_ptr() : nullptr, *sp = bytes ? scratch.data_ptr() : reinterpret_cast<void *>(uintptr_t(256));
+        const int one = g->numel() == 1;
+        Py_BEGIN_ALLOW_THREADS
+        rc = xent_sm100_linear_backward(gp, h.xr.p, h.wr.p, tp, ep, dxp, dwp, sp, h.xr.ld, h.wr.ld, dr.ld, one, h.type, h.ids, rows, V, K, on.stream);
+        Py_END_ALLOW_THREADS
+    }
+    if (failed(rc, "xent_sm100_linear_backward")) return nullptr;
+    if (!want_dx) Py_RETURN_NONE;
+    return THPVariable_Wrap(dx);
+    END_HANDLE_TH_ERRORS
+}
+
+// The table of an embedding or of its gradient: [rows, columns] of fp32 or bf16 beside the tokens.
+bool table_of(const at::Tensor &t, const at::Tensor &beside, Rows &r) {
+    return float_type(t) >= 0 && t.device() == beside.device() && t.dim() == 2 && r.read(t) && r.rows > 0;
+}
+// positions: like tokens, or None
+bool ids_of(const at::Tensor *tokens, const at::Tensor *positions) {
+    return id_type(*tokens) >= 0 && tokens->is_cuda() && tokens->is_contiguous() &&
+           (!positions || (is(*positions, tokens->scalar_type(), *tokens) && positions->is_contiguous() && positions->sizes() == tokens->sizes()));
+}
+int sequence_length(const at::Tensor &tokens) { return tokens.dim() ? (int)std::min<int64_t>(tokens.size(-1), 0x7fffffff) : 1; }
+
+// embedding_forward(tokens, table, positions or None, pos_table or None, scale, stream) -> y
+PyObject *embedding_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 6);
+    const at::Tensor *tokens = a.tensor(0), *table = a.tensor(1);
+    const at::Tensor *positions = a.ok && args[2] != Py_None ? a.tensor(2) : nullptr, *pos = a.ok && args[3] != Py_None ? a.tensor(3) : nullptr;
+    const double scale = a.real(4);
+    if (!a.ok) return nullptr;
+    if (!ids_of(tokens, positions)) return value_error("tokens, and positions if given, must be contiguous int32, int64 or fp32 CUDA tensors of the same type and shape");
+    Rows tr, pr;
+    if (!table_of(*table, *tokens, tr)) return value_error("table must be an fp32 or bf16 tensor of shape [tokens, features] on the same device, with its columns side by side");
+    if (pos && !(pos->scalar_type() == table->scalar_type() && table_of(*pos, *tokens, pr) && pr.columns == tr.columns))
+        return value_error("pos_table must be a tensor like table, with a row for each position");
+    if (positions && !pos) return value_error("positions without pos_table");
+    const On on(*tokens, args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    c10::SmallVector<int64_t, 6> shape(tokens->sizes().begin(), tokens->sizes().end());
+    shape.push_back(tr.columns);
+    at::Tensor y = alloc(shape, table->scalar_type(), *tokens);
+    const int64_t count = tokens->numel();
+    const void *tp = tokens->data_ptr(), *pp = positions ? positions->data_ptr() : nullptr;
+    void *yp = y.data_ptr();
+    const int type = float_type(*table), ids = id_type(*tokens), T = sequence_length(*tokens);
+    int rc = ATTN_OK;
+    Py_BEGIN_ALLOW_THREADS
+    if (count)
+        rc = tensor_sm100_embedding_forward(tp, tr.p, pp, pr.p, yp, count, tr.ld, pr.ld, (float)scale, type, ids, T, (int)tr.columns, (int)tr.rows, (int)pr.rows, on.stream);
+    Py_END_ALLOW_THREADS
+    if (failed(rc, "tensor_sm100_embedding_forward")) return nullptr;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// embedding_backward(dy, tokens, dtable or None, positions or None, dpos_table or None, scale, stream)
+PyObject *embedding_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a(args, n, 7);
+    const at::Tensor *dy = a.tensor(0), *tokens = a.tensor(1), *grad = a.ok && args[2] != Py_None ? a.tensor(2) : nullptr;
+    const at::Tensor *positions = a.ok && args[3] != Py_None ? a.tensor(3) : nullptr, *pos = a.ok && args[4] != Py_None ? a.tensor(4) : nullptr;
+    const double scale = a.real(5);
+    if (!a.ok) return nullptr;
+    if (!ids_of(tokens, positions)) return value_error("tokens, and positions if given, must be contiguous int32, int64 or fp32 CUDA tensors of the same type and shape");
+    Rows dr, gr, pr;
+    if (!(float_type(*dy) >= 0 && dy->device() == tokens->device() && dy->dim() == tokens->dim() + 1 && dy->sizes().slice(0, tokens->dim()) == tokens->sizes() && dr.read(*dy)))
+        return value_error("dy must be an fp32 or bf16 tensor with a row for each token on the same device, contiguous, or of two dimensions with its columns side by side");
+    if (!grad && !pos) return value_error("neither dtable nor dpos_table is given");
+    if (grad && !(table_of(*grad, *tokens, gr) && gr.columns == dr.columns))
+        return value_error("dtable must be an fp32 or bf16 tensor of shape [tokens, features] on the same device, with its columns side by side");
+    if (pos && !(table_of(*pos, *tokens, pr) && pr.columns == dr.columns && (!grad || pos->scalar_type() == grad->scalar_type())))
+        return value_error("dpos_table must be a tensor like dtable, with a row for each position");
+    if (positions && !pos) return value_error("positions without dpos_table");
+    const On on(*tokens, args[6]);
+    if (PyErr_Occurred()) return nullptr;
+    const int64_t count = tokens->numel();
+    int rc = ATTN_OK;
+    if (count) {
+        const int C = (int)dr.columns, V = (int)gr.rows, P = (int)pr.rows;
+        const size_t bytes = tensor_sm100_embedding_backward_scratch_bytes(count, C, V, positions ? P : 0);
+        at::Tensor scratch;
+        if (bytes) scratch = alloc({(int64_t)bytes}, at::kByte, *tokens);
+        void *sp = bytes ? scratch.data_ptr() : nullptr;
+        const void *tp = tokens->data_ptr(), *pp = positions ? positions->data_ptr() : nullptr;
+        const int type = float_type(*dy), grad_type = float_type(grad ? *grad : *pos), ids = id_type(*tokens), T = sequence_length(*tokens);
+        void *gp = const_cast<void *>(gr.p), *qp = const_cast<void *>(pr.p);
+        Py_BEGIN_ALLOW_THREADS
+        rc = tensor_sm100_embedding_backward(dr.p, tp, gp, pp, qp, sp, count, dr.ld, gr.ld, pr.ld, (float)scale, type, grad_type, ids, T, C, V, P, on.stream);
+        Py_END_ALLOW_THREADS
+    }
+    if (failed(rc, "tensor_sm100_embedding_backward")) return nullptr;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------
 // What calling a ctypes function of the library does instead, as the tp_call of its function object's class: a call with
 // exactly as many plain numbers (or None for a pointer) as the function has arguments goes to the C ABI from here, every
 // other one to ctypes.
@@ -562,6 +758,7 @@ PyObject *set_error(PyObject *, PyObject *cls) {
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {FAST(forward), FAST(backward), FAST(forward_into), FAST(backward_into), FAST(linear_forward),
                           FAST(linear_backward), FAST(layernorm_forward), FAST(layernorm_backward), FAST(paged_append), FAST(paged_attention), FAST(sample),
+                          FAST(linear_xent_forward), FAST(linear_xent_backward), FAST(embedding_forward), FAST(embedding_backward),
                           {"set_error", set_error, METH_O, nullptr}, {"shorten_calls", shorten_calls, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "gptc_b200_calls", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,880 @@
+// The vocabulary projection with the cross-entropy of its rows, and their gradients, without the logits in memory, for sm_100a.
+//
+//     z = x w^T             lse_r = log sum_v exp z_rv             loss_r = lse_r - z_r,t(r)
+//     G_rv = g_r (exp(z_rv - lse_r) - [v = t(r)])        dx = G w        dw += G^T x
+//
+// Forward: tiles of z are made in tensor memory and read once, for a maximum and a sum of exponentials of each row of the tile; a
+// second kernel joins them over the tiles of a row.
+// Backward: z is made again, a piece of the vocabulary at a time, and leaves its tile as G, in bf16, to a buffer that the two products
+// read.  The launch that makes the products of a piece also makes G of the next one, so its tail is filled with short tiles.
+//
+// All three products go through one loop over tiles of 256 x 256 and contraction blocks of 64:
+//     z   A: x,  contraction contiguous    B: w, contraction contiguous
+//     dx  A: G,  contraction contiguous    B: w, columns contiguous
+//     dw  A: G,  rows contiguous           B: x, columns contiguous
+// fp32 operands are two bf16 planes, hi and lo, and a product is hi hi + hi lo + lo hi: four tiles of a contraction block serve three
+// products.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+#include "attn_internal.h"
+#include "ids.cuh"
+#include "tc05.cuh"
+
+#include "../../include/xent_sm100.h"
+
+namespace head {
+namespace {
+
+using namespace tc05;
+
+constexpr int kTile = 256, kBlock = 64;
+constexpr int kEpiWarps = 16, kThreads = 32 * (2 + kEpiWarps);
+constexpr int kSlotBytes = kTile * kBlock * 2;
+constexpr int kQueue = 4;
+constexpr int kSegment = 16;           // contraction blocks of fp32 operands that one sum in tensor memory takes
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Site : int { SITE_EMPTY = 301, SITE_FULL, SITE_ACC_EMPTY, SITE_ACC_FULL, SITE_ITEM, SITE_ITEM_FREE, SITE_SMEM_ALIGN };
+enum Kind : int { kLogits, kDx, kDw };
+
+template <int kSlots, bool kBackward>
+struct __align__(1024) Smem {
+    uint8_t slot[kSlots][kSlotBytes];
+    float2 part[kBackward ? 1 : 2][kBackward ? 1 : 3][kBackward ? 1 : 128];  // maximum and sum of a row in three quarters of a tile
+    uint64_t full[kSlots], empty[kSlots];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t item_full[kQueue], item_empty[kQueue];
+    int item[kQueue];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+struct Maps {
+    CUtensorMap x, w;      // boxes of 64 contraction steps x 256 rows
+    CUtensorMap x_mn, w_mn;  // boxes of 64 columns x 64 contraction steps
+    CUtensorMap g, g_mn;   // the piece whose products are made, both ways
+};
+
+struct Problem {
+    int M, V, K;
+    int tiles_m, tiles_k;         // tiles of the rows of x, of its columns
+    int dx, dw, total;            // work items: dx first, then dw, then z
+    int dx_pieces, dx_blocks;     // pieces of the contraction of dx, blocks of each
+    int blocks_m, blocks_k;       // contraction blocks over the rows, over the columns of x
+    int v0, cols;                 // the piece of the vocabulary whose products are made
+    int next_v0, next_cols;       // the piece whose z is made
+    int first;                    // the first piece: what dx holds is not added to
+    int pitch;                    // columns of a row of G
+    long long plane;              // elements from the hi to the lo plane of G
+    Ids targets;
+    const float *g, *lse;
+    int one_g;
+    __nv_bfloat16 *out;           // G of the next piece
+    float *dxp;                   // [dx_pieces, M, dx_pitch]
+    long long dx_pitch;
+    void *dw_out;
+    long long lddw;
+    int dw_wide;                  // bytes that the rows of dw allow at a time: 32, 16, or an element
+    float2 *part;                 // forward: [tiles of V, M]
+    float *zt;                    // forward: the target's logit
+    int *counter;                 // items are handed out (else round robin)
+    float fix, log2e;             // z as the tensor cores leave it times `fix` is z; fix * log2(e)
+};
+
+struct Item {
+    int kind, m0, n0, n, halves;   // n: columns, a multiple of 32
+    int blocks, segment, block0;   // contraction blocks, of one sum; where they begin
+    int piece;
+};
+
+template <bool kBackward>
+__device__ __forceinline__ Item decode(const Problem &p, int w) {
+    Item it;
+    int rows, cols;
+    it.block0 = 0;
+    it.piece = 0;
+    if (kBackward && w < p.dx) {
+        it.kind = kDx;
+        const int t = w / p.dx_pieces;
+        it.piece = w - t * p.dx_pieces;
+        it.n0 = t % p.tiles_k * kTile;
+        it.m0 = t / p.tiles_k * kTile;
+        rows = p.M, cols = p.K;
+        it.block0 = it.piece * p.dx_blocks;
+        it.blocks = min(p.dx_blocks, p.cols / kBlock - it.block0);
+    } else if (kBackward && w < p.dx + p.dw) {
+        it.kind = kDw;
+        const int t = w - p.dx;
+        it.n0 = t % p.tiles_k * kTile;
+        it.m0 = t / p.tiles_k * kTile;  // in the piece
+        rows = min(p.cols, p.V - p.v0), cols = p.K;
+        it.blocks = p.blocks_m;
+    } else {
+        it.kind = kLogits;
+        const int t = kBackward ? w - p.dx - p.dw : w;
+        it.m0 = t % p.tiles_m * kTile;
+        it.n0 = t / p.tiles_m * kTile;  // in the piece
+        rows = p.M, cols = min(p.next_cols, p.V - p.next_v0);
+        it.blocks = p.blocks_k;
+    }
+    it.halves = rows - it.m0 > 128 ? 2 : 1;
+    it.n = min(kTile, (cols - it.n0 + 31) / 32 * 32);
+    it.segment = it.blocks;
+    return it;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+        : "memory");
+}
+
+__device__ __forceinline__ void load8(uint32_t (&r)[8], const void *p) {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store8(void *p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+                 "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
+// 64 sums of a row added to `at`, of which `left` (more than 0) are inside.
+template <bool kAdd>
+__device__ __forceinline__ void put_f32(float *at, const uint32_t (&z)[64], int left, int wide) {
+    if (wide == 32) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 16) {
+            uint32_t old[2][8];
+            if (kAdd) {
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    if (i + 8 * j < left) load8(old[j], at + i + 8 * j);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (i + 8 * j >= left) continue;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    old[j][e] = kAdd ? __float_as_uint(__uint_as_float(old[j][e]) + __uint_as_float(z[i + 8 * j + e])) : z[i + 8 * j + e];
+                store8(at + i + 8 * j, old[j]);
+            }
+        }
+    } else if (wide == 16) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 4) {
+            if (i >= left) continue;
+            float4 *q = reinterpret_cast<float4 *>(at + i);
+            float4 v = kAdd ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
+            v.x += __uint_as_float(z[i]), v.y += __uint_as_float(z[i + 1]), v.z += __uint_as_float(z[i + 2]), v.w += __uint_as_float(z[i + 3]);
+            *q = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 64; i++)
+            if (i < left) at[i] = kAdd ? at[i] + __uint_as_float(z[i]) : __uint_as_float(z[i]);
+    }
+}
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t old, uint32_t a, uint32_t b) {
+    return pack_bf16x2(__uint_as_float(old << 16) + __uint_as_float(a), __uint_as_float(old & 0xffff0000u) + __uint_as_float(b));
+}
+__device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&z)[64], int left, int wide) {
+    if (wide == 32) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 32) {
+            uint32_t old[2][8];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (i + 16 * j < left) load8(old[j], at + i + 16 * j);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                if (i + 16 * j >= left) continue;
+#pragma unroll
+                for (int e = 0; e < 8; e++) old[j][e] = add_bf16x2(old[j][e], z[i + 16 * j + 2 * e], z[i + 16 * j + 2 * e + 1]);
+                store8(at + i + 16 * j, old[j]);
+            }
+        }
+    } else if (wide == 16) {
+#pragma unroll
+        for (int i = 0; i < 64; i += 8) {
+            if (i >= left) continue;
+            uint4 *q = reinterpret_cast<uint4 *>(at + i);
+            uint4 v = *q;
+            v.x = add_bf16x2(v.x, z[i], z[i + 1]), v.y = add_bf16x2(v.y, z[i + 2], z[i + 3]);
+            v.z = add_bf16x2(v.z, z[i + 4], z[i + 5]), v.w = add_bf16x2(v.w, z[i + 6], z[i + 7]);
+            *q = v;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 64; i++)
+            if (i < left) at[i] = __float2bfloat16_rn(__bfloat162float(at[i]) + __uint_as_float(z[i]));
+    }
+}
+
+// kTerms 1: bf16 operands; 3: fp32 operands as two planes.
+template <int kTerms, bool kBackward, int kSlots>
+__global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, int *status) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    using S = Smem<kSlots, kBackward>;
+    S &sm = *reinterpret_cast<S *>(smem_raw);
+    if ((smem_u32(smem_raw) & 1023u) != 0) {
+        if (threadIdx.x == 0 && status) atomicCAS(status, 0, ST_TIMEOUT_BASE + SITE_SMEM_ALIGN);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int kLoads = kTerms == 1 ? 2 : 4;  // slots of a contraction block: A hi, B hi, B lo, A lo
+    WaitCtx ctx{&sm.abort_flag, status, 0};
+    if (threadIdx.x == 0) {
+        sm.abort_flag = 0;
+        for (int i = 0; i < kSlots; i++) {
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.acc_full[i], 1);
+            mbar_init(&sm.acc_empty[i], kEpiWarps);
+        }
+        for (int i = 0; i < kQueue; i++) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_empty[i], 1 + kEpiWarps);
+        }
+        fence_barrier_init();
+        tma_prefetch_desc(&maps.x);
+        tma_prefetch_desc(&maps.w);
+    }
+    if (warp == 1) tmem_alloc_then_launch_dependents(&sm.tmem_base, 512);
+    pdl_wait();  // every thread, before its first access to global memory
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sm.tmem_base;
+
+    if (warp == 0) {
+        // ------------------------------ hands out items, asks for tiles ------------------------------
+        if (lane == 0) {
+            int n = 0;  // slots filled
+            bool ok = true;
+            int w = blockIdx.x;
+            for (int j = 0;; j++) {
+                const int at = j % kQueue;
+                if (j >= kQueue && !(ok = mbar_wait(&sm.item_empty[at], (j / kQueue - 1) & 1, ctx, SITE_ITEM_FREE))) break;
+                sm.item[at] = w;
+                mbar_arrive(&sm.item_full[at]);
+                if (w >= p.total) break;
+                const Item it = decode<kBackward>(p, w);
+                w = p.counter ? (int)gridDim.x + atomicAdd(p.counter, 1) : w + (int)gridDim.x;
+                const int a_boxes = 2 * it.halves, b_boxes = (it.n + 63) / 64;
+                for (int b = it.block0; ok && b < it.block0 + it.blocks; b++) {
+#pragma unroll
+                    for (int l = 0; l < kLoads; l++, n++) {
+                        const int st = n % kSlots, plane = l >= 2 ? 1 : 0;
+                        const bool is_a = l == 0 || l == 3;
+                        if (n >= kSlots && !mbar_wait(&sm.empty[st], (n / kSlots - 1) & 1, ctx, SITE_EMPTY)) {
+                            ok = false;
+                            break;
+                        }
+                        uint8_t *dst = sm.slot[st];
+                        uint64_t *bar = &sm.full[st];
+                        if (it.kind == kLogits) {
+                            mbar_expect_tx(bar, kSlotBytes);
+                            if (is_a) tma_load_3d(dst, &maps.x, bar, b * kBlock, it.m0, plane);
+                            else tma_load_3d(dst, &maps.w, bar, b * kBlock, p.next_v0 + it.n0, plane);
+                        } else if (it.kind == kDx && is_a) {
+                            mbar_expect_tx(bar, kSlotBytes);
+                            tma_load_3d(dst, &maps.g, bar, b * kBlock, it.m0, plane);
+                        } else {
+                            const CUtensorMap *map = it.kind == kDx ? &maps.w_mn : is_a ? &maps.g_mn : &maps.x_mn;
+                            const int boxes = is_a ? a_boxes : b_boxes, c0 = is_a ? it.m0 : it.n0, row = (it.kind == kDx ? p.v0 : 0) + b * kBlock;
+                            mbar_expect_tx(bar, boxes * (kBlock * 128));
+                            for (int i = 0; i < boxes; i++) tma_load_3d(dst + i * (kBlock * 128), map, bar, c0 + 64 * i, row, plane);
+                        }
+                    }
+                }
+                if (!ok) break;
+            }
+            if (sm.abort_flag) {  // a wait has run out: shared memory is not given up before the copies that are under way have arrived
+                for (int i = max(0, n - kSlots); i < n; i++) {
+                    const uint64_t t0 = global_timer_ns();
+                    while (!mbar_test_wait(&sm.full[i % kSlots], (i / kSlots) & 1) && global_timer_ns() - t0 < 10000000ull) {
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------ issues the products ------------------------------
+        const uint32_t leader = elect_leader();
+        int n = 0, half = 0;
+        bool ok = true;
+        for (int j = 0; ok; j++) {
+            const int at = j % kQueue;
+            if (!mbar_wait_warp(&sm.item_full[at], (j / kQueue) & 1, ctx, SITE_ITEM)) break;
+            const int w = sm.item[at];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.item_empty[at]);
+            if (w >= p.total) break;
+            const Item it = decode<kBackward>(p, w);
+            const bool a_mn = it.kind == kDw, b_mn = it.kind != kLogits;
+            const uint32_t idesc = idesc_bf16_f32(128, it.n, a_mn, b_mn);
+            const uint32_t lbo_a = a_mn ? kBlock * 128 : 16, lbo_b = b_mn ? kBlock * 128 : 16, step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
+            const int seg = kTerms == 3 && kBackward && it.kind != kLogits ? kSegment : it.blocks;
+            for (int b0 = 0; ok && b0 < it.blocks; b0 += seg) {
+                const int b1 = min(it.blocks, b0 + seg);
+                for (int b = b0; b < b1; b++, n += kLoads) {
+#pragma unroll
+                    for (int l = 0; l < kLoads; l++)
+                        if (ok && !mbar_wait_warp(&sm.full[(n + l) % kSlots], ((n + l) / kSlots) & 1, ctx, SITE_FULL)) ok = false;
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    uint64_t d[kLoads];
+#pragma unroll
+                    for (int l = 0; l < kLoads; l++) {
+                        const bool is_a = l == 0 || l == 3;
+                        d[l] = smem_desc_sw128(smem_u32(sm.slot[(n + l) % kSlots]), is_a ? lbo_a : lbo_b, 1024);
+                    }
+                    for (int h = 0; h < it.halves; h++) {
+                        const int acc = (half + h) & 1;
+                        if (b == b0 && half + h >= 2) {
+                            if (!mbar_wait_warp(&sm.acc_empty[acc], ((half + h) / 2 - 1) & 1, ctx, SITE_ACC_EMPTY)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after_sync();
+                        }
+                        const uint32_t to = tmem + (uint32_t)acc * kTile;
+#pragma unroll
+                        for (int t = 0; t < kTerms; t++) {
+                            const uint64_t a = desc_advance(d[t == 2 ? kLoads - 1 : 0], h * 16384), bb = d[t == 1 ? 2 % kLoads : 1];
+#pragma unroll
+                            for (int k = 0; k < kBlock / 16; k++)
+                                mma_ss_lead(leader, to, desc_advance(a, k * step_a), desc_advance(bb, k * step_b), idesc, b > b0 || t > 0 || k > 0);
+                        }
+                        if (b == b1 - 1) tc_commit_lead(leader, &sm.acc_full[acc]);
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int l = 0; l < kLoads; l++) tc_commit_lead(leader, &sm.empty[(n + l) % kSlots]);
+                }
+                half += it.halves;
+            }
+        }
+    } else {
+        // ------------------------------ takes the sums out ------------------------------
+        // A warp reads 32 rows (its quarter of tensor memory's lanes) and 64 columns of each half of a tile.
+        const int quarter = warp & 3, group = (warp - 2) >> 2;
+        const uint32_t from = tmem + ((uint32_t)(quarter * 32) << 16) + 64 * group;
+        int half = 0;
+        bool ok = true;
+        for (int j = 0; ok; j++) {
+            const int at = j % kQueue;
+            if (!mbar_wait_warp(&sm.item_full[at], (j / kQueue) & 1, ctx, SITE_ITEM)) break;
+            const int w = sm.item[at];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.item_empty[at]);
+            if (w >= p.total) break;
+            const Item it = decode<kBackward>(p, w);
+            const int seg = kTerms == 3 && kBackward && it.kind != kLogits ? kSegment : it.blocks;
+            for (int b0 = 0; ok && b0 < it.blocks; b0 += seg) {
+                for (int h = 0; h < it.halves; h++, half++) {
+                    const int acc = half & 1;
+                    const int row = it.m0 + h * 128 + quarter * 32 + lane, off = 64 * group;
+                    const bool mine = off < it.n;  // (a whole warp)
+                    int target = -1;
+                    float gr = 0.f, nl = 0.f;
+                    if (it.kind == kLogits && row < p.M) {
+                        target = p.targets.at(row, p.V);
+                        if (kBackward) {
+                            gr = p.g[p.one_g ? 0 : row];
+                            nl = -p.lse[row] * kLog2e;
+                        }
+                    }
+                    if (!mbar_wait_warp(&sm.acc_full[acc], (half / 2) & 1, ctx, SITE_ACC_FULL)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after_sync();
+                    uint32_t z[64];
+                    tmem_ld32(from + acc * kTile, *reinterpret_cast<uint32_t(*)[32]>(z));
+                    tmem_ld32(from + acc * kTile + 32, *reinterpret_cast<uint32_t(*)[32]>(z + 32));
+                    tmem_wait_ld();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.acc_empty[acc]);
+                    if (it.kind == kLogits) {
+                        const int class0 = p.next_v0 + it.n0 + off;
+                        const int left = p.V - class0, place = target - class0;
+                        const bool here = target >= 0 && place >= 0 && place < 64;
+                        if (!kBackward) {
+                            float top = -INFINITY, sum = 0.f;
+                            if (left < 64) {
+#pragma unroll
+                                for (int e = 0; e < 64; e++)
+                                    if (e >= left) z[e] = __float_as_uint(-INFINITY);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 64; e++) top = fmaxf(top, __uint_as_float(z[e]));
+                            const float nt = top == -INFINITY ? 0.f : -top * p.log2e;
+                            float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int e = 0; e < 64; e++) s[e & 3] += ex2(fmaf(__uint_as_float(z[e]), p.log2e, nt));
+                            sum = (s[0] + s[1]) + (s[2] + s[3]);
+                            if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+                                for (int e = 0; e < 64; e++)
+                                    if (here && e == place) p.zt[row] = __uint_as_float(z[e]) * p.fix;
+                            }
+                            top *= p.fix;
+                            // the four quarters of the tile's columns
+                            if (group > 0) sm.part[half & 1][group - 1][quarter * 32 + lane] = make_float2(top, sum);
+                            asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+                            if (group == 0) {
+                                float2 q[4] = {make_float2(top, sum)};
+#pragma unroll
+                                for (int i = 0; i < 3; i++) q[i + 1] = sm.part[half & 1][i][quarter * 32 + lane];
+                                const float m = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), nm = m == -INFINITY ? 0.f : -m * kLog2e;
+                                sum = 0.f;
+#pragma unroll
+                                for (int i = 0; i < 4; i++) sum += q[i].y * ex2(fmaf(q[i].x, kLog2e, nm));
+                                if (row < p.M) p.part[(long long)(it.n0 / kTile) * p.M + row] = make_float2(m, sum);
+                            }
+                        } else if (off < p.pitch - it.n0) {
+#pragma unroll
+                            for (int e = 0; e < 64; e++) z[e] = __float_as_uint(ex2(fmaf(__uint_as_float(z[e]), p.log2e, nl)));
+                            if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+                                for (int e = 0; e < 64; e++)
+                                    if (here && e == place) z[e] = __float_as_uint(__uint_as_float(z[e]) - 1.f);
+                            }
+                            if (left < 64) {
+#pragma unroll
+                                for (int e = 0; e < 64; e++)
+                                    if (e >= left) z[e] = 0;
+                            }
+                            if (row < p.M) {
+                                __nv_bfloat16 *to = p.out + (long long)row * p.pitch + it.n0 + off;
+#pragma unroll
+                                for (int i = 0; i < 64; i += 16) {
+                                    uint32_t hi[8], lo[8];
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) {
+                                        const float a = __uint_as_float(z[i + 2 * e]) * gr, b = __uint_as_float(z[i + 2 * e + 1]) * gr;
+                                        if (kTerms == 1) hi[e] = pack_bf16x2(a, b);
+                                        else split_bf16x2(a, b, hi[e], lo[e]);
+                                        if (target < 0) hi[e] = lo[e] = 0;
+                                    }
+                                    store8(to + i, hi);
+                                    if (kTerms == 3) store8(to + p.plane + i, lo);
+                                }
+                            }
+                        }
+                    } else if (kBackward && mine) {
+                        const int left = p.K - it.n0 - off;
+                        if (it.kind == kDx) {
+                            if (row < p.M && left > 0) {
+                                float *to = p.dxp + ((long long)it.piece * p.M + row) * p.dx_pitch + it.n0 + off;
+                                if (p.first && b0 == 0) put_f32<false>(to, z, left, 32);
+                                else put_f32<true>(to, z, left, 32);
+                            }
+                        } else {
+                            const long long v = (long long)p.v0 + row;
+                            if (v < p.V && row < p.cols && left > 0) {
+                                if (kTerms == 1) add_bf16(static_cast<__nv_bfloat16 *>(p.dw_out) + v * p.lddw + it.n0 + off, z, left, p.dw_wide);
+                                else put_f32<true>(static_cast<float *>(p.dw_out) + v * p.lddw + it.n0 + off, z, left, p.dw_wide);
+                            }
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // ------------------------------ tear-down ------------------------------
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Maximum and sum of each row from those of its tiles.  A block takes 32 rows, a warp every eighth tile.
+__global__ void __launch_bounds__(256) join_kernel(const float2 *__restrict__ part, const float *__restrict__ zt, Ids targets, float *__restrict__ losses,
+                                                   float *__restrict__ lse, int tiles, int M, int V) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ float2 all[8][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = blockIdx.x * 32 + lane;
+    float m = -INFINITY, s = 0.f;
+    auto join = [&](float2 q) {
+        const float top = fmaxf(m, q.x), nt = top == -INFINITY ? 0.f : -top * kLog2e;
+        s = s * ex2(fmaf(m, kLog2e, nt)) + q.y * ex2(fmaf(q.x, kLog2e, nt));
+        m = top;
+    };
+    if (row < M) {
+        for (int t0 = warp; t0 < tiles; t0 += 32) {
+            float2 q[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) q[u] = t0 + 8 * u < tiles ? part[(long long)(t0 + 8 * u) * M + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; u++) join(q[u]);
+        }
+    }
+    all[warp][lane] = make_float2(m, s);
+    __syncthreads();
+    if (warp != 0 || row >= M) return;
+#pragma unroll
+    for (int i = 1; i < 8; i++) join(all[i][lane]);
+    const float l = m + logf(s);
+    lse[row] = l;
+    losses[row] = targets.at(row, V) >= 0 ? l - zt[row] : 0.f;
+}
+
+// src [R, K] as bf16 planes [R, pitch] (hi, and lo of fp32 values).  Rows without a target become zeros where targets are given.  Also
+// clears the counters of work items.
+template <class T>
+__global__ void __launch_bounds__(256) planes_kernel(const T *__restrict__ src, long long ld, __nv_bfloat16 *__restrict__ hi, __nv_bfloat16 *__restrict__ lo,
+                                                     int R, int K, int pitch, int wide, Ids targets, int V, int *counters, int count) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int words = pitch / 8;
+    const long long total = (long long)R * words;
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < count; i += 256) counters[i] = 0;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / words;
+        const int c = (int)(i - r * words) * 8;
+        const T *at = src + r * ld + c;
+        uint32_t h[4] = {}, l[4] = {};
+        const bool none = targets.p != nullptr && targets.at(r, V) < 0;
+        if (!none) {
+            if constexpr (sizeof(T) == 2) {
+                if (wide && c + 8 <= K) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(at);
+                    h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (c + e < K) h[e / 2] |= (uint32_t)reinterpret_cast<const unsigned short *>(at)[e] << (e & 1) * 16;
+                }
+            } else {
+                float v[8] = {};
+                if (wide && c + 8 <= K) {
+                    const float4 a = __ldcs(reinterpret_cast<const float4 *>(at)), b = __ldcs(reinterpret_cast<const float4 *>(at) + 1);
+                    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (c + e < K) v[e] = at[e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) split_bf16x2(v[2 * e], v[2 * e + 1], h[e], l[e]);
+            }
+        }
+        *reinterpret_cast<uint4 *>(hi + r * pitch + c) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(lo + r * pitch + c) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+
+// dx from the pieces of its contraction, in their order.
+template <class T>
+__global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int words = pitch / 4;
+    const long long total = (long long)M * words, apart = (long long)M * pitch;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const long long r = i / words;
+        const int c = (int)(i - r * words) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < count; p0 += 4) {
+            float4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                v[u] = p0 + u < count ? __ldcs(reinterpret_cast<const float4 *>(pieces + (p0 + u) * apart + r * pitch + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; u++) sum = make_float4(sum.x + v[u].x, sum.y + v[u].y, sum.z + v[u].z, sum.w + v[u].w);
+        }
+        T *at = dx + r * K + c;
+        const float s[4] = {sum.x, sum.y, sum.z, sum.w};
+        if (wide && c + 4 <= K) {
+            if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(at) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
+            else *reinterpret_cast<float4 *>(at) = sum;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c + e < K) at[e] = (T)s[e];
+        }
+    }
+}
+
+// ---- host side ----
+
+constexpr size_t kPieceBytes = (size_t)128 << 20;  // of G, about
+constexpr int kForwardSlots = 6, kBackwardSlots = 7;
+
+int up(int v, int to) { return (v + to - 1) / to * to; }
+size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// What a call reads in place and what it copies, and where everything lies in the scratch buffer.
+struct Layout {
+    bool copy_x, copy_w;
+    int pitch, planes;
+    size_t x, w, part, zt, counters, g[2], dxp, total;
+    int cols, pieces;         // of the vocabulary
+    int dx_pieces, dx_blocks, dx_pitch;
+    size_t plane_x, plane_w, plane_g;  // elements
+};
+
+bool in_place(const void *p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+
+Layout layout(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K, bool backward, int sms) {
+    Layout l = {};
+    l.planes = type == TENSOR_F32 ? 2 : 1;
+    l.pitch = up(K, 8);
+    l.copy_x = type == TENSOR_F32 || backward || !in_place(x, ldx);  // the gradients need rows of zeros where there is no target
+    l.copy_w = type == TENSOR_F32 || !in_place(w, ldw);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += up256(bytes);
+        return here;
+    };
+    l.plane_x = up256((size_t)M * l.pitch * 2) / 2;
+    l.plane_w = up256((size_t)V * l.pitch * 2) / 2;
+    if (l.copy_x) l.x = take(l.plane_x * 2 * l.planes);
+    if (l.copy_w) l.w = take(l.plane_w * 2 * l.planes);
+    const int tiles_v = (V + kTile - 1) / kTile, tiles_m = (M + kTile - 1) / kTile, tiles_k = (K + kTile - 1) / kTile;
+    if (!backward) {
+        l.part = take((size_t)tiles_v * M * sizeof(float2));
+        l.zt = take((size_t)M * sizeof(float));
+        l.total = at;
+        return l;
+    }
+    // pieces of the vocabulary: as many tiles each
+    const size_t tile_bytes = (size_t)M * kTile * 2 * l.planes;
+    const int most = (int)std::min<size_t>(tiles_v, std::max<size_t>(4, kPieceBytes / tile_bytes));
+    l.pieces = (tiles_v + most - 1) / most;
+    const int tiles = (tiles_v + l.pieces - 1) / l.pieces;
+    l.pieces = (tiles_v + tiles - 1) / tiles;
+    l.cols = tiles * kTile;
+    // pieces of the contraction of dx: none is longer than half of what an SM has to do for a piece of the vocabulary
+    const int blocks = l.cols / kBlock;
+    const double load = ((double)tiles_m * tiles_k * blocks + (double)tiles * tiles_k * std::max(4, (M + kBlock - 1) / kBlock)) / sms;
+    const int longest = std::max(12, (int)(load / 2));
+    l.dx_pieces = std::min(64, (blocks + longest - 1) / longest);
+    l.dx_blocks = (blocks + l.dx_pieces - 1) / l.dx_pieces;
+    l.dx_pieces = (blocks + l.dx_blocks - 1) / l.dx_blocks;
+    l.dx_pitch = up(K, 8);
+    l.counters = take(sizeof(int) * (l.pieces + 1));
+    l.plane_g = (size_t)M * l.cols;
+    for (int i = 0; i < (l.pieces > 1 ? 2 : 1); i++) l.g[i] = take(l.plane_g * 2 * l.planes);
+    l.dxp = take((size_t)l.dx_pieces * M * l.dx_pitch * sizeof(float));
+    l.total = at;
+    return l;
+}
+
+// [rows, cols] bf16 of `planes` planes: boxes of 64 columns by box_rows rows.
+int map_of(CUtensorMap *map, const void *base, long long rows, int cols, long long pitch, size_t plane, int planes, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, planes > 1 ? (cuuint64_t)plane * 2 : (cuuint64_t)pitch * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+    return attn::encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box);
+}
+
+// The tensor cores cut every sum of 16 products and what was there off to fp32: a sum of n such steps that grows evenly is on average n / 4 half
+// units too small, and so were the logits (K = 1600: by 26 2^-24 of themselves in bf16 and 84 in fp32, which has three products; 4096: by 68
+// and 212; without `fix` the log-sum-exp of logits of standard deviation 30 is 1.6e-6 off, with it 5e-7).
+void set_fix(Problem &p, int type) {
+    const double steps = (p.K + 15) / 16 * (type == TENSOR_F32 ? 3 : 1);
+    p.fix = (float)(1.0 + 0.26 * steps / 16777216.0);
+    p.log2e = (float)(1.4426950408889634 * (1.0 + 0.26 * steps / 16777216.0));
+}
+
+int blocks_for(long long words) { return (int)std::max(1ll, std::min(words / 256 + 1, 148ll * 16)); }
+
+cudaError_t launch_planes(const void *src, long long ld, int type, void *to, size_t plane, int R, int K, int pitch, Ids targets, int V, int *counters, int count,
+                          cudaStream_t s) {
+    __nv_bfloat16 *hi = static_cast<__nv_bfloat16 *>(to), *lo = hi + plane;
+    const int grid = blocks_for((long long)R * (pitch / 8));
+    const int each = type == TENSOR_F32 ? 4 : 2, wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld * each % 16 == 0;
+    if (type == TENSOR_F32)
+        return attn::launch_after_previous(planes_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<const float *>(src), ld, hi, lo, R, K, pitch, wide, targets, V,
+                                           counters, count);
+    return attn::launch_after_previous(planes_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, static_cast<const __nv_bfloat16 *>(src), ld, hi, lo, R, K, pitch, wide,
+                                       targets, V, counters, count);
+}
+
+template <int kTerms, bool kBackward>
+cudaError_t launch_tiles(const Maps &maps, const Problem &p, int sms, int *status, cudaStream_t s) {
+    constexpr int kSlots = kBackward ? kBackwardSlots : kForwardSlots;
+    return attn::launch_after_previous(tiles_kernel<kTerms, kBackward, kSlots>, dim3((unsigned)std::min(p.total, sms)), dim3(kThreads), sizeof(Smem<kSlots, kBackward>),
+                                       s, maps, p, status);
+}
+
+int check(const void *x, const void *w, const void *targets, const void *scratch, long long ldx, long long ldw, int type, int target_type, int rows, int V, int K) {
+    if (rows < 0 || V <= 0 || K <= 0 || ldx < K || ldw < K) return ATTN_ERR_ARGUMENT;
+    if ((type != TENSOR_F32 && type != TENSOR_BF16) || target_type < TENSOR_INT32 || target_type > TENSOR_IDS_F32) return ATTN_ERR_ARGUMENT;
+    const uintptr_t each = type == TENSOR_F32 ? 3 : 1, id = target_type == TENSOR_INT64 ? 7 : 3;
+    if ((reinterpret_cast<uintptr_t>(x) & each) || (reinterpret_cast<uintptr_t>(w) & each) || (reinterpret_cast<uintptr_t>(targets) & id) ||
+        (reinterpret_cast<uintptr_t>(scratch) & 255))
+        return ATTN_ERR_ALIGN;
+    // coordinates and numbers of tiles are 31-bit numbers, row strides of the copy engine 40-bit ones
+    if (rows > (1 << 30) || V > (1 << 30) || K > (1 << 24) || ldx > (1ll << 34) || ldw > (1ll << 34)) return ATTN_ERR_UNSUPPORTED;
+    if ((double)((rows + kTile - 1) / kTile + 1) * ((V + kTile - 1) / kTile + 1) > 1e9) return ATTN_ERR_UNSUPPORTED;
+    return ATTN_OK;
+}
+
+}  // namespace
+
+cudaError_t set_attributes() {
+    cudaError_t e = cudaSuccess;
+    auto set = [&](const void *kernel, size_t bytes) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    };
+    set(reinterpret_cast<const void *>(tiles_kernel<1, false, kForwardSlots>), sizeof(Smem<kForwardSlots, false>));
+    set(reinterpret_cast<const void *>(tiles_kernel<3, false, kForwardSlots>), sizeof(Smem<kForwardSlots, false>));
+    set(reinterpret_cast<const void *>(tiles_kernel<1, true, kBackwardSlots>), sizeof(Smem<kBackwardSlots, true>));
+    set(reinterpret_cast<const void *>(tiles_kernel<3, true, kBackwardSlots>), sizeof(Smem<kBackwardSlots, true>));
+    return e;
+}
+
+}  // namespace head
+
+extern "C" {
+
+size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
+    if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0) return 0;
+    return head::layout(x, w, ldx, ldw, type, rows, V, K, false, 148).total;
+}
+
+size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
+    if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0) return 0;
+    return head::layout(x, w, ldx, ldw, type, rows, V, K, true, attn::sm_count()).total;
+}
+
+int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
+                              int target_type, int rows, int V, int K, void *stream) {
+    using namespace head;
+    if (!x || !w || !targets || !losses || !lse || (rows > 0 && !scratch)) return ATTN_ERR_NULL;
+    int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
+    if (rc != ATTN_OK) return rc;
+    if ((reinterpret_cast<uintptr_t>(losses) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3)) return ATTN_ERR_ALIGN;
+    int *status = nullptr;
+    if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
+    if (rows == 0) return ATTN_OK;
+    const int sms = attn::sm_count();
+    const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, false, sms);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    char *base = static_cast<char *>(scratch);
+    cudaError_t e = cudaSuccess;
+    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
+    if (l.copy_x && (e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
+    Maps maps = {};
+    if ((rc = map_of(&maps.x, l.copy_x ? base + l.x : x, rows, K, l.copy_x ? l.pitch : rows > 1 ? ldx : l.pitch, l.plane_x, l.planes, kTile)) != 0) return rc;
+    if ((rc = map_of(&maps.w, l.copy_w ? base + l.w : w, V, K, l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch, l.plane_w, l.planes, kTile)) != 0) return rc;
+    Problem p = {};
+    p.M = rows, p.V = V, p.K = K;
+    set_fix(p, type);
+    p.tiles_m = (rows + kTile - 1) / kTile;
+    p.blocks_k = (K + kBlock - 1) / kBlock;
+    p.next_cols = up(V, kTile);
+    p.total = p.tiles_m * (p.next_cols / kTile);
+    p.targets = Ids{targets, target_type};
+    p.part = reinterpret_cast<float2 *>(base + l.part);
+    p.zt = reinterpret_cast<float *>(base + l.zt);
+    e = type == TENSOR_F32 ? launch_tiles<3, false>(maps, p, sms, status, s) : launch_tiles<1, false>(maps, p, sms, status, s);
+    if (e != cudaSuccess) return (int)e;
+    return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(256), 0, s, p.part, p.zt, p.targets, losses, lse, p.next_cols / kTile, rows, V);
+}
+
+int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw, void *scratch, long long ldx,
+                               long long ldw, long long lddw, int one_g, int type, int target_type, int rows, int V, int K, void *stream) {
+    using namespace head;
+    if (!g || !x || !w || !targets || !lse || (rows > 0 && !scratch) || (!dx && !dw)) return ATTN_ERR_NULL;
+    int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
+    if (rc != ATTN_OK) return rc;
+    if (dw && lddw < K) return ATTN_ERR_ARGUMENT;
+    const size_t each = type == TENSOR_F32 ? 4 : 2;
+    if ((reinterpret_cast<uintptr_t>(g) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3) || reinterpret_cast<uintptr_t>(dx) % each || reinterpret_cast<uintptr_t>(dw) % each)
+        return ATTN_ERR_ALIGN;
+    int *status = nullptr;
+    if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
+    if (rows == 0) return ATTN_OK;
+    const int sms = attn::sm_count();
+    const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, true, sms);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    char *base = static_cast<char *>(scratch);
+    cudaError_t e = cudaSuccess;
+    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
+    int *counters = reinterpret_cast<int *>(base + l.counters);
+    if ((e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{targets, target_type}, V, counters, l.pieces + 1, s)) != cudaSuccess) return (int)e;
+
+    const void *wp = l.copy_w ? base + l.w : w;
+    const long long pitch_w = l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch;
+    Maps maps = {};
+    if ((rc = map_of(&maps.x, base + l.x, rows, K, l.pitch, l.plane_x, l.planes, kTile)) != 0) return rc;
+    if ((rc = map_of(&maps.w, wp, V, K, pitch_w, l.plane_w, l.planes, kTile)) != 0) return rc;
+    if ((rc = map_of(&maps.x_mn, base + l.x, rows, K, l.pitch, l.plane_x, l.planes, kBlock)) != 0) return rc;
+    if ((rc = map_of(&maps.w_mn, wp, V, K, pitch_w, l.plane_w, l.planes, kBlock)) != 0) return rc;
+    Problem p = {};
+    p.M = rows, p.V = V, p.K = K;
+    set_fix(p, type);
+    p.tiles_m = (rows + kTile - 1) / kTile;
+    p.tiles_k = (K + kTile - 1) / kTile;
+    p.blocks_m = (rows + kBlock - 1) / kBlock;
+    p.blocks_k = (K + kBlock - 1) / kBlock;
+    p.dx_pieces = l.dx_pieces, p.dx_blocks = l.dx_blocks;
+    p.pitch = l.cols;
+    p.plane = (long long)l.plane_g;
+    p.targets = Ids{targets, target_type};
+    p.g = g, p.lse = lse, p.one_g = one_g;
+    p.dxp = reinterpret_cast<float *>(base + l.dxp);
+    p.dx_pitch = l.dx_pitch;
+    p.dw_out = dw, p.lddw = lddw;
+    for (int b : {32, 16})
+        if (!p.dw_wide && reinterpret_cast<uintptr_t>(dw) % b == 0 && (size_t)lddw * each % b == 0 && (size_t)K * each % b == 0) p.dw_wide = b;
+    for (int i = 0; i <= l.pieces; i++) {  // the products of piece i - 1, z of piece i
+        p.dx = i > 0 && dx ? p.tiles_m * p.tiles_k * l.dx_pieces : 0;
+        p.dw = 0;
+        if (i > 0) {
+            p.v0 = (i - 1) * l.cols;
+            p.cols = std::min(l.cols, up(V - p.v0, kTile));
+            if (dw) p.dw = p.cols / kTile * p.tiles_k;
+            p.first = i == 1;
+            const void *g0 = base + l.g[(i - 1) & 1];
+            if ((rc = map_of(&maps.g, g0, rows, p.cols, l.cols, l.plane_g, l.planes, kTile)) != 0) return rc;
+            if ((rc = map_of(&maps.g_mn, g0, rows, p.cols, l.cols, l.plane_g, l.planes, kBlock)) != 0) return rc;
+        }
+        int z = 0;
+        if (i < l.pieces) {
+            p.next_v0 = i * l.cols;
+            p.next_cols = std::min(l.cols, up(V - p.next_v0, kTile));
+            p.out = reinterpret_cast<__nv_bfloat16 *>(base + l.g[i & 1]);
+            z = p.tiles_m * (p.next_cols / kTile);
+        }
+        p.total = p.dx + p.dw + z;
+        p.counter = counters + i;
+        e = type == TENSOR_F32 ? launch_tiles<3, true>(maps, p, sms, status, s) : launch_tiles<1, true>(maps, p, sms, status, s);
+        if (e != cudaSuccess) return (int)e;
+    }
+    if (!dx) return ATTN_OK;
+    const int grid = blocks_for((long long)rows * (l.dx_pitch / 4));
+    const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
+    e = type == TENSOR_F32 ? attn::launch_after_previous(sum_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<float *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide)
+                         : attn::launch_after_previous(sum_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, static_cast<__nv_bfloat16 *>(dx), p.dxp, l.dx_pieces, rows, K,
+                                                       l.dx_pitch, wide);
+    return (int)e;
+}
+
+}  // extern "C"

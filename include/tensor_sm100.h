@@ -35,6 +35,40 @@ int tensor_sm100_gelu_forward(const float *x, float *y, size_t n, void *stream);
 /* dx[i] = g[i] * d/dx of the above at x[i] (overwritten, like the reference). */
 int tensor_sm100_gelu_backward(const float *g, const float *x, float *dx, size_t n, void *stream);
 
+/* Types of elements, and of tokens, positions and targets (the reference's dataloader.c:67-70 makes them fp32). */
+#define TENSOR_F32 0
+#define TENSOR_BF16 1
+#define TENSOR_INT32 0
+#define TENSOR_INT64 1
+#define TENSOR_IDS_F32 2
+
+/*
+ * y[t, :] = scale * table[tokens[t], :] + pos_table[positions[t], :] for t < n, computed in fp32 and rounded once.
+ *   table [V, C], pos_table [P, C]   of `type`, rows ld and pos_ld elements apart; pos_table may be NULL
+ *   tokens, positions [n]            of `id_type`; positions NULL: t % T, a token's place in its sequence of T
+ *   y [n, C]                         of `type`, contiguous
+ * A token outside 0 .. V - 1 (padding), or a position outside 0 .. P - 1, brings zeros.
+ * The reference's counterpart is embedding_forward_cuda_kernel (kernels/src/cuda/Embedding.cu:46-58), without scale and positions.
+ */
+int tensor_sm100_embedding_forward(const void *tokens, const void *table, const void *positions, const void *pos_table, void *y, long long n,
+                                   long long ld, long long pos_ld, float scale, int type, int id_type, int T, int C, int V, int P, void *stream);
+
+/*
+ * dtable[v, :]     += scale * sum of dy[t, :] over tokens[t] = v
+ * dpos_table[p, :] += sum of dy[t, :] over positions[t] = p
+ *   dy [n, C] of `type`, rows ld_dy elements apart; dtable [V, C], dpos_table [P, C] of `grad_type`, rows ld and pos_ld elements apart; one of
+ *   them may be NULL.  None of the three may overlap another (rows of one inside the gaps of another count as that).
+ * Sums are fp32 in an order that n fixes, rounded once where grad_type is TENSOR_BF16: the same bits in every call.  Tokens and positions
+ * outside their table have no part.  Rows that no token names are neither read nor written.
+ * scratch: tensor_sm100_embedding_backward_scratch_bytes bytes with P = 0 unless positions are given and V = 0 without dtable,
+ * 256-byte aligned (may be NULL if that is 0).
+ * The reference's counterpart is embedding_backward_cuda_kernel (kernels/src/cuda/Embedding.cu:60-74): an atomic addition a value.
+ */
+size_t tensor_sm100_embedding_backward_scratch_bytes(long long n, int C, int V, int P);
+int tensor_sm100_embedding_backward(const void *dy, const void *tokens, void *dtable, const void *positions, void *dpos_table, void *scratch,
+                                    long long n, long long ld_dy, long long ld, long long pos_ld, float scale, int type, int grad_type,
+                                    int id_type, int T, int C, int V, int P, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@
 #define XENT_SM100_H
 
 #include "attn_sm100.h"
+#include "tensor_sm100.h" /* types of elements and indices */
 
 #ifdef __cplusplus
 extern "C" {
@@ -59,6 +60,39 @@ int xent_sm100_backward(const float *g, const float *targets, const float *logsm
  */
 int xent_sm100_sample(const float *logits, const float *u, const float *temperature, const int *top_k, const float *top_p,
                       const float *min_p, int *tokens, long long ld, int rows, int C, void *stream);
+
+/*
+ * The vocabulary projection and the loss in one: z = x . w^T is never in memory.  (The reference keeps the logits, their log-softmax and
+ * their gradient: src/transformer.c:107-108, kernels/src/cuda/CrossEntropyLoss.cu.)
+ *
+ *   x [rows, K], w [V, K]   `type` TENSOR_F32 or TENSOR_BF16, rows ldx and ldw elements apart, any alignment of whole elements
+ *   targets [rows]          `target_type` TENSOR_INT32, TENSOR_INT64 or TENSOR_IDS_F32 (the reference's); a row whose target is not in 0 .. V - 1
+ *                           has no loss and no part in the gradients, whatever its x holds
+ *   lse[r]    = log sum_v exp z[r, v]
+ *   losses[r] = lse[r] - z[r, targets[r]], 0 for a row without a target
+ *
+ * The products of bf16 tensors are exact, those of fp32 tensors are made of two bf16 terms of each factor (16 bits of it; values
+ * above 3.38e38 in size have none); sums are fp32.  rows may be 0.
+ * scratch: xent_sm100_linear_forward_scratch_bytes bytes, 256-byte aligned; x and w are looked at for their alignment only there.
+ */
+size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K);
+int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch,
+                              long long ldx, long long ldw, int type, int target_type, int rows, int V, int K, void *stream);
+
+/*
+ * Its gradients, with lse from the forward call on the same x, w and targets:
+ *     G[r, v]  = g[r] (exp(z[r, v] - lse[r]) - [v = targets[r]])    g has one value per row, or one in all (one_g); 0 without a target
+ *     dx[r, :] = sum_v G[r, v] w[v, :]      overwritten, rows K elements apart, of `type`; may be NULL
+ *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call; may be NULL, but not both
+ * With bf16 tensors G is rounded to bf16 before these products, with fp32 tensors it is two bf16 terms like the others.  The results
+ * have the same bits in every call on GPUs of as many SMs.
+ * G is in memory for a piece of the vocabulary at a time: scratch of xent_sm100_linear_backward_scratch_bytes bytes (some hundred MB at
+ * most where rows are up to 100000, apart from copies of fp32 tensors), 256-byte aligned; 0: the sizes are refused.
+ */
+size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K);
+int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw,
+                               void *scratch, long long ldx, long long ldw, long long lddw, int one_g, int type, int target_type, int rows,
+                               int V, int K, void *stream);
 
 #ifdef __cplusplus
 }
