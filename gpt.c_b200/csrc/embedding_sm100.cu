@@ -35,42 +35,80 @@ constexpr int kThreads = 256, kUnits = 4;
 constexpr int kSortThreads = 1024, kSortCtas = 8, kSortWarps = kSortThreads / 32;
 constexpr int kBits = 9, kBins = 1 << kBits;  // of a pass of the sort, at most
 constexpr int kItems = 8;                     // places of a lane in a round of the sort
-constexpr int kAhead = 4;                     // places whose rows a thread asks for together
+constexpr int kAhead = 8;                     // places whose rows a thread asks for together
+constexpr int kBucketBits = 7, kBucketed = 8192;  // CTAs that sort without a cluster, and the longest list they take
+constexpr int kComparedBits = 9, kCompared = 1 << kComparedBits;  // places of a bucket that are compared each with each (tokens have 30 bits)
+constexpr int kFewTokens = 512;               // no sort is needed
 
-// kN columns of a row, as fp32.
+// kN columns of a row as they are in memory: one value, or 8, 16 or 32 bytes.  A thread asks for several before it looks at one: turned into fp32 where it
+// arrives, under a condition, each load was waited for by itself (runs of 49152 rows of 1600 bf16 values: 230 us).
 template <class T, int kN>
-__device__ __forceinline__ void load(float (&v)[kN], const T *p) {
-    if constexpr (kN == 1) {
-        v[0] = (float)*p;
-    } else if constexpr (sizeof(T) == 4) {
+struct Raw {
+    static constexpr int kWords = kN * sizeof(T) / 4;
+    uint32_t w[kWords ? kWords : 1];
+
+    // sum += these
+    __device__ __forceinline__ void add_to(float (&sum)[kN]) const {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(p + i);
-            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+            for (int i = 0; i < kN; i++) sum[i] += __uint_as_float(w[i]);
+        } else if constexpr (kN == 1) {
+            sum[0] += __uint_as_float(w[0] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN / 2; i++) sum[2 * i] += __uint_as_float(w[i] << 16), sum[2 * i + 1] += __uint_as_float(w[i] & 0xffff0000u);
         }
-    } else {
-        uint32_t w[kN / 2];
-        if constexpr (kN == 8) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p);
-        else *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p);
-#pragma unroll
-        for (int i = 0; i < kN / 2; i++) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
-}
-template <class T, int kN>
-__device__ __forceinline__ void store(T *p, const float (&v)[kN]) {
-    if constexpr (kN == 1) {
-        *p = (T)v[0];
-    } else if constexpr (sizeof(T) == 4) {
+    // these += scale * sum, rounded once
+    __device__ __forceinline__ void add(const float (&sum)[kN], float scale) {
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-    } else {
-        uint32_t w[kN / 2];
+            for (int i = 0; i < kN; i++) w[i] = __float_as_uint(fmaf(sum[i], scale, __uint_as_float(w[i])));
+        } else if constexpr (kN == 1) {
+            w[0] = pack_bf16x2(fmaf(sum[0], scale, __uint_as_float(w[0] << 16)), 0.f);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kN / 2; i++) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-        if constexpr (kN == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<uint4 *>(w);
-        else *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<uint2 *>(w);
+            for (int i = 0; i < kN / 2; i++)
+                w[i] = pack_bf16x2(fmaf(sum[2 * i], scale, __uint_as_float(w[i] << 16)), fmaf(sum[2 * i + 1], scale, __uint_as_float(w[i] & 0xffff0000u)));
+        }
     }
-}
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < (kWords ? kWords : 1); i++) w[i] = 0;
+    }
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (kWords == 8)
+            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+                         : "l"(p));
+        else if constexpr (kWords == 4) *reinterpret_cast<uint4 *>(w) = *reinterpret_cast<const uint4 *>(p);
+        else if constexpr (kWords == 2) *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(p);
+        else if constexpr (sizeof(T) == 4) w[0] = __float_as_uint(*p);
+        else w[0] = *reinterpret_cast<const unsigned short *>(p);
+    }
+    __device__ __forceinline__ void store(T *p) const {
+        if constexpr (kWords == 8)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                         "r"(w[6]), "r"(w[7])
+                         : "memory");
+        else if constexpr (kWords == 4) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(w);
+        else if constexpr (kWords == 2) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(w);
+        else if constexpr (sizeof(T) == 4) *p = __uint_as_float(w[0]);
+        else *reinterpret_cast<unsigned short *>(p) = (unsigned short)w[0];
+    }
+    // scale * this + y, rounded once to fp32, and to bf16 where the values are that
+    __device__ __forceinline__ void multiply_add(float scale, const Raw &y) {
+#pragma unroll
+        for (int i = 0; i < (kWords ? kWords : 1); i++) {
+            if constexpr (sizeof(T) == 4)
+                w[i] = __float_as_uint(fmaf(__uint_as_float(w[i]), scale, __uint_as_float(y.w[i])));
+            else
+                w[i] = pack_bf16x2(fmaf(__uint_as_float(w[i] << 16), scale, __uint_as_float(y.w[i] << 16)),
+                                   fmaf(__uint_as_float(w[i] & 0xffff0000u), scale, __uint_as_float(y.w[i] & 0xffff0000u)));
+        }
+    }
+};
 
 struct Lookup {
     const void *table, *pos_table;  // pos_table NULL: none
@@ -81,45 +119,42 @@ struct Lookup {
     float scale;
 };
 
-// kN columns at a time.
-template <class E, int kN>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(Lookup a, int words) {
+// kN columns at a time; a block takes `rows` rows of `words` such pieces.  i / words for i < 2^16 is the upper half of i * magic.
+template <class E, int kN, bool kPlaces>
+__global__ void __launch_bounds__(kThreads, 4) lookup_kernel(Lookup a, int rows, int words, unsigned magic) {
     pdl_launch_dependents();
     pdl_wait();
-    const long long total = a.n * words;
-    const long long first = (long long)blockIdx.x * (kThreads * kUnits) + threadIdx.x;
-    long long row[kUnits];
-    int col[kUnits], token[kUnits], place[kUnits];
+    const long long row0 = (long long)blockIdx.x * rows;
+    const int here = (int)min((long long)rows, a.n - row0) * words;
+    const unsigned place0 = kPlaces && !a.positions.p ? (unsigned)(row0 % a.T) : 0;
+    for (int i0 = threadIdx.x; i0 < here; i0 += kThreads * kUnits) {
+        int row[kUnits], col[kUnits], token[kUnits], place[kUnits];
 #pragma unroll
-    for (int u = 0; u < kUnits; u++) {
-        const long long i = first + u * kThreads;
-        row[u] = i / words;
-        col[u] = (int)(i - row[u] * words) * kN;
-        token[u] = place[u] = -1;
-        if (i >= total) {
-            row[u] = -1;
-            continue;
+        for (int u = 0; u < kUnits; u++) {
+            const int i = i0 + u * kThreads;
+            row[u] = rows == 1 ? 0 : words == 1 ? i : (int)__umulhi((unsigned)i, magic);
+            col[u] = (i - row[u] * words) * kN;
+            token[u] = place[u] = -1;
+            if (i >= here) continue;
+            token[u] = a.tokens.at(row0 + row[u], a.V);
+            if (kPlaces) {
+                const int p = a.positions.p ? a.positions.at(row0 + row[u], a.P) : (int)((place0 + (unsigned)row[u]) % (unsigned)a.T);
+                place[u] = p < a.P ? p : -1;
+            }
         }
-        token[u] = a.tokens.at(row[u], a.V);
-        if (a.pos_table) {
-            const long long p = a.positions.p ? a.positions.at(row[u], a.P) : row[u] % a.T;
-            place[u] = p < a.P ? (int)p : -1;
+        Raw<E, kN> x[kUnits], y[kPlaces ? kUnits : 1];
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) {
+            x[u].clear(), y[kPlaces ? u : 0].clear();
+            if (token[u] >= 0) x[u].load(static_cast<const E *>(a.table) + token[u] * a.ld + col[u]);
+            if (kPlaces && place[u] >= 0) y[u].load(static_cast<const E *>(a.pos_table) + place[u] * a.pos_ld + col[u]);
         }
-    }
-    float x[kUnits][kN], y[kUnits][kN];
 #pragma unroll
-    for (int u = 0; u < kUnits; u++) {
-#pragma unroll
-        for (int e = 0; e < kN; e++) x[u][e] = y[u][e] = 0.f;
-        if (token[u] >= 0) load<E, kN>(x[u], static_cast<const E *>(a.table) + token[u] * a.ld + col[u]);
-        if (place[u] >= 0) load<E, kN>(y[u], static_cast<const E *>(a.pos_table) + place[u] * a.pos_ld + col[u]);
-    }
-#pragma unroll
-    for (int u = 0; u < kUnits; u++) {
-        if (row[u] < 0) continue;
-#pragma unroll
-        for (int e = 0; e < kN; e++) x[u][e] = fmaf(x[u][e], a.scale, y[u][e]);
-        store<E, kN>(static_cast<E *>(a.y) + row[u] * a.C + col[u], x[u]);
+        for (int u = 0; u < kUnits; u++) {
+            if (i0 + u * kThreads >= here) continue;
+            x[u].multiply_add(a.scale, y[kPlaces ? u : 0]);
+            x[u].store(static_cast<E *>(a.y) + (row0 + row[u]) * a.C + col[u]);
+        }
     }
 }
 
@@ -130,7 +165,8 @@ struct List {
     long long ld;
     int V, n;
     float scale;
-    int *key[2], *at[2];  // tokens and their places, as the passes of the sort take turns
+    int2 *places[2];      // tokens and their places, as the passes of the sort take turns
+    const int2 *sorted;   // the one that holds the result
     int passes, bits;     // of a pass
     int length, ranges;   // places of a range
     float *head, *tail;   // [ranges, C]: parts of the run that came into a range, and of the one that leaves it
@@ -146,105 +182,331 @@ struct Gradient {
     long long pos_ld;
 };
 
+constexpr int kPitch = kBins + 1;  // four threads that add up a digit's counts read four rows of `warp` in different banks
+
 struct SortSmem {
-    int warp[kSortWarps][kBins];
-    int count[kBins], base[kBins], scan[kBins / 32];
+    int2 sorted[kSortThreads * kItems];  // a round's places by digit, so that they leave in runs
+    int warp[kSortWarps][kPitch];
+    int count[kBins], base[kBins], first[kBins], scan[kSortWarps];
+};
+
+// Running sums over the threads of a block: what is in front of `v`.
+__device__ __forceinline__ int in_front(int v, int *scan) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int left = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += left;
+    }
+    if (lane == 31) scan[warp] = sum;
+    __syncthreads();
+    const int other = lane < warp ? scan[lane] : 0;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, other) + sum - v;
+}
+
+// A block's round of a stable sort by one digit: up to kItems places a lane, all of a warp's next to each other.  Of places with the same digit, a
+// warp's own order is kept by votes on the digit's bits, that of the warps by running sums of their counts.
+struct Round {
+    int k[kItems], place[kItems], in_warp[kItems];  // k < 0: none
+    int items, bits, shift;
+
+    __device__ __forceinline__ int digit(int key) const { return key >> shift & ((1 << bits) - 1); }
+    __device__ __forceinline__ int first(int begin) const { return begin + (int)(threadIdx.x >> 5) * items * 32 + (int)(threadIdx.x & 31); }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int r = 0; r < kItems; r++) k[r] = -1;
+    }
+    // places[begin] to places[end - 1] (begin < end)
+    __device__ __forceinline__ void read(const int2 *places, int begin, int end) {
+        const int i0 = first(begin);
+        int2 e[kItems];
+#pragma unroll
+        for (int r = 0; r < kItems; r++) e[r] = __ldcg(places + min(i0 + 32 * r, end - 1));
+#pragma unroll
+        for (int r = 0; r < kItems; r++) k[r] = r < items && i0 + 32 * r < end ? e[r].x : -1, place[r] = e[r].y;
+    }
+    __device__ __forceinline__ void read(const Ids &ids, int V, int begin, int end) {
+        const int i0 = first(begin);
+        ids.many<kItems>(k, V, i0, 32, end);
+#pragma unroll
+        for (int r = 0; r < kItems; r++) {
+            place[r] = i0 + 32 * r;
+            if (r >= items || place[r] >= end) k[r] = -1;
+            else if (k[r] < 0) k[r] = V;
+        }
+    }
+    // What sm.warp and sm.count hold then: of each digit, places of the warps before each; of them all.
+    __device__ __forceinline__ void rank(SortSmem &sm) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bins = 1 << bits;
+        for (int i = lane; i < bins; i += 32) sm.warp[warp][i] = 0;
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < kItems; r++) {
+            if (r >= items) break;
+            const int d = digit(k[r]);
+            unsigned same = __ballot_sync(0xffffffffu, k[r] >= 0);  // lanes with this digit
+#pragma unroll
+            for (int b = 0; b < kBits; b++) {
+                if (b >= bits) break;
+                const bool set = d >> b & 1;
+                const unsigned vote = __ballot_sync(0xffffffffu, set);
+                same &= set ? vote : ~vote;
+            }
+            const int seen = k[r] < 0 ? 0 : sm.warp[warp][d];
+            __syncwarp();
+            if (k[r] >= 0 && lane == __ffs(same) - 1) sm.warp[warp][d] = seen + __popc(same);
+            __syncwarp();
+            in_warp[r] = seen + __popc(same & ((1u << lane) - 1));
+        }
+        __syncthreads();
+        for (int d0 = 0; d0 < bins; d0 += kSortThreads / 4) {  // two rounds of threads where there are 512 digits
+            const int d = d0 + (int)(threadIdx.x >> 2), q = threadIdx.x & 3;
+            int c[kSortWarps / 4], sum = 0;
+            if (d < bins) {
+#pragma unroll
+                for (int w = 0; w < kSortWarps / 4; w++) c[w] = sm.warp[q * (kSortWarps / 4) + w][d], sum += c[w];
+            }
+            int before = sum;
+            const int one = __shfl_up_sync(0xffffffffu, before, 1);
+            if (q >= 1) before += one;
+            const int two = __shfl_up_sync(0xffffffffu, before, 2);
+            if (q >= 2) before += two;
+            if (d < bins) {
+                if (q == 3) sm.count[d] = before;
+                before -= sum;
+#pragma unroll
+                for (int w = 0; w < kSortWarps / 4; w++) sm.warp[q * (kSortWarps / 4) + w][d] = before, before += c[w];
+            }
+        }
+        __syncthreads();
+    }
+    // The round's `count` places leave for out[sm.base[digit]] and on, by way of shared memory: stored there one by one each took a sector
+    // (49152 places: 14 us of 20 a pass).
+    __device__ __forceinline__ void scatter(SortSmem &sm, int2 *out, int count) {
+        const int d = threadIdx.x;
+        const int front = in_front(d < 1 << bits ? sm.count[d] : 0, sm.scan);
+        if (d < 1 << bits) sm.first[d] = front;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kItems; r++) {
+            if (k[r] < 0) continue;
+            const int digit_r = digit(k[r]);
+            sm.sorted[sm.first[digit_r] + sm.warp[threadIdx.x >> 5][digit_r] + in_warp[r]] = make_int2(k[r], place[r]);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < count; i += kSortThreads) {
+            const int2 e = sm.sorted[i];
+            out[sm.base[digit(e.x)] + i - sm.first[digit(e.x)]] = e;
+        }
+    }
 };
 
 // The places of a list in the order of their tokens, 2^bits tokens a pass, from the lowest digit on.  A cluster; each CTA has a piece.
 __device__ void sort_list(const List &l, SortSmem &sm) {
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int bins = 1 << l.bits;
+    const int rank = (int)cluster.block_rank(), bins = 1 << l.bits;
     const int piece = ((l.n + kSortCtas - 1) / kSortCtas + 31) / 32 * 32;
-    const int from = min((long long)l.n, (long long)rank * piece), to = min((long long)l.n, (long long)from + piece);
+    const int from = (int)min((long long)l.n, (long long)rank * piece), to = (int)min((long long)l.n, (long long)from + piece);
+    Round r;
+    r.items = min(kItems, (piece + kSortThreads - 1) / kSortThreads), r.bits = l.bits;
+    const int round = r.items * kSortThreads;
     for (int pass = 0; pass < l.passes; pass++) {
-        const int shift = pass * l.bits;
-        const volatile int *key = l.key[pass & 1], *at = l.at[pass & 1];
-        int *key_out = l.key[(pass & 1) ^ 1], *at_out = l.at[(pass & 1) ^ 1];
-        auto key_of = [&](int i) {
-            if (pass > 0) return (int)key[i];
-            const int k = l.ids.at(i, l.V);
-            return k < 0 ? l.V : k;
+        r.shift = pass * l.bits;
+        const int2 *in = l.places[pass & 1];
+        int2 *out = l.places[(pass & 1) ^ 1];
+        auto read = [&](int begin) {
+            if (begin >= to) r.clear();
+            else if (pass == 0) r.read(l.ids, l.V, begin, to);
+            else r.read(in, begin, to);
         };
-        for (int d = threadIdx.x; d < bins; d += kSortThreads) sm.count[d] = 0;
-        __syncthreads();
-        for (int i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(&sm.count[key_of(i) >> shift & (bins - 1)], 1);
+        const bool once = piece <= round;
+        const int d = threadIdx.x;
+        if (once) {  // the whole piece is in registers
+            read(from);
+            r.rank(sm);
+        } else {
+            if (d < bins) sm.count[d] = 0;
+            __syncthreads();
+            for (int begin = from; begin < to; begin += round) {
+                read(begin);
+#pragma unroll
+                for (int i = 0; i < kItems; i++)
+                    if (r.k[i] >= 0) atomicAdd(&sm.count[r.digit(r.k[i])], 1);
+            }
+        }
         cluster.sync();
         // where this CTA's places of each digit go
         int all = 0, before = 0;
-        const int d = threadIdx.x;
         if (d < bins) {
+            int v[kSortCtas];
+#pragma unroll
+            for (int c = 0; c < kSortCtas; c++) v[c] = cluster.map_shared_rank(sm.count, c)[d];
+#pragma unroll
             for (int c = 0; c < kSortCtas; c++) {
-                const int v = cluster.map_shared_rank(sm.count, c)[d];
-                if (c < rank) before += v;
-                all += v;
+                if (c < rank) before += v[c];
+                all += v[c];
             }
         }
-        int sum = all;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int left = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += left;
-        }
-        if (d < kBins && lane == 31) sm.scan[warp] = sum;
-        __syncthreads();
-        if (d < bins) {
-            int front = 0;
-            for (int k = 0; k < warp; k++) front += sm.scan[k];
-            sm.base[d] = front + sum - all + before;
-        }
-        for (int begin = from; begin < to; begin += kSortThreads * kItems) {
-            for (int i = lane; i < bins; i += 32) sm.warp[warp][i] = 0;
-            __syncwarp();
-            int k[kItems], place[kItems], in_warp[kItems];
-#pragma unroll
-            for (int r = 0; r < kItems; r++) {
-                const int i = begin + (warp * kItems + r) * 32 + lane;
-                k[r] = i < to ? key_of(i) : -1;
-                place[r] = i < to ? (pass > 0 ? at[i] : i) : 0;
+        const int front = in_front(all, sm.scan);
+        if (d < bins) sm.base[d] = front + before;
+        if (once) {
+            r.scatter(sm, out, to - from);
+        } else {
+            cluster.sync();  // the counts have been read
+            for (int begin = from; begin < to; begin += round) {
+                read(begin);
+                r.rank(sm);
+                r.scatter(sm, out, min(round, to - begin));
+                __syncthreads();
+                if (d < bins) sm.base[d] += sm.count[d];
+                __syncthreads();
             }
-#pragma unroll
-            for (int r = 0; r < kItems; r++) {
-                const int digit = k[r] < 0 ? -1 : k[r] >> shift & (bins - 1);
-                const unsigned same = __match_any_sync(0xffffffffu, digit);
-                const int seen = digit < 0 ? 0 : sm.warp[warp][digit];
-                __syncwarp();
-                if (digit >= 0 && lane == __ffs(same) - 1) sm.warp[warp][digit] = seen + __popc(same);
-                __syncwarp();
-                in_warp[r] = seen + __popc(same & ((1u << lane) - 1));
-            }
-            __syncthreads();
-            if (d < bins) {
-                int running = sm.base[d];
-                for (int w = 0; w < kSortWarps; w++) {
-                    const int c = sm.warp[w][d];
-                    sm.warp[w][d] = running;
-                    running += c;
-                }
-                sm.base[d] = running;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < kItems; r++) {
-                if (k[r] < 0) continue;
-                const int dst = sm.warp[warp][k[r] >> shift & (bins - 1)] + in_warp[r];
-                key_out[dst] = k[r];
-                at_out[dst] = place[r];
-            }
-            __syncthreads();
         }
         cluster.sync();  // what the others have written is there for the next pass, and nobody reads the counts any more
     }
 }
 
-// kN columns of grad += scale * sum.
-template <class G, int kN>
-__device__ __forceinline__ void add_to(G *p, const float (&old)[kN], const float (&sum)[kN], float scale) {
-    float v[kN];
+// The same for lists of up to kBucketed places, by CTAs that need not wait for each other: each looks through all tokens and takes those with its
+// lowest digit, whose order among each other it then makes by comparing each with each, or by the digits above.
+struct BucketSmem {
+    SortSmem sort;
+    int2 mine[kBucketed];
+};
+__device__ void sort_bucket(const List &l, int bucket, BucketSmem &sm) {
+    constexpr int kMost = kBucketed / kSortThreads;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int items = (l.n + kSortThreads - 1) / kSortThreads, i0 = warp * items * 32 + lane;
+    int less = 0, mine = 0;  // of this warp
+    unsigned votes[kMost];
+    int k[kMost];
+    l.ids.many<kMost>(k, l.V, i0, 32, l.n);
 #pragma unroll
-    for (int e = 0; e < kN; e++) v[e] = fmaf(sum[e], scale, old[e]);
-    store<G, kN>(p, v);
+    for (int r = 0; r < kMost; r++) {
+        const bool there = r < items && i0 + 32 * r < l.n;
+        if (k[r] < 0) k[r] = l.V;
+        const int d = k[r] & ((1 << kBucketBits) - 1);
+        less += __popc(__ballot_sync(0xffffffffu, there && d < bucket));
+        votes[r] = __ballot_sync(0xffffffffu, there && d == bucket);
+        mine += __popc(votes[r]);
+    }
+    int at = in_front(lane == 0 ? mine : 0, sm.sort.scan);
+    if (lane == 31) sm.sort.count[warp] = less, sm.sort.count[32 + warp] = mine;
+    at = __shfl_sync(0xffffffffu, at, 0);
+    __syncthreads();
+    const int base = __reduce_add_sync(0xffffffffu, sm.sort.count[lane]), count = __reduce_add_sync(0xffffffffu, sm.sort.count[32 + lane]);
+#pragma unroll
+    for (int r = 0; r < kMost; r++) {
+        if (votes[r] >> lane & 1) sm.mine[at + __popc(votes[r] & ((1u << lane) - 1))] = make_int2(k[r], i0 + 32 * r);
+        at += __popc(votes[r]);
+    }
+    __syncthreads();
+    if (count == 0) return;
+    if (count <= kCompared) {  // each with each: a token's other digits and its place in the bucket as one number
+        uint32_t *all = reinterpret_cast<uint32_t *>(sm.sort.sorted);
+        const int i = threadIdx.x, fours = (count + 3) / 4;
+        uint32_t own = 0xffffffffu;
+        if (i < count) own = (uint32_t)(sm.mine[i].x >> kBucketBits) << kComparedBits | (uint32_t)i;
+        if (i < 4 * fours) all[i] = own;
+        __syncthreads();
+        if (i >= count) return;
+        int rank = 0;
+        for (int j = 0; j < fours; j++) {
+            const uint4 o = reinterpret_cast<const uint4 *>(all)[j];
+            rank += (o.x < own) + (o.y < own) + (o.z < own) + (o.w < own);
+        }
+        const_cast<int2 *>(l.sorted)[base + rank] = sm.mine[i];
+        return;
+    }
+    Round r;
+    r.items = min(kItems, (count + kSortThreads - 1) / kSortThreads), r.bits = l.bits;
+    const int round = r.items * kSortThreads, d = threadIdx.x;
+    for (int pass = 0; pass < l.passes; pass++) {
+        r.shift = kBucketBits + pass * l.bits;
+        int2 *out = l.places[(l.passes - 1 - pass) & 1] + base;
+        const int2 *in = l.places[(l.passes - pass) & 1] + base;
+        auto read = [&](int begin) {
+            if (pass > 0) {
+                r.read(in, begin, count);
+                return;
+            }
+            const int first = r.first(begin);
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                const int2 e = sm.mine[min(first + 32 * i, count - 1)];
+                r.k[i] = i < r.items && first + 32 * i < count ? e.x : -1, r.place[i] = e.y;
+            }
+        };
+        if (count <= round) {
+            read(0);
+            r.rank(sm.sort);
+        } else {
+            if (d < 1 << r.bits) sm.sort.count[d] = 0;
+            __syncthreads();
+            for (int begin = 0; begin < count; begin += round) {
+                read(begin);
+#pragma unroll
+                for (int i = 0; i < kItems; i++)
+                    if (r.k[i] >= 0) atomicAdd(&sm.sort.count[r.digit(r.k[i])], 1);
+            }
+            __syncthreads();
+        }
+        const int front = in_front(d < 1 << r.bits ? sm.sort.count[d] : 0, sm.sort.scan);
+        if (d < 1 << r.bits) sm.sort.base[d] = front;
+        __syncthreads();
+        if (count <= round) {
+            r.scatter(sm.sort, out, count);
+        } else {
+            for (int begin = 0; begin < count; begin += round) {
+                read(begin);
+                r.rank(sm.sort);
+                r.scatter(sm.sort, out, min(round, count - begin));
+                __syncthreads();
+                if (d < 1 << r.bits) sm.sort.base[d] += sm.sort.count[d];
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int kN>
+__device__ __forceinline__ void put(float *p, const float (&sum)[kN]) {
+    Raw<float, kN> r;
+#pragma unroll
+    for (int e = 0; e < kN; e++) r.w[e] = __float_as_uint(sum[e]);
+    r.store(p);
+}
+template <int kN>
+__device__ __forceinline__ void clear(float (&v)[kN]) {
+#pragma unroll
+    for (int e = 0; e < kN; e++) v[e] = 0.f;
+}
+
+// The positions that are a token's place: dpos[t] += dy[t] + dy[t + T] + .., for the threads `first`, `first` + step, ..
+template <class E, class G, int kN>
+__device__ __forceinline__ void add_places(const Gradient &a, long long first, long long step) {
+    const int words = a.C / kN;
+    const long long T = min((long long)a.T, a.n), total = min(T, (long long)a.P) * words;
+    for (long long i = first; i < total; i += step) {
+        const long long t = i / words;
+        const int col = (int)(i - t * words) * kN;
+        float sum[kN] = {};
+        Raw<G, kN> old;
+        G *grad = static_cast<G *>(a.pos_grad) + t * a.pos_ld + col;
+        old.load(grad);
+        for (long long r = t; r < a.n; r += (long long)kAhead * a.T) {
+            Raw<E, kN> v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) v[u].load(static_cast<const E *>(a.dy) + min(r + (long long)u * a.T, a.n - 1) * a.ld + col);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++)
+                if (r + (long long)u * a.T < a.n) v[u].add_to(sum);
+        }
+        old.add(sum, 1.f);
+        old.store(grad);
+    }
 }
 
 // Clusters 0 .. lists - 1 sort; the others add up the positions that are a token's place.
@@ -253,131 +515,237 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const __grid_cons
     extern __shared__ __align__(16) uint8_t smem_raw[];
     pdl_launch_dependents();
     pdl_wait();
-    const int cluster = blockIdx.x / kSortCtas;
-    if (cluster < a.lists) {
-        sort_list(a.list[cluster], *reinterpret_cast<SortSmem *>(smem_raw));
-        return;
-    }
-    const int words = a.C / kN;
-    const long long T = min((long long)a.T, a.n), total = min(T, (long long)a.P) * words;
-    const long long step = (long long)(gridDim.x - a.lists * kSortCtas) * kSortThreads;
-    for (long long i = (long long)(blockIdx.x - a.lists * kSortCtas) * kSortThreads + threadIdx.x; i < total; i += step) {
-        const long long t = i / words;
-        const int col = (int)(i - t * words) * kN;
-        float sum[kN] = {}, old[kN];
-        G *grad = static_cast<G *>(a.pos_grad) + t * a.pos_ld + col;
-        load<G, kN>(old, grad);
-        for (long long r = t; r < a.n; r += (long long)kAhead * a.T) {
-            float v[kAhead][kN];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-#pragma unroll
-                for (int e = 0; e < kN; e++) v[u][e] = 0.f;
-                if (r + (long long)u * a.T < a.n) load<E, kN>(v[u], static_cast<const E *>(a.dy) + (r + (long long)u * a.T) * a.ld + col);
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-#pragma unroll
-                for (int e = 0; e < kN; e++) sum[e] += v[u][e];
-        }
-        add_to<G, kN>(grad, old, sum, 1.f);
-    }
+    const int cluster = blockIdx.x / kSortCtas, others = a.lists * kSortCtas;
+    if (cluster < a.lists) sort_list(a.list[cluster], *reinterpret_cast<SortSmem *>(smem_raw));
+    else add_places<E, G, kN>(a, (long long)(blockIdx.x - others) * kSortThreads + threadIdx.x, (long long)(gridDim.x - others) * kSortThreads);
 }
 
-// A range of a sorted list: blockIdx.x; columns: threads of blockIdx.y.
-template <class E, class G, int kN>
-__global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ Gradient a) {
+// A CTA for each bucket of each list.
+__global__ void __launch_bounds__(kSortThreads, 1) bucket_kernel(const __grid_constant__ Gradient a) {
+    extern __shared__ __align__(16) uint8_t smem_raw[];
     pdl_launch_dependents();
     pdl_wait();
-    const int which = blockIdx.x < (unsigned)a.list[0].ranges ? 0 : 1;
+    const int which = blockIdx.x >> kBucketBits;
+    sort_bucket(a.list[which], blockIdx.x & ((1 << kBucketBits) - 1), *reinterpret_cast<BucketSmem *>(smem_raw));
+}
+
+// A warp takes a range of a sorted list, and 32 kN columns (blockIdx.y).  Blocks behind the ranges add up the positions that are a token's place
+// where the sort was not a launch of few CTAs, which leaves room for that.
+template <class E, class G, int kN>
+__global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ Gradient a, int blocks) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if ((int)blockIdx.x >= blocks) {
+        const long long others = (long long)(gridDim.x - blocks) * gridDim.y;
+        add_places<E, G, kN>(a, ((long long)(blockIdx.x - blocks) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x, others * kThreads);
+        return;
+    }
+    const int lane = threadIdx.x & 31, unit = (int)blockIdx.x * (kThreads / 32) + (int)(threadIdx.x >> 5);
+    const int which = unit < a.list[0].ranges ? 0 : 1;
     const List &l = a.list[which];
-    const int range = blockIdx.x - (which ? a.list[0].ranges : 0);
-    const int *key = l.key[l.passes & 1], *at = l.at[l.passes & 1];
-    const int col = (blockIdx.y * blockDim.x + threadIdx.x) * kN;
-    if (col >= a.C) return;
-    const int from = range * l.length, to = min(l.n, from + l.length);
-    const bool from_before = from > 0 && key[from - 1] == key[from], goes_on = to < l.n && key[to] == key[to - 1];
+    const int range = unit - (which ? a.list[0].ranges : 0);
+    if (range >= l.ranges || which >= a.lists) return;
+    const int2 *places = l.sorted;
+    const int col = ((int)blockIdx.y * 32 + lane) * kN;
+    const bool inside = col < a.C;
+    const int from = range * l.length, count = min(l.n - from, l.length);  // up to 32
+    const int2 place = lane < count ? places[from + lane] : make_int2(-1, 0);
+    const int mine = place.x, row = place.y;
+    const int outer = lane == 0 ? (from > 0 ? places[from - 1].x : -1) : lane == 1 && from + count < l.n ? places[from + count].x : -1;
+    const int in_front = __shfl_sync(0xffffffffu, outer, 0), behind = __shfl_sync(0xffffffffu, outer, 1);
+    const int first = __shfl_sync(0xffffffffu, mine, 0), last = __shfl_sync(0xffffffffu, mine, count - 1);
+    bool began = in_front != first;  // the run began in this range
+    const bool goes_on = behind == last;
     float sum[kN] = {};
-    bool began = !from_before;  // the run began in this range
-    for (int i0 = from; i0 < to; i0 += kAhead) {
+    const E *dy = static_cast<const E *>(a.dy) + (inside ? col : 0);
+    G *grad = static_cast<G *>(l.grad) + (inside ? col : 0);
+    for (int i0 = 0; i0 < count; i0 += kAhead) {
+        Raw<E, kN> v[kAhead];
+        Raw<G, kN> old[kAhead];
         int k[kAhead + 1];
-        float v[kAhead][kN], old[kAhead][kN];
 #pragma unroll
-        for (int u = 0; u <= kAhead; u++) k[u] = i0 + u < to ? key[i0 + u] : -1;
+        for (int u = 0; u < kAhead; u++) v[u].load(dy + __shfl_sync(0xffffffffu, row, (i0 + u) & 31) * a.ld);  // (behind the range: the row of place 0)
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) {
-            if (k[u] < 0 || k[u] >= l.V) continue;
-            load<E, kN>(v[u], static_cast<const E *>(a.dy) + at[i0 + u] * a.ld + col);
-            if (k[u + 1] != k[u]) load<G, kN>(old[u], static_cast<G *>(l.grad) + k[u] * l.ld + col);
-        }
+        for (int u = 0; u <= kAhead; u++) k[u] = i0 + u < 32 ? __shfl_sync(0xffffffffu, mine, (i0 + u) & 31) : -1;
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+            if (k[u + 1] != k[u] && k[u] < l.V && k[u] >= 0) old[u].load(grad + k[u] * l.ld);
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-            if (k[u] < 0 || k[u] >= l.V) continue;
-#pragma unroll
-            for (int e = 0; e < kN; e++) sum[e] += v[u][e];
+            if (k[u] < 0) break;
+            if (k[u] >= l.V) {  // no token
+                began = true;
+                continue;
+            }
+            v[u].add_to(sum);
             if (k[u + 1] == k[u]) continue;
-            if (!began) store<float, kN>(l.head + (long long)range * a.C + col, sum);
-            else if (i0 + u == to - 1 && goes_on) store<float, kN>(l.tail + (long long)range * a.C + col, sum);
-            else add_to<G, kN>(static_cast<G *>(l.grad) + k[u] * l.ld + col, old[u], sum, l.scale);
+            if (inside) {
+                if (!began) {
+                    put<kN>(l.head + (long long)range * a.C + col, sum);
+                } else if (i0 + u == count - 1 && goes_on) {
+                    put<kN>(l.tail + (long long)range * a.C + col, sum);
+                } else {
+                    old[u].add(sum, l.scale);
+                    old[u].store(grad + k[u] * l.ld);
+                }
+            }
             began = true;
-#pragma unroll
-            for (int e = 0; e < kN; e++) sum[e] = 0.f;
+            clear(sum);
         }
     }
 }
 
-// Runs that leave the range blockIdx.x in which they began: their parts, warps taking every eighth.
+// Runs that leave the range in which they began: the sum of their parts, in the order of the list.  A warp looks at a range and takes runs of
+// up to kFew parts itself; a block takes the longer ones of its eight ranges one by one, its warps every eighth part.
+constexpr int kFew = 8;
 template <class G, int kN>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Gradient a) {
     pdl_launch_dependents();
     pdl_wait();
     __shared__ float part[8][32 * kN];
-    const int which = blockIdx.x < (unsigned)a.list[0].ranges ? 0 : 1;
+    __shared__ int last_of[8], key_of[8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = ((int)blockIdx.y * 32 + lane) * kN;
+    const bool inside = col < a.C;
+    const int blocks0 = (a.list[0].ranges + 7) / 8, which = blockIdx.x < (unsigned)blocks0 ? 0 : 1;
     const List &l = a.list[which];
-    const int range = blockIdx.x - (which ? a.list[0].ranges : 0);
-    const int *key = l.key[l.passes & 1];
-    const int from = range * l.length, to = min(l.n, from + l.length);
-    const int k = key[to - 1];
-    if (to >= l.n || k >= l.V || key[to] != k || (from > 0 && key[from - 1] == k)) return;
-    int lo = to, hi = l.n;  // the run ends in front of the first place behind `to` with another token
-    while (lo < hi) {
-        const int mid = lo + (hi - lo) / 2;
-        if (key[mid] == k) lo = mid + 1;
-        else hi = mid;
-    }
-    const int last = (lo - 1) / l.length;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = (blockIdx.y * 32 + lane) * kN;
-    float sum[kN] = {};
-    if (col < a.C) {
-        for (int r0 = range + 1 + warp; r0 <= last; r0 += 8 * kAhead) {
-            float v[kAhead][kN];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) {
-#pragma unroll
-                for (int e = 0; e < kN; e++) v[u][e] = 0.f;
-                if (r0 + 8 * u <= last) load<float, kN>(v[u], l.head + (long long)(r0 + 8 * u) * a.C + col);
+    const int range0 = ((int)blockIdx.x - (which ? blocks0 : 0)) * 8, range = range0 + warp;
+    const int2 *places = l.sorted;
+    int last = -1, k = -1;  // the last range that the run reaches, -1: none begins here and goes on
+    if (range < l.ranges) {
+        const int from = range * l.length, to = min(l.n, from + l.length);
+        const int at = lane == 0 ? to - 1 : lane == 1 ? to : from - 1;
+        const int seen = lane < 3 && at >= 0 && at < l.n ? places[at].x : -1;
+        k = __shfl_sync(0xffffffffu, seen, 0);
+        if (to < l.n && k < l.V && __shfl_sync(0xffffffffu, seen, 1) == k && __shfl_sync(0xffffffffu, seen, 2) != k) {
+            int lo = to, hi = l.n;  // places[lo] has k; where it ends is sought 32 places at a time
+            while (hi - lo > 1) {
+                const int step = (int)(((long long)hi - lo + 31) / 32);
+                const long long probe = lo + (lane + 1ll) * step;
+                const int same = __popc(__ballot_sync(0xffffffffu, probe < hi && places[probe < hi ? probe : lo].x == k));
+                lo += same * step;
+                hi = (int)min((long long)hi, (long long)lo + step);
             }
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-#pragma unroll
-                for (int e = 0; e < kN; e++) sum[e] += v[u][e];
+            last = lo / l.length;
         }
     }
+    if (lane == 0) last_of[warp] = last - range > kFew ? last : -1, key_of[warp] = k;
+    auto finish = [&](int r, int run, float(&sum)[kN]) {
+        Raw<float, kN> first;
+        Raw<G, kN> old;
+        G *grad = static_cast<G *>(l.grad) + run * l.ld + col;
+        old.load(grad);
+        first.load(l.tail + (long long)r * a.C + col);
+        first.add_to(sum);
+        old.add(sum, l.scale);
+        old.store(grad);
+    };
+    if (last >= 0 && last - range <= kFew && inside) {
+        Raw<float, kN> v[kFew];
+        float sum[kN] = {};
 #pragma unroll
-    for (int e = 0; e < kN; e++) part[warp][lane * kN + e] = sum[e];
-    __syncthreads();
-    if (warp != 0 || col >= a.C) return;
-    float old[kN], first[kN];
-    G *grad = static_cast<G *>(l.grad) + k * l.ld + col;
-    load<G, kN>(old, grad);
-    load<float, kN>(first, l.tail + (long long)range * a.C + col);
+        for (int u = 0; u < kFew; u++) v[u].load(l.head + (long long)min(range + 1 + u, last) * a.C + col);
 #pragma unroll
-    for (int e = 0; e < kN; e++) {
-        sum[e] = first[e];
-#pragma unroll
-        for (int w = 0; w < 8; w++) sum[e] += part[w][lane * kN + e];
+        for (int u = 0; u < kFew; u++)
+            if (range + 1 + u <= last) v[u].add_to(sum);
+        finish(range, k, sum);
     }
-    add_to<G, kN>(grad, old, sum, l.scale);
+    __syncthreads();
+    for (int w = 0; w < 8; w++) {
+        const int end = last_of[w];
+        if (end < 0) continue;
+        float sum[kN] = {};
+        if (inside) {
+            for (int r0 = range0 + w + 1 + warp; r0 <= end; r0 += 8 * kAhead) {
+                Raw<float, kN> v[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) v[u].load(l.head + (long long)min(r0 + 8 * u, end) * a.C + col);
+#pragma unroll
+                for (int u = 0; u < kAhead; u++)
+                    if (r0 + 8 * u <= end) v[u].add_to(sum);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kN; e++) part[warp][lane * kN + e] = sum[e];
+        __syncthreads();
+        if (warp == 0 && inside) {
+            clear(sum);
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int e = 0; e < kN; e++) sum[e] += part[i][lane * kN + e];
+            finish(range0 + w, key_of[w], sum);
+        }
+        __syncthreads();
+    }
+}
+
+// Few tokens: a block for each place t of each list.  The first place of a token adds up the rows of all; `groups` threads share a column's
+// rows, each taking every groups-th.  The blocks behind them add up the positions that are a token's place.
+template <class E, class G, int kN>
+__global__ void __launch_bounds__(kSortThreads) few_kernel(const __grid_constant__ Gradient a, int width, int groups) {
+    pdl_launch_dependents();
+    pdl_wait();
+    extern __shared__ __align__(16) float shared[];
+    __shared__ int list[kFewTokens], counts[kFewTokens / 32], of[1];
+    const int n = (int)a.n, which = blockIdx.x / n;
+    if (which >= a.lists) {
+        const int threads = width * groups, b = (int)blockIdx.x - a.lists * n;
+        if ((int)threadIdx.x < threads) add_places<E, G, kN>(a, (long long)b * threads + threadIdx.x, (long long)(gridDim.x - a.lists * n) * threads);
+        return;
+    }
+    const List &l = a.list[which];
+    const int t = blockIdx.x - which * n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // every warp but the last ones looks at 32 places; places in front of t with its token: nothing to do here
+    if (threadIdx.x == 0) of[0] = l.ids.at(t, l.V);
+    const int mine = (int)threadIdx.x < n ? l.ids.at(threadIdx.x, l.V) : -1;
+    __syncthreads();
+    const int k = of[0];
+    const unsigned same = __ballot_sync(0xffffffffu, mine == k && (int)threadIdx.x < n);
+    if (lane == 0 && warp < kFewTokens / 32) counts[warp] = __popc(same);
+    const bool before = mine == k && (int)threadIdx.x < t;
+    if (__syncthreads_or(before) || k < 0) return;
+    int front = 0, all = 0;
+    for (int w = 0; w < (n + 31) / 32; w++) {
+        if (w < warp) front += counts[w];
+        all += counts[w];
+    }
+    if (same >> lane & 1) list[front + __popc(same & ((1u << lane) - 1))] = threadIdx.x;
+    __syncthreads();
+    const int group = threadIdx.x / width, column = threadIdx.x - group * width;
+    for (int c0 = 0; c0 < a.C; c0 += width * kN) {
+        const int col = c0 + column * kN;
+        const bool inside = col < a.C && group < groups;
+        float sum[kN] = {};
+        Raw<G, kN> old;
+        G *grad = static_cast<G *>(l.grad) + k * l.ld + col;
+        if (inside && group == 0) old.load(grad);
+        if (inside) {
+            for (int i = group; i < all; i += groups * kAhead) {
+                Raw<E, kN> v[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; u++) v[u].load(static_cast<const E *>(a.dy) + list[min(i + u * groups, all - 1)] * a.ld + col);
+#pragma unroll
+                for (int u = 0; u < kAhead; u++)
+                    if (i + u * groups < all) v[u].add_to(sum);
+            }
+        }
+        if (all > 1 && groups > 1) {
+            if (group > 0 && group < groups) {
+#pragma unroll
+                for (int e = 0; e < kN; e++) shared[((group - 1) * width + column) * kN + e] = sum[e];
+            }
+            __syncthreads();
+            if (group == 0) {
+                for (int g = 1; g < groups; g++)
+#pragma unroll
+                    for (int e = 0; e < kN; e++) sum[e] += shared[((g - 1) * width + column) * kN + e];
+            }
+            __syncthreads();
+        }
+        if (inside && group == 0) {
+            old.add(sum, l.scale);
+            old.store(grad);
+        }
+    }
 }
 
 // ---- host side ----
@@ -395,8 +763,17 @@ bool overlap(const void *a, long long rows_a, long long ld_a, uintptr_t each_a, 
     return bits(a) < end_b && bits(b) < end_a;
 }
 
-// Places of a range: short ones where there are few, so that every SM has some.
-int range_length(long long n) { return n <= 2048 ? 4 : n <= 16384 ? 8 : n <= 32768 ? 16 : n <= 65536 ? 32 : 64; }
+// Places of a range, which a warp takes: 32 at most.
+int range_length(long long n) { return n <= 8192 ? 8 : n <= 32768 ? 16 : 32; }
+
+template <class E>
+cudaError_t launch_lookup(const Lookup &a, int bytes, int rows, int words, cudaStream_t s) {
+    const unsigned magic = words > 1 ? (unsigned)(((1ull << 32) + words - 1) / words) : 0;
+    const dim3 grid((unsigned)((a.n + rows - 1) / rows)), block(kThreads);
+    auto kernel = a.pos_table ? (bytes == 16 ? lookup_kernel<E, 16 / sizeof(E), true> : lookup_kernel<E, 1, true>)
+                              : (bytes == 32 ? lookup_kernel<E, 32 / sizeof(E), false> : bytes == 16 ? lookup_kernel<E, 16 / sizeof(E), false> : lookup_kernel<E, 1, false>);
+    return attn::launch_after_previous(kernel, grid, block, 0, s, a, rows, words, magic);
+}
 
 // Scratch of one list; where it is set up if `base` is given.
 size_t list_bytes(long long n, int C, int V, List *l, char *base) {
@@ -410,15 +787,17 @@ size_t list_bytes(long long n, int C, int V, List *l, char *base) {
     const long long ranges = (n + length - 1) / length;
     int need = 1;
     while (need < 31 && (1ll << need) <= V) need++;  // V itself stands for no token
+    if (n <= kBucketed) need = std::max(1, need - kBucketBits);
     const int passes = (need + kBits - 1) / kBits;
     if (l) {
         l->length = length, l->ranges = (int)ranges;
         l->passes = passes, l->bits = (need + passes - 1) / passes;
     }
     for (int i = 0; i < 2; i++) {
-        int *k = reinterpret_cast<int *>(take((size_t)n * 4)), *p = reinterpret_cast<int *>(take((size_t)n * 4));
-        if (l) l->key[i] = k, l->at[i] = p;
+        int2 *places = reinterpret_cast<int2 *>(take((size_t)n * sizeof(int2)));
+        if (l) l->places[i] = places;
     }
+    if (l) l->sorted = l->places[n <= kBucketed ? 0 : passes & 1];
     float *head = reinterpret_cast<float *>(take((size_t)ranges * C * 4)), *tail = reinterpret_cast<float *>(take((size_t)ranges * C * 4));
     if (l) l->head = head, l->tail = tail;
     return at;
@@ -427,32 +806,46 @@ size_t list_bytes(long long n, int C, int V, List *l, char *base) {
 template <class E, class G, int kN>
 cudaError_t launch_gradient(const Gradient &a, cudaStream_t s) {
     const int words = a.C / kN;
-    long long clusters = a.lists;
-    if (a.T > 0) {
-        const long long work = std::min(std::min((long long)a.T, a.n), (long long)a.P) * words;
-        clusters += std::max(1ll, std::min((work + kSortThreads * kSortCtas - 1) / (kSortThreads * kSortCtas), 17ll));
+    const long long places = a.T > 0 ? std::min(std::min((long long)a.T, a.n), (long long)a.P) * words : 0;
+    if (a.n <= kFewTokens) {
+        const int width = std::min(256, (words + 31) / 32 * 32), groups = std::max(1, std::min(4, kSortThreads / width));
+        const int threads = std::max(width * groups, kFewTokens);
+        const long long blocks = a.lists * a.n + std::min(600ll, (places + width * groups - 1) / (width * groups));
+        return attn::launch_after_previous(few_kernel<E, G, kN>, dim3((unsigned)blocks), dim3((unsigned)threads), sizeof(float) * kN * width * (groups - 1), s, a, width, groups);
     }
-    if (a.lists == 0 && a.T == 0) return cudaSuccess;
-    cudaError_t e = attn::launch_clusters_after_previous(sort_kernel<E, G, kN>, dim3((unsigned)(clusters * kSortCtas)), dim3(kSortThreads), sizeof(SortSmem), kSortCtas, s, a);
-    if (e != cudaSuccess || a.lists == 0) return e;
+    cudaError_t e;
+    const long long all = (places + kSortThreads - 1) / kSortThreads;  // blocks for the positions that are a token's place
+    if (a.n <= kBucketed) {
+        e = a.lists == 0 ? cudaSuccess : attn::launch_after_previous(bucket_kernel, dim3((unsigned)(a.lists << kBucketBits)), dim3(kSortThreads), sizeof(BucketSmem), s, a);
+    } else {
+        const long long clusters = a.lists + std::min((all + kSortCtas - 1) / kSortCtas, 17ll);
+        e = attn::launch_clusters_after_previous(sort_kernel<E, G, kN>, dim3((unsigned)(clusters * kSortCtas)), dim3(kSortThreads), sizeof(SortSmem), kSortCtas, s, a);
+    }
+    if (e != cudaSuccess || (a.lists == 0 && a.n > kBucketed)) return e;
+    const unsigned slices = (unsigned)((words + 31) / 32);
     const int ranges = a.list[0].ranges + (a.lists > 1 ? a.list[1].ranges : 0);
-    const int threads = std::min(kThreads, (words + 31) / 32 * 32), slices = (words + threads - 1) / threads;
-    e = attn::launch_after_previous(runs_kernel<E, G, kN>, dim3((unsigned)ranges, (unsigned)slices), dim3((unsigned)threads), 0, s, a);
-    if (e != cudaSuccess) return e;
-    return attn::launch_after_previous(join_kernel<G, kN>, dim3((unsigned)ranges, (unsigned)((words + 31) / 32)), dim3(256), 0, s, a);
+    const int groups = (ranges + kThreads / 32 - 1) / (kThreads / 32);
+    const long long others = a.n <= kBucketed ? (std::min((places + kThreads - 1) / kThreads, 1184ll) + slices - 1) / slices : 0;
+    e = attn::launch_after_previous(runs_kernel<E, G, kN>, dim3((unsigned)(groups + others), slices), dim3(kThreads), 0, s, a, groups);
+    if (e != cudaSuccess || a.lists == 0) return e;
+    const int blocks = (a.list[0].ranges + 7) / 8 + (a.lists > 1 ? (a.list[1].ranges + 7) / 8 : 0);
+    return attn::launch_after_previous(join_kernel<G, kN>, dim3((unsigned)blocks, slices), dim3(256), 0, s, a);
 }
 
 template <class E, class G>
 cudaError_t launch_gradient(const Gradient &a, bool wide, cudaStream_t s) {
-    return wide ? launch_gradient<E, G, 4>(a, s) : launch_gradient<E, G, 1>(a, s);
+    return wide ? launch_gradient<E, G, 16 / sizeof(E)>(a, s) : launch_gradient<E, G, 1>(a, s);
 }
 
 template <class E>
 cudaError_t set(cudaError_t e) {
-    auto one = [&](auto *kernel) {
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SortSmem));
+    auto one = [&](auto *kernel, size_t bytes) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     };
-    one(sort_kernel<E, float, 4>), one(sort_kernel<E, float, 1>), one(sort_kernel<E, __nv_bfloat16, 4>), one(sort_kernel<E, __nv_bfloat16, 1>);
+    constexpr int kN = 16 / sizeof(E);
+    one(sort_kernel<E, float, kN>, sizeof(SortSmem)), one(sort_kernel<E, float, 1>, sizeof(SortSmem));
+    one(sort_kernel<E, __nv_bfloat16, kN>, sizeof(SortSmem)), one(sort_kernel<E, __nv_bfloat16, 1>, sizeof(SortSmem));
+    one(bucket_kernel, sizeof(BucketSmem));
     return e;
 }
 
@@ -475,23 +868,21 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
     const int rc = attn::device_status_word(&status);
     if (rc != ATTN_OK) return rc;
     if (n == 0) return ATTN_OK;
-    const bool wide = ((embed::bits(table) | embed::bits(pos_table) | embed::bits(y)) & 15) == 0 && C * each % 16 == 0 && ld * each % 16 == 0 &&
-                      (!pos_table || pos_ld * each % 16 == 0);
-    const int words = wide ? (int)(C * each / 16) : C;
-    const long long per = embed::kThreads * embed::kUnits;
-    if (n > (1ll << 40) / C || (n * words + per - 1) / per > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;
+    if (n > (1ll << 40) / C || C > (1 << 20)) return ATTN_ERR_UNSUPPORTED;
+    // 32 bytes at a time where every row allows it and there is one table (two rows of four such pieces take too many registers), else 16, else a value
+    const uintptr_t all = embed::bits(table) | embed::bits(pos_table) | embed::bits(y) | C * each | (uintptr_t)ld * each | (pos_table ? (uintptr_t)pos_ld * each | 16 : 0);
+    const int bytes = all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : (int)each, words = (int)(C * each / bytes);
+    // a block has a piece for each thread, or four where that leaves blocks enough
+    const long long pieces = n * words, per = pieces >= embed::kThreads * embed::kUnits * 600ll ? embed::kThreads * embed::kUnits : embed::kThreads;
+    const int rows = (int)std::max(1ll, per / words);
+    if ((n + rows - 1) / rows > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;
     const embed::Lookup a{table, pos_table, y, ld, pos_ld, n, Ids{tokens, id_type}, Ids{positions, id_type}, T, C, V, P, scale};
-    const dim3 grid((unsigned)((n * words + per - 1) / per)), block(embed::kThreads);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (type == TENSOR_F32)
-        return (int)(wide ? attn::launch_after_previous(embed::lookup_kernel<float, 4>, grid, block, 0, s, a, words)
-                          : attn::launch_after_previous(embed::lookup_kernel<float, 1>, grid, block, 0, s, a, words));
-    return (int)(wide ? attn::launch_after_previous(embed::lookup_kernel<__nv_bfloat16, 8>, grid, block, 0, s, a, words)
-                      : attn::launch_after_previous(embed::lookup_kernel<__nv_bfloat16, 1>, grid, block, 0, s, a, words));
+    return (int)(type == TENSOR_F32 ? embed::launch_lookup<float>(a, bytes, rows, words, static_cast<cudaStream_t>(stream))
+                                    : embed::launch_lookup<__nv_bfloat16>(a, bytes, rows, words, static_cast<cudaStream_t>(stream)));
 }
 
 size_t tensor_sm100_embedding_backward_scratch_bytes(long long n, int C, int V, int P) {
-    if (n <= 0 || n > (1 << 30) || C <= 0 || V < 0 || P < 0) return 0;
+    if (n <= 0 || n > (1 << 30) || C <= 0 || C > (1 << 20) || V < 0 || V > (1 << 30) || P < 0 || P > (1 << 30)) return 0;
     return (V ? embed::list_bytes(n, C, V, nullptr, nullptr) : 0) + (P ? embed::list_bytes(n, C, P, nullptr, nullptr) : 0);
 }
 
@@ -507,7 +898,7 @@ int tensor_sm100_embedding_backward(const void *dy, const void *tokens, void *dt
     if (embed::bits(dy) % each || (embed::bits(dtable) | embed::bits(dpos_table)) % grad_each || (embed::bits(scratch) & 255) ||
         ((embed::bits(tokens) | embed::bits(positions)) & embed::id_mask(id_type)))
         return ATTN_ERR_ALIGN;
-    if (n > (1 << 30) || C > (1 << 20)) return ATTN_ERR_UNSUPPORTED;
+    if (n > (1 << 30) || C > (1 << 20) || V > (1 << 30) || P > (1 << 30)) return ATTN_ERR_UNSUPPORTED;
     if ((n && dtable && embed::overlap(dy, n, ld_dy, each, dtable, V, ld, grad_each, C)) || (n && dpos_table && embed::overlap(dy, n, ld_dy, each, dpos_table, P, pos_ld, grad_each, C)) ||
         (dtable && dpos_table && embed::overlap(dtable, V, ld, grad_each, dpos_table, P, pos_ld, grad_each, C)))
         return ATTN_ERR_ARGUMENT;
@@ -527,10 +918,11 @@ int tensor_sm100_embedding_backward(const void *dy, const void *tokens, void *dt
     if (dtable) add(tokens, dtable, ld, V, scale);
     if (dpos_table && positions) add(positions, dpos_table, pos_ld, P, 1.f);
     if (dpos_table && !positions) a.T = T, a.P = P, a.pos_grad = dpos_table, a.pos_ld = pos_ld;
-    // four columns at a time
-    const bool wide = C % 4 == 0 && (embed::bits(dy) | (uintptr_t)(ld_dy * each)) % (4 * each) == 0 &&
-                      (embed::bits(dtable) | embed::bits(dpos_table) | (uintptr_t)(dtable ? ld * grad_each : 0) | (uintptr_t)(dpos_table ? pos_ld * grad_each : 0)) %
-                              (4 * grad_each) == 0;
+    // 16 bytes of dy at a time, and as many columns of the gradients
+    const uintptr_t columns = 16 / each;
+    const bool wide = C % columns == 0 && (embed::bits(dy) | (uintptr_t)ld_dy * each) % 16 == 0 &&
+                      (embed::bits(dtable) | embed::bits(dpos_table) | (dtable ? (uintptr_t)ld * grad_each : 0) | (dpos_table ? (uintptr_t)pos_ld * grad_each : 0)) %
+                              (columns * grad_each) == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (type == TENSOR_F32)
         return (int)(grad_type == TENSOR_F32 ? embed::launch_gradient<float, float>(a, wide, s) : embed::launch_gradient<float, __nv_bfloat16>(a, wide, s));

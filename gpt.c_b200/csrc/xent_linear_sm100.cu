@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_internal.h"
 #include "ids.cuh"
@@ -60,7 +61,8 @@ struct Maps {
 struct Problem {
     int M, V, K;
     int tiles_m, tiles_k;         // tiles of the rows of x, of its columns
-    int dx, dw, total;            // work items: dx first, then dw, then z
+    int dx, dw, total;            // work items: dx, dw, z; those with the longest contraction of dx and dw first
+    int dw_first;
     int dx_pieces, dx_blocks;     // pieces of the contraction of dx, blocks of each
     int blocks_m, blocks_k;       // contraction blocks over the rows, over the columns of x
     int v0, cols;                 // the piece of the vocabulary whose products are made
@@ -95,6 +97,7 @@ __device__ __forceinline__ Item decode(const Problem &p, int w) {
     int rows, cols;
     it.block0 = 0;
     it.piece = 0;
+    if (kBackward && p.dw_first && w < p.dx + p.dw) w = w < p.dw ? p.dx + w : w - p.dw;
     if (kBackward && w < p.dx) {
         it.kind = kDx;
         const int t = w / p.dx_pieces;
@@ -314,59 +317,69 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     } else if (warp == 1) {
         // ------------------------------ issues the products ------------------------------
         const uint32_t leader = elect_leader();
-        int n = 0, half = 0;
+        int st = 0, half = 0;  // next slot; halves of tiles so far
+        uint32_t turn = 0;     // parity of the slots' phase
         bool ok = true;
-        for (int j = 0; ok; j++) {
-            const int at = j % kQueue;
-            if (!mbar_wait_warp(&sm.item_full[at], (j / kQueue) & 1, ctx, SITE_ITEM)) break;
-            const int w = sm.item[at];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.item_empty[at]);
-            if (w >= p.total) break;
-            const Item it = decode<kBackward>(p, w);
-            const bool a_mn = it.kind == kDw, b_mn = it.kind != kLogits;
+        // The products of an item, with what its operands' layout decides known to the compiler: the descriptors of an instruction are the slot's and
+        // constants (with steps known at run time alone an instruction took 230 cycles to issue, where the tensor cores take 128).
+        auto products = [&](const Item &it, auto a_mn_c, auto b_mn_c) {
+            constexpr bool a_mn = decltype(a_mn_c)::value, b_mn = decltype(b_mn_c)::value;
+            constexpr uint32_t step_a = a_mn ? 2048 / 16 : 32 / 16, step_b = b_mn ? 2048 / 16 : 32 / 16;
             const uint32_t idesc = idesc_bf16_f32(128, it.n, a_mn, b_mn);
-            const uint32_t lbo_a = a_mn ? kBlock * 128 : 16, lbo_b = b_mn ? kBlock * 128 : 16, step_a = a_mn ? 2048 : 32, step_b = b_mn ? 2048 : 32;
-            const int seg = kTerms == 3 && kBackward && it.kind != kLogits ? kSegment : it.blocks;
-            for (int b0 = 0; ok && b0 < it.blocks; b0 += seg) {
+            const uint64_t base_a = smem_desc_sw128(smem_u32(sm.slot[0]), a_mn ? kBlock * 128 : 16, 1024);
+            const uint64_t base_b = smem_desc_sw128(smem_u32(sm.slot[0]), b_mn ? kBlock * 128 : 16, 1024);
+            const int seg = kTerms == 3 && kBackward && b_mn ? kSegment : it.blocks;
+            for (int b0 = 0; b0 < it.blocks; b0 += seg) {
                 const int b1 = min(it.blocks, b0 + seg);
-                for (int b = b0; b < b1; b++, n += kLoads) {
+                for (int b = b0; b < b1; b++) {
+                    int slot[kLoads];
+                    auto wait = [&](int l) {
+                        slot[l] = st;
+                        if (!mbar_wait_warp(&sm.full[st], turn, ctx, SITE_FULL)) return false;
+                        if (++st == kSlots) st = 0, turn ^= 1;
+                        return true;
+                    };
+                    if (!wait(0) || !wait(1)) return false;
 #pragma unroll
-                    for (int l = 0; l < kLoads; l++)
-                        if (ok && !mbar_wait_warp(&sm.full[(n + l) % kSlots], ((n + l) / kSlots) & 1, ctx, SITE_FULL)) ok = false;
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    uint64_t d[kLoads];
+                    for (int t = 0; t < kTerms; t++) {
+                        if (t > 0 && !wait(1 + t)) return false;
+                        tc_fence_after_sync();
+                        const uint64_t a = base_a + (uint32_t)(slot[t == 2 ? kLoads - 1 : 0] * (kSlotBytes / 16));
+                        const uint64_t bb = base_b + (uint32_t)(slot[t == 1 ? 2 % kLoads : 1] * (kSlotBytes / 16));
 #pragma unroll
-                    for (int l = 0; l < kLoads; l++) {
-                        const bool is_a = l == 0 || l == 3;
-                        d[l] = smem_desc_sw128(smem_u32(sm.slot[(n + l) % kSlots]), is_a ? lbo_a : lbo_b, 1024);
-                    }
-                    for (int h = 0; h < it.halves; h++) {
-                        const int acc = (half + h) & 1;
-                        if (b == b0 && half + h >= 2) {
-                            if (!mbar_wait_warp(&sm.acc_empty[acc], ((half + h) / 2 - 1) & 1, ctx, SITE_ACC_EMPTY)) {
-                                ok = false;
-                                break;
+                        for (int h = 0; h < 2; h++) {
+                            if (h >= it.halves) break;
+                            const int acc = (half + h) & 1;
+                            if (t == 0 && b == b0 && half + h >= 2) {
+                                if (!mbar_wait_warp(&sm.acc_empty[acc], ((half + h) / 2 - 1) & 1, ctx, SITE_ACC_EMPTY)) return false;
+                                tc_fence_after_sync();
                             }
-                            tc_fence_after_sync();
-                        }
-                        const uint32_t to = tmem + (uint32_t)acc * kTile;
-#pragma unroll
-                        for (int t = 0; t < kTerms; t++) {
-                            const uint64_t a = desc_advance(d[t == 2 ? kLoads - 1 : 0], h * 16384), bb = d[t == 1 ? 2 % kLoads : 1];
+                            const uint32_t to = tmem + (uint32_t)acc * kTile;
 #pragma unroll
                             for (int k = 0; k < kBlock / 16; k++)
-                                mma_ss_lead(leader, to, desc_advance(a, k * step_a), desc_advance(bb, k * step_b), idesc, b > b0 || t > 0 || k > 0);
+                                mma_ss_lead(leader, to, a + h * (16384 / 16) + k * step_a, bb + k * step_b, idesc, b > b0 || t > 0 || k > 0);
+                            if (t == kTerms - 1 && b == b1 - 1) tc_commit_lead(leader, &sm.acc_full[acc]);
                         }
-                        if (b == b1 - 1) tc_commit_lead(leader, &sm.acc_full[acc]);
+                        // a slot is free as soon as its last product is done: hi of A and lo of B before the third one
+                        if (t == 1) tc_commit_lead(leader, &sm.empty[slot[0]]), tc_commit_lead(leader, &sm.empty[slot[2 % kLoads]]);
+                        if (t == 2) tc_commit_lead(leader, &sm.empty[slot[1]]), tc_commit_lead(leader, &sm.empty[slot[kLoads - 1]]);
+                        if (kTerms == 1) tc_commit_lead(leader, &sm.empty[slot[0]]), tc_commit_lead(leader, &sm.empty[slot[1]]);
                     }
-                    if (!ok) break;
-#pragma unroll
-                    for (int l = 0; l < kLoads; l++) tc_commit_lead(leader, &sm.empty[(n + l) % kSlots]);
                 }
                 half += it.halves;
             }
+            return true;
+        };
+        for (int j = 0; ok; j++) {
+            const int at = j % kQueue;
+            if (!mbar_wait_warp(&sm.item_full[at], (j / kQueue) & 1, ctx, SITE_ITEM)) break;
+            const int w = __reduce_max_sync(0xffffffffu, sm.item[at]);  // (the same in all lanes, in a register that the compiler knows to be)
+            if (lane == 0) mbar_arrive(&sm.item_empty[at]);
+            if (w >= p.total) break;
+            const Item it = decode<kBackward>(p, w);
+            if (!kBackward || it.kind == kLogits) ok = products(it, std::false_type{}, std::false_type{});
+            else if (it.kind == kDx) ok = products(it, std::false_type{}, std::true_type{});
+            else ok = products(it, std::true_type{}, std::true_type{});
         }
     } else {
         // ------------------------------ takes the sums out ------------------------------
@@ -864,6 +877,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
             z = p.tiles_m * (p.next_cols / kTile);
         }
         p.total = p.dx + p.dw + z;
+        p.dw_first = p.blocks_m > p.dx_blocks;
         p.counter = counters + i;
         e = type == TENSOR_F32 ? launch_tiles<3, true>(maps, p, sms, status, s) : launch_tiles<1, true>(maps, p, sms, status, s);
         if (e != cudaSuccess) return (int)e;
