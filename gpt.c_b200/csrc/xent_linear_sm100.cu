@@ -53,9 +53,9 @@ struct __align__(1024) Smem {
 };
 
 struct Maps {
-    CUtensorMap x, w;      // boxes of 64 contraction steps x 256 rows
+    CUtensorMap x, w;      // boxes of 64 contraction steps x 128 rows, x a tile's width
     CUtensorMap x_mn, w_mn;  // boxes of 64 columns x 64 contraction steps
-    CUtensorMap g, g_mn;   // the piece whose products are made, both ways
+    CUtensorMap g, g_mn;   // the piece whose products are made, like x and like x_mn
 };
 
 struct Problem {
@@ -66,7 +66,8 @@ struct Problem {
     int dx_pieces, dx_blocks;     // pieces of the contraction of dx, blocks of each
     int blocks_m, blocks_k;       // contraction blocks over the rows, over the columns of x
     int v0, cols;                 // the piece of the vocabulary whose products are made
-    int next_v0, next_cols;       // the piece whose z is made
+    int next_v0, next_cols;       // the piece whose z is made, in tiles of `wide` columns (a multiple of 16)
+    int wide;
     int first;                    // the first piece: what dx holds is not added to
     int pitch;                    // columns of a row of G
     long long plane;              // elements from the hi to the lo plane of G
@@ -86,7 +87,7 @@ struct Problem {
 };
 
 struct Item {
-    int kind, m0, n0, n, halves;   // n: columns, a multiple of 32
+    int kind, m0, n0, n, halves;   // n: columns, a multiple of 16
     int blocks, segment, block0;   // contraction blocks, of one sum; where they begin
     int piece;
 };
@@ -118,12 +119,12 @@ __device__ __forceinline__ Item decode(const Problem &p, int w) {
         it.kind = kLogits;
         const int t = kBackward ? w - p.dx - p.dw : w;
         it.m0 = t % p.tiles_m * kTile;
-        it.n0 = t / p.tiles_m * kTile;  // in the piece
+        it.n0 = t / p.tiles_m * p.wide;  // in the piece
         rows = p.M, cols = min(p.next_cols, p.V - p.next_v0);
         it.blocks = p.blocks_k;
     }
     it.halves = rows - it.m0 > 128 ? 2 : 1;
-    it.n = min(kTile, (cols - it.n0 + 31) / 32 * 32);
+    it.n = min(it.kind == kLogits ? p.wide : kTile, max(16, (cols - it.n0 + 15) / 16 * 16));
     it.segment = it.blocks;
     return it;
 }
@@ -153,64 +154,47 @@ __device__ __forceinline__ void store8(void *p, const uint32_t (&r)[8]) {
                  : "memory");
 }
 
-// 64 sums of a row added to `at`, of which `left` (more than 0) are inside.
-template <bool kAdd>
-__device__ __forceinline__ void put_f32(float *at, const uint32_t (&z)[64], int left, int wide) {
-    if (wide == 32) {
+// 32 sums of a row, of which `left` (more than 0) are inside, stored at `at`, 32-byte aligned.
+__device__ __forceinline__ void put_f32(float *at, const uint32_t (&z)[32], int left) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 16) {
-            uint32_t old[2][8];
-            if (kAdd) {
+    for (int i = 0; i < 32; i += 8) {
+        uint32_t v[8];
 #pragma unroll
-                for (int j = 0; j < 2; j++)
-                    if (i + 8 * j < left) load8(old[j], at + i + 8 * j);
-            }
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                if (i + 8 * j >= left) continue;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    old[j][e] = kAdd ? __float_as_uint(__uint_as_float(old[j][e]) + __uint_as_float(z[i + 8 * j + e])) : z[i + 8 * j + e];
-                store8(at + i + 8 * j, old[j]);
-            }
-        }
-    } else if (wide == 16) {
-#pragma unroll
-        for (int i = 0; i < 64; i += 4) {
-            if (i >= left) continue;
-            float4 *q = reinterpret_cast<float4 *>(at + i);
-            float4 v = kAdd ? *q : make_float4(0.f, 0.f, 0.f, 0.f);
-            v.x += __uint_as_float(z[i]), v.y += __uint_as_float(z[i + 1]), v.z += __uint_as_float(z[i + 2]), v.w += __uint_as_float(z[i + 3]);
-            *q = v;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 64; i++)
-            if (i < left) at[i] = kAdd ? at[i] + __uint_as_float(z[i]) : __uint_as_float(z[i]);
+        for (int e = 0; e < 8; e++) v[e] = z[i + e];
+        if (i < left) store8(at + i, v);
     }
 }
+// The same added to what is there.  One thread adds to a place, so the order of the sums is fixed; L2 adds, and nobody waits for what was there
+// (loaded and stored, a half of a tile took 6 us, in which the tensor cores waited for its accumulator).
+__device__ __forceinline__ void add_f32(float *at, const uint32_t (&z)[32], int left, bool wide) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+            if (i < left)
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at + i), "r"(z[i]), "r"(z[i + 1]), "r"(z[i + 2]), "r"(z[i + 3]) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++)
+            if (i < left) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + i), "r"(z[i]) : "memory");
+    }
+}
+// The same for bf16 values, which are rounded once: 32 sums added to what was there, 16 words of two values.
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t old, uint32_t a, uint32_t b) {
     return pack_bf16x2(__uint_as_float(old << 16) + __uint_as_float(a), __uint_as_float(old & 0xffff0000u) + __uint_as_float(b));
 }
-__device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&z)[64], int left, int wide) {
+__device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&old)[16], const uint32_t (&z)[32], int left, int wide) {
     if (wide == 32) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 32) {
-            uint32_t old[2][8];
+        for (int i = 0; i < 32; i += 16) {
+            if (i >= left) continue;
+            uint32_t v[8];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                if (i + 16 * j < left) load8(old[j], at + i + 16 * j);
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                if (i + 16 * j >= left) continue;
-#pragma unroll
-                for (int e = 0; e < 8; e++) old[j][e] = add_bf16x2(old[j][e], z[i + 16 * j + 2 * e], z[i + 16 * j + 2 * e + 1]);
-                store8(at + i + 16 * j, old[j]);
-            }
+            for (int e = 0; e < 8; e++) v[e] = add_bf16x2(old[i / 2 + e], z[i + 2 * e], z[i + 2 * e + 1]);
+            store8(at + i, v);
         }
     } else if (wide == 16) {
 #pragma unroll
-        for (int i = 0; i < 64; i += 8) {
+        for (int i = 0; i < 32; i += 8) {
             if (i >= left) continue;
             uint4 *q = reinterpret_cast<uint4 *>(at + i);
             uint4 v = *q;
@@ -220,7 +204,7 @@ __device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&z)[
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 64; i++)
+        for (int i = 0; i < 32; i++)
             if (i < left) at[i] = __float2bfloat16_rn(__bfloat162float(at[i]) + __uint_as_float(z[i]));
     }
 }
@@ -290,12 +274,13 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                         uint8_t *dst = sm.slot[st];
                         uint64_t *bar = &sm.full[st];
                         if (it.kind == kLogits) {
-                            mbar_expect_tx(bar, kSlotBytes);
-                            if (is_a) tma_load_3d(dst, &maps.x, bar, b * kBlock, it.m0, plane);
+                            mbar_expect_tx(bar, (is_a ? 128 * it.halves : p.wide) * (kBlock * 2));
+                            if (is_a)
+                                for (int h = 0; h < it.halves; h++) tma_load_3d(dst + h * 16384, &maps.x, bar, b * kBlock, it.m0 + h * 128, plane);
                             else tma_load_3d(dst, &maps.w, bar, b * kBlock, p.next_v0 + it.n0, plane);
                         } else if (it.kind == kDx && is_a) {
-                            mbar_expect_tx(bar, kSlotBytes);
-                            tma_load_3d(dst, &maps.g, bar, b * kBlock, it.m0, plane);
+                            mbar_expect_tx(bar, 16384 * it.halves);
+                            for (int h = 0; h < it.halves; h++) tma_load_3d(dst + h * 16384, &maps.g, bar, b * kBlock, it.m0 + h * 128, plane);
                         } else {
                             const CUtensorMap *map = it.kind == kDx ? &maps.w_mn : is_a ? &maps.g_mn : &maps.x_mn;
                             const int boxes = is_a ? a_boxes : b_boxes, c0 = is_a ? it.m0 : it.n0, row = (it.kind == kDx ? p.v0 : 0) + b * kBlock;
@@ -401,7 +386,6 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                 for (int h = 0; h < it.halves; h++, half++) {
                     const int acc = half & 1;
                     const int row = it.m0 + h * 128 + quarter * 32 + lane, off = 64 * group;
-                    const bool mine = off < it.n;  // (a whole warp)
                     int target = -1;
                     float gr = 0.f, nl = 0.f;
                     if (it.kind == kLogits && row < p.M) {
@@ -411,99 +395,126 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                             nl = -p.lse[row] * kLog2e;
                         }
                     }
-                    if (!mbar_wait_warp(&sm.acc_full[acc], (half / 2) & 1, ctx, SITE_ACC_FULL)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after_sync();
-                    uint32_t z[64];
-                    tmem_ld32(from + acc * kTile, *reinterpret_cast<uint32_t(*)[32]>(z));
-                    tmem_ld32(from + acc * kTile + 32, *reinterpret_cast<uint32_t(*)[32]>(z + 32));
-                    tmem_wait_ld();
-                    tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.acc_empty[acc]);
-                    if (it.kind == kLogits) {
-                        const int class0 = p.next_v0 + it.n0 + off;
-                        const int left = p.V - class0, place = target - class0;
-                        const bool here = target >= 0 && place >= 0 && place < 64;
-                        if (!kBackward) {
-                            float top = -INFINITY, sum = 0.f;
-                            if (left < 64) {
-#pragma unroll
-                                for (int e = 0; e < 64; e++)
-                                    if (e >= left) z[e] = __float_as_uint(-INFINITY);
-                            }
-#pragma unroll
-                            for (int e = 0; e < 64; e++) top = fmaxf(top, __uint_as_float(z[e]));
-                            const float nt = top == -INFINITY ? 0.f : -top * p.log2e;
-                            float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int e = 0; e < 64; e++) s[e & 3] += ex2(fmaf(__uint_as_float(z[e]), p.log2e, nt));
-                            sum = (s[0] + s[1]) + (s[2] + s[3]);
-                            if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-                                for (int e = 0; e < 64; e++)
-                                    if (here && e == place) p.zt[row] = __uint_as_float(z[e]) * p.fix;
-                            }
-                            top *= p.fix;
-                            // the four quarters of the tile's columns
-                            if (group > 0) sm.part[half & 1][group - 1][quarter * 32 + lane] = make_float2(top, sum);
-                            asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
-                            if (group == 0) {
-                                float2 q[4] = {make_float2(top, sum)};
-#pragma unroll
-                                for (int i = 0; i < 3; i++) q[i + 1] = sm.part[half & 1][i][quarter * 32 + lane];
-                                const float m = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), nm = m == -INFINITY ? 0.f : -m * kLog2e;
-                                sum = 0.f;
-#pragma unroll
-                                for (int i = 0; i < 4; i++) sum += q[i].y * ex2(fmaf(q[i].x, kLog2e, nm));
-                                if (row < p.M) p.part[(long long)(it.n0 / kTile) * p.M + row] = make_float2(m, sum);
-                            }
-                        } else if (off < p.pitch - it.n0) {
-#pragma unroll
-                            for (int e = 0; e < 64; e++) z[e] = __float_as_uint(ex2(fmaf(__uint_as_float(z[e]), p.log2e, nl)));
-                            if (__any_sync(0xffffffffu, here)) {
-#pragma unroll
-                                for (int e = 0; e < 64; e++)
-                                    if (here && e == place) z[e] = __float_as_uint(__uint_as_float(z[e]) - 1.f);
-                            }
-                            if (left < 64) {
-#pragma unroll
-                                for (int e = 0; e < 64; e++)
-                                    if (e >= left) z[e] = 0;
-                            }
-                            if (row < p.M) {
-                                __nv_bfloat16 *to = p.out + (long long)row * p.pitch + it.n0 + off;
-#pragma unroll
-                                for (int i = 0; i < 64; i += 16) {
-                                    uint32_t hi[8], lo[8];
-#pragma unroll
-                                    for (int e = 0; e < 8; e++) {
-                                        const float a = __uint_as_float(z[i + 2 * e]) * gr, b = __uint_as_float(z[i + 2 * e + 1]) * gr;
-                                        if (kTerms == 1) hi[e] = pack_bf16x2(a, b);
-                                        else split_bf16x2(a, b, hi[e], lo[e]);
-                                        if (target < 0) hi[e] = lo[e] = 0;
-                                    }
-                                    store8(to + i, hi);
-                                    if (kTerms == 3) store8(to + p.plane + i, lo);
-                                }
-                            }
+                    if constexpr (!kBackward) {
+                        if (!mbar_wait_warp(&sm.acc_full[acc], (half / 2) & 1, ctx, SITE_ACC_FULL)) {
+                            ok = false;
+                            break;
                         }
-                    } else if (kBackward && mine) {
-                        const int left = p.K - it.n0 - off;
-                        if (it.kind == kDx) {
-                            if (row < p.M && left > 0) {
-                                float *to = p.dxp + ((long long)it.piece * p.M + row) * p.dx_pitch + it.n0 + off;
-                                if (p.first && b0 == 0) put_f32<false>(to, z, left, 32);
-                                else put_f32<true>(to, z, left, 32);
+                        tc_fence_after_sync();
+                        uint32_t z[64];
+                        tmem_ld32(from + acc * kTile, *reinterpret_cast<uint32_t(*)[32]>(z));
+                        tmem_ld32(from + acc * kTile + 32, *reinterpret_cast<uint32_t(*)[32]>(z + 32));
+                        tmem_wait_ld();
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sm.acc_empty[acc]);
+                        const int left = min(p.V - it.n0, p.wide) - off, place = target - it.n0 - off;
+                        const bool here = target >= 0 && place >= 0 && place < min(64, left);
+                        float top = -INFINITY, sum = 0.f;
+                        if (left < 64) {
+#pragma unroll
+                            for (int e = 0; e < 64; e++)
+                                if (e >= left) z[e] = __float_as_uint(-INFINITY);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 64; e++) top = fmaxf(top, __uint_as_float(z[e]));
+                        const float nt = top == -INFINITY ? 0.f : -top * p.log2e;
+                        float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 64; e++) s[e & 3] += ex2(fmaf(__uint_as_float(z[e]), p.log2e, nt));
+                        sum = (s[0] + s[1]) + (s[2] + s[3]);
+                        if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+                            for (int e = 0; e < 64; e++)
+                                if (here && e == place) p.zt[row] = __uint_as_float(z[e]) * p.fix;
+                        }
+                        top *= p.fix;
+                        // the four quarters of the tile's columns
+                        if (group > 0) sm.part[half & 1][group - 1][quarter * 32 + lane] = make_float2(top, sum);
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+                        if (group == 0) {
+                            float2 q[4] = {make_float2(top, sum)};
+#pragma unroll
+                            for (int i = 0; i < 3; i++) q[i + 1] = sm.part[half & 1][i][quarter * 32 + lane];
+                            const float m = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), nm = m == -INFINITY ? 0.f : -m * kLog2e;
+                            sum = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) sum += q[i].y * ex2(fmaf(q[i].x, kLog2e, nm));
+                            if (row < p.M) p.part[(long long)(it.n0 / p.wide) * p.M + row] = make_float2(m, sum);
+                        }
+                    } else {
+                        // 32 columns at a time: registers that do not fit would be kept in L2, since shared memory leaves no room for L1
+                        const long long v = (long long)p.v0 + row;                                        // dw: the class
+                        const int left = (it.kind == kLogits ? min(p.wide, p.next_cols - it.n0) : min(it.n, p.K - it.n0)) - off;
+                        const bool inside = (it.kind == kDw ? v < p.V && row < p.cols : row < p.M) && left > 0;
+                        __nv_bfloat16 *dw = static_cast<__nv_bfloat16 *>(p.dw_out) + v * p.lddw + it.n0 + off;  // where it is bf16
+                        uint32_t old[16];
+                        auto ask = [&](int i) {  // for what dw holds, before the wait
+                            if (kTerms == 1 && it.kind == kDw && inside && p.dw_wide == 32) {
+                                if (i < left) load8(*reinterpret_cast<uint32_t(*)[8]>(old), dw + i);
+                                if (i + 16 < left) load8(*reinterpret_cast<uint32_t(*)[8]>(old + 8), dw + i + 16);
                             }
-                        } else {
-                            const long long v = (long long)p.v0 + row;
-                            if (v < p.V && row < p.cols && left > 0) {
-                                if (kTerms == 1) add_bf16(static_cast<__nv_bfloat16 *>(p.dw_out) + v * p.lddw + it.n0 + off, z, left, p.dw_wide);
-                                else put_f32<true>(static_cast<float *>(p.dw_out) + v * p.lddw + it.n0 + off, z, left, p.dw_wide);
+                        };
+                        ask(0);
+                        if (!mbar_wait_warp(&sm.acc_full[acc], (half / 2) & 1, ctx, SITE_ACC_FULL)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int i = 0; i < 64; i += 32) {
+                            uint32_t z[32];
+                            tmem_ld32(from + acc * kTile + i, z);
+                            tmem_wait_ld();
+                            if (i == 32) {
+                                tc_fence_before_sync();
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&sm.acc_empty[acc]);
                             }
+                            if (it.kind == kLogits) {
+                                if (i >= left) continue;  // (a whole warp)
+                                const int known = p.V - p.next_v0 - it.n0 - off - i, place = target - p.next_v0 - it.n0 - off - i;
+                                const bool here = target >= 0 && place >= 0 && place < 32;
+#pragma unroll
+                                for (int e = 0; e < 32; e++) z[e] = __float_as_uint(ex2(fmaf(__uint_as_float(z[e]), p.log2e, nl)));
+                                if (__any_sync(0xffffffffu, here)) {
+#pragma unroll
+                                    for (int e = 0; e < 32; e++)
+                                        if (here && e == place) z[e] = __float_as_uint(__uint_as_float(z[e]) - 1.f);
+                                }
+                                if (known < 32) {
+#pragma unroll
+                                    for (int e = 0; e < 32; e++)
+                                        if (e >= known) z[e] = 0;
+                                }
+                                if (inside) {
+                                    __nv_bfloat16 *to = p.out + (long long)row * p.pitch + it.n0 + off + i;
+#pragma unroll
+                                    for (int c = 0; c < 32; c += 16) {
+                                        uint32_t hi[8], lo[8];
+#pragma unroll
+                                        for (int e = 0; e < 8; e++) {
+                                            const float a = __uint_as_float(z[c + 2 * e]) * gr, b = __uint_as_float(z[c + 2 * e + 1]) * gr;
+                                            if (kTerms == 1) hi[e] = pack_bf16x2(a, b);
+                                            else split_bf16x2(a, b, hi[e], lo[e]);
+                                            if (target < 0) hi[e] = lo[e] = 0;
+                                        }
+                                        if (i + c < left) store8(to + c, hi);
+                                        if (kTerms == 3 && i + c < left) store8(to + p.plane + c, lo);
+                                    }
+                                }
+                            } else if (it.kind == kDx) {
+                                if (inside && i < left) {
+                                    float *to = p.dxp + ((long long)it.piece * p.M + row) * p.dx_pitch + it.n0 + off + i;
+                                    if (p.first && b0 == 0) put_f32(to, z, left - i);
+                                    else add_f32(to, z, left - i, true);
+                                }
+                            } else if (inside && i < left) {
+                                if (kTerms == 1) add_bf16(dw + i, old, z, left - i, p.dw_wide);
+                                else add_f32(static_cast<float *>(p.dw_out) + v * p.lddw + it.n0 + off + i, z, left - i, p.dw_wide >= 16);
+                            }
+                            __syncwarp();
+                            if (i == 0) ask(32);
                         }
                     }
                 }
@@ -520,35 +531,40 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
 }
 
-// Maximum and sum of each row from those of its tiles.  A block takes 32 rows, a warp every eighth tile.
-__global__ void __launch_bounds__(256) join_kernel(const float2 *__restrict__ part, const float *__restrict__ zt, Ids targets, float *__restrict__ losses,
-                                                   float *__restrict__ lse, int tiles, int M, int V) {
+// Maximum and sum of each row from those of its tiles.  A block takes 32 rows, a warp every 32nd tile, eight of them at a time.
+__global__ void __launch_bounds__(1024) join_kernel(const float2 *__restrict__ part, const float *__restrict__ zt, Ids targets, float *__restrict__ losses,
+                                                    float *__restrict__ lse, int tiles, int M, int V) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ float2 all[8][32];
+    constexpr int kAhead = 8;
+    __shared__ float2 all[32][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row = blockIdx.x * 32 + lane;
+    auto over = [](float m, float top) { return top == -INFINITY ? 0.f : ex2((m - top) * kLog2e); };  // exp(m - top); nothing there: 0
     float m = -INFINITY, s = 0.f;
-    auto join = [&](float2 q) {
-        const float top = fmaxf(m, q.x), nt = top == -INFINITY ? 0.f : -top * kLog2e;
-        s = s * ex2(fmaf(m, kLog2e, nt)) + q.y * ex2(fmaf(q.x, kLog2e, nt));
-        m = top;
-    };
     if (row < M) {
-        for (int t0 = warp; t0 < tiles; t0 += 32) {
-            float2 q[4];
+        for (int t0 = warp; t0 < tiles; t0 += 32 * kAhead) {
+            float2 q[kAhead];
 #pragma unroll
-            for (int u = 0; u < 4; u++) q[u] = t0 + 8 * u < tiles ? part[(long long)(t0 + 8 * u) * M + row] : make_float2(-INFINITY, 0.f);
+            for (int u = 0; u < kAhead; u++) q[u] = t0 + 32 * u < tiles ? part[(long long)(t0 + 32 * u) * M + row] : make_float2(-INFINITY, 0.f);
+            float top = m;
 #pragma unroll
-            for (int u = 0; u < 4; u++) join(q[u]);
+            for (int u = 0; u < kAhead; u++) top = fmaxf(top, q[u].x);
+            s *= over(m, top);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) s += q[u].y * over(q[u].x, top);
+            m = top;
         }
     }
     all[warp][lane] = make_float2(m, s);
     __syncthreads();
     if (warp != 0 || row >= M) return;
-#pragma unroll
-    for (int i = 1; i < 8; i++) join(all[i][lane]);
-    const float l = m + logf(s);
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < 32; i++) top = fmaxf(top, all[i][lane].x);
+#pragma unroll 8
+    for (int i = 0; i < 32; i++) sum += all[i][lane].y * over(all[i][lane].x, top);
+    const float l = top + logf(sum);
     lse[row] = l;
     losses[row] = targets.at(row, V) >= 0 ? l - zt[row] : 0.f;
 }
@@ -599,25 +615,39 @@ __global__ void __launch_bounds__(256) planes_kernel(const T *__restrict__ src, 
     }
 }
 
-// dx from the pieces of its contraction, in their order.
-template <class T>
+// dx from the pieces of its contraction.  kGroups threads share four columns, each taking every kGroups-th piece; their sums are added in order.
+template <class T, int kGroups>
 __global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide) {
     pdl_launch_dependents();
     pdl_wait();
-    const int words = pitch / 4;
+    constexpr int kWords = 256 / kGroups, kAhead = 4;
+    __shared__ float4 part[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kWords : 1];
+    const int words = pitch / 4, group = threadIdx.x / kWords, place = threadIdx.x % kWords;
     const long long total = (long long)M * words, apart = (long long)M * pitch;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / words;
+    for (long long i0 = (long long)blockIdx.x * kWords; i0 < total; i0 += (long long)gridDim.x * kWords) {
+        const long long i = i0 + place, r = i / words;
         const int c = (int)(i - r * words) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < count; p0 += 4) {
-            float4 v[4];
+        if (i < total) {
+            for (int p0 = group; p0 < count; p0 += kGroups * kAhead) {
+                float4 v[kAhead];
 #pragma unroll
-            for (int u = 0; u < 4; u++)
-                v[u] = p0 + u < count ? __ldcs(reinterpret_cast<const float4 *>(pieces + (p0 + u) * apart + r * pitch + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int u = 0; u < kAhead; u++) v[u] = __ldcs(reinterpret_cast<const float4 *>(pieces + min(p0 + kGroups * u, count - 1) * apart + r * pitch + c));
 #pragma unroll
-            for (int u = 0; u < 4; u++) sum = make_float4(sum.x + v[u].x, sum.y + v[u].y, sum.z + v[u].z, sum.w + v[u].w);
+                for (int u = 0; u < kAhead; u++)
+                    if (p0 + kGroups * u < count) sum = make_float4(sum.x + v[u].x, sum.y + v[u].y, sum.z + v[u].z, sum.w + v[u].w);
+            }
         }
+        if (kGroups > 1) {
+            part[group][place] = sum;
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int g = 1; g < kGroups; g++) sum = make_float4(sum.x + part[g][place].x, sum.y + part[g][place].y, sum.z + part[g][place].z, sum.w + part[g][place].w);
+            }
+            __syncthreads();
+        }
+        if (group > 0 || i >= total) continue;
         T *at = dx + r * K + c;
         const float s[4] = {sum.x, sum.y, sum.z, sum.w};
         if (wide && c + 4 <= K) {
@@ -645,11 +675,23 @@ struct Layout {
     int pitch, planes;
     size_t x, w, part, zt, counters, g[2], dxp, total;
     int cols, pieces;         // of the vocabulary
+    int wide;                 // columns of a tile of z
     int dx_pieces, dx_blocks, dx_pitch;
     size_t plane_x, plane_w, plane_g;  // elements
 };
 
 bool in_place(const void *p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
+
+// Columns of a tile of z: 256, but where they make few rounds of the SMs, what makes these rounds end together (40 x 50257: two rounds of 176
+// instead of 256).  A narrow tile costs a little more, as if it had 32 columns more.
+int tile_width(int tiles_m, int V, int sms) {
+    auto rounds = [&](int n) { return ((long long)tiles_m * ((V + n - 1) / n) + sms - 1) / sms; };
+    int best = kTile;
+    if (rounds(kTile) <= 8)
+        for (int n = kTile - 16; n >= 64; n -= 16)
+            if (rounds(n) * (n + 32) < rounds(best) * (best + 32)) best = n;
+    return best;
+}
 
 Layout layout(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K, bool backward, int sms) {
     Layout l = {};
@@ -669,7 +711,8 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     if (l.copy_w) l.w = take(l.plane_w * 2 * l.planes);
     const int tiles_v = (V + kTile - 1) / kTile, tiles_m = (M + kTile - 1) / kTile, tiles_k = (K + kTile - 1) / kTile;
     if (!backward) {
-        l.part = take((size_t)tiles_v * M * sizeof(float2));
+        l.wide = tile_width(tiles_m, V, sms);
+        l.part = take((size_t)((V + l.wide - 1) / l.wide) * M * sizeof(float2));
         l.zt = take((size_t)M * sizeof(float));
         l.total = at;
         return l;
@@ -680,7 +723,8 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     l.pieces = (tiles_v + most - 1) / most;
     const int tiles = (tiles_v + l.pieces - 1) / l.pieces;
     l.pieces = (tiles_v + tiles - 1) / tiles;
-    l.cols = tiles * kTile;
+    l.cols = l.pieces > 1 ? tiles * kTile : up(V, kBlock);
+    l.wide = l.pieces > 1 ? kTile : tile_width(tiles_m, l.cols, sms);
     // pieces of the contraction of dx: none is longer than half of what an SM has to do for a piece of the vocabulary
     const int blocks = l.cols / kBlock;
     const double load = ((double)tiles_m * tiles_k * blocks + (double)tiles * tiles_k * std::max(4, (M + kBlock - 1) / kBlock)) / sms;
@@ -728,6 +772,15 @@ cudaError_t launch_planes(const void *src, long long ld, int type, void *to, siz
                                        targets, V, counters, count);
 }
 
+// Eight threads share the pieces where there are more than four: 49 pieces of 40 x 768 18 -> XX us.
+template <class T>
+cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, cudaStream_t s) {
+    const int groups = count > 4 ? 8 : 1;
+    const int grid = blocks_for((long long)M * (pitch / 4) * groups);
+    return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide)
+                      : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide);
+}
+
 template <int kTerms, bool kBackward>
 cudaError_t launch_tiles(const Maps &maps, const Problem &p, int sms, int *status, cudaStream_t s) {
     constexpr int kSlots = kBackward ? kBackwardSlots : kForwardSlots;
@@ -768,7 +821,7 @@ extern "C" {
 
 size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
     if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0) return 0;
-    return head::layout(x, w, ldx, ldw, type, rows, V, K, false, 148).total;
+    return head::layout(x, w, ldx, ldw, type, rows, V, K, false, attn::sm_count()).total;
 }
 
 size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
@@ -794,21 +847,22 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
     if (l.copy_x && (e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
     Maps maps = {};
-    if ((rc = map_of(&maps.x, l.copy_x ? base + l.x : x, rows, K, l.copy_x ? l.pitch : rows > 1 ? ldx : l.pitch, l.plane_x, l.planes, kTile)) != 0) return rc;
-    if ((rc = map_of(&maps.w, l.copy_w ? base + l.w : w, V, K, l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch, l.plane_w, l.planes, kTile)) != 0) return rc;
+    if ((rc = map_of(&maps.x, l.copy_x ? base + l.x : x, rows, K, l.copy_x ? l.pitch : rows > 1 ? ldx : l.pitch, l.plane_x, l.planes, 128)) != 0) return rc;
+    if ((rc = map_of(&maps.w, l.copy_w ? base + l.w : w, V, K, l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch, l.plane_w, l.planes, l.wide)) != 0) return rc;
     Problem p = {};
     p.M = rows, p.V = V, p.K = K;
     set_fix(p, type);
     p.tiles_m = (rows + kTile - 1) / kTile;
     p.blocks_k = (K + kBlock - 1) / kBlock;
-    p.next_cols = up(V, kTile);
-    p.total = p.tiles_m * (p.next_cols / kTile);
+    p.next_cols = V, p.wide = l.wide;
+    const int tiles = (V + l.wide - 1) / l.wide;
+    p.total = p.tiles_m * tiles;
     p.targets = Ids{targets, target_type};
     p.part = reinterpret_cast<float2 *>(base + l.part);
     p.zt = reinterpret_cast<float *>(base + l.zt);
     e = type == TENSOR_F32 ? launch_tiles<3, false>(maps, p, sms, status, s) : launch_tiles<1, false>(maps, p, sms, status, s);
     if (e != cudaSuccess) return (int)e;
-    return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(256), 0, s, p.part, p.zt, p.targets, losses, lse, p.next_cols / kTile, rows, V);
+    return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, p.part, p.zt, p.targets, losses, lse, tiles, rows, V);
 }
 
 int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw, void *scratch, long long ldx,
@@ -836,8 +890,8 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     const void *wp = l.copy_w ? base + l.w : w;
     const long long pitch_w = l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch;
     Maps maps = {};
-    if ((rc = map_of(&maps.x, base + l.x, rows, K, l.pitch, l.plane_x, l.planes, kTile)) != 0) return rc;
-    if ((rc = map_of(&maps.w, wp, V, K, pitch_w, l.plane_w, l.planes, kTile)) != 0) return rc;
+    if ((rc = map_of(&maps.x, base + l.x, rows, K, l.pitch, l.plane_x, l.planes, 128)) != 0) return rc;
+    if ((rc = map_of(&maps.w, wp, V, K, pitch_w, l.plane_w, l.planes, l.wide)) != 0) return rc;
     if ((rc = map_of(&maps.x_mn, base + l.x, rows, K, l.pitch, l.plane_x, l.planes, kBlock)) != 0) return rc;
     if ((rc = map_of(&maps.w_mn, wp, V, K, pitch_w, l.plane_w, l.planes, kBlock)) != 0) return rc;
     Problem p = {};
@@ -848,7 +902,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     p.blocks_m = (rows + kBlock - 1) / kBlock;
     p.blocks_k = (K + kBlock - 1) / kBlock;
     p.dx_pieces = l.dx_pieces, p.dx_blocks = l.dx_blocks;
-    p.pitch = l.cols;
+    p.pitch = l.cols, p.wide = l.wide;
     p.plane = (long long)l.plane_g;
     p.targets = Ids{targets, target_type};
     p.g = g, p.lse = lse, p.one_g = one_g;
@@ -862,19 +916,19 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         p.dw = 0;
         if (i > 0) {
             p.v0 = (i - 1) * l.cols;
-            p.cols = std::min(l.cols, up(V - p.v0, kTile));
-            if (dw) p.dw = p.cols / kTile * p.tiles_k;
+            p.cols = std::min(l.cols, up(V - p.v0, kBlock));
+            if (dw) p.dw = (p.cols + kTile - 1) / kTile * p.tiles_k;
             p.first = i == 1;
             const void *g0 = base + l.g[(i - 1) & 1];
-            if ((rc = map_of(&maps.g, g0, rows, p.cols, l.cols, l.plane_g, l.planes, kTile)) != 0) return rc;
+            if ((rc = map_of(&maps.g, g0, rows, p.cols, l.cols, l.plane_g, l.planes, 128)) != 0) return rc;
             if ((rc = map_of(&maps.g_mn, g0, rows, p.cols, l.cols, l.plane_g, l.planes, kBlock)) != 0) return rc;
         }
         int z = 0;
         if (i < l.pieces) {
             p.next_v0 = i * l.cols;
-            p.next_cols = std::min(l.cols, up(V - p.next_v0, kTile));
+            p.next_cols = std::min(l.cols, up(V - p.next_v0, kBlock));
             p.out = reinterpret_cast<__nv_bfloat16 *>(base + l.g[i & 1]);
-            z = p.tiles_m * (p.next_cols / kTile);
+            z = p.tiles_m * ((p.next_cols + l.wide - 1) / l.wide);
         }
         p.total = p.dx + p.dw + z;
         p.dw_first = p.blocks_m > p.dx_blocks;
@@ -883,11 +937,9 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         if (e != cudaSuccess) return (int)e;
     }
     if (!dx) return ATTN_OK;
-    const int grid = blocks_for((long long)rows * (l.dx_pitch / 4));
     const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
-    e = type == TENSOR_F32 ? attn::launch_after_previous(sum_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<float *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide)
-                         : attn::launch_after_previous(sum_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, static_cast<__nv_bfloat16 *>(dx), p.dxp, l.dx_pieces, rows, K,
-                                                       l.dx_pitch, wide);
+    e = type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide, s)
+                           : launch_sum(static_cast<__nv_bfloat16 *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide, s);
     return (int)e;
 }
 
