@@ -19,9 +19,8 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "attn_internal.h"
-#include "ids.cuh"
 #include "tc05.cuh"
+#include "xent_linear.cuh"
 
 #include "../../include/xent_sm100.h"
 
@@ -331,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         }
     } else if (warp == 1) {
         // ------------------------------ issues the products ------------------------------
+        constexpr int kLead = kTerms == 1 ? 3 : 1;
         const uint32_t leader = elect_leader();
         int st = 0, half = 0;  // next slot; halves of tiles so far
         uint32_t turn = 0;     // parity of the slots' phase
@@ -346,35 +346,63 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
             const int seg = kTerms == 3 && kBackward && b_mn ? kSegment : it.blocks;
             for (int b0 = 0; b0 < it.blocks; b0 += seg) {
                 const int b1 = min(it.blocks, b0 + seg);
-                for (int b = b0; b < b1; b++) {
+                // One half's products of a block, term t, from the block's slots.
+                auto issue = [&](const int (&slot)[kLoads], int t, int h, int b) {
+                    const uint64_t a = base_a + (uint32_t)(slot[t == 2 ? kLoads - 1 : 0] * (kSlotBytes / 16)) + h * (16384 / 16);
+                    const uint64_t bb = base_b + (uint32_t)(slot[t == 1 ? 2 % kLoads : 1] * (kSlotBytes / 16));
+                    const uint32_t to = tmem + (uint32_t)((half + h) & 1) * kTile;
+#pragma unroll
+                    for (int k = 0; k < kBlock / 16; k++) mma_ss_lead(leader, to, a + k * step_a, bb + k * step_b, idesc, b > b0 || t > 0 || k > 0);
+                    if (t == kTerms - 1 && b == b1 - 1) tc_commit_lead(leader, &sm.acc_full[(half + h) & 1]);
+                };
+                auto wait = [&](int &slot) {
+                    slot = st;
+                    if (!mbar_wait_warp(&sm.full[st], turn, ctx, SITE_FULL)) return false;
+                    if (++st == kSlots) st = 0, turn ^= 1;
+                    return true;
+                };
+                auto wait_acc = [&](int h) {
+                    if (half + h >= 2 && !mbar_wait_warp(&sm.acc_empty[(half + h) & 1], ((half + h) / 2 - 1) & 1, ctx, SITE_ACC_EMPTY)) return false;
+                    tc_fence_after_sync();
+                    return true;
+                };
+                if (!wait_acc(0)) return false;
+                int b = b0;
+                if (it.halves == 2) {
+                    // The second accumulator is still being read when the first is free (the warps that read them take one after the other), so the
+                    // first half's products of kLead blocks come first.
+                    int slot[kLead][kLoads];
+                    const int n = min(kLead, b1 - b0);
+#pragma unroll
+                    for (int i = 0; i < kLead; i++) {
+                        if (i >= n) break;
+#pragma unroll
+                        for (int l = 0; l < kLoads; l++)
+                            if (!wait(slot[i][l])) return false;
+                        tc_fence_after_sync();
+#pragma unroll
+                        for (int t = 0; t < kTerms; t++) issue(slot[i], t, 0, b0 + i);
+                    }
+                    if (!wait_acc(1)) return false;
+#pragma unroll
+                    for (int i = 0; i < kLead; i++) {
+                        if (i >= n) break;
+#pragma unroll
+                        for (int t = 0; t < kTerms; t++) issue(slot[i], t, 1, b0 + i);
+#pragma unroll
+                        for (int l = 0; l < kLoads; l++) tc_commit_lead(leader, &sm.empty[slot[i][l]]);
+                    }
+                    b += n;
+                }
+                for (; b < b1; b++) {
                     int slot[kLoads];
-                    auto wait = [&](int l) {
-                        slot[l] = st;
-                        if (!mbar_wait_warp(&sm.full[st], turn, ctx, SITE_FULL)) return false;
-                        if (++st == kSlots) st = 0, turn ^= 1;
-                        return true;
-                    };
-                    if (!wait(0) || !wait(1)) return false;
+                    if (!wait(slot[0]) || !wait(slot[1])) return false;
 #pragma unroll
                     for (int t = 0; t < kTerms; t++) {
-                        if (t > 0 && !wait(1 + t)) return false;
+                        if (t > 0 && !wait(slot[(1 + t) % kLoads])) return false;
                         tc_fence_after_sync();
-                        const uint64_t a = base_a + (uint32_t)(slot[t == 2 ? kLoads - 1 : 0] * (kSlotBytes / 16));
-                        const uint64_t bb = base_b + (uint32_t)(slot[t == 1 ? 2 % kLoads : 1] * (kSlotBytes / 16));
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            if (h >= it.halves) break;
-                            const int acc = (half + h) & 1;
-                            if (t == 0 && b == b0 && half + h >= 2) {
-                                if (!mbar_wait_warp(&sm.acc_empty[acc], ((half + h) / 2 - 1) & 1, ctx, SITE_ACC_EMPTY)) return false;
-                                tc_fence_after_sync();
-                            }
-                            const uint32_t to = tmem + (uint32_t)acc * kTile;
-#pragma unroll
-                            for (int k = 0; k < kBlock / 16; k++)
-                                mma_ss_lead(leader, to, a + h * (16384 / 16) + k * step_a, bb + k * step_b, idesc, b > b0 || t > 0 || k > 0);
-                            if (t == kTerms - 1 && b == b1 - 1) tc_commit_lead(leader, &sm.acc_full[acc]);
-                        }
+                        issue(slot, t, 0, b);
+                        if (it.halves == 2) issue(slot, t, 1, b);
                         // a slot is free as soon as its last product is done: hi of A and lo of B before the third one
                         if (t == 1) tc_commit_lead(leader, &sm.empty[slot[0]]), tc_commit_lead(leader, &sm.empty[slot[2 % kLoads]]);
                         if (t == 2) tc_commit_lead(leader, &sm.empty[slot[1]]), tc_commit_lead(leader, &sm.empty[slot[kLoads - 1]]);
@@ -707,7 +735,8 @@ __global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const floa
 
 // ---- host side ----
 
-constexpr size_t kPieceBytes = (size_t)128 << 20;  // of G, about
+constexpr size_t kPieceBytes = (size_t)256 << 20;  // of G, at most, but for
+constexpr int kLeastTiles = 32;                    // tiles of classes
 constexpr int kFetchBlocks = 8;
 constexpr int kForwardSlots = 6, kBackwardSlots = 7;
 
@@ -716,7 +745,7 @@ size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 // What a call reads in place and what it copies, and where everything lies in the scratch buffer.
 struct Layout {
-    bool copy_x, copy_w;
+    bool few, copy_x, copy_w;
     int pitch, planes;
     size_t x, w, part, zt, counters, g[2], dxp, total;
     int cols, pieces;         // of the vocabulary
@@ -727,14 +756,16 @@ struct Layout {
 
 bool in_place(const void *p, long long ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0; }
 
-// Columns of a tile of z: 256, but where they make few rounds of the SMs, what makes these rounds end together (40 x 50257: two rounds of 176
-// instead of 256).  A narrow tile costs a little more, as if it had 32 columns more.
-int tile_width(int tiles_m, int V, int sms) {
+// Columns of a tile of z: 256, but where they make few rounds of the SMs, what makes these rounds end together (200 x 768 x 50257: two rounds of 176
+// instead of 256, 30.9 -> 29.8 us).  A narrow tile costs a little more, as if it had 32 columns more, and where a tile has only half of its rows
+// it waits for its operands anyway: 40 rows take 25.0 us at 256 columns, 26.4 at 176.
+int tile_width(int M, int V, int sms) {
+    const int tiles_m = (M + kTile - 1) / kTile, extra = M > 128 ? 32 : 256;
     auto rounds = [&](int n) { return ((long long)tiles_m * ((V + n - 1) / n) + sms - 1) / sms; };
     int best = kTile;
     if (rounds(kTile) <= 8)
         for (int n = kTile - 16; n >= 64; n -= 16)
-            if (rounds(n) * (n + 32) < rounds(best) * (best + 32)) best = n;
+            if (rounds(n) * (n + extra) < rounds(best) * (best + extra)) best = n;
     return best;
 }
 
@@ -742,6 +773,12 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     Layout l = {};
     l.planes = type == TENSOR_F32 ? 2 : 1;
     l.pitch = up(K, 8);
+    l.few = !backward && few_rows_fit(x, w, ldx, ldw, type, M, V, K, sms);
+    if (l.few) {
+        l.zt = up256((size_t)few_rows_parts(V, sms) * M * sizeof(float2));
+        l.total = l.zt + up256((size_t)M * sizeof(float));
+        return l;
+    }
     l.copy_x = type == TENSOR_F32 || backward || !in_place(x, ldx);  // the gradients need rows of zeros where there is no target
     l.copy_w = type == TENSOR_F32 || !in_place(w, ldw);
     size_t at = 0;
@@ -756,7 +793,7 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     if (l.copy_w) l.w = take(l.plane_w * 2 * l.planes);
     const int tiles_v = (V + kTile - 1) / kTile, tiles_m = (M + kTile - 1) / kTile, tiles_k = (K + kTile - 1) / kTile;
     if (!backward) {
-        l.wide = tile_width(tiles_m, V, sms);
+        l.wide = tile_width(M, V, sms);
         l.part = take((size_t)((V + l.wide - 1) / l.wide) * M * sizeof(float2));
         l.zt = take((size_t)M * sizeof(float));
         l.total = at;
@@ -764,12 +801,12 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     }
     // pieces of the vocabulary: as many tiles each
     const size_t tile_bytes = (size_t)M * kTile * 2 * l.planes;
-    const int most = (int)std::min<size_t>(tiles_v, std::max<size_t>(4, kPieceBytes / tile_bytes));
+    const int most = (int)std::min<size_t>(tiles_v, std::max<size_t>(kLeastTiles, kPieceBytes / tile_bytes));
     l.pieces = (tiles_v + most - 1) / most;
     const int tiles = (tiles_v + l.pieces - 1) / l.pieces;
     l.pieces = (tiles_v + tiles - 1) / tiles;
     l.cols = l.pieces > 1 ? tiles * kTile : up(V, kBlock);
-    l.wide = l.pieces > 1 ? kTile : tile_width(tiles_m, l.cols, sms);
+    l.wide = l.pieces > 1 ? kTile : tile_width(M, l.cols, sms);
     // pieces of the contraction of dx: none is longer than half of what an SM has to do for a piece of the vocabulary
     const int blocks = l.cols / kBlock;
     const double load = ((double)tiles_m * tiles_k * blocks + (double)tiles * tiles_k * std::max(4, (M + kBlock - 1) / kBlock)) / sms;
@@ -849,7 +886,7 @@ int check(const void *x, const void *w, const void *targets, const void *scratch
 }  // namespace
 
 cudaError_t set_attributes() {
-    cudaError_t e = cudaSuccess;
+    cudaError_t e = few_rows_set_attributes();
     auto set = [&](const void *kernel, size_t bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     };
@@ -889,6 +926,11 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
+    if (l.few) {
+        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K};
+        if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
+        return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, a.part, a.zt, a.targets, losses, lse, few_rows_parts(V, sms), rows, V);
+    }
     if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
     if (l.copy_x && (e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
     Maps maps = {};

@@ -92,9 +92,34 @@ def test_shapes(pkg, M, K, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,K,V", [(1, 64, 8000), (1, 768, 50257), (15, 40, 9001), (16, 200, 50257), (17, 72, 8192), (32, 768, 9999), (33, 136, 12001), (48, 8, 30011), (49, 264, 20000),
+                                   (64, 768, 16001), (65, 64, 16001)])
+def test_few_rows(pkg, M, K, V, dtype):
+    """Sizes at which the forward reads the weights into registers, and those beside them."""
+    for i, ignored in enumerate((0.0, 0.4)):
+        Case(M, K, V, dtype, ignored, seed=i, ids=IDS[(M + i) % 3]).check(pkg)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_rows_nan_and_infinity(pkg, dtype):
+    c = Case(9, 64, 9000, dtype, 0.0)
+    c.x[3, 5], c.x[4, 6] = float("nan"), float("inf")
+    losses, lse = pkg.linear_xent_forward(c.x, c.w, c.ids)
+    assert losses.isfinite().nonzero().flatten().tolist() == [0, 1, 2, 5, 6, 7, 8] and lse[3].isnan()
+    c = Case(9, 64, 9000, dtype, 0.0)  # classes that no row can have: their logits are -inf
+    c.w[100:9000, 0] = -float("inf")
+    c.x[:, 0] = 1.0
+    c.x[:, 1:], c.ids = (c.x[:, 1:].abs() + 0.1), c.ids % 100
+    if dtype == BF16:
+        losses, _ = pkg.linear_xent_forward(c.x, c.w, c.ids)
+        want = torch.nn.functional.cross_entropy(c.x.double() @ c.w[:100].double().T, c.ids, reduction="none")
+        assert ((losses - want).abs() <= 2.0 ** -14 * (1 + want)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_several_pieces_of_the_vocabulary(pkg, dtype):
     """G of the whole vocabulary is far above the size of a piece: products of one piece beside the logits of the next."""
-    Case(6000, 72, 40001, dtype, 0.1).check(pkg)
+    Case(9000, 72, 40001, dtype, 0.1).check(pkg)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
