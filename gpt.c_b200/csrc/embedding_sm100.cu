@@ -471,6 +471,30 @@ __device__ void sort_bucket(const List &l, int bucket, BucketSmem &sm) {
     }
 }
 
+// What a gradient holds, to which a sum is added: fp32 values where they are, by L2, so that nobody waits for them (one thread of a call adds to a
+// place, so the order is fixed); bf16 values are asked for ahead and rounded once.
+template <class G, int kN>
+struct Held {
+    Raw<G, sizeof(G) == 2 ? kN : 1> old;
+    __device__ __forceinline__ void ask(const G *p) {
+        if constexpr (sizeof(G) == 2) old.load(p);
+    }
+    __device__ __forceinline__ void add(G *p, const float (&sum)[kN], float scale) {
+        if constexpr (sizeof(G) == 2) {
+            old.add(sum, scale);
+            old.store(p);
+        } else if constexpr (kN == 1) {
+            asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(p), "f"(sum[0] * scale) : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; i += 4)
+                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + i), "f"(sum[i] * scale), "f"(sum[i + 1] * scale), "f"(sum[i + 2] * scale),
+                             "f"(sum[i + 3] * scale)
+                             : "memory");
+        }
+    }
+};
+
 template <int kN>
 __device__ __forceinline__ void put(float *p, const float (&sum)[kN]) {
     Raw<float, kN> r;
@@ -559,120 +583,136 @@ __global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ 
     float sum[kN] = {};
     const E *dy = static_cast<const E *>(a.dy) + (inside ? col : 0);
     G *grad = static_cast<G *>(l.grad) + (inside ? col : 0);
-    for (int i0 = 0; i0 < count; i0 += kAhead) {
+    struct Batch {
         Raw<E, kN> v[kAhead];
-        Raw<G, kN> old[kAhead];
+        Held<G, kN> old[kAhead];
         int k[kAhead + 1];
+    };
+    auto ask = [&](Batch &b, int i0) {
 #pragma unroll
-        for (int u = 0; u < kAhead; u++) v[u].load(dy + __shfl_sync(0xffffffffu, row, (i0 + u) & 31) * a.ld);  // (behind the range: the row of place 0)
+        for (int u = 0; u < kAhead; u++) b.v[u].load(dy + __shfl_sync(0xffffffffu, row, (i0 + u) & 31) * a.ld);  // (behind the range: the row of place 0)
 #pragma unroll
-        for (int u = 0; u <= kAhead; u++) k[u] = i0 + u < 32 ? __shfl_sync(0xffffffffu, mine, (i0 + u) & 31) : -1;
+        for (int u = 0; u <= kAhead; u++) {
+            const int next = __shfl_sync(0xffffffffu, mine, (i0 + u) & 31);
+            b.k[u] = i0 + u < 32 ? next : -1;
+        }
 #pragma unroll
         for (int u = 0; u < kAhead; u++)
-            if (k[u + 1] != k[u] && k[u] < l.V && k[u] >= 0) old[u].load(grad + k[u] * l.ld);
+            if (b.k[u + 1] != b.k[u] && b.k[u] < l.V && b.k[u] >= 0) b.old[u].ask(grad + b.k[u] * l.ld);
+    };
+    auto take = [&](Batch &b, int i0) {
 #pragma unroll
         for (int u = 0; u < kAhead; u++) {
-            if (k[u] < 0) break;
-            if (k[u] >= l.V) {  // no token
+            if (b.k[u] < 0) break;
+            if (b.k[u] >= l.V) {  // no token
                 began = true;
                 continue;
             }
-            v[u].add_to(sum);
-            if (k[u + 1] == k[u]) continue;
+            b.v[u].add_to(sum);
+            if (b.k[u + 1] == b.k[u]) continue;
             if (inside) {
-                if (!began) {
-                    put<kN>(l.head + (long long)range * a.C + col, sum);
-                } else if (i0 + u == count - 1 && goes_on) {
-                    put<kN>(l.tail + (long long)range * a.C + col, sum);
-                } else {
-                    old[u].add(sum, l.scale);
-                    old[u].store(grad + k[u] * l.ld);
-                }
+                if (!began) put<kN>(l.head + (long long)range * a.C + col, sum);
+                else if (i0 + u == count - 1 && goes_on) put<kN>(l.tail + (long long)range * a.C + col, sum);
+                else b.old[u].add(grad + b.k[u] * l.ld, sum, l.scale);
             }
             began = true;
             clear(sum);
+        }
+    };
+    if constexpr (sizeof(G) == 2) {
+        for (int i0 = 0; i0 < count; i0 += kAhead) {
+            Batch b;
+            ask(b, i0);
+            take(b, i0);
+        }
+    } else {  // what fp32 gradients hold takes no registers: one batch is on its way while the other is added up
+        Batch even, odd;
+        ask(even, 0);
+        for (int i0 = 0; i0 < count; i0 += 2 * kAhead) {
+            if (i0 + kAhead < count) ask(odd, i0 + kAhead);
+            take(even, i0);
+            if (i0 + kAhead >= count) break;
+            if (i0 + 2 * kAhead < count) ask(even, i0 + 2 * kAhead);
+            take(odd, i0 + kAhead);
         }
     }
 }
 
 // Runs that leave the range in which they began: the sum of their parts, in the order of the list.  A warp looks at a range and takes runs of
-// up to kFew parts itself; a block takes the longer ones of its eight ranges one by one, its warps every eighth part.
-constexpr int kFew = 8;
+// up to kFew parts itself; a block takes the longer ones of its 16 ranges one by one, its warps every 16th part.
+constexpr int kFew = 8, kJoinWarps = 16;
 template <class G, int kN>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Gradient a) {
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Gradient a) {
     pdl_launch_dependents();
     pdl_wait();
-    __shared__ float part[8][32 * kN];
-    __shared__ int last_of[8], key_of[8];
+    __shared__ float part[kJoinWarps][32 * kN];
+    __shared__ int last_of[kJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = ((int)blockIdx.y * 32 + lane) * kN;
     const bool inside = col < a.C;
-    const int blocks0 = (a.list[0].ranges + 7) / 8, which = blockIdx.x < (unsigned)blocks0 ? 0 : 1;
+    const int blocks0 = (a.list[0].ranges + kJoinWarps - 1) / kJoinWarps, which = blockIdx.x < (unsigned)blocks0 ? 0 : 1;
     const List &l = a.list[which];
-    const int range0 = ((int)blockIdx.x - (which ? blocks0 : 0)) * 8, range = range0 + warp;
+    const int range0 = ((int)blockIdx.x - (which ? blocks0 : 0)) * kJoinWarps, range = range0 + warp;
     const int2 *places = l.sorted;
-    int last = -1, k = -1;  // the last range that the run reaches, -1: none begins here and goes on
+    int parts = 0, k = -1;  // of the run that begins in this range and goes on: behind this one
     if (range < l.ranges) {
         const int from = range * l.length, to = min(l.n, from + l.length);
-        const int at = lane == 0 ? to - 1 : lane == 1 ? to : from - 1;
-        const int seen = lane < 3 && at >= 0 && at < l.n ? places[at].x : -1;
+        // lane 0: the last place, lanes 1 to 30: the first ones of the next ranges, lane 31: the place in front of this one
+        const int at = lane == 0 ? to - 1 : lane < 31 ? to + (lane - 1) * l.length : from - 1;
+        const int seen = at >= 0 && at < l.n ? places[at].x : -1;
         k = __shfl_sync(0xffffffffu, seen, 0);
-        if (to < l.n && k < l.V && __shfl_sync(0xffffffffu, seen, 1) == k && __shfl_sync(0xffffffffu, seen, 2) != k) {
-            int lo = to, hi = l.n;  // places[lo] has k; where it ends is sought 32 places at a time
+        const unsigned same = __ballot_sync(0xffffffffu, seen == k);
+        if (k < l.V && !(same >> 31)) parts = __ffs(~(same >> 1)) - 1;  // (a range's last place has its token: sorted)
+        if (parts == 30) {  // more: where the run ends is sought 32 ranges at a time
+            int lo = range + 30, hi = l.ranges;  // range lo begins with k
             while (hi - lo > 1) {
-                const int step = (int)(((long long)hi - lo + 31) / 32);
-                const long long probe = lo + (lane + 1ll) * step;
-                const int same = __popc(__ballot_sync(0xffffffffu, probe < hi && places[probe < hi ? probe : lo].x == k));
-                lo += same * step;
-                hi = (int)min((long long)hi, (long long)lo + step);
+                const int step = (hi - lo + 31) / 32, probe = lo + (lane + 1) * step;
+                const int more = __popc(__ballot_sync(0xffffffffu, probe < hi && places[(long long)min(probe, hi - 1) * l.length].x == k));
+                lo += more * step;
+                hi = min(hi, lo + step);
             }
-            last = lo / l.length;
+            parts = lo - range;
         }
     }
-    if (lane == 0) last_of[warp] = last - range > kFew ? last : -1, key_of[warp] = k;
-    auto finish = [&](int r, int run, float(&sum)[kN]) {
-        Raw<float, kN> first;
-        Raw<G, kN> old;
-        G *grad = static_cast<G *>(l.grad) + run * l.ld + col;
-        old.load(grad);
-        first.load(l.tail + (long long)r * a.C + col);
-        first.add_to(sum);
-        old.add(sum, l.scale);
-        old.store(grad);
+    if (lane == 0) last_of[warp] = parts > kFew ? range + parts : -1;
+    G *const grad = static_cast<G *>(l.grad) + col;
+    auto sum_of = [&](int first, int end, int step, float(&sum)[kN]) {  // parts first, first + step, .. up to end
+        for (int r0 = first; r0 <= end; r0 += step * kAhead) {
+            Raw<float, kN> v[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) v[u].load(l.head + (long long)min(r0 + step * u, end) * a.C + col);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++)
+                if (r0 + step * u <= end) v[u].add_to(sum);
+        }
     };
-    if (last >= 0 && last - range <= kFew && inside) {
-        Raw<float, kN> v[kFew];
-        float sum[kN] = {};
-#pragma unroll
-        for (int u = 0; u < kFew; u++) v[u].load(l.head + (long long)min(range + 1 + u, last) * a.C + col);
-#pragma unroll
-        for (int u = 0; u < kFew; u++)
-            if (range + 1 + u <= last) v[u].add_to(sum);
-        finish(range, k, sum);
+    Raw<float, kN> tail;
+    Held<G, kN> old;
+    if (parts > 0 && inside) {
+        old.ask(grad + k * l.ld);
+        tail.load(l.tail + (long long)range * a.C + col);
+        if (parts <= kFew) {
+            float sum[kN] = {};
+            tail.add_to(sum);
+            sum_of(range + 1, range + parts, 1, sum);
+            old.add(grad + k * l.ld, sum, l.scale);
+        }
     }
     __syncthreads();
-    for (int w = 0; w < 8; w++) {
+    for (int w = 0; w < kJoinWarps; w++) {
         const int end = last_of[w];
         if (end < 0) continue;
         float sum[kN] = {};
-        if (inside) {
-            for (int r0 = range0 + w + 1 + warp; r0 <= end; r0 += 8 * kAhead) {
-                Raw<float, kN> v[kAhead];
-#pragma unroll
-                for (int u = 0; u < kAhead; u++) v[u].load(l.head + (long long)min(r0 + 8 * u, end) * a.C + col);
-#pragma unroll
-                for (int u = 0; u < kAhead; u++)
-                    if (r0 + 8 * u <= end) v[u].add_to(sum);
-            }
-        }
+        if (inside) sum_of(range0 + w + 1 + warp, end, kJoinWarps, sum);
 #pragma unroll
         for (int e = 0; e < kN; e++) part[warp][lane * kN + e] = sum[e];
         __syncthreads();
-        if (warp == 0 && inside) {
+        if (warp == w && inside) {
             clear(sum);
-            for (int i = 0; i < 8; i++)
+            tail.add_to(sum);
+            for (int i = 0; i < kJoinWarps; i++)
 #pragma unroll
                 for (int e = 0; e < kN; e++) sum[e] += part[i][lane * kN + e];
-            finish(range0 + w, key_of[w], sum);
+            old.add(grad + k * l.ld, sum, l.scale);
         }
         __syncthreads();
     }
@@ -828,8 +868,9 @@ cudaError_t launch_gradient(const Gradient &a, cudaStream_t s) {
     const long long others = a.n <= kBucketed ? (std::min((places + kThreads - 1) / kThreads, 1184ll) + slices - 1) / slices : 0;
     e = attn::launch_after_previous(runs_kernel<E, G, kN>, dim3((unsigned)(groups + others), slices), dim3(kThreads), 0, s, a, groups);
     if (e != cudaSuccess || a.lists == 0) return e;
-    const int blocks = (a.list[0].ranges + 7) / 8 + (a.lists > 1 ? (a.list[1].ranges + 7) / 8 : 0);
-    return attn::launch_after_previous(join_kernel<G, kN>, dim3((unsigned)blocks, slices), dim3(256), 0, s, a);
+    const int joins = (a.list[0].ranges + kJoinWarps - 1) / kJoinWarps + (a.lists > 1 ? (a.list[1].ranges + kJoinWarps - 1) / kJoinWarps : 0);
+    constexpr int kJoined = kN > 4 ? 4 : kN;  // narrower, since one run may be all that there is to do
+    return attn::launch_after_previous(join_kernel<G, kJoined>, dim3((unsigned)joins, (unsigned)((a.C / kJoined + 31) / 32)), dim3(32 * kJoinWarps), 0, s, a);
 }
 
 template <class E, class G>

@@ -89,9 +89,9 @@ def test_shapes_and_types(pkg, shape, C, V, P, dtype, grad):
         b.check_backward(pkg, scale=[1.0, 3.5, -0.1][i])
 
 
-@pytest.mark.parametrize("n,V", [(1, 1), (7, 2), (31, 3), (4, 1 << 20), (1000, 1), (2047, 70000), (2049, 255), (16385, 256), (40000, 65536), (66000, 300000), (70000, 1)])
+@pytest.mark.parametrize("n,V", [(1, 1), (7, 2), (31, 3), (4, 1 << 20), (1000, 1), (2047, 70000), (2049, 255), (16385, 256), (40000, 65536), (66000, 300000), (70000, 1), (150000, 128), (150000, 1 << 17)])
 def test_runs_of_equal_tokens(pkg, n, V):
-    """Lists on both sides of where ranges change their length, sorts of one to three passes, runs over many ranges."""
+    """Lists on both sides of where ranges change their length, buckets that are compared, that take one pass and two, runs over many ranges."""
     for pad in (0.0, 0.7):
         Batch((n,), 8, V, 1, pad=pad, positions=None, out=0.05, seed=n).check_backward(pkg, 2.0)
 
