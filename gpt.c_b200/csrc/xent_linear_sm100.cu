@@ -12,8 +12,20 @@
 //     z   A: x,  contraction contiguous    B: w, contraction contiguous
 //     dx  A: G,  contraction contiguous    B: w, columns contiguous
 //     dw  A: G,  rows contiguous           B: x, columns contiguous
-// fp32 operands are two bf16 planes, hi and lo, and a product is hi hi + hi lo + lo hi: four tiles of a contraction block serve three
-// products.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks.
+// fp32 operands are two bf16 planes, hi and lo (16 bits, 2^-18 of a value is left), and a product is hi hi + hi lo + lo hi: four tiles of a
+// contraction block serve three products.  Six products of three planes would have all 24 bits in twice the time, TF32 operands
+// 11 bits in two thirds of it.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks.  With bf16 operands G is rounded
+// to bf16 like the activations and gradients around it; sums stay fp32 until one rounding at the end.
+//
+// A CTA has a tile of 256 x 256 in two accumulators of 128 rows: shared memory takes in 64 KB a block and hands out 96 in 1280 cycles, against
+// 1024 of the tensor cores.  (Two CTAs on a tile would take in half of B each; pairs have stopped for good on this GPU and are not used.)
+//
+// Warp 0 hands out items (from a counter in the backward, longest first) and asks for tiles, warp 1 issues the products, the others take the sums out.
+// The waits on barriers are bounded (tc05.cuh); the allocation of tensor memory and the wait for the previous kernel end for the reasons given there.
+//
+// Bound by the power limit where rows are many: 8192 x 768 x 50257 bf16, forward 475 to 510 us (1240 to 1330 TFLOP/s at 1.55 GHz, 1 kW), backward 1740 to 1850
+// (1370 to 1450, with z made again; the GPU's sustained rate for a matrix product alone is 1389); 4096 rows fp32 730 and 2580 to 2740 us (three products
+// each: 1300, 1380 to 1470).  Few rows wait for their operands: 40 rows bf16 23 to 26 and 98 us, where reading and writing takes 12 and 47.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -36,7 +48,7 @@ constexpr int kQueue = 4;
 constexpr int kSegment = 16;           // contraction blocks of fp32 operands that one sum in tensor memory takes
 constexpr float kLog2e = 1.4426950408889634f;
 
-enum Site : int { SITE_EMPTY = 301, SITE_FULL, SITE_ACC_EMPTY, SITE_ACC_FULL, SITE_ITEM, SITE_ITEM_FREE, SITE_SMEM_ALIGN };
+enum Site : int { SITE_EMPTY = 301, SITE_FULL, SITE_ACC_EMPTY, SITE_ACC_FULL, SITE_ITEM, SITE_ITEM_FREE, SITE_PART_FULL, SITE_PART_EMPTY, SITE_SMEM_ALIGN };
 enum Kind : int { kLogits, kDx, kDw };
 
 template <int kSlots, bool kBackward>
@@ -46,6 +58,7 @@ struct __align__(1024) Smem {
     uint64_t full[kSlots], empty[kSlots];
     uint64_t acc_full[2], acc_empty[2];
     uint64_t item_full[kQueue], item_empty[kQueue];
+    uint64_t part_full[2][4], part_empty[2][4];  // of each quarter of the lanes
     int item[kQueue];
     uint32_t tmem_base;
     int abort_flag;
@@ -89,7 +102,7 @@ struct Problem {
 
 struct Item {
     int kind, m0, n0, n, halves;   // n: columns, a multiple of 16
-    int blocks, segment, block0;   // contraction blocks, of one sum; where they begin
+    int blocks, block0;            // contraction blocks, and where they begin
     int piece;
 };
 
@@ -126,7 +139,6 @@ __device__ __forceinline__ Item decode(const Problem &p, int w) {
     }
     it.halves = rows - it.m0 > 128 ? 2 : 1;
     it.n = min(it.kind == kLogits ? p.wide : kTile, max(16, (cols - it.n0 + 15) / 16 * 16));
-    it.segment = it.blocks;
     return it;
 }
 
@@ -262,6 +274,10 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
         for (int i = 0; i < kQueue; i++) {
             mbar_init(&sm.item_full[i], 1);
             mbar_init(&sm.item_empty[i], 1 + kEpiWarps);
+        }
+        for (int i = 0; i < 8; i++) {
+            mbar_init(&sm.part_full[i / 4][i % 4], 3);
+            mbar_init(&sm.part_empty[i / 4][i % 4], 1);
         }
         fence_barrier_init();
         tma_prefetch_desc(&maps.x);
@@ -487,13 +503,27 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                 if (here && e == place) p.zt[row] = __uint_as_float(z[e]) * p.fix;
                         }
                         top *= p.fix;
-                        // the four quarters of the tile's columns
-                        if (group > 0) sm.part[half & 1][group - 1][quarter * 32 + lane] = make_float2(top, sum);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
-                        if (group == 0) {
+                        // the four quarters of the tile's columns: the first of these warps joins them
+                        const int buffer = half & 1, turn = (half / 2) & 1;
+                        uint64_t *const there = &sm.part_full[buffer][quarter], *const read = &sm.part_empty[buffer][quarter];
+                        if (group > 0) {
+                            if (half >= 2 && !mbar_wait_warp(read, turn ^ 1, ctx, SITE_PART_EMPTY)) {
+                                ok = false;
+                                break;
+                            }
+                            sm.part[buffer][group - 1][quarter * 32 + lane] = make_float2(top, sum);
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(there);
+                        } else {
+                            if (!mbar_wait_warp(there, turn, ctx, SITE_PART_FULL)) {
+                                ok = false;
+                                break;
+                            }
                             float2 q[4] = {make_float2(top, sum)};
 #pragma unroll
-                            for (int i = 0; i < 3; i++) q[i + 1] = sm.part[half & 1][i][quarter * 32 + lane];
+                            for (int i = 0; i < 3; i++) q[i + 1] = sm.part[buffer][i][quarter * 32 + lane];
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(read);
                             const float m = fmaxf(fmaxf(q[0].x, q[1].x), fmaxf(q[2].x, q[3].x)), nm = m == -INFINITY ? 0.f : -m * kLog2e;
                             sum = 0.f;
 #pragma unroll
@@ -595,6 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
     }
 
     // ------------------------------ tear-down ------------------------------
+    if (sm.abort_flag) __nanosleep(50000);  // products that have been issued end
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 1) {
@@ -735,9 +766,12 @@ __global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const floa
 
 // ---- host side ----
 
-constexpr size_t kPieceBytes = (size_t)256 << 20;  // of G, at most, but for
-constexpr int kLeastTiles = 32;                    // tiles of classes
-constexpr int kFetchBlocks = 8;
+// G of a piece takes 256 MB at most, but for pieces of 32 tiles of classes: below that an item of dw, whose contraction is all rows, is longer than what a
+// piece gives an SM to do.  Backward of 8192 x 768 x 50257 bf16 with 64, 128, 256, 512 MB: 2154, 1820, 1787, 1744 us; 16384 rows: 6324, 4293, 3671, 3629.
+constexpr size_t kPieceBytes = (size_t)256 << 20;
+constexpr int kLeastTiles = 32;
+constexpr int kMostRows = 1 << 20;  // of the backward: a sum of dw over more steps would be cut off by more than it is rounded
+constexpr int kFetchBlocks = 8;         // of 64 rows (40 rows, bf16 107 -> 98 us)
 constexpr int kForwardSlots = 6, kBackwardSlots = 7;
 
 int up(int v, int to) { return (v + to - 1) / to * to; }
@@ -854,7 +888,7 @@ cudaError_t launch_planes(const void *src, long long ld, int type, void *to, siz
                                        targets, V, counters, count);
 }
 
-// Eight threads share the pieces where there are more than four: 49 pieces of 40 x 768 18 -> XX us.
+// Eight threads share the pieces where there are more than four: 49 pieces of 40 x 768 18 -> 4.8 us.
 template <class T>
 cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, cudaStream_t s) {
     const int groups = count > 4 ? 8 : 1;
@@ -869,6 +903,14 @@ cudaError_t launch_tiles(const Maps &maps, const Problem &p, int sms, int *statu
     return attn::launch_after_previous(tiles_kernel<kTerms, kBackward, kSlots>, dim3((unsigned)std::min(p.total, sms)), dim3(kThreads), sizeof(Smem<kSlots, kBackward>),
                                        s, maps, p, status);
 }
+
+// The memory of a matrix; NULL: none.
+struct Span {
+    uintptr_t from, to;
+    Span(const void *p, long long rows, long long ld, long long columns, size_t each)
+        : from(reinterpret_cast<uintptr_t>(p)), to(p ? from + ((rows - 1) * ld + columns) * each : 0) {}
+    bool meets(const Span &o) const { return from && o.from && from < o.to && o.from < to; }
+};
 
 int check(const void *x, const void *w, const void *targets, const void *scratch, long long ldx, long long ldw, int type, int target_type, int rows, int V, int K) {
     if (rows < 0 || V <= 0 || K <= 0 || ldx < K || ldw < K) return ATTN_ERR_ARGUMENT;
@@ -907,7 +949,7 @@ size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, lon
 }
 
 size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
-    if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0) return 0;
+    if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0 || rows > head::kMostRows) return 0;
     return head::layout(x, w, ldx, ldw, type, rows, V, K, true, attn::sm_count()).total;
 }
 
@@ -959,9 +1001,18 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
     if (rc != ATTN_OK) return rc;
     if (dw && lddw < K) return ATTN_ERR_ARGUMENT;
+    if (rows > kMostRows) return ATTN_ERR_UNSUPPORTED;
     const size_t each = type == TENSOR_F32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(g) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3) || reinterpret_cast<uintptr_t>(dx) % each || reinterpret_cast<uintptr_t>(dw) % each)
         return ATTN_ERR_ALIGN;
+    if (rows > 0) {
+        const Span x_at(x, rows, ldx, K, each), w_at(w, V, ldw, K, each), dx_at(dx, rows, K, K, each), dw_at(dw, V, lddw, K, each);
+        const Span lse_at(lse, 1, rows, rows, 4), g_at(g, 1, rows, one_g ? 1 : rows, 4), t_at(targets, 1, rows, rows, target_type == TENSOR_INT64 ? 8 : 4);
+        for (const Span &out : {dx_at, dw_at})
+            for (const Span &in : {x_at, w_at, lse_at, g_at, t_at})
+                if (out.meets(in)) return ATTN_ERR_ARGUMENT;
+        if (dx_at.meets(dw_at)) return ATTN_ERR_ARGUMENT;
+    }
     int *status = nullptr;
     if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
     if (rows == 0) return ATTN_OK;

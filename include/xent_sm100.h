@@ -72,8 +72,9 @@ int xent_sm100_sample(const float *logits, const float *u, const float *temperat
  *   losses[r] = lse[r] - z[r, targets[r]], 0 for a row without a target
  *
  * The products of bf16 tensors are exact, those of fp32 tensors are made of two bf16 terms of each factor (16 bits of it; values
- * above 3.38e38 in size have none); sums are fp32.  rows may be 0.
- * scratch: xent_sm100_linear_forward_scratch_bytes bytes, 256-byte aligned; x and w are looked at for their alignment only there.
+ * above 3.38e38 in size have none); sums are fp32.  rows may be 0.  Outputs overlap no input.
+ * scratch: xent_sm100_linear_forward_scratch_bytes bytes for the same arguments on the same device, 256-byte aligned.  (Of the tensors their
+ * alignment matters there: bf16 ones on 16-byte boundaries are read where they are, others copied.)
  */
 size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K);
 int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch,
@@ -86,8 +87,9 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
  *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call; may be NULL, but not both
  * With bf16 tensors G is rounded to bf16 before these products, with fp32 tensors it is two bf16 terms like the others.  The results
  * have the same bits in every call on GPUs of as many SMs.
- * G is in memory for a piece of the vocabulary at a time: scratch of xent_sm100_linear_backward_scratch_bytes bytes (some hundred MB at
- * most where rows are up to 100000, apart from copies of fp32 tensors), 256-byte aligned; 0: the sizes are refused.
+ * G is in memory for two pieces of the vocabulary at a time, up to 256 MB each, or 16384 bytes a row (fp32 32768) where that is more:
+ * scratch of xent_sm100_linear_backward_scratch_bytes bytes, which also has room for dx in fp32 and for copies of x and, if fp32, of w;
+ * 256-byte aligned.  Up to 2^20 rows.  dx and dw overlap each other and the inputs in no byte (rows of one inside the gaps of another count as that).
  */
 size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K);
 int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw,

@@ -18,7 +18,7 @@ EMBED = dict(tokens=P, table=P, positions=None, pos_table=P, y=P, n=5, ld=64, po
 EMBED_GRAD = dict(dy=P, tokens=P, dtable=at(1 << 24), positions=None, dpos=at(1 << 25), scratch=at(1 << 26), n=5, ld_dy=64, ld=64, pos_ld=64, scale=1.0, type=0, grad=0,
                   ids=1, T=5, C=64, V=100, Pn=9, stream=None)
 LOSS = dict(x=P, w=P, targets=P, losses=P, lse=P, scratch=P, ldx=64, ldw=64, type=1, ids=1, rows=5, V=100, K=64, stream=None)
-LOSS_GRAD = dict(g=P, x=P, w=P, targets=P, lse=P, dx=P, dw=P, scratch=P, ldx=64, ldw=64, lddw=64, one=0, type=1, ids=1, rows=5, V=100, K=64, stream=None)
+LOSS_GRAD = dict(g=P, x=P, w=P, targets=P, lse=P, dx=at(1 << 21), dw=at(1 << 22), scratch=P, ldx=64, ldw=64, lddw=64, one=0, type=1, ids=1, rows=5, V=100, K=64, stream=None)
 
 
 @pytest.mark.parametrize("wrong,code", [
@@ -59,7 +59,9 @@ def test_linear_xent_forward_refuses(pkg, wrong, code):
 
 
 @pytest.mark.parametrize("wrong,code", HEAD_WRONG + [(dict(g=None), NULL), (dict(dx=None, dw=None), NULL), (dict(lddw=63), ARGUMENT), (dict(dx=ODD), ALIGN), (dict(dw=ODD), ALIGN),
-                                                     (dict(g=at((1 << 20) + 2)), ALIGN)])
+                                                     (dict(g=at((1 << 20) + 2)), ALIGN), (dict(rows=(1 << 20) + 1), UNSUPPORTED), (dict(dx=at(1 << 22)), ARGUMENT),
+                                                     (dict(dx=P), ARGUMENT), (dict(dw=P), ARGUMENT), (dict(dw=at((1 << 20) + 4 * 128)), ARGUMENT),
+                                                     (dict(w=at((1 << 22) + 99 * 128 + 62)), ARGUMENT), (dict(lse=at((1 << 21) + 16)), ARGUMENT)])
 def test_linear_xent_backward_refuses(pkg, wrong, code):
     assert pkg.lib().xent_sm100_linear_backward(*{**LOSS_GRAD, **wrong}.values()) == code
 
