@@ -120,10 +120,13 @@ struct Lookup {
 };
 
 // kN columns at a time; a block takes `rows` rows of `words` such pieces.  i / words for i < 2^16 is the upper half of i * magic.
+// Pieces of a thread: two where they are 32 bytes of two tables, whose four take too many registers.
+constexpr int units_of(int bytes, bool places) { return bytes == 32 && places ? 2 : kUnits; }
 template <class E, int kN, bool kPlaces>
 __global__ void __launch_bounds__(kThreads, 4) lookup_kernel(Lookup a, int rows, int words, unsigned magic) {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr int kUnits = units_of(kN * sizeof(E), kPlaces);
     const long long row0 = (long long)blockIdx.x * rows;
     const int here = (int)min((long long)rows, a.n - row0) * words;
     const unsigned place0 = kPlaces && !a.positions.p ? (unsigned)(row0 % a.T) : 0;
@@ -810,7 +813,7 @@ template <class E>
 cudaError_t launch_lookup(const Lookup &a, int bytes, int rows, int words, cudaStream_t s) {
     const unsigned magic = words > 1 ? (unsigned)(((1ull << 32) + words - 1) / words) : 0;
     const dim3 grid((unsigned)((a.n + rows - 1) / rows)), block(kThreads);
-    auto kernel = a.pos_table ? (bytes == 16 ? lookup_kernel<E, 16 / sizeof(E), true> : lookup_kernel<E, 1, true>)
+    auto kernel = a.pos_table ? (bytes == 32 ? lookup_kernel<E, 32 / sizeof(E), true> : bytes == 16 ? lookup_kernel<E, 16 / sizeof(E), true> : lookup_kernel<E, 1, true>)
                               : (bytes == 32 ? lookup_kernel<E, 32 / sizeof(E), false> : bytes == 16 ? lookup_kernel<E, 16 / sizeof(E), false> : lookup_kernel<E, 1, false>);
     return attn::launch_after_previous(kernel, grid, block, 0, s, a, rows, words, magic);
 }
@@ -910,11 +913,12 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
     if (rc != ATTN_OK) return rc;
     if (n == 0) return ATTN_OK;
     if (n > (1ll << 40) / C || C > (1 << 20)) return ATTN_ERR_UNSUPPORTED;
-    // 32 bytes at a time where every row allows it and there is one table (two rows of four such pieces take too many registers), else 16, else a value
-    const uintptr_t all = embed::bits(table) | embed::bits(pos_table) | embed::bits(y) | C * each | (uintptr_t)ld * each | (pos_table ? (uintptr_t)pos_ld * each | 16 : 0);
+    // 32 bytes at a time where every row allows it, else 16, else a value
+    const uintptr_t all = embed::bits(table) | embed::bits(pos_table) | embed::bits(y) | C * each | (uintptr_t)ld * each | (pos_table ? (uintptr_t)pos_ld * each : 0);
     const int bytes = all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : (int)each, words = (int)(C * each / bytes);
-    // a block has a piece for each thread, or four where that leaves blocks enough
-    const long long pieces = n * words, per = pieces >= embed::kThreads * embed::kUnits * 600ll ? embed::kThreads * embed::kUnits : embed::kThreads;
+    // a block has a piece for each thread, or all that one takes where that leaves blocks enough
+    const int units = embed::units_of(bytes, pos_table != nullptr);
+    const long long pieces = n * words, per = pieces >= embed::kThreads * units * 600ll ? embed::kThreads * units : embed::kThreads;
     const int rows = (int)std::max(1ll, per / words);
     if ((n + rows - 1) / rows > 0x7fffffffll) return ATTN_ERR_UNSUPPORTED;
     const embed::Lookup a{table, pos_table, y, ld, pos_ld, n, Ids{tokens, id_type}, Ids{positions, id_type}, T, C, V, P, scale};

@@ -725,10 +725,11 @@ __global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const floa
     pdl_wait();
     constexpr int kWords = 256 / kGroups, kAhead = 4;
     __shared__ float4 part[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kWords : 1];
-    const int words = pitch / 4, group = threadIdx.x / kWords, place = threadIdx.x % kWords;
+    const unsigned words = pitch / 4;
+    const int group = threadIdx.x / kWords, place = threadIdx.x % kWords;
     const long long total = (long long)M * words, apart = (long long)M * pitch;
     for (long long i0 = (long long)blockIdx.x * kWords; i0 < total; i0 += (long long)gridDim.x * kWords) {
-        const long long i = i0 + place, r = i / words;
+        const long long i = i0 + place, r = total <= 0xffffffffll ? (unsigned)i / words : i / words;
         const int c = (int)(i - r * words) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < total) {
@@ -841,10 +842,11 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     l.pieces = (tiles_v + tiles - 1) / tiles;
     l.cols = l.pieces > 1 ? tiles * kTile : up(V, kBlock);
     l.wide = l.pieces > 1 ? kTile : tile_width(M, l.cols, sms);
-    // pieces of the contraction of dx: none is longer than half of what an SM has to do for a piece of the vocabulary
+    // Pieces of the contraction of dx: none is longer than a share of what an SM has to do for a piece of the vocabulary.  Share 0.5, 0.7, 1.0: 40 rows bf16
+    // 98.6, 106, 106 us; 500 rows 187, 178, 173; 2048 x 768 x 16384 198, 198, 179; 4096 rows fp32 2661, 2609, 2705 (each more piece is 4 bytes a value of dx twice).
     const int blocks = l.cols / kBlock;
     const double load = ((double)tiles_m * tiles_k * blocks + (double)tiles * tiles_k * std::max(4, (M + kBlock - 1) / kBlock)) / sms;
-    const int longest = std::max(12, (int)(load / 2));
+    const int longest = std::max(12, (int)(load * (M <= 128 ? 0.5 : type == TENSOR_F32 ? 0.7 : 1.0)));
     l.dx_pieces = std::min(64, (blocks + longest - 1) / longest);
     l.dx_blocks = (blocks + l.dx_pieces - 1) / l.dx_pieces;
     l.dx_pieces = (blocks + l.dx_blocks - 1) / l.dx_blocks;
@@ -888,10 +890,10 @@ cudaError_t launch_planes(const void *src, long long ld, int type, void *to, siz
                                        targets, V, counters, count);
 }
 
-// Eight threads share the pieces where there are more than four: 49 pieces of 40 x 768 18 -> 4.8 us.
+// Eight threads share the pieces where there are more than four and few words: 49 pieces of 40 x 768 18 -> 4.8 us, 7 of 2048 x 768 23.5 us by eight (11 by one).
 template <class T>
 cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, cudaStream_t s) {
-    const int groups = count > 4 ? 8 : 1;
+    const int groups = count > 4 && (long long)M * (pitch / 4) < 100000 ? 8 : 1;
     const int grid = blocks_for((long long)M * (pitch / 4) * groups);
     return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide)
                       : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide);
