@@ -36,16 +36,10 @@ template <class T>
 struct Piece {
     static constexpr int kValues = 32 / sizeof(T);
     uint32_t v[8];
-    __device__ __forceinline__ void load(const T *p, int left) {  // `left`: values that are inside, a multiple of 8
-        if (left >= kValues) {
-            asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                         : "l"(p));
-        } else {
+    __device__ __forceinline__ void load(const T *p, int left) {  // `left`: values that are inside, as many as 16 bytes at a time
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 0;
-            if (sizeof(T) == 2 && left > 0) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
-        }
+        for (int i = 0; i < 2; i++)
+            *reinterpret_cast<uint4 *>(v + 4 * i) = left > i * kValues / 2 ? *reinterpret_cast<const uint4 *>(p + i * kValues / 2) : make_uint4(0, 0, 0, 0);
     }
     // kValues / 2 words of two bf16 values
     __device__ __forceinline__ void split(uint32_t (&hi)[kValues / 2], uint32_t (&lo)[kValues / 2]) const {
@@ -57,10 +51,17 @@ struct Piece {
     }
 };
 
-// kTiles: of 16 rows of x.  `classes`: of a CTA, a multiple of 16.
-template <class T, int kTiles>
+// What the backward makes of z: G[v, 0 .. stride - 1], of up to 16 rows.
+struct ToG {
+    float *out;
+    const float *g, *lse;
+    int one_g, stride;
+};
+
+// kTiles: of 16 rows of x.  `classes`: of a CTA, a multiple of 16.  kGradient: G instead of maxima and sums.
+template <class T, int kTiles, bool kGradient>
 __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, Ids targets,
-                                                                   float2 *__restrict__ part, float *__restrict__ zt, int M, int V, int K, int classes, int pitch) {
+                                                                   float2 *__restrict__ part, float *__restrict__ zt, ToG to, int M, int V, int K, int classes, int pitch) {
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(16) uint8_t rows[];  // [plane][16 kTiles][pitch bytes]
@@ -109,6 +110,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
             const int row = 16 * m + 8 * r + g;
             target[m][r] = row < M ? targets.at(row, V) : -1;
             top[m][r] = -INFINITY, sum[m][r] = 0.f;
+            if (kGradient && row < M) top[m][r] = to.lse[row], sum[m][r] = target[m][r] < 0 ? 0.f : to.g[to.one_g ? 0 : row];
         }
     __syncthreads();
 
@@ -160,45 +162,166 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
             for (int m = 0; m < kTiles; m++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float v[4];
+                    if constexpr (kGradient) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int c = first + 8 * (i / 2) + i % 2;
-                        v[i] = c < V ? z[m][i / 2][2 * h + i % 2] : -INFINITY;
-                        if (c < V && c == target[m][h]) zt[16 * m + 8 * h + g] = v[i];
+                        for (int i = 0; i < 4; i++) {
+                            const int c = first + 8 * (i / 2) + i % 2, row = 8 * h + g;
+                            const float p = exp_of(z[m][i / 2][2 * h + i % 2] - top[m][h]) - (c == target[m][h] ? 1.f : 0.f);
+                            if (c < V && row < to.stride) to.out[(long long)c * to.stride + row] = target[m][h] < 0 ? 0.f : p * sum[m][h];
+                        }
+                    } else {
+                        float v[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int c = first + 8 * (i / 2) + i % 2;
+                            v[i] = c < V ? z[m][i / 2][2 * h + i % 2] : -INFINITY;
+                            if (c < V && c == target[m][h]) zt[16 * m + 8 * h + g] = v[i];
+                        }
+                        const float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), top[m][h]), by = most == -INFINITY ? 0.f : most;
+                        sum[m][h] *= exp_of(top[m][h] - by);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sum[m][h] += exp_of(v[i] - by);
+                        top[m][h] = most;
                     }
-                    const float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), top[m][h]), by = most == -INFINITY ? 0.f : most;
-                    sum[m][h] *= exp_of(top[m][h] - by);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sum[m][h] += exp_of(v[i] - by);
-                    top[m][h] = most;
                 }
         }
     }
-    // the lanes of a row, then the warps
-    auto join = [](float &m, float &s, float m2, float s2) {
-        const float most = fmaxf(m, m2), by = most == -INFINITY ? 0.f : most;
-        s = s * exp_of(m - by) + s2 * exp_of(m2 - by);
-        m = most;
-    };
+    if constexpr (!kGradient) {
+        // the lanes of a row, then the warps
+        auto join = [](float &m, float &s, float m2, float s2) {
+            const float most = fmaxf(m, m2), by = most == -INFINITY ? 0.f : most;
+            s = s * exp_of(m - by) + s2 * exp_of(m2 - by);
+            m = most;
+        };
 #pragma unroll
-    for (int m = 0; m < kTiles; m++)
+        for (int m = 0; m < kTiles; m++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+            for (int h = 0; h < 2; h++) {
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1)
-                join(top[m][h], sum[m][h], __shfl_xor_sync(0xffffffffu, top[m][h], o), __shfl_xor_sync(0xffffffffu, sum[m][h], o));
-            if (q == 0) all[warp][16 * m + 8 * h + g] = make_float2(top[m][h], sum[m][h]);
+                for (int o = 1; o < 4; o <<= 1)
+                    join(top[m][h], sum[m][h], __shfl_xor_sync(0xffffffffu, top[m][h], o), __shfl_xor_sync(0xffffffffu, sum[m][h], o));
+                if (q == 0) all[warp][16 * m + 8 * h + g] = make_float2(top[m][h], sum[m][h]);
+            }
+        __syncthreads();
+        const int row = threadIdx.x;
+        if (row < M) {
+            float m = -INFINITY, s = 0.f;
+            for (int i = 0; i < warps; i++) join(m, s, all[i][row].x, all[i][row].y);
+            part[(long long)blockIdx.x * M + row] = make_float2(m, s);
         }
-    __syncthreads();
-    const int row = threadIdx.x;
-    if (row >= M) return;
-    float m = -INFINITY, s = 0.f;
-    for (int i = 0; i < warps; i++) join(m, s, all[i][row].x, all[i][row].y);
-    part[(long long)blockIdx.x * M + row] = make_float2(m, s);
+    }
 }
 
 // Eight lanes read four pieces of 16 bytes each of two rows, next to each other (fp32: hi or lo of 8 values) or 32 bytes apart.
+// ---------------------------------------------------------------------------------------------
+// The two products of the backward for up to 16 rows, in fp32 arithmetic: a thread has four columns of x and of the sums of dx for all rows, and goes through
+// classes of its block: w once for dx, dw once for what is added to it.  G of a class is the same for all threads.
+//
+// Bound by HBM: w is read again (with the G kernel twice in all) and dw read and written, 617 MB of fp32 and 309 of bf16 at 768 x 50257: 94 and 47 us.
+// Measured with G and the sum of dx, in brackets with tiles: 1 row fp32 113 us (216; 780 features 121, 371), 16 rows 162 (214), where the multiplications
+// take as long; bf16, whose values come eight bytes a thread, 82 for 1 row, 80 for 4, 100 for 8 (98; 9000 classes
+// of 200 features 20, with tiles 33), but 145 for 16, which tiles keep.
+// ---------------------------------------------------------------------------------------------
+constexpr int kProductThreads = 256, kClasses = 64, kAheadClasses = 8;
+
+template <class T>
+struct Four {
+    static constexpr int kWords = sizeof(T);  // of four values
+    uint32_t v[kWords];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+        else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
+    }
+    __device__ __forceinline__ void values(float (&f)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = sizeof(T) == 4 ? __uint_as_float(v[i % kWords]) : __uint_as_float(i & 1 ? v[i / 2 % kWords] & 0xffff0000u : v[i / 2 % kWords] << 16);
+    }
+};
+
+template <class T, int kRows>
+__global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_products_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, Ids targets,
+                                                                                                const float *__restrict__ G, T *dw, long long lddw, float *__restrict__ dxp,
+                                                                                                int dx_pitch, int M, int V, int K, int classes, int width) {
+    pdl_launch_dependents();
+    pdl_wait();
+    __shared__ __align__(16) float of_class[kClasses][kRows];
+    const int groups = (int)blockDim.x / width, group = (int)threadIdx.x / width, column = (int)threadIdx.x - group * width;
+    const int col = ((int)blockIdx.y * width + column) * 4;
+    const bool inside = col < K;
+    const int begin = blockIdx.x * classes, end = min(V, begin + classes);
+    float xs[kRows][4], sum[kRows][4];
+#pragma unroll
+    for (int m = 0; m < kRows; m++) {
+        Four<T> f;
+#pragma unroll
+        for (int i = 0; i < Four<T>::kWords; i++) f.v[i] = 0;
+        if (dw != nullptr && inside && m < M && targets.at(m, V) >= 0) f.load(x + m * ldx + col);  // rows without a target may hold anything
+        f.values(xs[m]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum[m][e] = 0.f;
+    }
+    for (int v0 = begin; v0 < end; v0 += kClasses) {
+        const int count = min(kClasses, end - v0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < count * kRows / 4; i += (int)blockDim.x)
+            reinterpret_cast<float4 *>(&of_class[0][0])[i] = reinterpret_cast<const float4 *>(G + (long long)v0 * kRows)[i];
+        __syncthreads();
+        for (int c0 = group * kAheadClasses; c0 < count; c0 += groups * kAheadClasses) {
+            Four<T> ws[kAheadClasses], old[sizeof(T) == 2 ? kAheadClasses : 1];
+            if (!inside) continue;
+#pragma unroll
+            for (int u = 0; u < kAheadClasses; u++) {
+                const long long v = v0 + min(c0 + u, count - 1);
+                if (dxp) ws[u].load(w + v * ldw + col);
+                if (sizeof(T) == 2 && dw) old[u % (sizeof(T) == 2 ? kAheadClasses : 1)].load(dw + v * lddw + col);
+            }
+#pragma unroll
+            for (int u = 0; u < kAheadClasses; u++) {
+                if (c0 + u >= count) break;
+                float f[4], add[4] = {0.f, 0.f, 0.f, 0.f};
+                ws[u].values(f);
+#pragma unroll
+                for (int m = 0; m < kRows; m++) {
+                    const float g = of_class[c0 + u][m];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sum[m][e] = fmaf(g, f[e], sum[m][e]), add[e] = fmaf(g, xs[m][e], add[e]);
+                }
+                if (!dw) continue;
+                T *at = dw + (long long)(v0 + c0 + u) * lddw + col;
+                if constexpr (sizeof(T) == 4) {
+                    asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(add[0]), "f"(add[1]), "f"(add[2]), "f"(add[3]) : "memory");
+                } else {
+                    float h[4];
+                    old[u].values(h);
+                    *reinterpret_cast<uint2 *>(at) = make_uint2(pack_bf16x2(h[0] + add[0], h[1] + add[1]), pack_bf16x2(h[2] + add[2], h[3] + add[3]));
+                }
+            }
+        }
+    }
+    if (!dxp) return;
+    if (groups > 1) {  // their sums, in order
+        __shared__ float4 part[kProductThreads];
+#pragma unroll
+        for (int m = 0; m < kRows; m++) {
+            if (m >= M) break;
+            part[threadIdx.x] = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+            __syncthreads();
+            if (group == 0) {
+                for (int i = 1; i < groups; i++) {
+                    const float4 other = part[i * width + column];
+                    sum[m][0] += other.x, sum[m][1] += other.y, sum[m][2] += other.z, sum[m][3] += other.w;
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (group == 0 && inside) {
+#pragma unroll
+        for (int m = 0; m < kRows; m++)
+            if (m < M) *reinterpret_cast<float4 *>(dxp + ((long long)blockIdx.x * M + m) * dx_pitch + col) = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+    }
+}
+
 int row_pitch(int K, int planes) { return (K * 2 + 127) / 128 * 128 + (planes == 2 ? 64 : 16); }
 size_t shared_bytes(int M, int K, int planes) { return (size_t)(M + 15) / 16 * 16 * row_pitch(K, planes) * planes; }
 constexpr size_t kMostShared = 200 << 10;
@@ -218,16 +341,37 @@ Split split_of(int M, int V, int sms) {
 template <class T>
 cudaError_t launch(const FewRows &a, int sms, cudaStream_t s) {
     const auto [tiles, each, rounds, warps] = split_of(a.M, a.V, sms);
-    auto kernel = a.M <= 16 ? few_rows_kernel<T, 1> : a.M <= 32 ? few_rows_kernel<T, 2> : a.M <= 48 ? few_rows_kernel<T, 3> : few_rows_kernel<T, 4>;
+    auto kernel = a.grad_g ? few_rows_kernel<T, 1, true> : a.M <= 16 ? few_rows_kernel<T, 1, false> : few_rows_kernel<T, 2, false>;
+    if constexpr (sizeof(T) == 4)
+        if (a.M > 32) kernel = a.M <= 48 ? few_rows_kernel<T, 3, false> : few_rows_kernel<T, 4, false>;
+    const ToG to{a.G, a.grad_g, a.lse, a.one_g, few_rows_stride(a.M)};
     return attn::launch_after_previous(kernel, dim3((unsigned)((tiles + each - 1) / each)), dim3(32 * warps), shared_bytes(a.M, a.K, sizeof(T) / 2), s, static_cast<const T *>(a.x), a.ldx,
-                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
+                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
+}
+
+// Threads along the columns of a block of the products (as many groups of them as fit share its classes), blocks along the columns, and blocks of
+// classes: as many as an SM holds, since each has a piece of dx.
+int product_width(int K) { return std::min(kProductThreads, ((K + 3) / 4 + 31) / 32 * 32); }
+int product_columns(int K) { return (K + 4 * product_width(K) - 1) / (4 * product_width(K)); }
+int product_blocks(int M, int V, int K, int sms) { return std::min(std::max(1, sms * (M <= 8 ? 2 : 1) / product_columns(K)), (V + 7) / 8); }
+template <class T>
+cudaError_t launch_products(const FewRows &a, T *dw, long long lddw, float *dxp, int dx_pitch, int sms, cudaStream_t s) {
+    const int blocks = product_blocks(a.M, a.V, a.K, sms), classes = (a.V + blocks - 1) / blocks, stride = few_rows_stride(a.M), width = product_width(a.K);
+    auto kernel = stride == 4 ? few_rows_products_kernel<T, 4> : few_rows_products_kernel<T, 8>;
+    if constexpr (sizeof(T) == 4)
+        if (stride == 16) kernel = few_rows_products_kernel<T, 16>;
+    return attn::launch_after_previous(kernel, dim3((unsigned)few_rows_pieces(a.M, a.V, a.K, sms), (unsigned)product_columns(a.K)), dim3((unsigned)(kProductThreads / width * width)), 0, s,
+                                       static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w), a.ldw, a.targets, a.G, dw, lddw, dxp, dx_pitch, a.M, a.V, a.K, classes, width);
 }
 
 template <class T>
 cudaError_t set() {
     cudaError_t e = cudaSuccess;
-    for (auto kernel : {few_rows_kernel<T, 1>, few_rows_kernel<T, 2>, few_rows_kernel<T, 3>, few_rows_kernel<T, 4>})
+    auto one = [&](auto *kernel) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
+    };
+    one(few_rows_kernel<T, 1, true>), one(few_rows_kernel<T, 1, false>), one(few_rows_kernel<T, 2, false>);
+    if constexpr (sizeof(T) == 4) one(few_rows_kernel<T, 3, false>), one(few_rows_kernel<T, 4, false>);
     return e;
 }
 
@@ -238,14 +382,31 @@ cudaError_t few_rows_set_attributes() {
     return e != cudaSuccess ? e : set<__nv_bfloat16>();
 }
 
+static bool fits(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int K) {
+    const int each = type == TENSOR_F32 ? 4 : 2;
+    return K * each % 16 == 0 && shared_bytes(M, K, each / 2) <= kMostShared && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0 &&
+           (M == 1 || ldx * each % 16 == 0) && ldw * each % 16 == 0;
+}
 bool few_rows_fit(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K, int sms) {
-    const int each = type == TENSOR_F32 ? 4 : 2, tiles_m = (M + 15) / 16;
-    if (M > kFewRows || K % 8 || shared_bytes(M, K, each / 2) > kMostShared) return false;
-    if (((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 31) || (M > 1 && ldx * each % 32) || ldw * each % 32) return false;
+    const int tiles_m = (M + 15) / 16;
+    if (M > kFewRows || !fits(x, w, ldx, ldw, type, M, K)) return false;
     // fp32 weights: from about as many classes on as the planes of the other way take time for.  bf16 ones: up to 32 rows, and warps enough.
     if (type == TENSOR_F32) return V >= 4000 * tiles_m;
     const Split p = split_of(M, V, sms);
     return tiles_m <= 2 && V >= 8000 && (p.rounds == 1 || p.warps >= 10);
+}
+int few_rows_stride(int M) { return M <= 4 ? 4 : M <= 8 ? 8 : 16; }
+bool few_rows_gradients_fit(const void *x, const void *w, const void *dw, long long ldx, long long ldw, long long lddw, int type, int M, int V, int K) {
+    const int each = type == TENSOR_F32 ? 4 : 2;
+    return M <= (type == TENSOR_F32 ? 16 : 8) && V >= 2000 && fits(x, w, ldx, ldw, type, M, K) && (!dw || ((reinterpret_cast<uintptr_t>(dw) & 15) == 0 && lddw * each % 16 == 0));
+}
+int few_rows_pieces(int M, int V, int K, int sms) {
+    const int blocks = product_blocks(M, V, K, sms), classes = (V + blocks - 1) / blocks;
+    return (V + classes - 1) / classes;
+}
+cudaError_t launch_few_rows_products(const FewRows &a, int type, void *dw, long long lddw, float *dxp, int dx_pitch, int sms, cudaStream_t s) {
+    return type == TENSOR_F32 ? launch_products(a, static_cast<float *>(dw), lddw, dxp, dx_pitch, sms, s)
+                              : launch_products(a, static_cast<__nv_bfloat16 *>(dw), lddw, dxp, dx_pitch, sms, s);
 }
 int few_rows_parts(int V, int sms) {
     const Split p = split_of(1, V, sms);

@@ -859,6 +859,19 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     return l;
 }
 
+// The backward of up to 16 rows: G, and the pieces of dx.
+struct FewLayout {
+    size_t g, dxp, total;
+    int pieces, dx_pitch;
+};
+FewLayout few_layout(int M, int V, int K, int sms) {
+    FewLayout l;
+    l.pieces = few_rows_pieces(M, V, K, sms), l.dx_pitch = up(K, 8);
+    l.g = 0, l.dxp = up256((size_t)V * few_rows_stride(M) * sizeof(float));
+    l.total = l.dxp + up256((size_t)l.pieces * M * l.dx_pitch * sizeof(float));
+    return l;
+}
+
 // [rows, cols] bf16 of `planes` planes: boxes of 64 columns by box_rows rows.
 int map_of(CUtensorMap *map, const void *base, long long rows, int cols, long long pitch, size_t plane, int planes, int box_rows) {
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
@@ -952,7 +965,8 @@ size_t xent_sm100_linear_forward_scratch_bytes(const void *x, const void *w, lon
 
 size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, long long ldx, long long ldw, int type, int rows, int V, int K) {
     if (head::check(x, w, nullptr, nullptr, ldx, ldw, type, TENSOR_INT32, rows, V, K) != ATTN_OK || rows == 0 || rows > head::kMostRows) return 0;
-    return head::layout(x, w, ldx, ldw, type, rows, V, K, true, attn::sm_count()).total;
+    const size_t tiles = head::layout(x, w, ldx, ldw, type, rows, V, K, true, attn::sm_count()).total;
+    return rows <= 16 ? std::max(tiles, head::few_layout(rows, V, K, attn::sm_count()).total) : tiles;  // (which of them depends on dw too)
 }
 
 int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
@@ -971,7 +985,7 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
     if (l.few) {
-        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K};
+        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K, nullptr, nullptr, 0, nullptr};
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
         return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, a.part, a.zt, a.targets, losses, lse, few_rows_parts(V, sms), rows, V);
     }
@@ -1019,10 +1033,23 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
     if (rows == 0) return ATTN_OK;
     const int sms = attn::sm_count();
-    const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, true, sms);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
+    auto sum = [&](const float *pieces, int count, int pitch) {
+        const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
+        return (int)(type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), pieces, count, rows, K, pitch, wide, s)
+                                        : launch_sum(static_cast<__nv_bfloat16 *>(dx), pieces, count, rows, K, pitch, wide, s));
+    };
+    if (few_rows_gradients_fit(x, w, dw, ldx, ldw, lddw, type, rows, V, K)) {
+        const FewLayout f = few_layout(rows, V, K, sms);
+        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, nullptr, nullptr, rows, V, K, g, lse, one_g, reinterpret_cast<float *>(base + f.g)};
+        float *dxp = dx ? reinterpret_cast<float *>(base + f.dxp) : nullptr;
+        if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
+        if ((e = launch_few_rows_products(a, type, dw, lddw, dxp, f.dx_pitch, sms, s)) != cudaSuccess) return (int)e;
+        return dx ? sum(dxp, f.pieces, f.dx_pitch) : ATTN_OK;
+    }
+    const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, true, sms);
     if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
     int *counters = reinterpret_cast<int *>(base + l.counters);
     if ((e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{targets, target_type}, V, counters, l.pieces + 1, s)) != cudaSuccess) return (int)e;
@@ -1085,11 +1112,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         e = type == TENSOR_F32 ? launch_tiles<3, true>(maps, p, sms, status, s) : launch_tiles<1, true>(maps, p, sms, status, s);
         if (e != cudaSuccess) return (int)e;
     }
-    if (!dx) return ATTN_OK;
-    const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
-    e = type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide, s)
-                           : launch_sum(static_cast<__nv_bfloat16 *>(dx), p.dxp, l.dx_pieces, rows, K, l.dx_pitch, wide, s);
-    return (int)e;
+    return dx ? sum(p.dxp, l.dx_pieces, l.dx_pitch) : ATTN_OK;
 }
 
 }  // extern "C"

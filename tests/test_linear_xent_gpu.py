@@ -101,6 +101,20 @@ def test_few_rows(pkg, M, K, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,K,V", [(1, 8, 2000), (1, 780, 50257), (3, 1100, 2001), (4, 64, 9000), (5, 2048, 3000), (8, 768, 30000), (9, 40, 2063), (16, 768, 50257), (16, 2056, 2500),
+                                   (16, 4, 5000), (16, 64, 1999), (17, 64, 5000), (12, 12, 4000)])
+def test_gradients_of_few_rows(pkg, M, K, V, dtype):
+    """Sizes at which the backward works on few rows in fp32 arithmetic, and those beside them."""
+    for i, ignored in enumerate((0.0, 0.4)):
+        c = Case(M, K, V, dtype, ignored, seed=i, ids=IDS[(M + i) % 3])
+        c.check(pkg)
+        held, lse = c.dw.clone(), pkg.linear_xent_forward(c.x, c.w, c.ids)[1]
+        dx = pkg.linear_xent_backward(c.g, c.x, c.w, c.ids, lse, c.dw)
+        assert torch.equal(pkg.linear_xent_backward(c.g, c.x, c.w, c.ids, lse), dx)
+        assert pkg.linear_xent_backward(c.g, c.x, c.w, c.ids, lse, held, want_dx=False) is None and torch.equal(held, c.dw)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_few_rows_nan_and_infinity(pkg, dtype):
     c = Case(9, 64, 9000, dtype, 0.0)
     c.x[3, 5], c.x[4, 6] = float("nan"), float("inf")
@@ -134,10 +148,11 @@ def test_rows_without_targets(pkg, dtype):
 @pytest.mark.parametrize("value", [float("inf"), float("nan"), -float("inf")])
 def test_what_rows_without_targets_hold(pkg, dtype, value):
     """Padding may hold anything: it reaches neither a loss nor a gradient."""
-    c = Case(300, 96, 1000, dtype, 0.3)
-    c.x[(c.t < 0) | (c.t >= c.V), ::5] = value
-    dx = c.check(pkg)
-    assert dx.isfinite().all() and c.dw.isfinite().all()
+    for M, K, V in ((300, 96, 1000), (13, 96, 9000)):
+        c = Case(M, K, V, dtype, 0.3)
+        c.x[(c.t < 0) | (c.t >= c.V), ::5] = value
+        dx = c.check(pkg)
+        assert dx.isfinite().all() and c.dw.isfinite().all()
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -165,7 +180,12 @@ def test_large_and_equal_logits(pkg, dtype):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("apart,start", [(80, 0), (72, 8), (67, 1), (73, 4)])
 def test_rows_that_lie_apart(pkg, dtype, apart, start):
-    c = Case(140, 60, 333, dtype)
+    for M, V in ((140, 333), (7, 9001)):
+        c = Case(M, 60, V, dtype)
+        rows_apart(pkg, c, dtype, apart, start)
+
+
+def rows_apart(pkg, c, dtype, apart, start):
     wide = lambda t: torch.full((t.shape[0], apart + 8), 7.0, device="cuda", dtype=dtype)  # noqa: E731
     held = {k: wide(getattr(c, k)) for k in ("x", "w", "dw")}
     for k, v in held.items():

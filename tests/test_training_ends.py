@@ -72,6 +72,11 @@ def test_scratch_sizes(pkg):
     for bad in [(0, 10, 8), (5, 0, 8), (5, 10, 0), (-1, 10, 8)]:
         rows, V, K = bad
         assert backward(P, P, 8, 8, 1, rows, V, K) == 0 and forward(P, P, 8, 8, 1, rows, V, K) == 0
+    for rows in (1, 16, 17, 300):
+        for V in (1, 2, 5000):
+            for K in (1, 2, 3, 7, 1600):
+                for type in (0, 1):
+                    assert forward(P, P, K, K, type, rows, V, K) > 0 and backward(P, P, K, K, type, rows, V, K) >= rows * K * 4
     assert forward(P, P, 8, 8, 2, 5, 10, 8) == 0 and backward(P, P, 7, 8, 1, 5, 10, 8) == 0
     # bf16 tensors on 16-byte boundaries are read where they are; others are copied, and fp32 ones become two planes
     direct, moved, strided, fp32 = forward(P, P, 768, 768, 1, 100, 50257, 768), forward(P, at((1 << 20) + 2), 768, 768, 1, 100, 50257, 768), forward(P, P, 768, 770, 1, 100, 50257, 768), \
