@@ -93,7 +93,7 @@ struct Problem {
     void *dw_out;
     long long lddw;
     int fetch_dw;                 // a tile of dw is asked for into L2 when its item is handed out
-    int dw_wide;                  // bytes that the rows of dw allow at a time: 32, 16, or an element
+    int dw_wide;                  // bytes that the rows of dw allow at a time: 32, 16, or (0) an element
     float2 *part;                 // forward: [tiles of V, M]
     float *zt;                    // forward: the target's logit
     int *counter;                 // items are handed out (else round robin)
@@ -202,20 +202,28 @@ __device__ __forceinline__ void four_rows(int lane, uint32_t (&z)[32]) {
         z[e + 16] = high ? z[e + 16] : got;
     }
 }
+// A lane has 32 columns of its row; afterwards it has its column of 32 rows, so that an instruction touches one row.
+__device__ __forceinline__ void transpose(int lane, uint32_t (&z)[32]) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+            if (e & o) continue;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? z[e] : z[e + o], o);
+            z[e] = up ? got : z[e];
+            z[e + o] = up ? z[e + o] : got;
+        }
+    }
+}
 // kN sums of a row added to what is there, as far as `left` goes.  One thread adds to a place, so the order of the sums is fixed; L2 adds, and nobody
 // waits for what was there (loaded and stored, a half of a tile took 6 us, in which the tensor cores waited for its accumulator).
 template <int kN>
-__device__ __forceinline__ void add_f32(float *at, const uint32_t *z, int left, bool wide) {
-    if (wide) {
+__device__ __forceinline__ void add_f32(float *at, const uint32_t *z, int left) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 4)
-            if (i < left)
-                asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at + i), "r"(z[i]), "r"(z[i + 1]), "r"(z[i + 2]), "r"(z[i + 3]) : "memory");
-    } else {
-#pragma unroll
-        for (int i = 0; i < kN; i++)
-            if (i < left) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + i), "r"(z[i]) : "memory");
-    }
+    for (int i = 0; i < kN; i += 4)
+        if (i < left)
+            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at + i), "r"(z[i]), "r"(z[i + 1]), "r"(z[i + 2]), "r"(z[i + 3]) : "memory");
 }
 // The same for bf16 values, which are rounded once: 32 sums added to what was there, 16 words of two values.
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t old, uint32_t a, uint32_t b) {
@@ -241,15 +249,34 @@ __device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&old
             v.z = add_bf16x2(v.z, z[i + 4], z[i + 5]), v.w = add_bf16x2(v.w, z[i + 6], z[i + 7]);
             *q = v;
         }
+    }
+}
+// 32 x 32 sums added to rows of dw that start anywhere, an element at a time; `z`: the lane's column, `count` rows and `left` columns are inside.
+// (With the rows that lanes have from tensor memory an instruction touched 32: forward and backward of 100 x 1001 x 50257 bf16 1407 -> 316 us, fp32 611 -> 439.)
+template <class T>
+__device__ __forceinline__ void add_anywhere(int lane, T *at, long long ld, const uint32_t (&z)[32], int count, int left) {
+    if (lane >= left) return;
+    at += lane;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int r = 0; r < 32; r++)
+            if (r < count) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + r * ld), "r"(z[r]) : "memory");
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; i++)
-            if (i < left) at[i] = __float2bfloat16_rn(__bfloat162float(at[i]) + __uint_as_float(z[i]));
+        for (int r = 0; r < 32; r += 8) {
+            uint16_t old[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) old[e] = r + e < count ? *reinterpret_cast<const uint16_t *>(at + (r + e) * ld) : 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (r + e < count) at[(r + e) * ld] = __float2bfloat16_rn(__uint_as_float((uint32_t)old[e] << 16) + __uint_as_float(z[r + e]));
+        }
     }
 }
 
-// kTerms 1: bf16 operands; 3: fp32 operands as two planes.
-template <int kTerms, bool kBackward, int kSlots>
+// kTerms 1: bf16 operands; 3: fp32 operands as two planes.  kAnywhere: the rows of dw may start anywhere (a kernel of its own: the registers of
+// both ways together spill, 60 x 768 x 50257 bf16 127 -> 147 us).
+template <int kTerms, bool kBackward, int kSlots, bool kAnywhere>
 __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Problem p, int *status) {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     using S = Smem<kSlots, kBackward>;
@@ -538,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                         __nv_bfloat16 *dw = static_cast<__nv_bfloat16 *>(p.dw_out) + v * p.lddw + it.n0 + off;  // where it is bf16
                         uint32_t old[16];
                         auto ask = [&](int i) {  // for what dw holds, before the wait
-                            if (kTerms == 1 && it.kind == kDw && inside && p.dw_wide == 32) {
+                            if (kTerms == 1 && !kAnywhere && it.kind == kDw && inside && p.dw_wide == 32) {
                                 if (i < left) load8(*reinterpret_cast<uint32_t(*)[8]>(old), dw + i);
                                 if (i + 16 < left) load8(*reinterpret_cast<uint32_t(*)[8]>(old + 8), dw + i + 16);
                             }
@@ -591,6 +618,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                         if (kTerms == 3 && i + c < left) store8(to + p.plane + c, lo);
                                     }
                                 }
+                            } else if (kAnywhere && it.kind == kDw) {
+                                using T = std::conditional_t<kTerms == 3, float, __nv_bfloat16>;
+                                transpose(lane, z);
+                                const int row0 = row - lane;
+                                add_anywhere(lane, static_cast<T *>(p.dw_out) + ((long long)p.v0 + row0) * p.lddw + it.n0 + off + i, p.lddw, z, min(p.cols, p.V - p.v0) - row0, left - i);
                             } else if (kTerms == 3) {
                                 four_rows(lane, z);
                                 const int row4 = row - lane + (lane & ~3), column = i + 8 * (lane & 3);
@@ -601,9 +633,9 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                     if (it.kind == kDx) {
                                         float *to = p.dxp + ((long long)it.piece * p.M + row4 + t) * p.dx_pitch + it.n0 + off + column;
                                         if (p.first && b0 == 0) store8(to, *reinterpret_cast<const uint32_t(*)[8]>(z + 8 * t));
-                                        else add_f32<8>(to, z + 8 * t, 8, true);
+                                        else add_f32<8>(to, z + 8 * t, 8);
                                     } else {
-                                        add_f32<8>(static_cast<float *>(p.dw_out) + ((long long)p.v0 + row4 + t) * p.lddw + it.n0 + off + column, z + 8 * t, left - column, p.dw_wide >= 16);
+                                        add_f32<8>(static_cast<float *>(p.dw_out) + ((long long)p.v0 + row4 + t) * p.lddw + it.n0 + off + column, z + 8 * t, left - column);
                                     }
                                 }
                             } else if (inside && i < left) {
@@ -612,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                 } else {
                                     float *to = p.dxp + ((long long)it.piece * p.M + row) * p.dx_pitch + it.n0 + off + i;
                                     if (p.first && b0 == 0) put_f32(to, z, left - i);
-                                    else add_f32<32>(to, z, left - i, true);
+                                    else add_f32<32>(to, z, left - i);
                                 }
                             }
                             __syncwarp();
@@ -915,7 +947,10 @@ cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int 
 template <int kTerms, bool kBackward>
 cudaError_t launch_tiles(const Maps &maps, const Problem &p, int sms, int *status, cudaStream_t s) {
     constexpr int kSlots = kBackward ? kBackwardSlots : kForwardSlots;
-    return attn::launch_after_previous(tiles_kernel<kTerms, kBackward, kSlots>, dim3((unsigned)std::min(p.total, sms)), dim3(kThreads), sizeof(Smem<kSlots, kBackward>),
+    auto kernel = tiles_kernel<kTerms, kBackward, kSlots, false>;
+    if constexpr (kBackward)
+        if (p.dw && p.dw_wide < 16) kernel = tiles_kernel<kTerms, kBackward, kSlots, true>;
+    return attn::launch_after_previous(kernel, dim3((unsigned)std::min(p.total, sms)), dim3(kThreads), sizeof(Smem<kSlots, kBackward>),
                                        s, maps, p, status);
 }
 
@@ -947,10 +982,12 @@ cudaError_t set_attributes() {
     auto set = [&](const void *kernel, size_t bytes) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     };
-    set(reinterpret_cast<const void *>(tiles_kernel<1, false, kForwardSlots>), sizeof(Smem<kForwardSlots, false>));
-    set(reinterpret_cast<const void *>(tiles_kernel<3, false, kForwardSlots>), sizeof(Smem<kForwardSlots, false>));
-    set(reinterpret_cast<const void *>(tiles_kernel<1, true, kBackwardSlots>), sizeof(Smem<kBackwardSlots, true>));
-    set(reinterpret_cast<const void *>(tiles_kernel<3, true, kBackwardSlots>), sizeof(Smem<kBackwardSlots, true>));
+    set(reinterpret_cast<const void *>(tiles_kernel<1, false, kForwardSlots, false>), sizeof(Smem<kForwardSlots, false>));
+    set(reinterpret_cast<const void *>(tiles_kernel<3, false, kForwardSlots, false>), sizeof(Smem<kForwardSlots, false>));
+    set(reinterpret_cast<const void *>(tiles_kernel<1, true, kBackwardSlots, false>), sizeof(Smem<kBackwardSlots, true>));
+    set(reinterpret_cast<const void *>(tiles_kernel<1, true, kBackwardSlots, true>), sizeof(Smem<kBackwardSlots, true>));
+    set(reinterpret_cast<const void *>(tiles_kernel<3, true, kBackwardSlots, false>), sizeof(Smem<kBackwardSlots, true>));
+    set(reinterpret_cast<const void *>(tiles_kernel<3, true, kBackwardSlots, true>), sizeof(Smem<kBackwardSlots, true>));
     return e;
 }
 
