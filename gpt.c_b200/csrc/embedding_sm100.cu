@@ -3,14 +3,16 @@
 //     y[t] = scale table[tokens[t]] + pos_table[positions[t]]
 //     dtable[v] += scale sum over tokens[t] = v of dy[t]          dpos_table[p] += sum over positions[t] = p of dy[t]
 //
-// Lookup: bound by HBM, a thread takes four words of 16 bytes, whose rows it asks for together.
+// Lookup: a copy, bound by HBM where the rows are many and by a launch where they are few.
 //
 // Gradient: the places t are put in the order of their tokens (equal tokens by t), and the sorted list is cut into ranges of the same
 // number of places, whatever the tokens are.  A thread keeps the sum of a few columns over a run of equal tokens and adds it to the table
 // where the run ends; the parts of runs that cross a border of a range are kept, and a last kernel adds them up in the order of the
-// list.  So every sum has a fixed order, and a token that takes half of the batch is spread over the GPU.  The list is sorted by one
-// cluster, while the other CTAs of that launch make the gradient of positions that are a token's place in its sequence, where no list is
-// needed.
+// list.  So every sum has a fixed order, and a token that takes half of the batch is spread over the GPU.
+//
+// Three ways to the order, by the number of places: up to 512 no list at all (few_kernel); up to 8192 one CTA for each of 128 buckets of tokens
+// (bucket_kernel), since the GPU is empty meanwhile; above, one cluster (sort_kernel), next to which the other CTAs of that launch make the
+// gradient of positions that are a token's place in its sequence, where no list is needed.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -36,9 +38,13 @@ constexpr int kSortThreads = 1024, kSortCtas = 8, kSortWarps = kSortThreads / 32
 constexpr int kBits = 9, kBins = 1 << kBits;  // of a pass of the sort, at most
 constexpr int kItems = 8;                     // places of a lane in a round of the sort
 constexpr int kAhead = 8;                     // places whose rows a thread asks for together
-constexpr int kBucketBits = 7, kBucketed = 8192;  // CTAs that sort without a cluster, and the longest list they take
+// CTAs that sort without a cluster, and the longest list they take, which is what their shared memory holds.  (8192 places of 768 fp32 columns, the whole
+// gradient: 16.5 us, by the cluster 30.)
+constexpr int kBucketBits = 7, kBucketed = 8192;
 constexpr int kComparedBits = 9, kCompared = 1 << kComparedBits;  // places of a bucket that are compared each with each (tokens have 30 bits)
-constexpr int kFewTokens = 512;               // no sort is needed
+// Where each place can look at all others.  (768 fp32 columns, by buckets in brackets: 16 places 3.4 us (10.5), 512 places 6.8 (11.2); its time grows with
+// the square.)
+constexpr int kFewTokens = 512;
 
 // kN columns of a row as they are in memory: one value, or 8, 16 or 32 bytes.  A thread asks for several before it looks at one: turned into fp32 where it
 // arrives, under a condition, each load was waited for by itself (runs of 49152 rows of 1600 bf16 values: 230 us).
@@ -121,6 +127,7 @@ struct Lookup {
 
 // kN columns at a time; a block takes `rows` rows of `words` such pieces.  i / words for i < 2^16 is the upper half of i * magic.
 // Pieces of a thread: two where they are 32 bytes of two tables, whose four take too many registers.
+// 8192 rows of 768 fp32 values with positions 6.5 us (they are in L2 then; from HBM 8.9, 4500 GB/s), 49152 of 1600 bf16 values 46 to 48 us (5500 GB/s).
 constexpr int units_of(int bytes, bool places) { return bytes == 32 && places ? 2 : kUnits; }
 template <class E, int kN, bool kPlaces>
 __global__ void __launch_bounds__(kThreads, 4) lookup_kernel(Lookup a, int rows, int words, unsigned magic) {
@@ -536,7 +543,9 @@ __device__ __forceinline__ void add_places(const Gradient &a, long long first, l
     }
 }
 
-// Clusters 0 .. lists - 1 sort; the others add up the positions that are a token's place.
+// Clusters 0 .. lists - 1 sort; the others add up the positions that are a token's place.  Bound by the passes, two of
+// 8 bits for 50257 tokens, whose CTAs wait for each other; it hides the 157 MB of dy that the others read.  49152 places of 1600 bf16 columns, half of them one
+// token: 99 us, of which sort, runs and joins have 31, 48 and 21 %.
 template <class E, class G, int kN>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const __grid_constant__ Gradient a) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -547,7 +556,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const __grid_cons
     else add_places<E, G, kN>(a, (long long)(blockIdx.x - others) * kSortThreads + threadIdx.x, (long long)(gridDim.x - others) * kSortThreads);
 }
 
-// A CTA for each bucket of each list.
+// A CTA for each bucket of each list.  Bound by latency: no more than 4 MB are moved, most of them from L2.  8192 places of 768 fp32
+// columns: 18.5 us with positions, of which this, runs and joins have 27, 46 and 27 %.
 __global__ void __launch_bounds__(kSortThreads, 1) bucket_kernel(const __grid_constant__ Gradient a) {
     extern __shared__ __align__(16) uint8_t smem_raw[];
     pdl_launch_dependents();
@@ -558,6 +568,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) bucket_kernel(const __grid_co
 
 // A warp takes a range of a sorted list, and 32 kN columns (blockIdx.y).  Blocks behind the ranges add up the positions that are a token's place
 // where the sort was not a launch of few CTAs, which leaves room for that.
+// Bound by what 16 warps an SM have on their way, since sums and two batches of rows take 114 registers: half of
+// the memory's rate for 49152 rows of 1600 bf16 columns.
 template <class E, class G, int kN>
 __global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ Gradient a, int blocks) {
     pdl_launch_dependents();
@@ -643,6 +655,7 @@ __global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ 
 
 // Runs that leave the range in which they began: the sum of their parts, in the order of the list.  A warp looks at a range and takes runs of
 // up to kFew parts itself; a block takes the longer ones of its 16 ranges one by one, its warps every 16th part.
+// Bound by the longest run, whose parts are read by one block of each 128 columns (one token has half of the places in the case above).
 constexpr int kFew = 8, kJoinWarps = 16;
 template <class G, int kN>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Gradient a) {
@@ -722,7 +735,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 }
 
 // Few tokens: a block for each place t of each list.  The first place of a token adds up the rows of all; `groups` threads share a column's
-// rows, each taking every groups-th.  The blocks behind them add up the positions that are a token's place.
+// rows, each taking every groups-th.  The blocks behind them add up the positions that are a token's place.  Bound by the launch and two loads that wait for
+// each other: 3.4 us from 1 to 128 places.
 template <class E, class G, int kN>
 __global__ void __launch_bounds__(kSortThreads) few_kernel(const __grid_constant__ Gradient a, int width, int groups) {
     pdl_launch_dependents();
@@ -806,8 +820,9 @@ bool overlap(const void *a, long long rows_a, long long ld_a, uintptr_t each_a, 
     return bits(a) < end_b && bits(b) < end_a;
 }
 
-// Places of a range, which a warp takes: 32 at most.
-int range_length(long long n) { return n <= 8192 ? 8 : n <= 32768 ? 16 : 32; }
+// Places of a range, which a warp takes: 32 at most.  Short ranges make more warps, long ones fewer parts of runs.  (768 fp32 columns: 8192 places
+// 16.5 us by 8, 17.8 by 16; 16384 places 40 by 8, 36.6 by 16; 32768 places 72 by 16, 69 by 32; 49152 places 93.6 by 16, 90 by 32.)
+int range_length(long long n) { return n <= 8192 ? 8 : n <= 16384 ? 16 : 32; }
 
 template <class E>
 cudaError_t launch_lookup(const Lookup &a, int bytes, int rows, int words, cudaStream_t s) {

@@ -69,7 +69,8 @@ extern "C" {
 #define ATTN_ERR_DEVICE (-5)      /* current device is not an sm_100 GPU, or a driver entry point is missing */
 #define ATTN_ERR_KERNEL (-6)      /* reported by attn_sm100_device_status: a kernel gave up a bounded wait */
 #define ATTN_ERR_STATIC_CAPACITY (-7) /* attn_sm100_forward_static: the problem needs more than ATTN_STATIC_SCRATCH_BYTES */
-#define ATTN_ERR_ARGUMENT (-8)        /* attn_sm100_paged_*, xent_sm100_sample: an argument outside what its description allows */
+#define ATTN_ERR_ARGUMENT (-8)        /* attn_sm100_paged_*, xent_sm100_sample, xent_sm100_linear_*, tensor_sm100_embedding_*:
+                                       * an argument outside what its description allows */
 
 /* flags */
 #define ATTN_FLAG_FORCE_GENERIC 1 /* use the general kernels even when those for D = 64 apply */

@@ -48,6 +48,7 @@ int tensor_sm100_gelu_backward(const float *g, const float *x, float *dx, size_t
  *   tokens, positions [n]            of `id_type`; positions NULL: t % T, a token's place in its sequence of T
  *   y [n, C]                         of `type`, contiguous
  * A token outside 0 .. V - 1 (padding), or a position outside 0 .. P - 1, brings zeros.
+ * Up to 2^20 columns, and 2^40 values of y; ATTN_ERR_UNSUPPORTED beyond.  y overlaps neither table.
  * The reference's counterpart is embedding_forward_cuda_kernel (kernels/src/cuda/Embedding.cu:46-58), without scale and positions.
  */
 int tensor_sm100_embedding_forward(const void *tokens, const void *table, const void *positions, const void *pos_table, void *y, long long n,
@@ -62,6 +63,7 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
  * outside their table have no part.  Rows that no token names are neither read nor written.
  * scratch: tensor_sm100_embedding_backward_scratch_bytes bytes with P = 0 unless positions are given and V = 0 without dtable,
  * 256-byte aligned (may be NULL if that is 0).
+ * Up to 2^30 places, 2^20 columns and 2^30 rows of a table; ATTN_ERR_UNSUPPORTED beyond.
  * The reference's counterpart is embedding_backward_cuda_kernel (kernels/src/cuda/Embedding.cu:60-74): an atomic addition a value.
  */
 size_t tensor_sm100_embedding_backward_scratch_bytes(long long n, int C, int V, int P);
