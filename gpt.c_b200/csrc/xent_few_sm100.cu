@@ -8,7 +8,7 @@
 //
 // Bound by HBM where there are up to 16 rows, then by the products (mma.sync has a quarter of the rate) and what they wait for.  Classes of 768 features, us with the
 // join, in brackets with tiles: 16 x 50257 bf16 18.7 (25.4), fp32 38 (110); 32 rows 22.3 (24.9), 45 (103); 48 rows 25.7 (22.8), 57 (104); 32 x 8000 13.4 (12.5),
-// 23 (25); 16 x 32000 bf16, whose CTAs have work for seven warps, 17.5 (15.8).  Reading takes 12 us of bf16 and 24 of fp32 weights.
+// 23 (25); 16 x 32000 bf16, whose CTAs have work for seven warps, 17.5 (15.8).  Reading takes 12 us of bf16 and 24 of fp32 weights.  fp32 rows that start anywhere: 5 x 1001 x 50257 55 us (146).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -41,6 +41,12 @@ struct Piece {
         for (int i = 0; i < 2; i++)
             *reinterpret_cast<uint4 *>(v + 4 * i) = left > i * kValues / 2 ? *reinterpret_cast<const uint4 *>(p + i * kValues / 2) : make_uint4(0, 0, 0, 0);
     }
+    // fp32 values that start anywhere: every fourth one from the lane's on, so that four lanes read 16 bytes of a row next to each other.  (The order of the
+    // contraction is free as long as both factors have the same.)
+    __device__ __forceinline__ void load_fourths(const T *p, int left) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = left > 4 * i ? *reinterpret_cast<const uint32_t *>(p + 4 * i) : 0;
+    }
     // kValues / 2 words of two bf16 values
     __device__ __forceinline__ void split(uint32_t (&hi)[kValues / 2], uint32_t (&lo)[kValues / 2]) const {
 #pragma unroll
@@ -59,7 +65,8 @@ struct ToG {
 };
 
 // kTiles: of 16 rows of x.  `classes`: of a CTA, a multiple of 16.  kGradient: G instead of maxima and sums.
-template <class T, int kTiles, bool kGradient>
+// kAnywhere: rows of fp32 values that do not all start on 16 bytes.
+template <class T, int kTiles, bool kGradient, bool kAnywhere>
 __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, Ids targets,
                                                                    float2 *__restrict__ part, float *__restrict__ zt, ToG to, int M, int V, int K, int classes, int pitch) {
     pdl_launch_dependents();
@@ -77,11 +84,15 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
     const T *from[2];
     auto rows_of = [&](int t) {
 #pragma unroll
-        for (int r = 0; r < 2; r++) from[r] = w + (long long)min(class0 + 16 * t + 8 * r + g, V - 1) * ldw + kEach * q;
+        for (int r = 0; r < 2; r++) from[r] = w + (long long)min(class0 + 16 * t + 8 * r + g, V - 1) * ldw + (kAnywhere ? q : kEach * q);
     };
     auto ask = [&](Piece<T>(&to)[2], int n) {
 #pragma unroll
-        for (int r = 0; r < 2; r++) to[r].load(from[r] + kBlock * load_b, n < total ? K - kBlock * load_b - kEach * q : 0);
+        for (int r = 0; r < 2; r++) {
+            const int left = n < total ? K - kBlock * load_b : 0;
+            if constexpr (kAnywhere) to[r].load_fourths(from[r] + kBlock * load_b, left - q);
+            else to[r].load(from[r] + kBlock * load_b, left - kEach * q);
+        }
         if (++load_b == blocks) load_b = 0, load_t += warps, rows_of(load_t);
     };
     rows_of(load_t);
@@ -93,7 +104,12 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
         const int row = i / words, c = (i - row * words) * kEach;
         uint32_t hi[kWords], lo[kWords];
         Piece<T> e;
-        e.load(x + row * ldx + c, row < M ? K - c : 0);
+        if constexpr (kAnywhere) {
+            const int first = c / kBlock * kBlock + c / kEach % 4;
+            e.load_fourths(x + row * ldx + first, row < M ? K - first : 0);
+        } else {
+            e.load(x + row * ldx + c, row < M ? K - c : 0);
+        }
         e.split(hi, lo);
 #pragma unroll
         for (int k = 0; k < kWords; k += 4) {
@@ -212,7 +228,6 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
     }
 }
 
-// Eight lanes read four pieces of 16 bytes each of two rows, next to each other (fp32: hi or lo of 8 values) or 32 bytes apart.
 // ---------------------------------------------------------------------------------------------
 // The two products of the backward for up to 16 rows, in fp32 arithmetic: a thread has four columns of x and of the sums of dx for all rows, and goes through
 // classes of its block: w once for dx, dw once for what is added to it.  G of a class is the same for all threads.
@@ -220,16 +235,22 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
 // Bound by HBM: w is read again (with the G kernel twice in all) and dw read and written, 617 MB of fp32 and 309 of bf16 at 768 x 50257: 94 and 47 us.
 // Measured with G and the sum of dx, in brackets with tiles: 1 row fp32 113 us (216; 780 features 121, 371), 16 rows 162 (214), where the multiplications
 // take as long; bf16, whose values come eight bytes a thread, 82 for 1 row, 80 for 4, 100 for 8 (98; 9000 classes
-// of 200 features 20, with tiles 33), but 145 for 16, which tiles keep.
+// of 200 features 20, with tiles 33), but 145 for 16, which tiles keep.  fp32 rows that start anywhere, with the forward: 1 x 1001 x 50257 224 (465), 3 x 333 x 50257
+// 87 (197).
 // ---------------------------------------------------------------------------------------------
 constexpr int kProductThreads = 256, kClasses = 64, kAheadClasses = 8;
 
-template <class T>
+// Four columns of a thread: next to each other, or (kAnywhere: rows of fp32 values that do not all start on 16 bytes) `step` apart, so that a warp's are next to
+// each other; `left` of the columns from the first on are inside.
+template <class T, bool kAnywhere>
 struct Four {
     static constexpr int kWords = sizeof(T);  // of four values
     uint32_t v[kWords];
-    __device__ __forceinline__ void load(const T *p) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
+    __device__ __forceinline__ void load(const T *p, int step, int left) {
+        if constexpr (kAnywhere) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] = e * step < left ? *reinterpret_cast<const uint32_t *>(p + e * step) : 0;
+        } else if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(p);
         else *reinterpret_cast<uint2 *>(v) = *reinterpret_cast<const uint2 *>(p);
     }
     __device__ __forceinline__ void values(float (&f)[4]) const {
@@ -238,7 +259,7 @@ struct Four {
     }
 };
 
-template <class T, int kRows>
+template <class T, int kRows, bool kAnywhere>
 __global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_products_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, Ids targets,
                                                                                                 const float *__restrict__ G, T *dw, long long lddw, float *__restrict__ dxp,
                                                                                                 int dx_pitch, int M, int V, int K, int classes, int width) {
@@ -246,16 +267,16 @@ __global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_
     pdl_wait();
     __shared__ __align__(16) float of_class[kClasses][kRows];
     const int groups = (int)blockDim.x / width, group = (int)threadIdx.x / width, column = (int)threadIdx.x - group * width;
-    const int col = ((int)blockIdx.y * width + column) * 4;
-    const bool inside = col < K;
+    const int col = kAnywhere ? (int)blockIdx.y * width * 4 + column : ((int)blockIdx.y * width + column) * 4, step = kAnywhere ? width : 1, left = K - col;
+    const bool inside = left > 0;
     const int begin = blockIdx.x * classes, end = min(V, begin + classes);
     float xs[kRows][4], sum[kRows][4];
 #pragma unroll
     for (int m = 0; m < kRows; m++) {
-        Four<T> f;
+        Four<T, kAnywhere> f;
 #pragma unroll
-        for (int i = 0; i < Four<T>::kWords; i++) f.v[i] = 0;
-        if (dw != nullptr && inside && m < M && targets.at(m, V) >= 0) f.load(x + m * ldx + col);  // rows without a target may hold anything
+        for (int i = 0; i < f.kWords; i++) f.v[i] = 0;
+        if (dw != nullptr && inside && m < M && targets.at(m, V) >= 0) f.load(x + m * ldx + col, step, left);  // rows without a target may hold anything
         f.values(xs[m]);
 #pragma unroll
         for (int e = 0; e < 4; e++) sum[m][e] = 0.f;
@@ -267,13 +288,13 @@ __global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_
             reinterpret_cast<float4 *>(&of_class[0][0])[i] = reinterpret_cast<const float4 *>(G + (long long)v0 * kRows)[i];
         __syncthreads();
         for (int c0 = group * kAheadClasses; c0 < count; c0 += groups * kAheadClasses) {
-            Four<T> ws[kAheadClasses], old[sizeof(T) == 2 ? kAheadClasses : 1];
+            Four<T, kAnywhere> ws[kAheadClasses], old[sizeof(T) == 2 ? kAheadClasses : 1];
             if (!inside) continue;
 #pragma unroll
             for (int u = 0; u < kAheadClasses; u++) {
                 const long long v = v0 + min(c0 + u, count - 1);
-                if (dxp) ws[u].load(w + v * ldw + col);
-                if (sizeof(T) == 2 && dw) old[u % (sizeof(T) == 2 ? kAheadClasses : 1)].load(dw + v * lddw + col);
+                if (dxp) ws[u].load(w + v * ldw + col, step, left);
+                if (sizeof(T) == 2 && dw) old[u % (sizeof(T) == 2 ? kAheadClasses : 1)].load(dw + v * lddw + col, step, left);
             }
 #pragma unroll
             for (int u = 0; u < kAheadClasses; u++) {
@@ -288,7 +309,11 @@ __global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_
                 }
                 if (!dw) continue;
                 T *at = dw + (long long)(v0 + c0 + u) * lddw + col;
-                if constexpr (sizeof(T) == 4) {
+                if constexpr (kAnywhere) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (e * step < left) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(at + e * step), "f"(add[e]) : "memory");
+                } else if constexpr (sizeof(T) == 4) {
                     asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(add[0]), "f"(add[1]), "f"(add[2]), "f"(add[3]) : "memory");
                 } else {
                     float h[4];
@@ -318,10 +343,21 @@ __global__ void __launch_bounds__(kProductThreads, kRows <= 8 ? 2 : 1) few_rows_
     if (group == 0 && inside) {
 #pragma unroll
         for (int m = 0; m < kRows; m++)
-            if (m < M) *reinterpret_cast<float4 *>(dxp + ((long long)blockIdx.x * M + m) * dx_pitch + col) = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+            if (m < M) {
+                float *to = dxp + ((long long)blockIdx.x * M + m) * dx_pitch + col;
+                if constexpr (kAnywhere) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (e * step < left) to[e * step] = sum[m][e];
+                } else {
+                    *reinterpret_cast<float4 *>(to) = make_float4(sum[m][0], sum[m][1], sum[m][2], sum[m][3]);
+                }
+            }
     }
 }
 
+// Eight lanes read four pieces of 16 bytes each of two rows, next to each other (fp32: hi or lo of 8 values) or 32 bytes apart: the pitch keeps them in
+// different banks.
 int row_pitch(int K, int planes) { return (K * 2 + 127) / 128 * 128 + (planes == 2 ? 64 : 16); }
 size_t shared_bytes(int M, int K, int planes) { return (size_t)(M + 15) / 16 * 16 * row_pitch(K, planes) * planes; }
 constexpr size_t kMostShared = 200 << 10;
@@ -338,12 +374,22 @@ Split split_of(int M, int V, int sms) {
     return p;
 }
 
+// Rows that can be read by 16 bytes.
+bool aligned(const void *p, long long rows, long long ld, int K, int each) { return !p || (((reinterpret_cast<uintptr_t>(p) | (uintptr_t)K * each) & 15) == 0 && (rows == 1 || ld * each % 16 == 0)); }
+
+template <class T, bool kAnywhere>
+auto kernel_of(int M, bool gradient) {
+    auto kernel = gradient ? few_rows_kernel<T, 1, true, kAnywhere> : M <= 16 ? few_rows_kernel<T, 1, false, kAnywhere> : few_rows_kernel<T, 2, false, kAnywhere>;
+    if constexpr (sizeof(T) == 4)
+        if (M > 32) kernel = M <= 48 ? few_rows_kernel<T, 3, false, kAnywhere> : few_rows_kernel<T, 4, false, kAnywhere>;
+    return kernel;
+}
 template <class T>
 cudaError_t launch(const FewRows &a, int sms, cudaStream_t s) {
     const auto [tiles, each, rounds, warps] = split_of(a.M, a.V, sms);
-    auto kernel = a.grad_g ? few_rows_kernel<T, 1, true> : a.M <= 16 ? few_rows_kernel<T, 1, false> : few_rows_kernel<T, 2, false>;
+    auto kernel = kernel_of<T, false>(a.M, a.grad_g != nullptr);
     if constexpr (sizeof(T) == 4)
-        if (a.M > 32) kernel = a.M <= 48 ? few_rows_kernel<T, 3, false> : few_rows_kernel<T, 4, false>;
+        if (!aligned(a.x, a.M, a.ldx, a.K, 4) || !aligned(a.w, a.V, a.ldw, a.K, 4)) kernel = kernel_of<T, true>(a.M, a.grad_g != nullptr);
     const ToG to{a.G, a.grad_g, a.lse, a.one_g, few_rows_stride(a.M)};
     return attn::launch_after_previous(kernel, dim3((unsigned)((tiles + each - 1) / each)), dim3(32 * warps), shared_bytes(a.M, a.K, sizeof(T) / 2), s, static_cast<const T *>(a.x), a.ldx,
                                        static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
@@ -357,9 +403,12 @@ int product_blocks(int M, int V, int K, int sms) { return std::min(std::max(1, s
 template <class T>
 cudaError_t launch_products(const FewRows &a, T *dw, long long lddw, float *dxp, int dx_pitch, int sms, cudaStream_t s) {
     const int blocks = product_blocks(a.M, a.V, a.K, sms), classes = (a.V + blocks - 1) / blocks, stride = few_rows_stride(a.M), width = product_width(a.K);
-    auto kernel = stride == 4 ? few_rows_products_kernel<T, 4> : few_rows_products_kernel<T, 8>;
-    if constexpr (sizeof(T) == 4)
-        if (stride == 16) kernel = few_rows_products_kernel<T, 16>;
+    auto kernel = stride == 4 ? few_rows_products_kernel<T, 4, false> : few_rows_products_kernel<T, 8, false>;
+    if constexpr (sizeof(T) == 4) {
+        if (!aligned(a.x, a.M, a.ldx, a.K, 4) || !aligned(a.w, a.V, a.ldw, a.K, 4) || !aligned(dw, a.V, lddw, a.K, 4))
+            kernel = stride == 4 ? few_rows_products_kernel<T, 4, true> : stride == 8 ? few_rows_products_kernel<T, 8, true> : few_rows_products_kernel<T, 16, true>;
+        else if (stride == 16) kernel = few_rows_products_kernel<T, 16, false>;
+    }
     return attn::launch_after_previous(kernel, dim3((unsigned)few_rows_pieces(a.M, a.V, a.K, sms), (unsigned)product_columns(a.K)), dim3((unsigned)(kProductThreads / width * width)), 0, s,
                                        static_cast<const T *>(a.x), a.ldx, static_cast<const T *>(a.w), a.ldw, a.targets, a.G, dw, lddw, dxp, dx_pitch, a.M, a.V, a.K, classes, width);
 }
@@ -370,8 +419,11 @@ cudaError_t set() {
     auto one = [&](auto *kernel) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
     };
-    one(few_rows_kernel<T, 1, true>), one(few_rows_kernel<T, 1, false>), one(few_rows_kernel<T, 2, false>);
-    if constexpr (sizeof(T) == 4) one(few_rows_kernel<T, 3, false>), one(few_rows_kernel<T, 4, false>);
+    for (int M : {16, 32, 48, 64}) {
+        if (sizeof(T) == 2 && M > 32) continue;
+        one(kernel_of<T, false>(M, false)), one(kernel_of<T, false>(M, true));
+        if constexpr (sizeof(T) == 4) one(kernel_of<T, true>(M, false)), one(kernel_of<T, true>(M, true));
+    }
     return e;
 }
 
@@ -382,14 +434,13 @@ cudaError_t few_rows_set_attributes() {
     return e != cudaSuccess ? e : set<__nv_bfloat16>();
 }
 
-static bool fits(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int K) {
-    const int each = type == TENSOR_F32 ? 4 : 2;
-    return K * each % 16 == 0 && shared_bytes(M, K, each / 2) <= kMostShared && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) == 0 &&
-           (M == 1 || ldx * each % 16 == 0) && ldw * each % 16 == 0;
+// (bf16 rows that start anywhere would be read by 2 bytes: the other kernel's copy is faster.)
+static bool fits(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K) {
+    return shared_bytes(M, K, type == TENSOR_F32 ? 2 : 1) <= kMostShared && (type == TENSOR_F32 || (aligned(x, M, ldx, K, 2) && aligned(w, V, ldw, K, 2)));
 }
 bool few_rows_fit(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K, int sms) {
     const int tiles_m = (M + 15) / 16;
-    if (M > kFewRows || !fits(x, w, ldx, ldw, type, M, K)) return false;
+    if (M > kFewRows || !fits(x, w, ldx, ldw, type, M, V, K)) return false;
     // fp32 weights: from about as many classes on as the planes of the other way take time for.  bf16 ones: up to 32 rows, and warps enough.
     if (type == TENSOR_F32) return V >= 4000 * tiles_m;
     const Split p = split_of(M, V, sms);
@@ -397,8 +448,7 @@ bool few_rows_fit(const void *x, const void *w, long long ldx, long long ldw, in
 }
 int few_rows_stride(int M) { return M <= 4 ? 4 : M <= 8 ? 8 : 16; }
 bool few_rows_gradients_fit(const void *x, const void *w, const void *dw, long long ldx, long long ldw, long long lddw, int type, int M, int V, int K) {
-    const int each = type == TENSOR_F32 ? 4 : 2;
-    return M <= (type == TENSOR_F32 ? 16 : 8) && V >= 2000 && fits(x, w, ldx, ldw, type, M, K) && (!dw || ((reinterpret_cast<uintptr_t>(dw) & 15) == 0 && lddw * each % 16 == 0));
+    return M <= (type == TENSOR_F32 ? 16 : 8) && V >= 2000 && fits(x, w, ldx, ldw, type, M, V, K) && (type == TENSOR_F32 || aligned(dw, V, lddw, K, 2));
 }
 int few_rows_pieces(int M, int V, int K, int sms) {
     const int blocks = product_blocks(M, V, K, sms), classes = (V + blocks - 1) / blocks;

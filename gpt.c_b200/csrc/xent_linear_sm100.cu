@@ -24,8 +24,9 @@
 // The waits on barriers are bounded (tc05.cuh); the allocation of tensor memory and the wait for the previous kernel end for the reasons given there.
 //
 // Bound by the power limit where rows are many: 8192 x 768 x 50257 bf16, forward 475 to 510 us (1240 to 1330 TFLOP/s at 1.55 GHz, 1 kW), backward 1740 to 1850
-// (1370 to 1450, with z made again; the GPU's sustained rate for a matrix product alone is 1389); 4096 rows fp32 730 and 2580 to 2740 us (three products
-// each: 1300, 1380 to 1470).  Few rows wait for their operands: 40 rows bf16 23 to 26 and 98 us, where reading and writing takes 12 and 47.
+// (three products with z made again: 1025 to 1090; the GPU's sustained rate for one matrix product is 1389); 4096 rows fp32 730 and 2580 to 2740 us (three
+// times the products: 1300, 1040 to 1100).  The backward moves 700 MB of G and dw a piece besides, and the launches of the first and last piece have z or products
+// alone, whose tensor cores are busy for 53 % of the time instead of 66 %.  Few rows wait for their operands: 40 rows bf16 23 to 26 and 98 us, where reading and writing takes 12 and 47.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -93,7 +93,7 @@ def test_shapes(pkg, M, K, V, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K,V", [(1, 64, 8000), (1, 768, 50257), (15, 40, 9001), (16, 200, 50257), (17, 72, 8192), (32, 768, 9999), (33, 136, 12001), (48, 8, 30011), (49, 264, 20000),
-                                   (64, 768, 16001), (65, 64, 16001)])
+                                   (64, 768, 16001), (65, 64, 16001), (1, 1, 8001), (2, 33, 9000), (16, 1001, 8003), (31, 201, 8009), (47, 770, 13000), (64, 67, 16003)])
 def test_few_rows(pkg, M, K, V, dtype):
     """Sizes at which the forward reads the weights into registers, and those beside them."""
     for i, ignored in enumerate((0.0, 0.4)):
@@ -102,7 +102,8 @@ def test_few_rows(pkg, M, K, V, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K,V", [(1, 8, 2000), (1, 780, 50257), (3, 1100, 2001), (4, 64, 9000), (5, 2048, 3000), (8, 768, 30000), (9, 40, 2063), (16, 768, 50257), (16, 2056, 2500),
-                                   (16, 4, 5000), (16, 64, 1999), (17, 64, 5000), (12, 12, 4000)])
+                                   (16, 4, 5000), (16, 64, 1999), (17, 64, 5000), (12, 12, 4000), (1, 1, 2000), (2, 1033, 2003), (5, 201, 9001), (7, 770, 4000), (13, 1027, 3001),
+                                   (16, 3, 8001)])
 def test_gradients_of_few_rows(pkg, M, K, V, dtype):
     """Sizes at which the backward works on few rows in fp32 arithmetic, and those beside them."""
     for i, ignored in enumerate((0.0, 0.4)):
