@@ -68,7 +68,7 @@ struct ToG {
 // kAnywhere: rows of fp32 values that do not all start on 16 bytes.
 template <class T, int kTiles, bool kGradient, bool kAnywhere>
 __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__restrict__ x, long long ldx, const T *__restrict__ w, long long ldw, Ids targets,
-                                                                   float2 *__restrict__ part, float *__restrict__ zt, ToG to, int M, int V, int K, int classes, int pitch) {
+                                                                   float2 *__restrict__ part, float *__restrict__ zt, ToG to, float fix, int M, int V, int K, int classes, int pitch) {
     pdl_launch_dependents();
     pdl_wait();
     extern __shared__ __align__(16) uint8_t rows[];  // [plane][16 kTiles][pitch bytes]
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int c = first + 8 * (i / 2) + i % 2, row = 8 * h + g;
-                            const float p = exp_of(z[m][i / 2][2 * h + i % 2] - top[m][h]) - (c == target[m][h] ? 1.f : 0.f);
+                            const float p = exp_of(fmaf(z[m][i / 2][2 * h + i % 2], fix, -top[m][h])) - (c == target[m][h] ? 1.f : 0.f);
                             if (c < V && row < to.stride) to.out[(long long)c * to.stride + row] = target[m][h] < 0 ? 0.f : p * sum[m][h];
                         }
                     } else {
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             const int c = first + 8 * (i / 2) + i % 2;
-                            v[i] = c < V ? z[m][i / 2][2 * h + i % 2] : -INFINITY;
+                            v[i] = c < V ? z[m][i / 2][2 * h + i % 2] * fix : -INFINITY;
                             if (c < V && c == target[m][h]) zt[16 * m + 8 * h + g] = v[i];
                         }
                         const float most = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), top[m][h]), by = most == -INFINITY ? 0.f : most;
@@ -392,7 +392,7 @@ cudaError_t launch(const FewRows &a, int sms, cudaStream_t s) {
         if (!aligned(a.x, a.M, a.ldx, a.K, 4) || !aligned(a.w, a.V, a.ldw, a.K, 4)) kernel = kernel_of<T, true>(a.M, a.grad_g != nullptr);
     const ToG to{a.G, a.grad_g, a.lse, a.one_g, few_rows_stride(a.M)};
     return attn::launch_after_previous(kernel, dim3((unsigned)((tiles + each - 1) / each)), dim3(32 * warps), shared_bytes(a.M, a.K, sizeof(T) / 2), s, static_cast<const T *>(a.x), a.ldx,
-                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
+                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.fix, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
 }
 
 // Threads along the columns of a block of the products (as many groups of them as fit share its classes), blocks along the columns, and blocks of

@@ -14,7 +14,7 @@
 //     dw  A: G,  rows contiguous           B: x, columns contiguous
 // fp32 operands are two bf16 planes, hi and lo (16 bits, 2^-18 of a value is left), and a product is hi hi + hi lo + lo hi: four tiles of a
 // contraction block serve three products.  Six products of three planes would have all 24 bits in twice the time, TF32 operands
-// 11 bits in two thirds of it.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks.  With bf16 operands G is rounded
+// 11 bits in two thirds of it.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks, and what that takes on average is put back (cut_of).  With bf16 operands G is rounded
 // to bf16 like the activations and gradients around it; sums stay fp32 until one rounding at the end.
 //
 // A CTA has a tile of 256 x 256 in two accumulators of 128 rows: shared memory takes in 64 KB a block and hands out 96 in 1280 cycles, against
@@ -99,6 +99,7 @@ struct Problem {
     float *zt;                    // forward: the target's logit
     int *counter;                 // items are handed out (else round robin)
     float fix, log2e;             // z as the tensor cores leave it times `fix` is z; fix * log2(e)
+    float fix_g;                  // of G, which makes up for what the sums of dw lose
 };
 
 struct Item {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                     if (it.kind == kLogits && row < p.M) {
                         target = p.targets.at(row, p.V);
                         if (kBackward) {
-                            gr = p.g[p.one_g ? 0 : row];
+                            gr = p.g[p.one_g ? 0 : row] * p.fix_g;
                             nl = -p.lse[row] * kLog2e;
                         }
                     }
@@ -751,9 +752,9 @@ __global__ void __launch_bounds__(256) planes_kernel(const T *__restrict__ src, 
     }
 }
 
-// dx from the pieces of its contraction.  kGroups threads share four columns, each taking every kGroups-th piece; their sums are added in order.
+// dx from the pieces of its contraction, times `by`.  kGroups threads share four columns, each taking every kGroups-th piece; their sums are added in order.
 template <class T, int kGroups>
-__global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide) {
+__global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide, float by) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int kWords = 256 / kGroups, kAhead = 4;
@@ -786,6 +787,7 @@ __global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const floa
         }
         if (group > 0 || i >= total) continue;
         T *at = dx + r * K + c;
+        sum = make_float4(sum.x * by, sum.y * by, sum.z * by, sum.w * by);
         const float s[4] = {sum.x, sum.y, sum.z, sum.w};
         if (wide && c + 4 <= K) {
             if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2 *>(at) = make_uint2(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]));
@@ -913,13 +915,17 @@ int map_of(CUtensorMap *map, const void *base, long long rows, int cols, long lo
     return attn::encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box);
 }
 
-// The tensor cores cut every sum of 16 products and what was there off to fp32: a sum of n such steps that grows evenly is on average n / 4 half
-// units too small, and so were the logits (K = 1600: by 26 2^-24 of themselves in bf16 and 84 in fp32, which has three products; 4096: by 68
-// and 212; without `fix` the log-sum-exp of logits of standard deviation 30 is 1.6e-6 off, with it 5e-7).
 void set_fix(Problem &p, int type) {
-    const double steps = (p.K + 15) / 16 * (type == TENSOR_F32 ? 3 : 1);
-    p.fix = (float)(1.0 + 0.26 * steps / 16777216.0);
-    p.log2e = (float)(1.4426950408889634 * (1.0 + 0.26 * steps / 16777216.0));
+    const double fix = fix_of(p.K, type);
+    p.fix = (float)fix, p.log2e = (float)(1.4426950408889634 * fix);
+}
+
+// What a gradient loses, as a share of it: sums of fp32 operands end after kSegment blocks or with the contraction of `blocks`.  dw is what G makes up for, before
+// the sums, and dx the rest, behind them: neither costs anything there.  (4096 x 768 x 50257: dx and dw were 2.8e-6 too small and 4.1e-6 of their norm off, now
+// 1e-7 and 3.0e-6.)  bf16 gradients are rounded to 2^-9 of themselves, next to which it is nothing.  (0.9: these sums grow less evenly.)
+double cut_of(int blocks) {
+    const int full = blocks / kSegment, rest = blocks % kSegment;
+    return 0.9 * kCut * 3 * (kBlock / 16) * ((double)full * kSegment * kSegment + (double)rest * rest) / blocks;
 }
 
 int blocks_for(long long words) { return (int)std::max(1ll, std::min(words / 256 + 1, 148ll * 16)); }
@@ -938,11 +944,11 @@ cudaError_t launch_planes(const void *src, long long ld, int type, void *to, siz
 
 // Eight threads share the pieces where there are more than four and few words: 49 pieces of 40 x 768 18 -> 4.8 us, 7 of 2048 x 768 23.5 us by eight (11 by one).
 template <class T>
-cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, cudaStream_t s) {
+cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, float by, cudaStream_t s) {
     const int groups = count > 4 && (long long)M * (pitch / 4) < 100000 ? 8 : 1;
     const int grid = blocks_for((long long)M * (pitch / 4) * groups);
-    return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide)
-                      : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide);
+    return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by)
+                      : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by);
 }
 
 template <int kTerms, bool kBackward>
@@ -1023,7 +1029,7 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
     if (l.few) {
-        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K, nullptr, nullptr, 0, nullptr};
+        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K, nullptr, nullptr, 0, nullptr, (float)fix_of(K, type)};
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
         return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, a.part, a.zt, a.targets, losses, lse, few_rows_parts(V, sms), rows, V);
     }
@@ -1074,18 +1080,18 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
-    auto sum = [&](const float *pieces, int count, int pitch) {
+    auto sum = [&](const float *pieces, int count, int pitch, double by) {
         const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
-        return (int)(type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), pieces, count, rows, K, pitch, wide, s)
-                                        : launch_sum(static_cast<__nv_bfloat16 *>(dx), pieces, count, rows, K, pitch, wide, s));
+        return (int)(type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), pieces, count, rows, K, pitch, wide, (float)by, s)
+                                        : launch_sum(static_cast<__nv_bfloat16 *>(dx), pieces, count, rows, K, pitch, wide, (float)by, s));
     };
     if (few_rows_gradients_fit(x, w, dw, ldx, ldw, lddw, type, rows, V, K)) {
         const FewLayout f = few_layout(rows, V, K, sms);
-        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, nullptr, nullptr, rows, V, K, g, lse, one_g, reinterpret_cast<float *>(base + f.g)};
+        const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, nullptr, nullptr, rows, V, K, g, lse, one_g, reinterpret_cast<float *>(base + f.g), (float)fix_of(K, type)};
         float *dxp = dx ? reinterpret_cast<float *>(base + f.dxp) : nullptr;
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
         if ((e = launch_few_rows_products(a, type, dw, lddw, dxp, f.dx_pitch, sms, s)) != cudaSuccess) return (int)e;
-        return dx ? sum(dxp, f.pieces, f.dx_pitch) : ATTN_OK;
+        return dx ? sum(dxp, f.pieces, f.dx_pitch, 1.0) : ATTN_OK;
     }
     const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, true, sms);
     if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
@@ -1102,12 +1108,15 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     Problem p = {};
     p.M = rows, p.V = V, p.K = K;
     set_fix(p, type);
+    p.fix_g = 1.f;
+    double fix_dx = 1.0;
     p.tiles_m = (rows + kTile - 1) / kTile;
     p.tiles_k = (K + kTile - 1) / kTile;
     p.blocks_m = (rows + kBlock - 1) / kBlock;
     p.blocks_k = (K + kBlock - 1) / kBlock;
     p.dx_pieces = l.dx_pieces, p.dx_blocks = l.dx_blocks;
     p.pitch = l.cols, p.wide = l.wide;
+    if (type == TENSOR_F32) p.fix_g = (float)(1.0 + cut_of(p.blocks_m)), fix_dx = 1.0 + cut_of(p.dx_blocks) - cut_of(p.blocks_m);
     p.plane = (long long)l.plane_g;
     p.targets = Ids{targets, target_type};
     p.g = g, p.lse = lse, p.one_g = one_g;
@@ -1150,7 +1159,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         e = type == TENSOR_F32 ? launch_tiles<3, true>(maps, p, sms, status, s) : launch_tiles<1, true>(maps, p, sms, status, s);
         if (e != cudaSuccess) return (int)e;
     }
-    return dx ? sum(p.dxp, l.dx_pieces, l.dx_pitch) : ATTN_OK;
+    return dx ? sum(p.dxp, l.dx_pieces, l.dx_pitch, fix_dx) : ATTN_OK;
 }
 
 }  // extern "C"

@@ -323,3 +323,33 @@ def test_refusals(pkg):
                   dict(dw=w.T.contiguous().T)):
         with pytest.raises(ValueError):
             pkg.linear_xent_backward(**{**dict(g=one, x=x, w=w, targets=t, lse=torch.zeros(4, device="cuda")), **wrong})
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,K,V", [(9, 1600, 9000), (40, 1600, 9000), (200, 2560, 3000)])
+def test_logits_are_not_too_small(pkg, dtype, M, K, V):
+    """The tensor cores cut every sum off, on average 0.28 2^-24 of it for each step of 16 products.  What is left of that is far less: a third would be the sign of
+    a way that does not make up for it."""
+    c = Case(M, K, V, dtype, 0.0, spread=20.0)
+    z = c.x.double() @ c.w.double().T
+    want = torch.logsumexp(z, -1)
+    t = z.argmin(-1)
+    losses, lse = pkg.linear_xent_forward(c.x, c.w, t)
+    steps = K // 16 * (3 if dtype == F32 else 1)
+    # the mean over the rows of roundings (2^-24 of a value each, and 2^-17 of a logit's terms, as many of either sign) is less than half of the limit
+    limit = 0.28 / 3 * steps * 2.0 ** -24 + (2.0 ** -22 if dtype == F32 else 2.0 ** -23)
+    at = z.gather(1, t[:, None])[:, 0]
+    assert abs(((lse.double() - want) / want).mean()) < limit and abs(((lse.double() - losses.double() - at) / at).mean()) < limit
+
+
+def test_fp32_gradients_are_not_too_small(pkg):
+    """Segments of 192 steps take 0.25 2^-24 of a sum a step: 2.9e-6."""
+    c = Case(2048, 64, 9000, F32, 0.0)
+    z = c.x.double() @ c.w.double().T
+    G = torch.softmax(z, -1)
+    G[torch.arange(c.M), c.t] -= 1
+    G *= c.g.double()[:, None]
+    c.dw.zero_()
+    dx = pkg.linear_xent_backward(c.g, c.x, c.w, c.ids, pkg.linear_xent_forward(c.x, c.w, c.ids)[1], c.dw)
+    for got, want in ((dx, G @ c.w.double()), (c.dw, G.T @ c.x.double())):
+        assert abs((got.double() * want).sum() / (want * want).sum() - 1) < 1.2e-6
