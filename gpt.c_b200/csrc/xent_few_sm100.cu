@@ -1,14 +1,16 @@
 // The forward of projection and loss (xent_linear_sm100.cu) for few rows: the weights are read once, straight into registers, for sm_100a.
 //
-// With up to 64 rows the products are few and the weights all that has to be moved.  The tiles of the other kernel have half of their shared memory
+// With up to 48 rows the products are few and the weights all that has to be moved.  The tiles of the other kernel have half of their shared memory
 // for rows that are not there, and fp32 weights are written and read again as bf16 planes.  Here a warp takes 16 classes at a time: a lane reads eight
 // values of a row, 32 or 16 bytes, which are the lane's part of two mma fragments if the contraction is taken in that order, and splits fp32 values into
 // hi and lo on the way.  x is in shared memory, bf16 (hi and lo), its rows so far apart that eight lanes that read two of them meet no bank twice.
 // Maximum and sum of each row stay in registers until the end.
 //
 // Bound by HBM where there are up to 16 rows, then by the products (mma.sync has a quarter of the rate) and what they wait for.  Classes of 768 features, us with the
-// join, in brackets with tiles: 16 x 50257 bf16 18.7 (25.4), fp32 38 (110); 32 rows 22.3 (24.9), 45 (103); 48 rows 25.7 (22.8), 57 (104); 32 x 8000 13.4 (12.5),
-// 23 (25); 16 x 32000 bf16, whose CTAs have work for seven warps, 17.5 (15.8).  Reading takes 12 us of bf16 and 24 of fp32 weights.  fp32 rows that start anywhere: 5 x 1001 x 50257 55 us (146).
+// join, in brackets with tiles: 16 x 50257 bf16 15.6 (26), fp32 37 (110); 32 rows 20.1 (25), 46 (103); 48 rows fp32 58 (104), bf16 25.7 (22.8); 64 rows fp32 104 (104);
+// 16 x 100 bf16 8.2 (11.3), fp32 11.5 (20).  Reading takes 12 us of bf16 and 24 of fp32 weights.  fp32 rows that start anywhere: 5 x 1001 x 50257 55 us (146).  All
+// warps help with x, whether there are classes for them or not (16 x 2000 bf16 14.2 -> 9.0); bf16 values are asked for where the products have taken the ones before,
+// since registers would be copied otherwise (16 x 1600 x 50257 45.3 -> 35.5).
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -73,7 +75,8 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
     pdl_wait();
     extern __shared__ __align__(16) uint8_t rows[];  // [plane][16 kTiles][pitch bytes]
     __shared__ float2 all[kMostWarps][16 * kTiles];
-    constexpr int kPlanes = sizeof(T) / 2, kAhead = 3, kBlock = 128 / sizeof(T), kEach = Piece<T>::kValues, kWords = kEach / 2;
+    constexpr int kAhead = sizeof(T) == 2 ? 7 - kTiles : kTiles == 1 ? 4 : 3;  // as many as there are registers for
+    constexpr int kPlanes = sizeof(T) / 2, kBlock = 128 / sizeof(T), kEach = Piece<T>::kValues, kWords = kEach / 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5, g = lane >> 2, q = lane & 3;
     const int class0 = blockIdx.x * classes, tiles = (min(V, class0 + classes) - class0 + 15) / 16, blocks = (K + kBlock - 1) / kBlock;
     const int mine = tiles > warp ? (tiles - warp + warps - 1) / warps : 0, total = mine * blocks;
@@ -145,7 +148,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
             uint32_t hi[2][kWords], lo[2][kWords];
 #pragma unroll
             for (int r = 0; r < 2; r++) ahead[u][r].split(hi[r], lo[r]);
-            ask(ahead[u], n0 + u + kAhead);
+            if (sizeof(T) == 4) ask(ahead[u], n0 + u + kAhead);
 #pragma unroll
             for (int m = 0; m < kTiles; m++) {
 #pragma unroll
@@ -169,6 +172,7 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
                     }
                 }
             }
+            if (sizeof(T) == 2) ask(ahead[u], n0 + u + kAhead);  // (its values go to the products as they are)
             if (++b < blocks) continue;
             b = 0;
             // 16 classes are done: a lane has classes 8 r + 2 q and the next of rows g and 8 + g of each tile
@@ -233,10 +237,9 @@ __global__ void __launch_bounds__(32 * kMostWarps) few_rows_kernel(const T *__re
 // classes of its block: w once for dx, dw once for what is added to it.  G of a class is the same for all threads.
 //
 // Bound by HBM: w is read again (with the G kernel twice in all) and dw read and written, 617 MB of fp32 and 309 of bf16 at 768 x 50257: 94 and 47 us.
-// Measured with G and the sum of dx, in brackets with tiles: 1 row fp32 113 us (216; 780 features 121, 371), 16 rows 162 (214), where the multiplications
-// take as long; bf16, whose values come eight bytes a thread, 82 for 1 row, 80 for 4, 100 for 8 (98; 9000 classes
-// of 200 features 20, with tiles 33), but 145 for 16, which tiles keep.  fp32 rows that start anywhere, with the forward: 1 x 1001 x 50257 224 (465), 3 x 333 x 50257
-// 87 (197).
+// Measured with G and the sum of dx, in brackets with tiles: 1 row fp32 111 us (216; 780 features 121, 371), 16 rows 166 (214), where the multiplications
+// take as long; bf16, whose values come eight bytes a thread, 75 for 1 row, 80 for 4, 92 for 8 (98), but 145 for 16, which tiles keep.  With the forward: 100 to
+// 4000 classes, 1 row bf16 18 to 27 (27 to 36), 16 rows fp32 31 to 44 (39 to 52); fp32 rows that start anywhere, 1 x 1001 x 50257 224 (465), 3 x 333 x 50257 87 (197).
 // ---------------------------------------------------------------------------------------------
 constexpr int kProductThreads = 256, kClasses = 64, kAheadClasses = 8;
 
@@ -362,15 +365,15 @@ int row_pitch(int K, int planes) { return (K * 2 + 127) / 128 * 128 + (planes ==
 size_t shared_bytes(int M, int K, int planes) { return (size_t)(M + 15) / 16 * 16 * row_pitch(K, planes) * planes; }
 constexpr size_t kMostShared = 200 << 10;
 
-// Tiles of a CTA, and its warps: as many as end together.
+// Tiles of a CTA, the rounds of its warps, and how many warps would do in as many.
 struct Split {
     int tiles, each, rounds, warps;
 };
-Split split_of(int M, int V, int sms) {
+Split split_of(int V, int sms) {
     Split p;
     p.tiles = (V + 15) / 16, p.each = (p.tiles + sms - 1) / sms;
     p.rounds = (p.each + kMostWarps - 1) / kMostWarps;
-    p.warps = std::max((p.each + p.rounds - 1) / p.rounds, (M + 31) / 32);
+    p.warps = (p.each + p.rounds - 1) / p.rounds;
     return p;
 }
 
@@ -381,18 +384,18 @@ template <class T, bool kAnywhere>
 auto kernel_of(int M, bool gradient) {
     auto kernel = gradient ? few_rows_kernel<T, 1, true, kAnywhere> : M <= 16 ? few_rows_kernel<T, 1, false, kAnywhere> : few_rows_kernel<T, 2, false, kAnywhere>;
     if constexpr (sizeof(T) == 4)
-        if (M > 32) kernel = M <= 48 ? few_rows_kernel<T, 3, false, kAnywhere> : few_rows_kernel<T, 4, false, kAnywhere>;
+        if (M > 32) kernel = few_rows_kernel<T, 3, false, kAnywhere>;
     return kernel;
 }
 template <class T>
 cudaError_t launch(const FewRows &a, int sms, cudaStream_t s) {
-    const auto [tiles, each, rounds, warps] = split_of(a.M, a.V, sms);
+    const Split p = split_of(a.V, sms);
     auto kernel = kernel_of<T, false>(a.M, a.grad_g != nullptr);
     if constexpr (sizeof(T) == 4)
         if (!aligned(a.x, a.M, a.ldx, a.K, 4) || !aligned(a.w, a.V, a.ldw, a.K, 4)) kernel = kernel_of<T, true>(a.M, a.grad_g != nullptr);
     const ToG to{a.G, a.grad_g, a.lse, a.one_g, few_rows_stride(a.M)};
-    return attn::launch_after_previous(kernel, dim3((unsigned)((tiles + each - 1) / each)), dim3(32 * warps), shared_bytes(a.M, a.K, sizeof(T) / 2), s, static_cast<const T *>(a.x), a.ldx,
-                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.fix, a.M, a.V, a.K, each * 16, row_pitch(a.K, sizeof(T) / 2));
+    return attn::launch_after_previous(kernel, dim3((unsigned)((p.tiles + p.each - 1) / p.each)), dim3(32 * kMostWarps), shared_bytes(a.M, a.K, sizeof(T) / 2), s, static_cast<const T *>(a.x), a.ldx,
+                                       static_cast<const T *>(a.w), a.ldw, a.targets, a.part, a.zt, to, a.fix, a.M, a.V, a.K, p.each * 16, row_pitch(a.K, sizeof(T) / 2));
 }
 
 // Threads along the columns of a block of the products (as many groups of them as fit share its classes), blocks along the columns, and blocks of
@@ -419,7 +422,7 @@ cudaError_t set() {
     auto one = [&](auto *kernel) {
         if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void *>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
     };
-    for (int M : {16, 32, 48, 64}) {
+    for (int M : {16, 32, 48}) {
         if (sizeof(T) == 2 && M > 32) continue;
         one(kernel_of<T, false>(M, false)), one(kernel_of<T, false>(M, true));
         if constexpr (sizeof(T) == 4) one(kernel_of<T, true>(M, false)), one(kernel_of<T, true>(M, true));
@@ -441,14 +444,13 @@ static bool fits(const void *x, const void *w, long long ldx, long long ldw, int
 bool few_rows_fit(const void *x, const void *w, long long ldx, long long ldw, int type, int M, int V, int K, int sms) {
     const int tiles_m = (M + 15) / 16;
     if (M > kFewRows || !fits(x, w, ldx, ldw, type, M, V, K)) return false;
-    // fp32 weights: from about as many classes on as the planes of the other way take time for.  bf16 ones: up to 32 rows, and warps enough.
-    if (type == TENSOR_F32) return V >= 4000 * tiles_m;
-    const Split p = split_of(M, V, sms);
-    return tiles_m <= 2 && V >= 8000 && (p.rounds == 1 || p.warps >= 10);
+    // bf16 weights: up to 32 rows, more than 16 only where the warps end together (32 x 768 x 32000, 7 warps' work in two rounds: 17.2 us, with tiles 15.7).
+    const Split p = split_of(V, sms);
+    return type == TENSOR_F32 || tiles_m == 1 || (tiles_m == 2 && (p.rounds == 1 || p.warps >= 9));
 }
 int few_rows_stride(int M) { return M <= 4 ? 4 : M <= 8 ? 8 : 16; }
 bool few_rows_gradients_fit(const void *x, const void *w, const void *dw, long long ldx, long long ldw, long long lddw, int type, int M, int V, int K) {
-    return M <= (type == TENSOR_F32 ? 16 : 8) && V >= 2000 && fits(x, w, ldx, ldw, type, M, V, K) && (type == TENSOR_F32 || aligned(dw, V, lddw, K, 2));
+    return M <= (type == TENSOR_F32 ? 16 : 8) && fits(x, w, ldx, ldw, type, M, V, K) && (type == TENSOR_F32 || aligned(dw, V, lddw, K, 2));
 }
 int few_rows_pieces(int M, int V, int K, int sms) {
     const int blocks = product_blocks(M, V, K, sms), classes = (V + blocks - 1) / blocks;
@@ -459,7 +461,7 @@ cudaError_t launch_few_rows_products(const FewRows &a, int type, void *dw, long 
                               : launch_products(a, static_cast<__nv_bfloat16 *>(dw), lddw, dxp, dx_pitch, sms, s);
 }
 int few_rows_parts(int V, int sms) {
-    const Split p = split_of(1, V, sms);
+    const Split p = split_of(V, sms);
     return (p.tiles + p.each - 1) / p.each;
 }
 cudaError_t launch_few_rows(const FewRows &a, int type, int sms, cudaStream_t s) { return type == TENSOR_F32 ? launch<float>(a, sms, s) : launch<__nv_bfloat16>(a, sms, s); }

@@ -14,7 +14,7 @@ inline double fix_of(int K, int type) { return 1.0 + kCut * ((K + 15) / 16 * (ty
 
 // Up to kFewRows rows (xent_few_sm100.cu).  The forward: maxima and sums of each row over the classes of each CTA.  The backward of up to 16 rows, where grad_g
 // is given: G, then the products.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 48;
 struct FewRows {
     const void *x, *w;
     long long ldx, ldw;

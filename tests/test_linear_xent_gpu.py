@@ -102,7 +102,7 @@ def test_few_rows(pkg, M, K, V, dtype):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K,V", [(1, 8, 2000), (1, 780, 50257), (3, 1100, 2001), (4, 64, 9000), (5, 2048, 3000), (8, 768, 30000), (9, 40, 2063), (16, 768, 50257), (16, 2056, 2500),
-                                   (16, 4, 5000), (16, 64, 1999), (17, 64, 5000), (12, 12, 4000), (1, 1, 2000), (2, 1033, 2003), (5, 201, 9001), (7, 770, 4000), (13, 1027, 3001),
+                                   (16, 4, 5000), (16, 64, 1999), (3, 40, 1), (16, 768, 9), (8, 1600, 17), (17, 64, 5000), (12, 12, 4000), (1, 1, 2000), (2, 1033, 2003), (5, 201, 9001), (7, 770, 4000), (13, 1027, 3001),
                                    (16, 3, 8001)])
 def test_gradients_of_few_rows(pkg, M, K, V, dtype):
     """Sizes at which the backward works on few rows in fp32 arithmetic, and those beside them."""
