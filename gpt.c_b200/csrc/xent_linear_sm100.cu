@@ -15,7 +15,7 @@
 // fp32 operands are two bf16 planes, hi and lo (16 bits, 2^-18 of a value is left), and a product is hi hi + hi lo + lo hi: four tiles of a
 // contraction block serve three products.  Six products of three planes would have all 24 bits in twice the time, TF32 operands
 // 11 bits in two thirds of it.  fp32 sums of dx and dw leave the tensor cores, which truncate every sum, after 16 blocks, and what that takes on average is put back (cut_of).  With bf16 operands G is rounded
-// to bf16 like the activations and gradients around it; sums stay fp32 until one rounding at the end.
+// to bf16 like the activations and gradients around it, without the factor that its rows share (common_of), which the sums take; they stay fp32 until one rounding at the end.
 //
 // A CTA has a tile of 256 x 256 in two accumulators of 128 rows: shared memory takes in 64 KB a block and hands out 96 in 1280 cycles, against
 // 1024 of the tensor cores.  (Two CTAs on a tile would take in half of B each; pairs have stopped for good on this GPU and are not used.)
@@ -100,6 +100,7 @@ struct Problem {
     int *counter;                 // items are handed out (else round robin)
     float fix, log2e;             // z as the tensor cores leave it times `fix` is z; fix * log2(e)
     float fix_g;                  // of G, which makes up for what the sums of dw lose
+    const float *common;          // bf16: what the sums of dx and dw are multiplied by, and what G is (common_of)
 };
 
 struct Item {
@@ -227,18 +228,18 @@ __device__ __forceinline__ void add_f32(float *at, const uint32_t *z, int left) 
         if (i < left)
             asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at + i), "r"(z[i]), "r"(z[i + 1]), "r"(z[i + 2]), "r"(z[i + 3]) : "memory");
 }
-// The same for bf16 values, which are rounded once: 32 sums added to what was there, 16 words of two values.
-__device__ __forceinline__ uint32_t add_bf16x2(uint32_t old, uint32_t a, uint32_t b) {
-    return pack_bf16x2(__uint_as_float(old << 16) + __uint_as_float(a), __uint_as_float(old & 0xffff0000u) + __uint_as_float(b));
+// The same for bf16 values, which are rounded once: 32 sums, times `by`, added to what was there, 16 words of two values.
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t old, uint32_t a, uint32_t b, float by) {
+    return pack_bf16x2(fmaf(__uint_as_float(a), by, __uint_as_float(old << 16)), fmaf(__uint_as_float(b), by, __uint_as_float(old & 0xffff0000u)));
 }
-__device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&old)[16], const uint32_t (&z)[32], int left, int wide) {
+__device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&old)[16], const uint32_t (&z)[32], int left, int wide, float by) {
     if (wide == 32) {
 #pragma unroll
         for (int i = 0; i < 32; i += 16) {
             if (i >= left) continue;
             uint32_t v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = add_bf16x2(old[i / 2 + e], z[i + 2 * e], z[i + 2 * e + 1]);
+            for (int e = 0; e < 8; e++) v[e] = add_bf16x2(old[i / 2 + e], z[i + 2 * e], z[i + 2 * e + 1], by);
             store8(at + i, v);
         }
     } else if (wide == 16) {
@@ -247,16 +248,16 @@ __device__ __forceinline__ void add_bf16(__nv_bfloat16 *at, const uint32_t (&old
             if (i >= left) continue;
             uint4 *q = reinterpret_cast<uint4 *>(at + i);
             uint4 v = *q;
-            v.x = add_bf16x2(v.x, z[i], z[i + 1]), v.y = add_bf16x2(v.y, z[i + 2], z[i + 3]);
-            v.z = add_bf16x2(v.z, z[i + 4], z[i + 5]), v.w = add_bf16x2(v.w, z[i + 6], z[i + 7]);
+            v.x = add_bf16x2(v.x, z[i], z[i + 1], by), v.y = add_bf16x2(v.y, z[i + 2], z[i + 3], by);
+            v.z = add_bf16x2(v.z, z[i + 4], z[i + 5], by), v.w = add_bf16x2(v.w, z[i + 6], z[i + 7], by);
             *q = v;
         }
     }
 }
-// 32 x 32 sums added to rows of dw that start anywhere, an element at a time; `z`: the lane's column, `count` rows and `left` columns are inside.
+// 32 x 32 sums (of bf16 rows times `by`) added to rows of dw that start anywhere, an element at a time; `z`: the lane's column, `count` rows and `left` columns are inside.
 // (With the rows that lanes have from tensor memory an instruction touched 32: forward and backward of 100 x 1001 x 50257 bf16 1407 -> 316 us, fp32 611 -> 439.)
 template <class T>
-__device__ __forceinline__ void add_anywhere(int lane, T *at, long long ld, const uint32_t (&z)[32], int count, int left) {
+__device__ __forceinline__ void add_anywhere(int lane, T *at, long long ld, const uint32_t (&z)[32], int count, int left, float by) {
     if (lane >= left) return;
     at += lane;
     if constexpr (sizeof(T) == 4) {
@@ -271,7 +272,7 @@ __device__ __forceinline__ void add_anywhere(int lane, T *at, long long ld, cons
             for (int e = 0; e < 8; e++) old[e] = r + e < count ? *reinterpret_cast<const uint16_t *>(at + (r + e) * ld) : 0;
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (r + e < count) at[(r + e) * ld] = __float2bfloat16_rn(__uint_as_float((uint32_t)old[e] << 16) + __uint_as_float(z[r + e]));
+                if (r + e < count) at[(r + e) * ld] = __float2bfloat16_rn(fmaf(__uint_as_float(z[r + e]), by, __uint_as_float((uint32_t)old[e] << 16)));
         }
     }
 }
@@ -490,11 +491,11 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                     const int acc = half & 1;
                     const int row = it.m0 + h * 128 + quarter * 32 + lane, off = 64 * group;
                     int target = -1;
-                    float gr = 0.f, nl = 0.f;
+                    float by = kBackward && kTerms == 1 && it.kind == kDw ? p.common[0] : 0.f, nl = 0.f;  // by: what G, or sums of bf16 rows of dw, are multiplied by
                     if (it.kind == kLogits && row < p.M) {
                         target = p.targets.at(row, p.V);
                         if (kBackward) {
-                            gr = p.g[p.one_g ? 0 : row] * p.fix_g;
+                            by = p.g[p.one_g ? 0 : row] * (kTerms == 1 ? p.common[1] : p.fix_g);
                             nl = -p.lse[row] * kLog2e;
                         }
                     }
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                         uint32_t hi[8], lo[8];
 #pragma unroll
                                         for (int e = 0; e < 8; e++) {
-                                            const float a = __uint_as_float(z[c + 2 * e]) * gr, b = __uint_as_float(z[c + 2 * e + 1]) * gr;
+                                            const float a = __uint_as_float(z[c + 2 * e]) * by, b = __uint_as_float(z[c + 2 * e + 1]) * by;
                                             if (kTerms == 1) hi[e] = pack_bf16x2(a, b);
                                             else split_bf16x2(a, b, hi[e], lo[e]);
                                             if (target < 0) hi[e] = lo[e] = 0;
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                 using T = std::conditional_t<kTerms == 3, float, __nv_bfloat16>;
                                 transpose(lane, z);
                                 const int row0 = row - lane;
-                                add_anywhere(lane, static_cast<T *>(p.dw_out) + ((long long)p.v0 + row0) * p.lddw + it.n0 + off + i, p.lddw, z, min(p.cols, p.V - p.v0) - row0, left - i);
+                                add_anywhere(lane, static_cast<T *>(p.dw_out) + ((long long)p.v0 + row0) * p.lddw + it.n0 + off + i, p.lddw, z, min(p.cols, p.V - p.v0) - row0, left - i, by);
                             } else if (kTerms == 3) {
                                 four_rows(lane, z);
                                 const int row4 = row - lane + (lane & ~3), column = i + 8 * (lane & 3);
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                                 }
                             } else if (inside && i < left) {
                                 if (it.kind == kDw) {
-                                    add_bf16(dw + i, old, z, left - i, p.dw_wide);
+                                    add_bf16(dw + i, old, z, left - i, p.dw_wide, by);
                                 } else {
                                     float *to = p.dxp + ((long long)it.piece * p.M + row) * p.dx_pitch + it.n0 + off + i;
                                     if (p.first && b0 == 0) put_f32(to, z, left - i);
@@ -706,18 +707,61 @@ __global__ void __launch_bounds__(1024) join_kernel(const float2 *__restrict__ p
     losses[row] = targets.at(row, V) >= 0 ? l - zt[row] : 0.f;
 }
 
+// The factor of all rows' G that bf16 gradients do not take into it: the significand c, 1 to 2, of the largest |g| of a row that has a target.  With
+// g = 1 / rows, or the same g for each row, G / c is p - [v = t] times a power of two; with g in it, nearly every target's entry, -g, would be rounded to the
+// same side by the same share, up to 2^-8, and so would everything that is made of it (3001 x 1600 x 50257: 1.7e-3).  Where rows have factors of
+// their own each rounds its own entries.  A power of two stays in G, so that no product leaves the range it had.  out: c, 1 / c.
+struct Common {
+    const float *g;
+    float *out;
+    int one_g;
+};
+__device__ __forceinline__ void common_of(const Common &a, const Ids &targets, int rows, int V) {
+    constexpr int kAhead = 8;
+    __shared__ float most[8];
+    float top = 0.f;
+    if (a.one_g) {
+        top = fabsf(a.g[0]);
+    } else {
+        for (int r0 = threadIdx.x; r0 < rows; r0 += 256 * kAhead) {
+            int t[kAhead];
+            float v[kAhead];
+            targets.many<kAhead>(t, V, r0, 256, rows);
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) v[u] = a.g[min(r0 + 256 * u, rows - 1)];  // (behind the last row: that one again)
+#pragma unroll
+            for (int u = 0; u < kAhead; u++)
+                if (t[u] >= 0) top = fmaxf(top, fabsf(v[u]));
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x > 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = fmaxf(top, most[i]);
+    const float c = top >= 1.1754944e-38f && top < INFINITY ? __uint_as_float((__float_as_uint(top) & 0x007fffffu) | 0x3f800000u) : 1.f;
+    a.out[0] = c, a.out[1] = 1.f / c;
+}
+
 // src [R, K] as bf16 planes [R, pitch] (hi, and lo of fp32 values).  Rows without a target become zeros where targets are given.  Also
-// clears the counters of work items.
+// clears the counters of work items; one more block finds the common factor where it is asked for.
 template <class T>
 __global__ void __launch_bounds__(256) planes_kernel(const T *__restrict__ src, long long ld, __nv_bfloat16 *__restrict__ hi, __nv_bfloat16 *__restrict__ lo,
-                                                     int R, int K, int pitch, int wide, Ids targets, int V, int *counters, int count) {
+                                                     int R, int K, int pitch, int wide, Ids targets, int V, int *counters, int count, Common common) {
     pdl_launch_dependents();
     pdl_wait();
+    const int blocks = common.out ? (int)gridDim.x - 1 : (int)gridDim.x;
+    if ((int)blockIdx.x == blocks) {
+        common_of(common, targets, R, V);
+        return;
+    }
     const int words = pitch / 8;
     const long long total = (long long)R * words;
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i < count; i += 256) counters[i] = 0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)blocks * 256) {
         const long long r = i / words;
         const int c = (int)(i - r * words) * 8;
         const T *at = src + r * ld + c;
@@ -752,11 +796,12 @@ __global__ void __launch_bounds__(256) planes_kernel(const T *__restrict__ src, 
     }
 }
 
-// dx from the pieces of its contraction, times `by`.  kGroups threads share four columns, each taking every kGroups-th piece; their sums are added in order.
+// dx from the pieces of its contraction, times `by`, and times the common factor where there is one.  kGroups threads share four columns, each taking every kGroups-th piece; their sums are added in order.
 template <class T, int kGroups>
-__global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide, float by) {
+__global__ void __launch_bounds__(256) sum_kernel(T *__restrict__ dx, const float *__restrict__ pieces, int count, int M, int K, int pitch, int wide, float by, const float *__restrict__ common) {
     pdl_launch_dependents();
     pdl_wait();
+    if (common) by *= common[0];
     constexpr int kWords = 256 / kGroups, kAhead = 4;
     __shared__ float4 part[kGroups > 1 ? kGroups : 1][kGroups > 1 ? kWords : 1];
     const unsigned words = pitch / 4;
@@ -886,7 +931,7 @@ Layout layout(const void *x, const void *w, long long ldx, long long ldw, int ty
     l.dx_blocks = (blocks + l.dx_pieces - 1) / l.dx_pieces;
     l.dx_pieces = (blocks + l.dx_blocks - 1) / l.dx_blocks;
     l.dx_pitch = up(K, 8);
-    l.counters = take(sizeof(int) * (l.pieces + 1));
+    l.counters = take(sizeof(int) * (l.pieces + 3));  // and the common factor
     l.plane_g = (size_t)M * l.cols;
     for (int i = 0; i < (l.pieces > 1 ? 2 : 1); i++) l.g[i] = take(l.plane_g * 2 * l.planes);
     l.dxp = take((size_t)l.dx_pieces * M * l.dx_pitch * sizeof(float));
@@ -931,24 +976,24 @@ double cut_of(int blocks) {
 int blocks_for(long long words) { return (int)std::max(1ll, std::min(words / 256 + 1, 148ll * 16)); }
 
 cudaError_t launch_planes(const void *src, long long ld, int type, void *to, size_t plane, int R, int K, int pitch, Ids targets, int V, int *counters, int count,
-                          cudaStream_t s) {
+                          Common common, cudaStream_t s) {
     __nv_bfloat16 *hi = static_cast<__nv_bfloat16 *>(to), *lo = hi + plane;
-    const int grid = blocks_for((long long)R * (pitch / 8));
+    const int grid = blocks_for((long long)R * (pitch / 8)) + (common.out != nullptr);
     const int each = type == TENSOR_F32 ? 4 : 2, wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld * each % 16 == 0;
     if (type == TENSOR_F32)
         return attn::launch_after_previous(planes_kernel<float>, dim3(grid), dim3(256), 0, s, static_cast<const float *>(src), ld, hi, lo, R, K, pitch, wide, targets, V,
-                                           counters, count);
+                                           counters, count, common);
     return attn::launch_after_previous(planes_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, static_cast<const __nv_bfloat16 *>(src), ld, hi, lo, R, K, pitch, wide,
-                                       targets, V, counters, count);
+                                       targets, V, counters, count, common);
 }
 
 // Eight threads share the pieces where there are more than four and few words: 49 pieces of 40 x 768 18 -> 4.8 us, 7 of 2048 x 768 23.5 us by eight (11 by one).
 template <class T>
-cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, float by, cudaStream_t s) {
+cudaError_t launch_sum(T *dx, const float *pieces, int count, int M, int K, int pitch, int wide, float by, const float *common, cudaStream_t s) {
     const int groups = count > 4 && (long long)M * (pitch / 4) < 100000 ? 8 : 1;
     const int grid = blocks_for((long long)M * (pitch / 4) * groups);
-    return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by)
-                      : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by);
+    return groups > 1 ? attn::launch_after_previous(sum_kernel<T, 8>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by, common)
+                      : attn::launch_after_previous(sum_kernel<T, 1>, dim3(grid), dim3(256), 0, s, dx, pieces, count, M, K, pitch, wide, by, common);
 }
 
 template <int kTerms, bool kBackward>
@@ -1033,8 +1078,8 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
         return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, a.part, a.zt, a.targets, losses, lse, few_rows_parts(V, sms), rows, V);
     }
-    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
-    if (l.copy_x && (e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
+    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, Common{}, s)) != cudaSuccess) return (int)e;
+    if (l.copy_x && (e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, Common{}, s)) != cudaSuccess) return (int)e;
     Maps maps = {};
     if ((rc = map_of(&maps.x, l.copy_x ? base + l.x : x, rows, K, l.copy_x ? l.pitch : rows > 1 ? ldx : l.pitch, l.plane_x, l.planes, 128)) != 0) return rc;
     if ((rc = map_of(&maps.w, l.copy_w ? base + l.w : w, V, K, l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch, l.plane_w, l.planes, l.wide)) != 0) return rc;
@@ -1080,10 +1125,10 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
-    auto sum = [&](const float *pieces, int count, int pitch, double by) {
+    auto sum = [&](const float *pieces, int count, int pitch, double by, const float *common) {
         const int wide = (reinterpret_cast<uintptr_t>(dx) & 15) == 0 && (size_t)K * each % 16 == 0;
-        return (int)(type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), pieces, count, rows, K, pitch, wide, (float)by, s)
-                                        : launch_sum(static_cast<__nv_bfloat16 *>(dx), pieces, count, rows, K, pitch, wide, (float)by, s));
+        return (int)(type == TENSOR_F32 ? launch_sum(static_cast<float *>(dx), pieces, count, rows, K, pitch, wide, (float)by, common, s)
+                                        : launch_sum(static_cast<__nv_bfloat16 *>(dx), pieces, count, rows, K, pitch, wide, (float)by, common, s));
     };
     if (few_rows_gradients_fit(x, w, dw, ldx, ldw, lddw, type, rows, V, K)) {
         const FewLayout f = few_layout(rows, V, K, sms);
@@ -1091,12 +1136,13 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         float *dxp = dx ? reinterpret_cast<float *>(base + f.dxp) : nullptr;
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
         if ((e = launch_few_rows_products(a, type, dw, lddw, dxp, f.dx_pitch, sms, s)) != cudaSuccess) return (int)e;
-        return dx ? sum(dxp, f.pieces, f.dx_pitch, 1.0) : ATTN_OK;
+        return dx ? sum(dxp, f.pieces, f.dx_pitch, 1.0, nullptr) : ATTN_OK;
     }
     const Layout l = layout(x, w, ldx, ldw, type, rows, V, K, true, sms);
-    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, s)) != cudaSuccess) return (int)e;
+    if (l.copy_w && (e = launch_planes(w, ldw, type, base + l.w, l.plane_w, V, K, l.pitch, Ids{nullptr, 0}, 0, nullptr, 0, Common{}, s)) != cudaSuccess) return (int)e;
     int *counters = reinterpret_cast<int *>(base + l.counters);
-    if ((e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{targets, target_type}, V, counters, l.pieces + 1, s)) != cudaSuccess) return (int)e;
+    const Common common{g, type == TENSOR_BF16 ? reinterpret_cast<float *>(counters + l.pieces + 1) : nullptr, one_g};
+    if ((e = launch_planes(x, ldx, type, base + l.x, l.plane_x, rows, K, l.pitch, Ids{targets, target_type}, V, counters, l.pieces + 1, common, s)) != cudaSuccess) return (int)e;
 
     const void *wp = l.copy_w ? base + l.w : w;
     const long long pitch_w = l.copy_w ? l.pitch : V > 1 ? ldw : l.pitch;
@@ -1108,7 +1154,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
     Problem p = {};
     p.M = rows, p.V = V, p.K = K;
     set_fix(p, type);
-    p.fix_g = 1.f;
+    p.fix_g = 1.f, p.common = common.out;
     double fix_dx = 1.0;
     p.tiles_m = (rows + kTile - 1) / kTile;
     p.tiles_k = (K + kTile - 1) / kTile;
@@ -1159,7 +1205,7 @@ int xent_sm100_linear_backward(const float *g, const void *x, const void *w, con
         e = type == TENSOR_F32 ? launch_tiles<3, true>(maps, p, sms, status, s) : launch_tiles<1, true>(maps, p, sms, status, s);
         if (e != cudaSuccess) return (int)e;
     }
-    return dx ? sum(p.dxp, l.dx_pieces, l.dx_pitch, fix_dx) : ATTN_OK;
+    return dx ? sum(p.dxp, l.dx_pieces, l.dx_pitch, fix_dx, common.out) : ATTN_OK;
 }
 
 }  // extern "C"

@@ -86,7 +86,8 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
  *     G[r, v]  = g[r] (exp(z[r, v] - lse[r]) - [v = targets[r]])    g has one value per row, or one in all (one_g); 0 without a target
  *     dx[r, :] = sum_v G[r, v] w[v, :]      overwritten, rows K elements apart, of `type`; may be NULL
  *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call; may be NULL, but not both
- * With bf16 tensors G is rounded to bf16 before these products, with fp32 tensors it is two bf16 terms like the others.  The results
+ * With bf16 tensors G is rounded to bf16 before these products (above 8 rows; without the significand of the largest |g| of a row that has a target, which the
+ * sums are multiplied by: one factor for all rows costs no accuracy), with fp32 tensors it is two bf16 terms like the others.  The results
  * have the same bits in every call on GPUs of as many SMs.
  * G is in memory for two pieces of the vocabulary at a time, up to 256 MB each, or 16384 bytes a row (fp32 32768) where that is more:
  * scratch of xent_sm100_linear_backward_scratch_bytes bytes, which also has room for dx in fp32 and for copies of x and, if fp32, of w;
