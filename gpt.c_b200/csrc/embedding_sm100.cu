@@ -41,7 +41,9 @@ constexpr int kAhead = 8;                     // places whose rows a thread asks
 // CTAs that sort without a cluster, and the longest list they take, which is what their shared memory holds.  (8192 places of 768 fp32 columns, the whole
 // gradient: 16.5 us, by the cluster 30.)
 constexpr int kBucketBits = 7, kBucketed = 8192;
-constexpr int kComparedBits = 9, kCompared = 1 << kComparedBits;  // places of a bucket that are compared each with each (tokens have 30 bits)
+// Places of a bucket that are compared each with each, by numbers of 32 bits: no token's own, V, has to have 30 bits as well, so a table of 2^30 rows takes the other way.
+constexpr int kComparedBits = 9, kCompared = 1 << kComparedBits, kComparedRows = (1 << 30) - 1;
+static_assert((kComparedRows >> kBucketBits) < 1 << (32 - kComparedBits), "a token's digits above its bucket's, V's among them, fit above a place");
 // Where each place can look at all others.  (768 fp32 columns, by buckets in brackets: 16 places 3.4 us (10.5), 512 places 6.8 (11.2); its time grows with
 // the square.)
 constexpr int kFewTokens = 512;
@@ -413,7 +415,7 @@ __device__ void sort_bucket(const List &l, int bucket, BucketSmem &sm) {
     }
     __syncthreads();
     if (count == 0) return;
-    if (count <= kCompared) {  // each with each: a token's other digits and its place in the bucket as one number
+    if (count <= kCompared && l.V <= kComparedRows) {  // each with each: a token's other digits and its place in the bucket as one number
         uint32_t *all = reinterpret_cast<uint32_t *>(sm.sort.sorted);
         const int i = threadIdx.x, fours = (count + 3) / 4;
         uint32_t own = 0xffffffffu;
