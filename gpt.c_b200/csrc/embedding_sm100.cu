@@ -431,54 +431,29 @@ __device__ void sort_bucket(const List &l, int bucket, BucketSmem &sm) {
         const_cast<int2 *>(l.sorted)[base + rank] = sm.mine[i];
         return;
     }
+    static_assert(kBucketed <= kItems * kSortThreads, "a bucket is one round");
     Round r;
     r.items = min(kItems, (count + kSortThreads - 1) / kSortThreads), r.bits = l.bits;
-    const int round = r.items * kSortThreads, d = threadIdx.x;
+    const int d = threadIdx.x;
     for (int pass = 0; pass < l.passes; pass++) {
         r.shift = kBucketBits + pass * l.bits;
         int2 *out = l.places[(l.passes - 1 - pass) & 1] + base;
         const int2 *in = l.places[(l.passes - pass) & 1] + base;
-        auto read = [&](int begin) {
-            if (pass > 0) {
-                r.read(in, begin, count);
-                return;
-            }
-            const int first = r.first(begin);
+        if (pass > 0) {
+            r.read(in, 0, count);
+        } else {
+            const int first = r.first(0);
 #pragma unroll
             for (int i = 0; i < kItems; i++) {
                 const int2 e = sm.mine[min(first + 32 * i, count - 1)];
                 r.k[i] = i < r.items && first + 32 * i < count ? e.x : -1, r.place[i] = e.y;
             }
-        };
-        if (count <= round) {
-            read(0);
-            r.rank(sm.sort);
-        } else {
-            if (d < 1 << r.bits) sm.sort.count[d] = 0;
-            __syncthreads();
-            for (int begin = 0; begin < count; begin += round) {
-                read(begin);
-#pragma unroll
-                for (int i = 0; i < kItems; i++)
-                    if (r.k[i] >= 0) atomicAdd(&sm.sort.count[r.digit(r.k[i])], 1);
-            }
-            __syncthreads();
         }
+        r.rank(sm.sort);
         const int front = in_front(d < 1 << r.bits ? sm.sort.count[d] : 0, sm.sort.scan);
         if (d < 1 << r.bits) sm.sort.base[d] = front;
         __syncthreads();
-        if (count <= round) {
-            r.scatter(sm.sort, out, count);
-        } else {
-            for (int begin = 0; begin < count; begin += round) {
-                read(begin);
-                r.rank(sm.sort);
-                r.scatter(sm.sort, out, min(round, count - begin));
-                __syncthreads();
-                if (d < 1 << r.bits) sm.sort.base[d] += sm.sort.count[d];
-                __syncthreads();
-            }
-        }
+        r.scatter(sm.sort, out, count);
         __syncthreads();
     }
 }
