@@ -189,6 +189,7 @@ struct Gradient {
     List list[2];
     int lists, C;
     int T, P;             // positions that are a token's place: sequences of T, table of P (T 0: none)
+    int place_width;      // pieces of rows of that table that a block has at a time, a power of two
     long long n;
     void *pos_grad;
     long long pos_ld;
@@ -495,28 +496,64 @@ __device__ __forceinline__ void clear(float (&v)[kN]) {
     for (int e = 0; e < kN; e++) v[e] = 0.f;
 }
 
-// The positions that are a token's place: dpos[t] += dy[t] + dy[t + T] + .., for the threads `first`, `first` + step, ..
+// Rows t, t + step, .. of dy, eight at a time.
+template <class E, int kN>
+__device__ __forceinline__ void add_rows(const Gradient &a, long long t, long long step, int col, float (&sum)[kN]) {
+    for (; t < a.n; t += kAhead * step) {
+        Raw<E, kN> v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) v[u].load(static_cast<const E *>(a.dy) + min(t + u * step, a.n - 1) * a.ld + col);
+        float part[kN] = {};  // (a sum of every term behind the other loses bits where they are many)
+#pragma unroll
+        for (int u = 0; u < kAhead; u++)
+            if (t + u * step < a.n) v[u].add_to(part);
+#pragma unroll
+        for (int e = 0; e < kN; e++) sum[e] += part[e];
+    }
+}
+
+// The positions that are a token's place: dpos[t] += dy[t] + dy[t + T] + .., by block `block` of `blocks`, of which all threads come here and `threads` work.
+// a.place_width of them have a piece of a row of the table each (place_width() says how many); `threads` / place_width share its sequences, each taking every so many-th, and
+// their sums are added up in pairs.  `shared`: threads / 2 * kN values, unless every thread has a piece of its own.
 template <class E, class G, int kN>
-__device__ __forceinline__ void add_places(const Gradient &a, long long first, long long step) {
-    const int words = a.C / kN;
-    const long long T = min((long long)a.T, a.n), total = min(T, (long long)a.P) * words;
-    for (long long i = first; i < total; i += step) {
-        const long long t = i / words;
-        const int col = (int)(i - t * words) * kN;
-        float sum[kN] = {};
-        Raw<G, kN> old;
-        G *grad = static_cast<G *>(a.pos_grad) + t * a.pos_ld + col;
-        old.load(grad);
-        for (long long r = t; r < a.n; r += (long long)kAhead * a.T) {
-            Raw<E, kN> v[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; u++) v[u].load(static_cast<const E *>(a.dy) + min(r + (long long)u * a.T, a.n - 1) * a.ld + col);
-#pragma unroll
-            for (int u = 0; u < kAhead; u++)
-                if (r + (long long)u * a.T < a.n) v[u].add_to(sum);
+__device__ __forceinline__ void add_places(const Gradient &a, int block, int blocks, int threads, float *shared) {
+    const int words = a.C / kN, width = a.place_width;
+    const long long total = min(min((long long)a.T, a.n), (long long)a.P) * words;
+    Held<G, kN> old;
+    if (width == threads) {  // (the loop below with one group: 4 % slower in the largest case)
+        for (long long i = (long long)block * width + threadIdx.x; i < total && (int)threadIdx.x < threads; i += (long long)blocks * width) {
+            const long long t = i / words;
+            const int col = (int)(i - t * words) * kN;
+            G *grad = static_cast<G *>(a.pos_grad) + t * a.pos_ld + col;
+            float sum[kN] = {};
+            old.ask(grad);
+            add_rows<E, kN>(a, t, a.T, col, sum);
+            old.add(grad, sum, 1.f);
         }
-        old.add(sum, 1.f);
-        old.store(grad);
+        return;
+    }
+    const int groups = threads / width, group = (int)threadIdx.x / width, own = (int)threadIdx.x & (width - 1);
+    for (long long i0 = (long long)block * width; i0 < total; i0 += (long long)blocks * width) {
+        const long long i = i0 + own, t = i / words;
+        const int col = (int)(i - t * words) * kN;
+        const bool inside = i < total && group < groups;
+        G *grad = static_cast<G *>(a.pos_grad) + t * a.pos_ld + col;
+        float sum[kN] = {};
+        if (inside && group == 0) old.ask(grad);
+        if (inside) add_rows<E, kN>(a, t + (long long)group * a.T, (long long)groups * a.T, col, sum);
+        for (int half = groups / 2; half > 0; half /= 2) {
+            if (inside && group >= half && group < 2 * half) {
+#pragma unroll
+                for (int e = 0; e < kN; e++) shared[e * (threads / 2) + (group - half) * width + own] = sum[e];
+            }
+            __syncthreads();
+            if (inside && group < half) {
+#pragma unroll
+                for (int e = 0; e < kN; e++) sum[e] += shared[e * (threads / 2) + group * width + own];
+            }
+            __syncthreads();
+        }
+        if (inside && group == 0) old.add(grad, sum, 1.f);
     }
 }
 
@@ -530,7 +567,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_kernel(const __grid_cons
     pdl_wait();
     const int cluster = blockIdx.x / kSortCtas, others = a.lists * kSortCtas;
     if (cluster < a.lists) sort_list(a.list[cluster], *reinterpret_cast<SortSmem *>(smem_raw));
-    else add_places<E, G, kN>(a, (long long)(blockIdx.x - others) * kSortThreads + threadIdx.x, (long long)(gridDim.x - others) * kSortThreads);
+    else add_places<E, G, kN>(a, (int)blockIdx.x - others, (int)gridDim.x - others, kSortThreads, reinterpret_cast<float *>(smem_raw));
 }
 
 // A CTA for each bucket of each list.  Bound by latency: no more than 4 MB are moved, most of them from L2.  8192 places of 768 fp32
@@ -552,8 +589,8 @@ __global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ 
     pdl_launch_dependents();
     pdl_wait();
     if ((int)blockIdx.x >= blocks) {
-        const long long others = (long long)(gridDim.x - blocks) * gridDim.y;
-        add_places<E, G, kN>(a, ((long long)(blockIdx.x - blocks) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x, others * kThreads);
+        __shared__ float shared[kThreads / 2 * kN];
+        add_places<E, G, kN>(a, (int)((blockIdx.x - blocks) * gridDim.y + blockIdx.y), (int)((gridDim.x - blocks) * gridDim.y), kThreads, shared);
         return;
     }
     const int lane = threadIdx.x & 31, unit = (int)blockIdx.x * (kThreads / 32) + (int)(threadIdx.x >> 5);
@@ -722,8 +759,7 @@ __global__ void __launch_bounds__(kSortThreads) few_kernel(const __grid_constant
     __shared__ int list[kFewTokens], counts[kFewTokens / 32], of[1];
     const int n = (int)a.n, which = blockIdx.x / n;
     if (which >= a.lists) {
-        const int threads = width * groups, b = (int)blockIdx.x - a.lists * n;
-        if ((int)threadIdx.x < threads) add_places<E, G, kN>(a, (long long)b * threads + threadIdx.x, (long long)(gridDim.x - a.lists * n) * threads);
+        add_places<E, G, kN>(a, (int)blockIdx.x - a.lists * n, (int)gridDim.x - a.lists * n, kFewTokens, shared);
         return;
     }
     const List &l = a.list[which];
@@ -838,18 +874,32 @@ size_t list_bytes(long long n, int C, int V, List *l, char *base) {
     return at;
 }
 
+// How many pieces of rows of the position table a block of `threads` takes at a time: one a thread, but fewer, whose sequences threads share, where that makes fewer than `blocks`
+// blocks, there are eight sequences for each thread, and a row is still read 32 bytes at a time.  us of the whole gradient of 768 fp32 columns with one a thread, in brackets by
+// this rule: 8192 places in sequences of 1 518 (46), of 8 88 (34), of 64 35 (29); 65536 in sequences of 1 5983 (148), of 16 584 (123).  Halved once more where blocks are
+// enough, 48 sequences of 1024 x 1600 bf16 columns took 119 instead of 100.
+int place_width(long long places, const Gradient &a, int threads, int blocks) {
+    const long long sequences = a.T > 0 ? (a.n + a.T - 1) / a.T : 0;
+    int width = threads;
+    while (width > 2 && sequences * width > 8ll * threads && (places + width - 1) / width < blocks) width /= 2;
+    return width;
+}
+
 template <class E, class G, int kN>
-cudaError_t launch_gradient(const Gradient &a, cudaStream_t s) {
+cudaError_t launch_gradient(Gradient a, cudaStream_t s) {
     const int words = a.C / kN;
     const long long places = a.T > 0 ? std::min(std::min((long long)a.T, a.n), (long long)a.P) * words : 0;
     if (a.n <= kFewTokens) {
         const int width = std::min(256, (words + 31) / 32 * 32), groups = std::max(1, std::min(4, kSortThreads / width));
         const int threads = std::max(width * groups, kFewTokens);
-        const long long blocks = a.lists * a.n + std::min(600ll, (places + width * groups - 1) / (width * groups));
-        return attn::launch_after_previous(few_kernel<E, G, kN>, dim3((unsigned)blocks), dim3((unsigned)threads), sizeof(float) * kN * width * (groups - 1), s, a, width, groups);
+        a.place_width = place_width(places, a, kFewTokens, 148);
+        const long long blocks = a.lists * a.n + std::min(600ll, (places + a.place_width - 1) / a.place_width);
+        const int shared = std::max(width * (groups - 1), a.place_width < kFewTokens ? kFewTokens / 2 : 0);
+        return attn::launch_after_previous(few_kernel<E, G, kN>, dim3((unsigned)blocks), dim3((unsigned)threads), sizeof(float) * kN * shared, s, a, width, groups);
     }
     cudaError_t e;
-    const long long all = (places + kSortThreads - 1) / kSortThreads;  // blocks for the positions that are a token's place
+    a.place_width = a.n <= kBucketed ? place_width(places, a, kThreads, 296) : place_width(places, a, kSortThreads, 136);
+    const long long all = (places + a.place_width - 1) / a.place_width;  // blocks for the positions that are a token's place
     if (a.n <= kBucketed) {
         e = a.lists == 0 ? cudaSuccess : attn::launch_after_previous(bucket_kernel, dim3((unsigned)(a.lists << kBucketBits)), dim3(kSortThreads), sizeof(BucketSmem), s, a);
     } else {
@@ -860,7 +910,7 @@ cudaError_t launch_gradient(const Gradient &a, cudaStream_t s) {
     const unsigned slices = (unsigned)((words + 31) / 32);
     const int ranges = a.list[0].ranges + (a.lists > 1 ? a.list[1].ranges : 0);
     const int groups = (ranges + kThreads / 32 - 1) / (kThreads / 32);
-    const long long others = a.n <= kBucketed ? (std::min((places + kThreads - 1) / kThreads, 1184ll) + slices - 1) / slices : 0;
+    const long long others = a.n <= kBucketed ? (std::min(all, 1184ll) + slices - 1) / slices : 0;
     e = attn::launch_after_previous(runs_kernel<E, G, kN>, dim3((unsigned)(groups + others), slices), dim3(kThreads), 0, s, a, groups);
     if (e != cudaSuccess || a.lists == 0) return e;
     const int joins = (a.list[0].ranges + kJoinWarps - 1) / kJoinWarps + (a.lists > 1 ? (a.list[1].ranges + kJoinWarps - 1) / kJoinWarps : 0);
