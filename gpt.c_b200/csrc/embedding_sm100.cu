@@ -979,13 +979,12 @@ int tensor_sm100_embedding_backward(const void *dy, const void *tokens, void *dt
     if (!dy || (!dtable && !dpos_table) || (dtable && !tokens)) return ATTN_ERR_NULL;
     if (n < 0 || C <= 0 || ld_dy < C || !embed::float_type(type) || !embed::float_type(grad_type) || !embed::id_type(id_type)) return ATTN_ERR_ARGUMENT;
     if ((dtable && (V <= 0 || ld < C)) || (dpos_table && (P <= 0 || pos_ld < C || (!positions && T <= 0)))) return ATTN_ERR_ARGUMENT;
-    const bool listed = dtable || positions;
-    if (n > 0 && listed && !scratch) return ATTN_ERR_NULL;
     const uintptr_t each = embed::each_of(type), grad_each = embed::each_of(grad_type);
     if (embed::bits(dy) % each || (embed::bits(dtable) | embed::bits(dpos_table)) % grad_each || (embed::bits(scratch) & 255) ||
         ((embed::bits(tokens) | embed::bits(positions)) & embed::id_mask(id_type)))
         return ATTN_ERR_ALIGN;
     if (n > (1 << 30) || C > (1 << 20) || V > (1 << 30) || P > (1 << 30)) return ATTN_ERR_UNSUPPORTED;
+    if (n > 0 && (dtable || positions) && !scratch) return ATTN_ERR_NULL;  // (behind the sizes that have none)
     if ((n && dtable && embed::overlap(dy, n, ld_dy, each, dtable, V, ld, grad_each, C)) || (n && dpos_table && embed::overlap(dy, n, ld_dy, each, dpos_table, P, pos_ld, grad_each, C)) ||
         (dtable && dpos_table && embed::overlap(dtable, V, ld, grad_each, dpos_table, P, pos_ld, grad_each, C)))
         return ATTN_ERR_ARGUMENT;
