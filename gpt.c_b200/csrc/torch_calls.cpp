@@ -551,7 +551,7 @@ PyObject *linear_xent_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
         scratch = alloc({(int64_t)bytes}, at::kByte, *h.x);
         float *lp = static_cast<float *>(losses.data_ptr()), *ep = static_cast<float *>(lse.data_ptr());
         const void *tp = h.targets->data_ptr();
-        void *sp = bytes ? scratch.data_ptr() : reinterpret_cast<void *>(uintptr_t(256));  // (sizes that the call refuses)
+        void *sp = bytes ? scratch.data_ptr() : nullptr;  // (none: sizes that the call refuses)
         Py_BEGIN_ALLOW_THREADS
         rc = xent_sm100_linear_forward(h.xr.p, h.wr.p, tp, lp, ep, sp, h.xr.ld, h.wr.ld, h.type, h.ids, rows, V, K, on.stream);
         Py_END_ALLOW_THREADS
@@ -590,7 +590,7 @@ PyObject *linear_xent_backward(PyObject *, PyObject *const *args, Py_ssize_t n) 
         scratch = alloc({(int64_t)bytes}, at::kByte, *h.x);
         const float *gp = static_cast<const float *>(g->data_ptr()), *ep = static_cast<const float *>(lse->data_ptr());
         const void *tp = h.targets->data_ptr();
-        void *dxp = want_dx ? dx.data_ptr() : nullptr, *dwp = dw ? dw->data_ptr() : nullptr, *sp = bytes ? scratch.data_ptr() : reinterpret_cast<void *>(uintptr_t(256));
+        void *dxp = want_dx ? dx.data_ptr() : nullptr, *dwp = dw ? dw->data_ptr() : nullptr, *sp = bytes ? scratch.data_ptr() : nullptr;
         const int one = g->numel() == 1;
         Py_BEGIN_ALLOW_THREADS
         rc = xent_sm100_linear_backward(gp, h.xr.p, h.wr.p, tp, ep, dxp, dwp, sp, h.xr.ld, h.wr.ld, dr.ld, one, h.type, h.ids, rows, V, K, on.stream);

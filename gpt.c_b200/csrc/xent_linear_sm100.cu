@@ -1061,9 +1061,10 @@ size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, lo
 int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
                               int target_type, int rows, int V, int K, void *stream) {
     using namespace head;
-    if (!x || !w || !targets || !losses || !lse || (rows > 0 && !scratch)) return ATTN_ERR_NULL;
+    if (!x || !w || !targets || !losses || !lse) return ATTN_ERR_NULL;
     int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
     if (rc != ATTN_OK) return rc;
+    if (rows > 0 && !scratch) return ATTN_ERR_NULL;  // (behind the sizes that have none)
     if ((reinterpret_cast<uintptr_t>(losses) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3)) return ATTN_ERR_ALIGN;
     int *status = nullptr;
     if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
@@ -1102,11 +1103,12 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
 int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw, void *scratch, long long ldx,
                                long long ldw, long long lddw, int one_g, int type, int target_type, int rows, int V, int K, void *stream) {
     using namespace head;
-    if (!g || !x || !w || !targets || !lse || (rows > 0 && !scratch) || (!dx && !dw)) return ATTN_ERR_NULL;
+    if (!g || !x || !w || !targets || !lse || (!dx && !dw)) return ATTN_ERR_NULL;
     int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
     if (rc != ATTN_OK) return rc;
     if (dw && lddw < K) return ATTN_ERR_ARGUMENT;
     if (rows > kMostRows) return ATTN_ERR_UNSUPPORTED;
+    if (rows > 0 && !scratch) return ATTN_ERR_NULL;
     const size_t each = type == TENSOR_F32 ? 4 : 2;
     if ((reinterpret_cast<uintptr_t>(g) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3) || reinterpret_cast<uintptr_t>(dx) % each || reinterpret_cast<uintptr_t>(dw) % each)
         return ATTN_ERR_ALIGN;
