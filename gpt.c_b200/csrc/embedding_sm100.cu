@@ -828,10 +828,12 @@ uintptr_t id_mask(int t) { return t == TENSOR_INT64 ? 7 : 3; }
 uintptr_t each_of(int t) { return t == TENSOR_F32 ? 4 : 2; }
 uintptr_t bits(const void *p) { return reinterpret_cast<uintptr_t>(p); }
 
-bool overlap(const void *a, long long rows_a, long long ld_a, uintptr_t each_a, const void *b, long long rows_b, long long ld_b, uintptr_t each_b, int C) {
-    const uintptr_t end_a = bits(a) + ((rows_a - 1) * ld_a + C) * each_a, end_b = bits(b) + ((rows_b - 1) * ld_b + C) * each_b;
-    return bits(a) < end_b && bits(b) < end_a;
-}
+// The memory from a matrix's first row to its last; NULL: none.
+struct Span {
+    uintptr_t from, to;
+    Span(const void *p, long long rows, long long ld, long long columns, uintptr_t each) : from(bits(p)), to(p ? bits(p) + ((rows - 1) * ld + columns) * each : 0) {}
+    bool meets(const Span &o) const { return from && o.from && from < o.to && o.from < to; }
+};
 
 // Places of a range, which a warp takes: 32 at most.  Short ranges make more warps, long ones fewer parts of runs.  (768 fp32 columns: 8192 places
 // 16.5 us by 8, 17.8 by 16; 16384 places 40 by 8, 36.6 by 16; 32768 places 72 by 16, 69 by 32; 49152 places 93.6 by 16, 90 by 32.)
@@ -950,11 +952,17 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
     if (pos_table && (P <= 0 || pos_ld < C || (!positions && T <= 0))) return ATTN_ERR_ARGUMENT;
     const uintptr_t each = embed::each_of(type);
     if ((embed::bits(table) | embed::bits(pos_table) | embed::bits(y)) % each || ((embed::bits(tokens) | embed::bits(positions)) & embed::id_mask(id_type))) return ATTN_ERR_ALIGN;
+    if (n > 0) {
+        if (n > (1ll << 40) / C || C > (1 << 20)) return ATTN_ERR_UNSUPPORTED;
+        const uintptr_t id_bytes = embed::id_mask(id_type) + 1;
+        const embed::Span out(y, n, C, C, each);
+        for (const embed::Span &in : {embed::Span(table, V, ld, C, each), embed::Span(pos_table, P, pos_ld, C, each), embed::Span(tokens, 1, n, n, id_bytes), embed::Span(positions, 1, n, n, id_bytes)})
+            if (out.meets(in)) return ATTN_ERR_ARGUMENT;
+    }
     int *status = nullptr;
     const int rc = attn::device_status_word(&status);
     if (rc != ATTN_OK) return rc;
     if (n == 0) return ATTN_OK;
-    if (n > (1ll << 40) / C || C > (1 << 20)) return ATTN_ERR_UNSUPPORTED;
     // 32 bytes at a time where every row allows it, else 16, else a value
     const uintptr_t all = embed::bits(table) | embed::bits(pos_table) | embed::bits(y) | C * each | (uintptr_t)ld * each | (pos_table ? (uintptr_t)pos_ld * each : 0);
     const int bytes = all % 32 == 0 ? 32 : all % 16 == 0 ? 16 : (int)each, words = (int)(C * each / bytes);
@@ -985,9 +993,13 @@ int tensor_sm100_embedding_backward(const void *dy, const void *tokens, void *dt
         return ATTN_ERR_ALIGN;
     if (n > (1 << 30) || C > (1 << 20) || V > (1 << 30) || P > (1 << 30)) return ATTN_ERR_UNSUPPORTED;
     if (n > 0 && (dtable || positions) && !scratch) return ATTN_ERR_NULL;  // (behind the sizes that have none)
-    if ((n && dtable && embed::overlap(dy, n, ld_dy, each, dtable, V, ld, grad_each, C)) || (n && dpos_table && embed::overlap(dy, n, ld_dy, each, dpos_table, P, pos_ld, grad_each, C)) ||
-        (dtable && dpos_table && embed::overlap(dtable, V, ld, grad_each, dpos_table, P, pos_ld, grad_each, C)))
-        return ATTN_ERR_ARGUMENT;
+    const embed::Span table_at(dtable, V, ld, C, grad_each), pos_at(dpos_table, P, pos_ld, C, grad_each);
+    if (n > 0) {
+        const uintptr_t id_bytes = embed::id_mask(id_type) + 1;
+        for (const embed::Span &in : {embed::Span(dy, n, ld_dy, C, each), embed::Span(tokens, 1, n, n, id_bytes), embed::Span(positions, 1, n, n, id_bytes)})
+            if (table_at.meets(in) || pos_at.meets(in)) return ATTN_ERR_ARGUMENT;
+    }
+    if (table_at.meets(pos_at)) return ATTN_ERR_ARGUMENT;
     int *status = nullptr;
     const int rc = attn::device_status_word(&status);
     if (rc != ATTN_OK) return rc;

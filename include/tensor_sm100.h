@@ -48,7 +48,7 @@ int tensor_sm100_gelu_backward(const float *g, const float *x, float *dx, size_t
  *   tokens, positions [n]            of `id_type`; positions NULL: t % T, a token's place in its sequence of T
  *   y [n, C]                         of `type`, contiguous
  * A token outside 0 .. V - 1 (padding), or a position outside 0 .. P - 1, brings zeros.
- * Up to 2^20 columns, and 2^40 values of y; ATTN_ERR_UNSUPPORTED beyond.  y overlaps neither table.
+ * Up to 2^20 columns, and 2^40 values of y; ATTN_ERR_UNSUPPORTED beyond.  y overlaps no input.
  * The reference's counterpart is embedding_forward_cuda_kernel (kernels/src/cuda/Embedding.cu:46-58), without scale and positions.
  */
 int tensor_sm100_embedding_forward(const void *tokens, const void *table, const void *positions, const void *pos_table, void *y, long long n,
@@ -58,7 +58,7 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
  * dtable[v, :]     += scale * sum of dy[t, :] over tokens[t] = v
  * dpos_table[p, :] += sum of dy[t, :] over positions[t] = p
  *   dy [n, C] of `type`, rows ld_dy elements apart; dtable [V, C], dpos_table [P, C] of `grad_type`, rows ld and pos_ld elements apart; one of
- *   them may be NULL.  None of the three may overlap another (rows of one inside the gaps of another count as that).
+ *   them may be NULL.  None of the three may overlap another (rows of one inside the gaps of another count as that), nor the gradients tokens or positions.
  * Sums are fp32 in an order that n fixes, rounded once where grad_type is TENSOR_BF16: the same bits in every call.  Tokens and positions
  * outside their table have no part.  Rows that no token names are neither read nor written.
  * scratch: tensor_sm100_embedding_backward_scratch_bytes bytes with P = 0 unless positions are given and V = 0 without dtable,
