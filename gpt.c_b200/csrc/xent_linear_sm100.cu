@@ -1066,6 +1066,13 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     if (rc != ATTN_OK) return rc;
     if (rows > 0 && !scratch) return ATTN_ERR_NULL;  // (behind the sizes that have none)
     if ((reinterpret_cast<uintptr_t>(losses) & 3) || (reinterpret_cast<uintptr_t>(lse) & 3)) return ATTN_ERR_ALIGN;
+    if (rows > 0) {
+        const size_t each = type == TENSOR_F32 ? 4 : 2;
+        const Span losses_at(losses, 1, rows, rows, 4), lse_at(lse, 1, rows, rows, 4);
+        for (const Span &in : {Span(x, rows, ldx, K, each), Span(w, V, ldw, K, each), Span(targets, 1, rows, rows, target_type == TENSOR_INT64 ? 8 : 4)})
+            if (losses_at.meets(in) || lse_at.meets(in)) return ATTN_ERR_ARGUMENT;
+        if (losses_at.meets(lse_at)) return ATTN_ERR_ARGUMENT;
+    }
     int *status = nullptr;
     if ((rc = attn::device_status_word(&status)) != ATTN_OK) return rc;
     if (rows == 0) return ATTN_OK;

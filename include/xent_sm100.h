@@ -72,7 +72,7 @@ int xent_sm100_sample(const float *logits, const float *u, const float *temperat
  *   losses[r] = lse[r] - z[r, targets[r]], 0 for a row without a target
  *
  * The products of bf16 tensors are exact, those of fp32 tensors are made of two bf16 terms of each factor (16 bits of it; values
- * above 3.38e38 in size have none); sums are fp32.  rows may be 0.  Outputs overlap no input.
+ * above 3.38e38 in size have none); sums are fp32.  rows may be 0.  Outputs overlap no input and not each other.
  * Up to 2^30 rows and classes and 2^24 features, rows of x and w up to 2^34 elements apart; ATTN_ERR_UNSUPPORTED beyond.
  * scratch: xent_sm100_linear_forward_scratch_bytes bytes for the same arguments on the same device, 256-byte aligned.  (Of the tensors their
  * alignment matters there: bf16 ones on 16-byte boundaries are read where they are, others copied.)

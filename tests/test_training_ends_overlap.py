@@ -3,7 +3,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_training_ends import EMBED, EMBED_GRAD, at  # noqa: E402
+from test_training_ends import EMBED, EMBED_GRAD, LOSS, at  # noqa: E402
 
 ARGUMENT = -8
 LOOKUP = {**EMBED, "tokens": at(1 << 20), "table": at(1 << 21), "pos_table": at(1 << 22), "y": at(1 << 23), "ld": 72}
@@ -21,3 +21,15 @@ def test_embedding_forward(pkg, y):
 def test_embedding_backward(pkg, wrong):
     call = pkg.lib().tensor_sm100_embedding_backward
     assert call(*{**EMBED_GRAD, **wrong}.values()) == ARGUMENT
+
+
+SCORE = {**LOSS, "x": at(1 << 20), "w": at(1 << 21), "targets": at(1 << 22), "losses": at(1 << 23), "lse": at(1 << 24)}
+
+
+@pytest.mark.parametrize("result", ["losses", "lse"])
+@pytest.mark.parametrize("place", [1 << 20, (1 << 20) + 5 * 128 - 4, (1 << 20) - 16, (1 << 21) + 100 * 128 - 4, (1 << 22) + 4 * 8 + 4, (1 << 22) - 4])
+def test_linear_xent_forward(pkg, result, place):
+    call = pkg.lib().xent_sm100_linear_forward
+    assert call(*{**SCORE, result: at(place)}.values()) == ARGUMENT
+    assert call(*{**SCORE, "lse": at((1 << 23) + 16)}.values()) == ARGUMENT
+    assert call(*{**SCORE, "rows": 0, result: at(place)}.values()) != ARGUMENT  # nothing is written
