@@ -61,6 +61,7 @@ SIGNATURES = {
     "xent_sm100_sample": (_c.c_int, [_c.c_void_p] * 7 + [_c.c_longlong] + [_c.c_int] * 2 + [_c.c_void_p]),
     "xent_sm100_linear_forward_scratch_bytes": (_c.c_size_t, [_c.c_void_p] * 2 + [_c.c_longlong] * 2 + [_c.c_int] * 4),
     "xent_sm100_linear_forward": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_longlong] * 2 + [_c.c_int] * 5 + [_c.c_void_p]),
+    "xent_sm100_selftest_linear_wait_limit": (_c.c_int, [_c.c_void_p] * 6 + [_c.c_longlong] * 2 + [_c.c_int] * 6 + [_c.c_void_p]),
     "xent_sm100_linear_backward_scratch_bytes": (_c.c_size_t, [_c.c_void_p] * 2 + [_c.c_longlong] * 2 + [_c.c_int] * 4),
     "xent_sm100_linear_backward": (_c.c_int, [_c.c_void_p] * 8 + [_c.c_longlong] * 3 + [_c.c_int] * 6 + [_c.c_void_p]),
     "xent_sm100_backward": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 2 + [_c.c_void_p]),

@@ -101,6 +101,7 @@ struct Problem {
     float fix, log2e;             // z as the tensor cores leave it times `fix` is z; fix * log2(e)
     float fix_g;                  // of G, which makes up for what the sums of dw lose
     const float *common;          // bf16: what the sums of dx and dw are multiplied by, and what G is (common_of)
+    int loaded;                   // forward: items whose operands are asked for, all but in a test of the waits
 };
 
 struct Item {
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) tiles_kernel(const __grid_constan
                 if (j >= kQueue && !(ok = mbar_wait(&sm.item_empty[at], (j / kQueue - 1) & 1, ctx, SITE_ITEM_FREE))) break;
                 sm.item[at] = w;
                 mbar_arrive(&sm.item_full[at]);
-                if (w >= p.total) break;
+                if (w >= p.total || (!kBackward && w >= p.loaded)) break;
                 const Item it = decode<kBackward>(p, w);
                 w = p.counter ? (int)gridDim.x + atomicAdd(p.counter, 1) : w + (int)gridDim.x;
                 if (kBackward && it.kind == kDw && p.fetch_dw)
@@ -1058,8 +1059,9 @@ size_t xent_sm100_linear_backward_scratch_bytes(const void *x, const void *w, lo
     return rows <= 16 ? std::max(tiles, head::few_layout(rows, V, K, attn::sm_count()).total) : tiles;  // (which of them depends on dw too)
 }
 
-int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
-                              int target_type, int rows, int V, int K, void *stream) {
+// loaded < 0: all items are loaded.  Otherwise only rows that go by tiles.
+static int linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
+                          int target_type, int rows, int V, int K, int loaded, void *stream) {
     using namespace head;
     if (!x || !w || !targets || !losses || !lse) return ATTN_ERR_NULL;
     int rc = check(x, w, targets, scratch, ldx, ldw, type, target_type, rows, V, K);
@@ -1081,6 +1083,7 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     char *base = static_cast<char *>(scratch);
     cudaError_t e = cudaSuccess;
+    if (l.few && loaded >= 0) return ATTN_ERR_SHAPE;
     if (l.few) {
         const FewRows a{x, w, ldx, ldw, Ids{targets, target_type}, reinterpret_cast<float2 *>(base), reinterpret_cast<float *>(base + l.zt), rows, V, K, nullptr, nullptr, 0, nullptr, (float)fix_of(K, type)};
         if ((e = launch_few_rows(a, type, sms, s)) != cudaSuccess) return (int)e;
@@ -1099,12 +1102,24 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
     p.next_cols = V, p.wide = l.wide;
     const int tiles = (V + l.wide - 1) / l.wide;
     p.total = p.tiles_m * tiles;
+    p.loaded = loaded < 0 ? p.total : loaded;
     p.targets = Ids{targets, target_type};
     p.part = reinterpret_cast<float2 *>(base + l.part);
     p.zt = reinterpret_cast<float *>(base + l.zt);
     e = type == TENSOR_F32 ? launch_tiles<3, false>(maps, p, sms, status, s) : launch_tiles<1, false>(maps, p, sms, status, s);
     if (e != cudaSuccess) return (int)e;
     return (int)attn::launch_after_previous(join_kernel, dim3((rows + 31) / 32), dim3(1024), 0, s, p.part, p.zt, p.targets, losses, lse, tiles, rows, V);
+}
+
+int xent_sm100_linear_forward(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
+                              int target_type, int rows, int V, int K, void *stream) {
+    return linear_forward(x, w, targets, losses, lse, scratch, ldx, ldw, type, target_type, rows, V, K, -1, stream);
+}
+
+int xent_sm100_selftest_linear_wait_limit(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch, long long ldx, long long ldw, int type,
+                                          int target_type, int rows, int V, int K, int loaded, void *stream) {
+    if (loaded < 0) return ATTN_ERR_SHAPE;
+    return linear_forward(x, w, targets, losses, lse, scratch, ldx, ldw, type, target_type, rows, V, K, loaded, stream);
 }
 
 int xent_sm100_linear_backward(const float *g, const void *x, const void *w, const void *targets, const float *lse, void *dx, void *dw, void *scratch, long long ldx,

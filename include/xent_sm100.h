@@ -82,6 +82,15 @@ int xent_sm100_linear_forward(const void *x, const void *w, const void *targets,
                               long long ldx, long long ldw, int type, int target_type, int rows, int V, int K, void *stream);
 
 /*
+ * What that call does when operands never arrive, without a fault: the same kernels, for more than 48 rows, ask only for the operands of the first `loaded` tiles
+ * (256 rows by up to 256 classes).  The waits for the others run out after their second, attn_sm100_device_status reports 1302 or 1304, whichever
+ * wait was first, and losses and lse are not defined.
+ */
+int xent_sm100_selftest_linear_wait_limit(const void *x, const void *w, const void *targets, float *losses, float *lse, void *scratch,
+                                          long long ldx, long long ldw, int type, int target_type, int rows, int V, int K, int loaded,
+                                          void *stream);
+
+/*
  * Its gradients, with lse from the forward call on the same x, w and targets:
  *     G[r, v]  = g[r] (exp(z[r, v] - lse[r]) - [v = targets[r]])    g has one value per row, or one in all (one_g); 0 without a target
  *     dx[r, :] = sum_v G[r, v] w[v, :]      overwritten, rows K elements apart, of `type`; may be NULL
