@@ -72,7 +72,9 @@ int xent_sm100_sample(const float *logits, const float *u, const float *temperat
  *   losses[r] = lse[r] - z[r, targets[r]], 0 for a row without a target
  *
  * The products of bf16 tensors are exact, those of fp32 tensors are made of two bf16 terms of each factor (16 bits of it; values
- * above 3.38e38 in size have none); sums are fp32.  rows may be 0.  Outputs overlap no input and not each other.
+ * above 3.38e38 in size have none); sums are fp32.  The tensor cores cut sums off: logits are multiplied by what that takes on average, 1 + 0.28 2^-24 for each
+ * 16 features (fp32 tensors: three times that), so where nothing is cut off, as with one feature that is not zero, they are too large by it (768 bf16 features: 8e-7
+ * of themselves; 4096 of fp32: 1.3e-5).  rows may be 0.  Outputs overlap no input and not each other.
  * Up to 2^30 rows and classes and 2^24 features, rows of x and w up to 2^34 elements apart; ATTN_ERR_UNSUPPORTED beyond.
  * scratch: xent_sm100_linear_forward_scratch_bytes bytes for the same arguments on the same device, 256-byte aligned.  (Of the tensors their
  * alignment matters there: bf16 ones on 16-byte boundaries are read where they are, others copied.)
@@ -96,7 +98,8 @@ int xent_sm100_selftest_linear_wait_limit(const void *x, const void *w, const vo
  *     dx[r, :] = sum_v G[r, v] w[v, :]      overwritten, rows K elements apart, of `type`; may be NULL
  *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call; may be NULL, but not both
  * With bf16 tensors G is rounded to bf16 before these products (above 8 rows; without the significand of the largest |g| of a row that has a target, which the
- * sums are multiplied by: one factor for all rows costs no accuracy), with fp32 tensors it is two bf16 terms like the others.  The results
+ * sums are multiplied by: one factor for all rows costs no accuracy), with fp32 tensors it is two bf16 terms like the others, and above 16 rows dx and dw are multiplied by
+ * what the tensor cores cut off of them on average, up to 1 + 2.9e-6.  The results
  * have the same bits in every call on GPUs of as many SMs.
  * G is in memory for two pieces of the vocabulary at a time, up to 256 MB each, or 16384 bytes a row (fp32 32768) where that is more:
  * scratch of xent_sm100_linear_backward_scratch_bytes bytes, which also has room for dx in fp32 and for copies of x and, if fp32, of w;
