@@ -65,7 +65,7 @@ class Case:
             assert ((got.double() - want).abs() <= half_unit(want.abs() + off) + off).all()
 
 
-@pytest.mark.parametrize("M,V,apart", [(6, 4096, 64), (10, 4096, 64), (40, 1024, 72), (300, 4096, 64), (300, 4096, 67), (1000, 2048, 64), (9000, 16384, 64)])
+@pytest.mark.parametrize("M,V,apart", [(6, 4096, 64), (10, 4096, 64), (40, 1024, 72), (300, 4096, 64), (6, 4096, 67), (300, 4096, 67), (1000, 2048, 64), (9000, 16384, 64)])
 def test_a_factor_that_all_rows_share_is_not_rounded(pkg, M, V, apart):
     c = Case(M, V, apart)
     for g in (torch.tensor([G], device="cuda"), torch.tensor([-G * 2.0 ** 40], device="cuda"), torch.full((M,), G, device="cuda")):
