@@ -129,7 +129,9 @@ struct Lookup {
 
 // kN columns at a time; a block takes `rows` rows of `words` such pieces.  i / words for i < 2^16 is the upper half of i * magic.
 // Pieces of a thread: two where they are 32 bytes of two tables, whose four take too many registers.
-// 8192 rows of 768 fp32 values with positions 6.5 us (they are in L2 then; from HBM 8.9, 4500 GB/s), 49152 of 1600 bf16 values 46 to 48 us (5500 GB/s).
+// 8192 rows of 768 fp32 values with positions 6.5 us with everything in L2, 8.9 from HBM (4500 GB/s): two loads that wait for each other, 2.8 rounds of blocks, and 97 MB from
+// L2, a quarter of them rows of positions that each sequence reads again; 49152 of 1600 bf16 values without positions 46 to 48 us (5500 GB/s, HBM).  Rows that start anywhere go a
+// value at a time: 8192 x 767 28 us (fp32) and 35 (bf16), 49152 x 1599 bf16 350.
 constexpr int units_of(int bytes, bool places) { return bytes == 32 && places ? 2 : kUnits; }
 template <class E, int kN, bool kPlaces>
 __global__ void __launch_bounds__(kThreads, 4) lookup_kernel(Lookup a, int rows, int words, unsigned magic) {
@@ -582,8 +584,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) bucket_kernel(const __grid_co
 
 // A warp takes a range of a sorted list, and 32 kN columns (blockIdx.y).  Blocks behind the ranges add up the positions that are a token's place
 // where the sort was not a launch of few CTAs, which leaves room for that.
-// Bound by what 16 warps an SM have on their way, since sums and two batches of rows take 114 registers: half of
-// the memory's rate for 49152 rows of 1600 bf16 columns.
+// Bound by what 16 warps an SM have on their way, since a thread takes 113 or 114 registers: sums and two batches of rows where the table is fp32 (which ranges of up to 8192
+// places, one batch long, do not use), sums, one batch and what the table holds where it is bf16.  Half of the memory's rate for 49152 rows of 1600 bf16 columns.
 template <class E, class G, int kN>
 __global__ void __launch_bounds__(kThreads) runs_kernel(const __grid_constant__ Gradient a, int blocks) {
     pdl_launch_dependents();

@@ -96,7 +96,8 @@ int xent_sm100_selftest_linear_wait_limit(const void *x, const void *w, const vo
  * Its gradients, with lse from the forward call on the same x, w and targets:
  *     G[r, v]  = g[r] (exp(z[r, v] - lse[r]) - [v = targets[r]])    g has one value per row, or one in all (one_g); 0 without a target
  *     dx[r, :] = sum_v G[r, v] w[v, :]      overwritten, rows K elements apart, of `type`; may be NULL
- *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call; may be NULL, but not both
+ *     dw[v, :] += sum_r G[r, v] x[r, :]     rows lddw elements apart, of `type`, one rounding a call (fp32: one for every 1024 rows; values below 2^-126 in size
+ *                                           may become 0, L2 adds); may be NULL, but not both
  * With bf16 tensors G is rounded to bf16 before these products (above 8 rows; without the significand of the largest |g| of a row that has a target, which the
  * sums are multiplied by: one factor for all rows costs no accuracy), with fp32 tensors it is two bf16 terms like the others, and above 16 rows dx and dw are multiplied by
  * what the tensor cores cut off of them on average, up to 1 + 2.9e-6.  The results
