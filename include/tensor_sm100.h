@@ -59,7 +59,7 @@ int tensor_sm100_embedding_forward(const void *tokens, const void *table, const 
  * dpos_table[p, :] += sum of dy[t, :] over positions[t] = p
  *   dy [n, C] of `type`, rows ld_dy elements apart; dtable [V, C], dpos_table [P, C] of `grad_type`, rows ld and pos_ld elements apart; one of
  *   them may be NULL.  None of the three may overlap another (rows of one inside the gaps of another count as that), nor the gradients tokens or positions.
- * Sums are fp32 in an order that n fixes, rounded once where grad_type is TENSOR_BF16: the same bits in every call.  Tokens and positions
+ * Sums are fp32 in an order that the sizes fix, rounded once where grad_type is TENSOR_BF16: the same bits in every call.  Tokens and positions
  * outside their table have no part.  Rows that no token names are neither read nor written.
  * An fp32 gradient, what it holds or becomes, that is below 2^-126 in size may become 0 (L2 adds).
  * scratch: tensor_sm100_embedding_backward_scratch_bytes bytes with P = 0 unless positions are given and V = 0 without dtable,
